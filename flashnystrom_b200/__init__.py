@@ -17,10 +17,12 @@ import sys
 from .nystrom_config import NystromConfig
 from .flash_nystrom import (HAS_CUDA, FlashNystromAttention, FlashNystromFunction,
                             flash_nystrom_attention)
+from .decay import DecayAttention, decay_attention, decay_attention_step, default_log_decay
+from .norm import LayerNorm, layer_norm
 
 __version__ = "0.2.0"
 __all__ = ["FlashNystromAttention", "FlashNystromFunction", "flash_nystrom_attention",
-           "NystromConfig", "HAS_CUDA", "install_as", "__version__"]
+           "NystromConfig", "DecayAttention", "decay_attention", "decay_attention_step", "default_log_decay", "LayerNorm", "layer_norm", "HAS_CUDA", "install_as", "__version__"]
 
 
 def install_as(name="flash_nystrom"):

@@ -83,6 +83,53 @@ class ConvDwArgs(C.Structure):
                 ("device", C.c_int32), ("stream", C.c_void_p)]
 
 
+class Rows(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("stride_b", C.c_int64), ("stride_h", C.c_int64), ("stride_n", C.c_int64)]
+
+
+class DecayShape(C.Structure):
+    _fields_ = [("batch", C.c_int64), ("heads", C.c_int64), ("seq_len", C.c_int64), ("head_dim", C.c_int32), ("dtype", C.c_int32),
+                ("scale", C.c_float), ("flags", C.c_uint32)]
+
+
+class DecayFwdArgs(C.Structure):
+    _fields_ = [("shape", DecayShape), ("q", Rows), ("k", Rows), ("v", Rows), ("out", Rows),
+                ("log_decay", C.c_void_p), ("seq_lens", C.c_void_p), ("initial_state", C.c_void_p), ("final_state", C.c_void_p),
+                ("segment_states", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+                ("device", C.c_int32), ("stream", C.c_void_p), ("device_status", C.c_void_p)]
+
+
+class DecayBwdArgs(C.Structure):
+    _fields_ = [("shape", DecayShape), ("q", Rows), ("k", Rows), ("v", Rows), ("d_out", Rows), ("dq", Rows), ("dk", Rows), ("dv", Rows),
+                ("log_decay", C.c_void_p), ("seq_lens", C.c_void_p), ("initial_state", C.c_void_p), ("d_final_state", C.c_void_p),
+                ("d_initial_state", C.c_void_p), ("segment_states", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+                ("device", C.c_int32), ("stream", C.c_void_p), ("device_status", C.c_void_p)]
+
+
+class DecayStepArgs(C.Structure):
+    _fields_ = [("batch", C.c_int64), ("heads", C.c_int64), ("num_states", C.c_int64), ("head_dim", C.c_int32), ("dtype", C.c_int32),
+                ("scale", C.c_float), ("q", Rows), ("k", Rows), ("v", Rows), ("out", Rows), ("log_decay", C.c_void_p), ("states", C.c_void_p),
+                ("slots", C.c_void_p), ("device", C.c_int32), ("stream", C.c_void_p)]
+
+
+class NormShape(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("cols", C.c_int32), ("groups", C.c_int32), ("dtype", C.c_int32), ("param_dtype", C.c_int32),
+                ("eps", C.c_float)]
+
+
+class NormFwdArgs(C.Structure):
+    _fields_ = [("shape", NormShape), ("x", C.c_void_p), ("x_stride", C.c_int64), ("y", C.c_void_p), ("y_stride", C.c_int64),
+                ("weight", C.c_void_p), ("bias", C.c_void_p), ("mean", C.c_void_p), ("rstd", C.c_void_p), ("device", C.c_int32),
+                ("stream", C.c_void_p)]
+
+
+class NormBwdArgs(C.Structure):
+    _fields_ = [("shape", NormShape), ("x", C.c_void_p), ("x_stride", C.c_int64), ("d_y", C.c_void_p), ("d_y_stride", C.c_int64),
+                ("d_x", C.c_void_p), ("d_x_stride", C.c_int64), ("weight", C.c_void_p), ("mean", C.c_void_p), ("rstd", C.c_void_p),
+                ("d_weight", C.c_void_p), ("d_bias", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+                ("device", C.c_int32), ("stream", C.c_void_p)]
+
+
 # every symbol include/flashnystrom_b200.h declares, with its ctypes signature
 SIGNATURES = {
     "fnb_last_error": (C.c_char_p, []),
@@ -115,6 +162,16 @@ SIGNATURES = {
     "fnb_conv_residual": (C.c_int, [C.POINTER(ConvArgs)]),
     "fnb_conv_dweight_workspace_bytes": (C.c_size_t, [C.c_int64, C.c_int64, C.c_int64, C.c_int32]),
     "fnb_conv_residual_dweight": (C.c_int, [C.POINTER(ConvDwArgs)]),
+    "fnb_check_decay_shape": (C.c_int, [C.POINTER(DecayShape)]),
+    "fnb_decay_segment_floats": (C.c_size_t, [C.POINTER(DecayShape)]),
+    "fnb_decay_workspace_bytes": (C.c_size_t, [C.POINTER(DecayShape)]),
+    "fnb_decay_forward": (C.c_int, [C.POINTER(DecayFwdArgs)]),
+    "fnb_decay_backward": (C.c_int, [C.POINTER(DecayBwdArgs)]),
+    "fnb_decay_step": (C.c_int, [C.POINTER(DecayStepArgs)]),
+    "fnb_check_norm_shape": (C.c_int, [C.POINTER(NormShape)]),
+    "fnb_norm_workspace_bytes": (C.c_size_t, [C.POINTER(NormShape)]),
+    "fnb_norm_forward": (C.c_int, [C.POINTER(NormFwdArgs)]),
+    "fnb_norm_backward": (C.c_int, [C.POINTER(NormBwdArgs)]),
     "fnb_set_profiling": (C.c_int, [C.c_int]),
     "fnb_last_profile": (C.c_int, [C.POINTER(KernelTime), C.c_int]),
 }

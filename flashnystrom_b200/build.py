@@ -26,7 +26,7 @@ CSRC = os.path.join(PKG, "csrc")
 LIB_DIR = os.path.join(PKG, "lib")
 PACKAGE_LIB = os.path.join(LIB_DIR, "libflashnystrom_b200.so")
 LIB_PATH = os.path.join(LIB_DIR, os.environ.get("FNB_LIB_NAME", os.path.basename(PACKAGE_LIB)))
-SOURCES = ["fnb_api.cu"]
+SOURCES = ["fnb_api.cu", "fnb_operators.cu"]
 NATIVE_SOURCE = os.path.join(CSRC, "native.cpp")
 NATIVE_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden"]
 HEADER = os.path.join(os.path.dirname(PKG), "include", "flashnystrom_b200.h")
@@ -34,6 +34,7 @@ HEADER = os.path.join(os.path.dirname(PKG), "include", "flashnystrom_b200.h")
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden", "-shared",
+    "--threads", "0",      # the sources side by side
 ]
 if os.environ.get("FNB_PTXAS_VERBOSE"):      # registers, spills, shared memory per kernel
     NVCC_FLAGS += ["-Xptxas", "-v"]
@@ -96,6 +97,18 @@ def native_path():
     return os.path.join(LIB_DIR, f"_native.{versions}.{digest.hexdigest()[:16]}.so")
 
 
+def _loaded_libstdcxx():
+    """The C++ runtime of this process, to link to by its path: a compiler that finds a static one alone would put a second copy
+    of its streams and locales into the module, and printing a number into a message then ends the process."""
+    with contextlib.suppress(OSError):
+        with open("/proc/self/maps") as f:
+            for line in f:
+                path = line.split(None, 5)[-1].strip()
+                if os.path.basename(path).startswith("libstdc++.so"):
+                    return [path]
+    return []
+
+
 def build_native(force=False, verbose=False):
     """The C++ module: host code only, linked to the CUDA library that the package loads."""
     path = native_path()
@@ -111,7 +124,7 @@ def build_native(force=False, verbose=False):
     cmd += ["-I" + sysconfig.get_paths()["include"], "-I" + os.path.join(cuda, "include"),
             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", NATIVE_SOURCE,
             "-L" + torch_lib, "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python",
-            "-L" + LIB_DIR, "-l:" + os.path.basename(PACKAGE_LIB), "-Wl,-rpath,$ORIGIN"]
+            "-L" + LIB_DIR, "-l:" + os.path.basename(PACKAGE_LIB), "-Wl,-rpath,$ORIGIN"] + _loaded_libstdcxx()
     with _one_at_a_time():
         if not force and os.path.exists(path):      # (another process was faster)
             return path

@@ -1,0 +1,457 @@
+// Causal attention with a decay for each head, on the CUDA cores: the chunked form for sequences, the sum of states over the
+// cuts of a sequence, and the step for single tokens.
+//
+// Output and all three gradients are one form, taken forwards or backwards in time:
+//     A(x, y, z)_s  = sum over t <= s of  exp(g (s - t)) (x_s . y_t) z_t          o = A(q, k, v),  dq = A(do, v, k)
+//     A'(x, y, z)_s = sum over t >= s of  exp(g (t - s)) (x_s . y_t) z_t          dk = A'(v, do, q),  dv = A'(k, q, do)
+// A chunk of C rows takes the pairs inside it from the C x C product x y^T, masked and weighted, and everything before it from
+// the D x D state S = sum exp(..) y z^T, which goes on from chunk to chunk.  Exponents are never negative distances:
+// nothing is divided by a power of exp(g), so that no decay, however strong, leaves the range.
+#pragma once
+#include "common.cuh"
+
+namespace fnb {
+
+struct DecayRows {
+  const void* p;
+  int64_t sb, sh, sn;
+};
+struct DecayParams {
+  DecayRows x, y, z, out;
+  const float* log_decay;     // [H]
+  const int32_t* seq_lens;    // [B] or null
+  const float* state_in;      // [BH][ncut][D][D] or null (zeros): the state that enters each run of rows
+  float* state_out;           // chunk kernel with outputs: [BH][D][D] or null, the state that leaves the last run of a slice;
+                              // without: [BH][ncut][D][D], the sum of each run alone
+  int64_t N;
+  int H, ncut;                // runs of rows per slice
+  int cut0, nrun;             // the runs of this launch: nrun of them from cut0 on
+  int64_t seg_rows;           // rows of a segment (a multiple of the chunk)
+  int sub;                    // runs per segment
+  int64_t sub_rows;           // rows of a run but the last of its segment
+  float scale;                // of the output's part from the run's own chunks
+  float inter;                // of its part from the state: scale, or 1 where the state has it already (gradients of states)
+  float sum_scale;            // of the state's own sums: 1, or scale there
+  int transposed;             // the state is read as its transpose
+  int vec;                    // every pointer and stride is a multiple of 16 bytes
+};
+
+__host__ __device__ inline int64_t decay_cut_begin(int64_t seg_rows, int sub, int64_t sub_rows, int i) {
+  return (int64_t)(i / sub) * seg_rows + (int64_t)(i % sub) * sub_rows;
+}
+// rows [begin, end) of run i, before the sequence's own length is taken into account
+__host__ __device__ inline int64_t decay_cut_end(int64_t seg_rows, int sub, int64_t sub_rows, int64_t N, int i) {
+  const int64_t seg = (int64_t)(i / sub + 1) * seg_rows;
+  int64_t e = i % sub == sub - 1 ? seg : decay_cut_begin(seg_rows, sub, sub_rows, i + 1);
+  if (e > seg) e = seg;
+  return e < N ? e : N;
+}
+
+__device__ __forceinline__ int64_t decay_len(const int32_t* seq_lens, int64_t b, int64_t N) {
+  if (!seq_lens) return N;
+  const int64_t n = seq_lens[b];
+  return n < 0 ? 0 : n > N ? N : n;
+}
+// -inf stands for "nothing of the past": a finite exponent that gives zero at every distance but 0 (-inf * 0 would be NaN)
+__device__ __forceinline__ double decay_log(float g) { return g == -INFINITY ? -1e30 : (double)g; }
+// exp(g n) as the sum of two floats.  The state is multiplied by it once a chunk: a factor rounded to one float would be off by
+// 2^-24 each time in the same direction, 1e-5 over a few hundred chunks of a slow decay.
+struct DecayPair { float hi, lo; };
+__device__ __forceinline__ DecayPair decay_pair(double g, int64_t n) {
+  const double w = exp(g * (double)n);
+  DecayPair p;
+  p.hi = (float)w;
+  p.lo = p.hi < INFINITY ? (float)(w - (double)p.hi) : 0.f;
+  return p;
+}
+__device__ __forceinline__ float decay_by(const DecayPair& p, float s) { return s == 0.f ? 0.f : fmaf(s, p.hi, s * p.lo); }
+
+// ---- chunked form ------------------------------------------------------------------------------------------
+// A CTA walks one run of rows, C at a time; tiles in shared memory as FP32.  Thread (ty, tx) of a 16 x 16 grid holds rows
+// ty + 16 i of the score and output tiles and a (D / 16)^2 piece of the state.  Bound by the shared-memory loads of its FP32 products.
+constexpr int kDecayC = 64;
+template <int D> struct DecaySmem {
+  static constexpr int LD = D + 4, LP = kDecayC + 4;      // (padded rows: 16 rows read at once fall on different banks)
+  static constexpr int kFloats = 3 * kDecayC * LD + kDecayC * LP + D * LD + 80;
+  static constexpr int kBytes = kFloats * 4;
+};
+
+template <class T, int D>
+__device__ __forceinline__ void decay_load_tile(float* dst, const DecayRows& t, int64_t base, int64_t row0, int nv, int vec) {
+  constexpr int V = Vec16<T>::n, CH = D / V, LD = DecaySmem<D>::LD;
+  const T* src = static_cast<const T*>(t.p) + base + row0 * t.sn;
+  for (int i = threadIdx.x; i < kDecayC * CH; i += kThreads) {
+    const int r = i / CH, c = (i % CH) * V;
+    float v[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = 0.f;
+    if (r < nv) {
+      const T* p = src + (int64_t)r * t.sn + c;
+      if (vec) {
+        load16<T>(p, v);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = to_f<T>(p[j]);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < V; j += 4) *reinterpret_cast<float4*>(dst + r * LD + c + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+  }
+}
+
+// CW consecutive floats from shared memory (CW = 1, 2, 4)
+template <int CW> __device__ __forceinline__ void decay_lds(const float* p, float* v) {
+  if (CW == 4) {
+    const float4 x = *reinterpret_cast<const float4*>(p);
+    v[0] = x.x; v[1 % CW] = x.y; v[2 % CW] = x.z; v[3 % CW] = x.w;
+  } else {
+#pragma unroll
+    for (int j = 0; j < CW; ++j) v[j] = p[j];
+  }
+}
+
+template <class T, int D, bool REV, bool OUT>
+__global__ void __launch_bounds__(kThreads, D <= 64 ? 2 : 1) decay_chunk_kernel(DecayParams p) {
+  using L = DecaySmem<D>;
+  constexpr int LD = L::LD, LP = L::LP, C = kDecayC;
+  constexpr int CW = D / 16 < 4 ? D / 16 : 4, CG = D / 16 / CW;      // a thread's columns (and state rows): CG groups of CW
+  extern __shared__ float4 smem4[];
+  float* xs = reinterpret_cast<float*>(smem4);
+  float* ys = xs + C * LD;
+  float* zs = ys + C * LD;
+  float* ps = zs + C * LD;
+  float* ss = ps + C * LP;
+  float* pw = ss + D * LD;           // exp(g n), n = 0 .. C
+
+  const int bh = blockIdx.x / p.nrun, cut = p.cut0 + blockIdx.x % p.nrun;
+  const int b = bh / p.H, h = bh % p.H;
+  const int64_t len = decay_len(p.seq_lens, b, p.N);
+  const int64_t r0 = decay_cut_begin(p.seg_rows, p.sub, p.sub_rows, cut);
+  const int64_t r1 = decay_cut_end(p.seg_rows, p.sub, p.sub_rows, p.N, cut);
+  const int64_t end = r1 < len ? r1 : len;            // rows that count
+  if (!OUT && r0 >= end) return;                       // (what joins the runs knows that there is nothing)
+  const double g = decay_log(p.log_decay[h]);
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  for (int i = threadIdx.x; i <= C; i += kThreads) pw[i] = (float)exp(g * i);
+  const DecayPair full = decay_pair(g, C);
+
+  T* out = OUT ? static_cast<T*>(const_cast<void*>(p.out.p)) + b * p.out.sb + h * p.out.sh : nullptr;
+  if (OUT) {
+    const int64_t z0 = r0 > end ? r0 : end;
+    for (int64_t i = threadIdx.x; i < (r1 - z0) * D; i += kThreads) out[(z0 + i / D) * p.out.sn + i % D] = from_f<T>(0.f);
+  }
+  float S[CG][CW][CG][CW];
+#pragma unroll
+  for (int a = 0; a < CG; ++a)
+#pragma unroll
+    for (int i = 0; i < CW; ++i)
+#pragma unroll
+      for (int c = 0; c < CG; ++c)
+#pragma unroll
+        for (int j = 0; j < CW; ++j) {
+          float s = 0.f;
+          if (OUT && p.state_in) {
+            const int si = a * 64 + ty * CW + i, sj = c * 64 + tx * CW + j;
+            s = p.state_in[((size_t)bh * p.ncut + cut) * D * D + (p.transposed ? sj * D + si : si * D + sj)];
+          }
+          S[a][i][c][j] = s;
+        }
+  const int64_t bx = b * p.x.sb + h * p.x.sh, by = b * p.y.sb + h * p.y.sh, bz = b * p.z.sb + h * p.z.sh;
+  const int chunks = r0 < end ? (int)((end - r0 + C - 1) / C) : 0;
+  for (int ci = 0; ci < chunks; ++ci) {
+    const int64_t c0 = r0 + (int64_t)(REV ? chunks - 1 - ci : ci) * C;
+    const int nv = end - c0 < C ? (int)(end - c0) : C;
+    __syncthreads();
+    decay_load_tile<T, D>(ys, p.y, by, c0, nv, p.vec);
+    decay_load_tile<T, D>(zs, p.z, bz, c0, nv, p.vec);
+    if (OUT) {
+      decay_load_tile<T, D>(xs, p.x, bx, c0, nv, p.vec);
+#pragma unroll
+      for (int a = 0; a < CG; ++a)
+#pragma unroll
+        for (int i = 0; i < CW; ++i)
+#pragma unroll
+          for (int c = 0; c < CG; ++c)
+#pragma unroll
+            for (int j = 0; j < CW; ++j) ss[(a * 64 + ty * CW + i) * LD + c * 64 + tx * CW + j] = S[a][i][c][j];
+      __syncthreads();
+      float acc[4][4] = {};
+      for (int k = 0; k < D; k += 4) {
+        float4 xv[4], yv[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          xv[i] = *reinterpret_cast<const float4*>(xs + (ty + 16 * i) * LD + k);
+          yv[i] = *reinterpret_cast<const float4*>(ys + (tx + 16 * i) * LD + k);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            acc[i][j] = fmaf(xv[i].w, yv[j].w, fmaf(xv[i].z, yv[j].z, fmaf(xv[i].y, yv[j].y, fmaf(xv[i].x, yv[j].x, acc[i][j]))));
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int s = ty + 16 * i, t = tx + 16 * j, d = REV ? t - s : s - t;
+          ps[s * LP + t] = d >= 0 ? acc[i][j] * pw[d] : 0.f;
+        }
+      __syncthreads();
+      float o[4][CG][CW], q[4][CG][CW];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int c = 0; c < CG; ++c)
+#pragma unroll
+          for (int j = 0; j < CW; ++j) o[i][c][j] = q[i][c][j] = 0.f;
+#pragma unroll
+      for (int tb = 0; tb < 4; ++tb)
+        for (int t = tb * 16; t < tb * 16 + 16; t += 4) {
+          float pv[4][4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (REV ? i <= tb : i >= tb) decay_lds<4>(ps + (ty + 16 * i) * LP + t, pv[i]);
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int c = 0; c < CG; ++c) {
+              float zv[CW];
+              decay_lds<CW>(zs + (t + u) * LD + c * 64 + tx * CW, zv);
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (REV ? i <= tb : i >= tb)
+#pragma unroll
+                  for (int j = 0; j < CW; ++j) o[i][c][j] = fmaf(pv[i][u], zv[j], o[i][c][j]);
+            }
+        }
+      for (int k = 0; k < D; k += 4) {
+        float xv[4][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) decay_lds<4>(xs + (ty + 16 * i) * LD + k, xv[i]);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+          for (int c = 0; c < CG; ++c) {
+            float sv[CW];
+            decay_lds<CW>(ss + (k + u) * LD + c * 64 + tx * CW, sv);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+              for (int j = 0; j < CW; ++j) q[i][c][j] = fmaf(xv[i][u], sv[j], q[i][c][j]);
+          }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int s = ty + 16 * i;
+        if (s >= nv) continue;
+        const float w = p.inter * pw[REV ? nv - 1 - s : s + 1];
+        T* to = out + (c0 + s) * p.out.sn;
+#pragma unroll
+        for (int c = 0; c < CG; ++c) {
+          T v[CW];
+#pragma unroll
+          for (int j = 0; j < CW; ++j) v[j] = from_f<T>(w == 0.f ? p.scale * o[i][c][j] : fmaf(w, q[i][c][j], p.scale * o[i][c][j]));
+          if (CW == 4 && p.vec) {
+            if (sizeof(T) == 4) *reinterpret_cast<uint4*>(to + c * 64 + tx * CW) = *reinterpret_cast<uint4*>(v);
+            else *reinterpret_cast<uint2*>(to + c * 64 + tx * CW) = *reinterpret_cast<uint2*>(v);
+          } else {
+#pragma unroll
+            for (int j = 0; j < CW; ++j) to[c * 64 + tx * CW + j] = v[j];
+          }
+        }
+      }
+    } else {
+      __syncthreads();
+    }
+    // the state: U = sum over the chunk's rows, then S = exp(g nv) S + U
+    float U[CG][CW][CG][CW];
+#pragma unroll
+    for (int a = 0; a < CG; ++a)
+#pragma unroll
+      for (int i = 0; i < CW; ++i)
+#pragma unroll
+        for (int c = 0; c < CG; ++c)
+#pragma unroll
+          for (int j = 0; j < CW; ++j) U[a][i][c][j] = 0.f;
+#pragma unroll 4
+    for (int t = 0; t < nv; ++t) {
+      const float w = p.sum_scale * pw[REV ? t + 1 : nv - 1 - t];
+      float yv[CG][CW], zv[CG][CW];
+#pragma unroll
+      for (int a = 0; a < CG; ++a) {
+        decay_lds<CW>(ys + t * LD + a * 64 + ty * CW, yv[a]);
+        decay_lds<CW>(zs + t * LD + a * 64 + tx * CW, zv[a]);
+#pragma unroll
+        for (int i = 0; i < CW; ++i) yv[a][i] = w == 0.f ? 0.f : yv[a][i] * w;
+      }
+#pragma unroll
+      for (int a = 0; a < CG; ++a)
+#pragma unroll
+        for (int i = 0; i < CW; ++i)
+#pragma unroll
+          for (int c = 0; c < CG; ++c)
+#pragma unroll
+            for (int j = 0; j < CW; ++j) U[a][i][c][j] = fmaf(yv[a][i], zv[c][j], U[a][i][c][j]);
+    }
+    const DecayPair by_nv = nv == C ? full : decay_pair(g, nv);
+#pragma unroll
+    for (int a = 0; a < CG; ++a)
+#pragma unroll
+      for (int i = 0; i < CW; ++i)
+#pragma unroll
+        for (int c = 0; c < CG; ++c)
+#pragma unroll
+          for (int j = 0; j < CW; ++j) S[a][i][c][j] = decay_by(by_nv, S[a][i][c][j]) + U[a][i][c][j];
+  }
+  if (!p.state_out) return;
+  if (OUT) {
+    const int64_t last = len > 0 ? (len - 1) / p.seg_rows : 0;      // (with outputs a run is a segment)
+    if (cut != (REV ? 0 : (int)last)) return;
+  }
+  float* to = p.state_out + (OUT ? (size_t)bh : (size_t)bh * p.ncut + cut) * D * D;
+#pragma unroll
+  for (int a = 0; a < CG; ++a)
+#pragma unroll
+    for (int i = 0; i < CW; ++i)
+#pragma unroll
+      for (int c = 0; c < CG; ++c)
+#pragma unroll
+        for (int j = 0; j < CW; ++j) to[(a * 64 + ty * CW + i) * D + c * 64 + tx * CW + j] = S[a][i][c][j];
+}
+
+// ---- the runs of a slice joined -----------------------------------------------------------------------------
+// One thread per element of the state of a slice goes through the runs in the order of time: before the first run of a segment
+// the state so far is what enters that segment.
+struct DecayJoinParams {
+  const float* sums;          // [BH][ncut][D][D]: each run alone
+  const float* state_in;      // [BH][D][D] or null
+  float* seg_states;          // [BH][nseg][D][D] or null
+  float* state_out;           // [BH][D][D] or null
+  const float* log_decay;
+  const int32_t* seq_lens;
+  int64_t N;
+  int H, D, nseg, sub;
+  int64_t seg_rows, sub_rows;
+  int count;                  // runs with a sum, in the order of time; with fewer than all of them there is no state_out
+};
+template <bool REV>
+__global__ void __launch_bounds__(kThreads) decay_join_kernel(DecayJoinParams p) {
+  const int bh = blockIdx.y, e = blockIdx.x * kThreads + threadIdx.x, DD = p.D * p.D, ncut = p.nseg * p.sub;
+  if (e >= DD) return;
+  const double g = decay_log(p.log_decay[bh % p.H]);
+  const int64_t len = decay_len(p.seq_lens, bh / p.H, p.N);
+  float s = p.state_in ? p.state_in[(size_t)bh * DD + e] : 0.f;
+  int64_t known = -1;
+  DecayPair w{1.f, 0.f};
+  constexpr int kAhead = 8;      // sums fetched ahead: the walk is a chain, its loads are not
+  const int walk = min(ncut, p.count + 1);
+  for (int i0 = 0; i0 < walk; i0 += kAhead) {
+    float u[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int i = REV ? ncut - 1 - (i0 + k) : i0 + k;
+      u[k] = 0.f;
+      if (i0 + k < p.count && decay_cut_begin(p.seg_rows, p.sub, p.sub_rows, i) < len &&
+          decay_cut_begin(p.seg_rows, p.sub, p.sub_rows, i) < decay_cut_end(p.seg_rows, p.sub, p.sub_rows, p.N, i))
+        u[k] = p.sums[((size_t)bh * ncut + i) * DD + e];
+    }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      if (i0 + k >= walk) break;
+      const int i = REV ? ncut - 1 - (i0 + k) : i0 + k;
+      if (p.seg_states && i % p.sub == (REV ? p.sub - 1 : 0)) p.seg_states[((size_t)bh * p.nseg + i / p.sub) * DD + e] = s;
+      int64_t n = decay_cut_end(p.seg_rows, p.sub, p.sub_rows, p.N, i);
+      n = (n < len ? n : len) - decay_cut_begin(p.seg_rows, p.sub, p.sub_rows, i);
+      if (n <= 0) continue;
+      if (n != known) { w = decay_pair(g, n); known = n; }
+      s = decay_by(w, s) + u[k];
+    }
+  }
+  if (p.state_out) p.state_out[(size_t)bh * DD + e] = s;
+}
+
+// ---- one token ----------------------------------------------------------------------------------------------
+// A CTA takes W columns of one head's state: LPR = W / 4 threads hold a row's columns as float4, the rows are spread over the CTA.
+// Columns are independent of one another, the sum over the rows ends in shared memory.  Bound by the state, read and written once.
+struct DecayStepParams {
+  const void *q, *k, *v;
+  void* out;
+  int64_t qb, qh, kb, kh, vb, vh, ob, oh;
+  const float* log_decay;
+  float* states;
+  const int32_t* slots;
+  int64_t num_states;
+  int B, H;
+  float scale;
+};
+template <class T, int D, int W>
+__global__ void __launch_bounds__(D * W / 4 < 256 ? D * W / 4 : 256) decay_step_kernel(DecayStepParams p) {
+  constexpr int NT = D * W / 4 < 256 ? D * W / 4 : 256, LPR = W / 4, RPI = NT / LPR, ITERS = D / RPI;
+  __shared__ float s_q[D], s_k[D], s_sum[RPI][W];
+  __shared__ int s_next, s_early;
+  const int b0 = blockIdx.x / p.H, h = blockIdx.x % p.H, col = blockIdx.y * W + (threadIdx.x % LPR) * 4, row = threadIdx.x / LPR;
+  T* out = static_cast<T*>(p.out);
+  int64_t slot = b0;
+  if (p.slots) {
+    slot = p.slots[b0];
+    if (slot < 0 || slot >= p.num_states) {
+      if (threadIdx.x < W) out[b0 * p.ob + h * p.oh + blockIdx.y * W + threadIdx.x] = from_f<T>(0.f);
+      return;
+    }
+  }
+  float4* S = reinterpret_cast<float4*>(p.states + ((size_t)slot * p.H + h) * D * D + col);
+  float4 s[ITERS];
+#pragma unroll
+  for (int i = 0; i < ITERS; ++i) s[i] = S[(size_t)(row + i * RPI) * (D / 4)];
+  const float decay = (float)exp(decay_log(p.log_decay[h]));
+  int b = b0;
+  if (p.slots) {
+    // rows of the batch that name one state are tokens in a row: the first of them takes all, the others leave
+    if (threadIdx.x == 0) { s_early = 0; s_next = p.B; }
+    __syncthreads();
+    for (int i = threadIdx.x; i < p.B; i += NT)
+      if (i != b0 && p.slots[i] == slot) {
+        if (i < b0) s_early = 1;
+        else atomicMin(&s_next, i);
+      }
+    __syncthreads();
+    if (s_early) return;
+  }
+  for (;;) {
+    const T* q = static_cast<const T*>(p.q) + b * p.qb + h * p.qh;
+    const T* k = static_cast<const T*>(p.k) + b * p.kb + h * p.kh;
+    const T* v = static_cast<const T*>(p.v) + b * p.vb + h * p.vh + col;
+    for (int i = threadIdx.x; i < D; i += NT) { s_q[i] = to_f<T>(q[i]); s_k[i] = to_f<T>(k[i]); }
+    const float v0 = to_f<T>(v[0]), v1 = to_f<T>(v[1]), v2 = to_f<T>(v[2]), v3 = to_f<T>(v[3]);
+    __syncthreads();
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < ITERS; ++i) {
+      const float kr = s_k[row + i * RPI], qr = s_q[row + i * RPI];
+      float4& x = s[i];
+      x.x = fmaf(kr, v0, decay == 0.f ? 0.f : decay * x.x); x.y = fmaf(kr, v1, decay == 0.f ? 0.f : decay * x.y);
+      x.z = fmaf(kr, v2, decay == 0.f ? 0.f : decay * x.z); x.w = fmaf(kr, v3, decay == 0.f ? 0.f : decay * x.w);
+      o.x = fmaf(qr, x.x, o.x); o.y = fmaf(qr, x.y, o.y); o.z = fmaf(qr, x.z, o.z); o.w = fmaf(qr, x.w, o.w);
+    }
+    *reinterpret_cast<float4*>(&s_sum[row][(threadIdx.x % LPR) * 4]) = o;
+    const int next = p.slots ? s_next : p.B;
+    __syncthreads();
+    if (threadIdx.x < W) {
+      float t = 0.f;
+#pragma unroll
+      for (int r = 0; r < RPI; ++r) t += s_sum[r][threadIdx.x];
+      out[b * p.ob + h * p.oh + blockIdx.y * W + threadIdx.x] = from_f<T>(t * p.scale);
+    }
+    if (next >= p.B) break;
+    b = next;                       // (rare: further tokens for the same state)
+    if (threadIdx.x == 0) s_next = p.B;
+    __syncthreads();
+    for (int i = b + 1 + threadIdx.x; i < p.B; i += NT)
+      if (p.slots[i] == slot) atomicMin(&s_next, i);
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < ITERS; ++i) S[(size_t)(row + i * RPI) * (D / 4)] = s[i];
+}
+
+}  // namespace fnb

@@ -13,6 +13,7 @@
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include <atomic>
 #include <cmath>
@@ -371,11 +372,427 @@ std::optional<at::Tensor> module_forward(const at::Tensor& x, const at::Tensor& 
   return project_out(o, wo);
 }
 
+// ---- causal attention with a decay, layer norm ------------------------------------------------------------------
+using OptTensor = std::optional<at::Tensor>;
+
+void check_cuda(const at::Tensor& t, const char* name, const at::Tensor& like) {
+  TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor (flashnystrom_b200 has no CPU path)");
+  TORCH_CHECK(t.layout() == at::kStrided, name, " must be a strided tensor");
+  TORCH_CHECK(t.device() == like.device(), name, " is on ", t.device(), ", the others on ", like.device());
+}
+// Results of a backward that is itself not differentiable: a second derivative raises instead of leaving a term out.  `of`: what the
+// results depend on; the node that raises lies between them and these, so that no way to them goes past it.
+variable_list once_differentiable(variable_list grads, const char* what, const variable_list& of) {
+  if (!at::GradMode::is_enabled()) return grads;
+  const size_t n = grads.size();
+  for (const at::Tensor& t : of) grads.push_back(t);
+  variable_list r = (*std::make_shared<torch::autograd::DelayedError>(std::string(what) + " has no second derivative", grads.size()))(std::move(grads));
+  r.resize(n);
+  return r;
+}
+
+// (B, H, N, D) rows that the kernels can read where they lie: last dimension contiguous, no dimension spread out of one element
+at::Tensor rows_in_place(const at::Tensor& t) {
+  bool fine = t.stride(3) == 1 || t.size(3) == 1;
+  for (int i = 0; i < 3; ++i) fine = fine && (t.size(i) == 1 || t.stride(i) > 0);
+  return fine ? t : t.contiguous();
+}
+fnb_rows rows_arg(const at::Tensor& t) { return {t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)}; }
+// uninitialised, in the order that t's heads and rows have in memory
+at::Tensor empty_rows_like(const at::Tensor& t) { return empty_in(t, t.stride(1) < t.stride(2) ? FNB_LAYOUT_BNHD : FNB_LAYOUT_BHND); }
+
+struct DecayArgs {
+  at::Tensor q, k, v, log_decay, initial, seq_lens;      // (the last two may be undefined)
+  double scale;
+  at::Tensor status;
+};
+fnb_decay_shape decay_shape(const at::Tensor& q, double scale) {
+  fnb_decay_shape s{};
+  s.batch = q.size(0); s.heads = q.size(1); s.seq_len = q.size(2); s.head_dim = (int32_t)std::min<int64_t>(q.size(3), INT32_MAX);
+  s.dtype = dtype_of(q); s.scale = (float)scale; s.flags = g_flags.load() & FNB_FLAG_FORCE_GENERIC;
+  return s;
+}
+float* floats_or_null(const at::Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
+const int32_t* lens_or_null(const at::Tensor& t) { return t.defined() ? t.data_ptr<int32_t>() : nullptr; }
+
+void check_state(const at::Tensor& t, const char* name, const at::Tensor& q) {
+  check_cuda(t, name, q);
+  TORCH_CHECK(t.scalar_type() == at::kFloat, name, " must be float32, got ", t.scalar_type());
+  TORCH_CHECK(t.sizes() == at::IntArrayRef({q.size(0), q.size(1), q.size(3), q.size(3)}), name, " must be (B, H, D, D), got ", t.sizes());
+}
+void check_log_decay(const at::Tensor& g, const at::Tensor& q) {
+  check_cuda(g, "log_decay", q);
+  TORCH_CHECK(g.scalar_type() == at::kFloat && g.dim() == 1 && g.size(0) == q.size(1), "log_decay must be a float32 tensor with one value a head (", q.size(1),
+              "), got ", g.scalar_type(), " ", g.sizes());
+  TORCH_CHECK(!(at::GradMode::is_enabled() && g.requires_grad()), "log_decay is a constant here: it has no gradient");
+}
+DecayArgs decay_args(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& log_decay, double scale, const OptTensor& initial,
+                     const OptTensor& seq_lens, const at::Tensor& status) {
+  TORCH_CHECK(q.is_cuda(), "q must be a CUDA tensor (flashnystrom_b200 has no CPU path)");
+  TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && v.dim() == 4, "q, k, v must be 4D (B, H, N, D)");
+  check_cuda(q, "q", q);
+  check_cuda(k, "k", q);
+  check_cuda(v, "v", q);
+  TORCH_CHECK(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(), "q, k, v dtypes must match");
+  TORCH_CHECK(k.sizes() == q.sizes() && v.sizes() == q.sizes(), "q, k, v shapes must match, got ", q.sizes(), ", ", k.sizes(), " and ", v.sizes());
+  TORCH_CHECK(dtype_of(q) >= 0, "Supported dtypes: float32, float16, bfloat16");
+  check_log_decay(log_decay, q);
+  if (initial) check_state(*initial, "initial_state", q);
+  if (seq_lens) {
+    check_cuda(*seq_lens, "seq_lens", q);
+    TORCH_CHECK(seq_lens->scalar_type() == at::kInt && seq_lens->dim() == 1 && seq_lens->size(0) == q.size(0),
+                "seq_lens must be an int32 tensor with one length a sequence (", q.size(0), "), got ", seq_lens->scalar_type(), " ", seq_lens->sizes());
+  }
+  return {q, k, v, log_decay, initial ? *initial : at::Tensor(), seq_lens ? *seq_lens : at::Tensor(), scale, status};
+}
+at::Tensor contiguous_or_none(const at::Tensor& t) { return t.defined() ? t.contiguous() : t; }
+
+// out, the state behind the last row (undefined unless wanted), the states at the cuts
+struct DecayResult { at::Tensor out, final, segments; };
+DecayResult run_decay_forward(const DecayArgs& c, bool want_state) {
+  const at::Tensor q = rows_in_place(c.q), k = rows_in_place(c.k), v = rows_in_place(c.v);
+  const at::Tensor g = c.log_decay.contiguous(), initial = contiguous_or_none(c.initial), lens = contiguous_or_none(c.seq_lens);
+  fnb_decay_fwd_args a{};
+  a.shape = decay_shape(q, c.scale);
+  check(fnb_check_decay_shape(&a.shape));
+  DecayResult r;
+  const auto f32 = q.options().dtype(at::kFloat);
+  r.out = empty_rows_like(q);
+  if (want_state) r.final = at::empty({q.size(0), q.size(1), q.size(3), q.size(3)}, f32);
+  r.segments = at::empty({(int64_t)fnb_decay_segment_floats(&a.shape)}, f32);
+  const at::Tensor ws = bytes(fnb_decay_workspace_bytes(&a.shape), q);
+  a.q = rows_arg(q); a.k = rows_arg(k); a.v = rows_arg(v); a.out = rows_arg(r.out);
+  a.log_decay = g.data_ptr<float>(); a.seq_lens = lens_or_null(lens);
+  a.initial_state = floats_or_null(initial); a.final_state = floats_or_null(r.final);
+  a.segment_states = r.segments.numel() ? r.segments.data_ptr<float>() : nullptr;
+  a.workspace = ws.data_ptr(); a.workspace_bytes = (size_t)ws.numel();
+  a.device = q.device().index();
+  a.stream = c10::cuda::getCurrentCUDAStream(q.device().index()).stream();
+  a.device_status = c.status.data_ptr<int32_t>();
+  check(fnb_decay_forward(&a));
+  return r;
+}
+// dq, dk, dv, d_initial (undefined unless wanted)
+variable_list run_decay_backward(const DecayArgs& c, const at::Tensor& segments, const at::Tensor& d_out, const at::Tensor& d_final, bool want_initial) {
+  const at::Tensor q = rows_in_place(c.q), k = rows_in_place(c.k), v = rows_in_place(c.v), d = rows_in_place(d_out);
+  const at::Tensor g = c.log_decay.contiguous(), initial = contiguous_or_none(c.initial), lens = contiguous_or_none(c.seq_lens),
+                   df = contiguous_or_none(d_final);
+  fnb_decay_bwd_args a{};
+  a.shape = decay_shape(q, c.scale);
+  check(fnb_check_decay_shape(&a.shape));
+  TORCH_CHECK(segments.scalar_type() == at::kFloat && segments.device() == q.device() && segments.is_contiguous() &&
+                  segments.numel() == (int64_t)fnb_decay_segment_floats(&a.shape),
+              "the saved states do not match q");
+  at::Tensor dq = empty_rows_like(q), dk = empty_rows_like(k), dv = empty_rows_like(v), d_initial;
+  if (want_initial) d_initial = at::empty({q.size(0), q.size(1), q.size(3), q.size(3)}, q.options().dtype(at::kFloat));
+  const at::Tensor ws = bytes(fnb_decay_workspace_bytes(&a.shape), q);
+  a.q = rows_arg(q); a.k = rows_arg(k); a.v = rows_arg(v); a.d_out = rows_arg(d);
+  a.dq = rows_arg(dq); a.dk = rows_arg(dk); a.dv = rows_arg(dv);
+  a.log_decay = g.data_ptr<float>(); a.seq_lens = lens_or_null(lens); a.initial_state = floats_or_null(initial);
+  a.d_final_state = floats_or_null(df); a.d_initial_state = floats_or_null(d_initial);
+  a.segment_states = segments.numel() ? segments.data_ptr<float>() : nullptr;
+  a.workspace = ws.data_ptr(); a.workspace_bytes = (size_t)ws.numel();
+  a.device = q.device().index();
+  a.stream = c10::cuda::getCurrentCUDAStream(q.device().index()).stream();
+  a.device_status = c.status.data_ptr<int32_t>();
+  check(fnb_decay_backward(&a));
+  return {dq, dk, dv, d_initial};
+}
+
+struct DecayNode : torch::autograd::Function<DecayNode> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const OptTensor& initial,
+                               const DecayArgs& c, bool want_state) {
+    const at::Tensor s0 = initial ? *initial : at::Tensor();
+    const DecayResult r = run_decay_forward({q, k, v, c.log_decay, s0, c.seq_lens, c.scale, c.status}, want_state);
+    ctx->save_for_backward({q, k, v, s0, c.log_decay, c.seq_lens, r.segments});
+    ctx->saved_data["scale"] = c.scale;
+    ctx->saved_data["status"] = c.status;
+    ctx->set_materialize_grads(false);
+    if (want_state) return {r.out, r.final};
+    return {r.out};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list kept = ctx->get_saved_variables();
+    const DecayArgs c{kept[0], kept[1], kept[2], kept[4], kept[3], kept[5], ctx->saved_data["scale"].toDouble(), ctx->saved_data["status"].toTensor()};
+    c10::cuda::CUDAGuard guard(c.q.device());
+    at::Tensor d = grads[0], df = grads.size() > 1 ? grads[1] : at::Tensor();
+    variable_list result(6);
+    if (!d.defined() && !df.defined()) return result;
+    if (!d.defined()) d = at::zeros_like(c.q);
+    TORCH_CHECK(d.is_cuda() && d.device() == c.q.device() && d.sizes() == c.q.sizes() && d.scalar_type() == c.q.scalar_type(),
+                "the gradient of the output does not match q in shape, dtype or device");
+    if (df.defined()) check_state(df, "the gradient of the state", c.q);
+    variable_list g;
+    {
+      at::AutoGradMode off(false);
+      g = run_decay_backward(c, kept[6], d, df, c.initial.defined() && ctx->needs_input_grad(3));
+    }
+    for (int i = 0; i < 4; ++i)
+      if (g[i].defined() && ctx->needs_input_grad(i)) result[i] = g[i];
+    return once_differentiable(std::move(result), "decay_attention", {c.q, c.k, c.v, c.initial, d, df});
+  }
+};
+
+// (out, final state or nothing)
+std::pair<at::Tensor, OptTensor> decay_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& log_decay,
+                                                 double scale, const OptTensor& initial, const OptTensor& seq_lens, bool want_state,
+                                                 const at::Tensor& status) {
+  const DecayArgs c = decay_args(q, k, v, log_decay, scale, initial, seq_lens, status);
+  py::gil_scoped_release nogil;
+  c10::cuda::CUDAGuard guard(q.device());
+  if (q.numel() == 0) {      // nothing to attend to: the state goes through
+    TORCH_CHECK(q.size(3) > 0, "head_dim must be 16, 32, 64 or 128, got 0");
+    OptTensor state;
+    if (want_state) state = initial ? initial->clone() : at::zeros({q.size(0), q.size(1), q.size(3), q.size(3)}, q.options().dtype(at::kFloat));
+    return {q.clone(), state};
+  }
+  if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() || (initial && initial->requires_grad()))) {
+    const variable_list r = DecayNode::apply(q, k, v, initial, c, want_state);
+    return {r[0], want_state ? OptTensor(r[1]) : std::nullopt};
+  }
+  at::AutoGradMode off(false);
+  const DecayResult r = run_decay_forward(c, want_state);
+  return {r.out, want_state ? OptTensor(r.final) : std::nullopt};
+}
+std::tuple<at::Tensor, at::Tensor, at::Tensor> decay_forward(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& log_decay,
+                                                             double scale, const OptTensor& initial, const OptTensor& seq_lens,
+                                                             const at::Tensor& status) {
+  at::AutoGradMode off(false);
+  const DecayArgs c = decay_args(q, k, v, log_decay, scale, initial, seq_lens, status);
+  c10::cuda::CUDAGuard guard(q.device());
+  const DecayResult r = run_decay_forward(c, true);
+  return {r.out, r.final, r.segments};
+}
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> decay_backward(const at::Tensor& d, const at::Tensor& df, const at::Tensor& q,
+                                                                          const at::Tensor& k, const at::Tensor& v, const at::Tensor& log_decay,
+                                                                          double scale, const OptTensor& initial, const OptTensor& seq_lens,
+                                                                          const at::Tensor& segments, const at::Tensor& status) {
+  at::AutoGradMode off(false);
+  const DecayArgs c = decay_args(q, k, v, log_decay, scale, initial, seq_lens, status);
+  TORCH_CHECK(d.sizes() == q.sizes() && d.scalar_type() == q.scalar_type() && d.device() == q.device(), "d_out does not match q");
+  check_state(df, "d_final_state", q);
+  c10::cuda::CUDAGuard guard(q.device());
+  const variable_list g = run_decay_backward(c, segments, d, df, true);
+  return {g[0], g[1], g[2], g[3]};
+}
+
+at::Tensor decay_step(const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_, const at::Tensor& state, const at::Tensor& log_decay,
+                      double scale, const OptTensor& slots) {
+  TORCH_CHECK(q_.is_cuda(), "q must be a CUDA tensor (flashnystrom_b200 has no CPU path)");
+  TORCH_CHECK(q_.dim() == 3 && k_.dim() == 3 && v_.dim() == 3, "q, k, v must be 3D (B, H, D)");
+  check_cuda(q_, "q", q_);
+  check_cuda(k_, "k", q_);
+  check_cuda(v_, "v", q_);
+  check_cuda(state, "state", q_);
+  TORCH_CHECK(k_.scalar_type() == q_.scalar_type() && v_.scalar_type() == q_.scalar_type(), "q, k, v dtypes must match");
+  TORCH_CHECK(k_.sizes() == q_.sizes() && v_.sizes() == q_.sizes(), "q, k, v shapes must match");
+  TORCH_CHECK(dtype_of(q_) >= 0, "Supported dtypes: float32, float16, bfloat16");
+  check_log_decay(log_decay, q_);
+  const int64_t B = q_.size(0), H = q_.size(1), D = q_.size(2);
+  TORCH_CHECK(state.scalar_type() == at::kFloat && state.dim() == 4 && state.size(1) == H && state.size(2) == D && state.size(3) == D && state.is_contiguous(),
+              "state must be a contiguous float32 tensor of shape (states, ", H, ", ", D, ", ", D, "), got ", state.scalar_type(), " ", state.sizes());
+  TORCH_CHECK(slots || state.size(0) == B, "state must have one entry for each row (", B, ") where no slots are given, got ", state.size(0));
+  if (slots) {
+    check_cuda(*slots, "slots", q_);
+    TORCH_CHECK(slots->scalar_type() == at::kInt && slots->dim() == 1 && slots->size(0) == B, "slots must be an int32 tensor with one value a row (", B, "), got ",
+                slots->scalar_type(), " ", slots->sizes());
+  }
+  TORCH_CHECK(!(at::GradMode::is_enabled() && (q_.requires_grad() || k_.requires_grad() || v_.requires_grad() || state.requires_grad())),
+              "decay_attention_step updates the state in place and has no gradient: use decay_attention, or torch.no_grad()");
+  TORCH_CHECK(!state.is_inference() || c10::InferenceMode::is_enabled(), "an inference tensor cannot be updated in place outside InferenceMode");
+  py::gil_scoped_release nogil;
+  c10::cuda::CUDAGuard guard(q_.device());
+  at::AutoGradMode off(false);
+  const auto in_place = [](const at::Tensor& t) { return t.stride(2) == 1 ? t : t.contiguous(); };
+  const at::Tensor q = in_place(q_), k = in_place(k_), v = in_place(v_), g = log_decay.contiguous();
+  at::Tensor out = at::empty({B, H, D}, q.options());
+  if (B == 0 || H == 0) return out;
+  if (state.size(0) == 0) return out.zero_();      // (slots of no state: every row is idle)
+  const at::Tensor s = slots ? slots->contiguous() : at::Tensor();
+  fnb_decay_step_args a{};
+  const auto arg = [](const at::Tensor& t) { return fnb_rows{t.data_ptr(), t.stride(0), t.stride(1), 0}; };
+  a.batch = B; a.heads = H; a.num_states = state.size(0); a.head_dim = (int32_t)std::min<int64_t>(D, INT32_MAX); a.dtype = dtype_of(q);
+  a.scale = (float)scale;
+  a.q = arg(q); a.k = arg(k); a.v = arg(v); a.out = arg(out);
+  a.log_decay = g.data_ptr<float>(); a.states = state.data_ptr<float>(); a.slots = lens_or_null(s);
+  a.device = q.device().index();
+  a.stream = c10::cuda::getCurrentCUDAStream(q.device().index()).stream();
+  check(fnb_decay_step(&a));
+  if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();
+  return out;
+}
+
+// x as rows of its last dimension that lie one stride apart; contiguous where it is not so
+at::Tensor norm_rows(const at::Tensor& x) {
+  const int64_t C = x.size(-1);
+  if (C == 1 || x.stride(-1) == 1) {
+    int64_t stride = -1, size = 1;      // of the innermost leading dimension that counts; rows so far
+    bool fine = true;
+    for (int64_t i = x.dim() - 2; i >= 0 && fine; --i) {
+      if (x.size(i) == 1) continue;
+      if (stride < 0) stride = x.stride(i);
+      else fine = x.stride(i) == size * stride;
+      size *= x.size(i);
+    }
+    if (fine && (stride < 0 || stride >= C)) return x.as_strided({size, C}, {stride < 0 ? C : stride, 1});
+  }
+  return x.contiguous().view({-1, C});
+}
+struct NormArgs {
+  at::Tensor x, weight, bias;      // (weight and bias may be undefined)
+  int64_t groups;
+  double eps;
+};
+fnb_norm_shape norm_shape(const at::Tensor& x, at::ScalarType param, int64_t groups, double eps) {
+  fnb_norm_shape s{};
+  TORCH_CHECK(x.size(-1) <= INT32_MAX, "the last dimension is too large (", x.size(-1), ")");
+  s.rows = x.numel() / x.size(-1); s.cols = (int32_t)x.size(-1); s.groups = (int32_t)groups;
+  s.dtype = dtype_of(x); s.param_dtype = param == at::kFloat ? FNB_F32 : s.dtype; s.eps = (float)eps;
+  return s;
+}
+at::ScalarType norm_param_type(const NormArgs& c) {
+  return c.weight.defined() ? c.weight.scalar_type() : c.bias.defined() ? c.bias.scalar_type() : at::kFloat;
+}
+NormArgs norm_args(const at::Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps, int64_t groups) {
+  TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor (flashnystrom_b200 has no CPU path)");
+  check_cuda(x, "x", x);
+  TORCH_CHECK(dtype_of(x) >= 0, "Supported dtypes: float32, float16, bfloat16");
+  TORCH_CHECK(x.dim() >= 1 && x.size(-1) > 0, "x must have a last dimension to normalise, got ", x.sizes());
+  TORCH_CHECK(groups >= 1 && x.size(-1) % groups == 0, "num_groups (", groups, ") must divide the last dimension (", x.size(-1), ")");
+  const struct { const OptTensor& t; const char* name; } params[] = {{weight, "weight"}, {bias, "bias"}};
+  for (const auto& p : params)
+    if (p.t) {
+      check_cuda(*p.t, p.name, x);
+      TORCH_CHECK(p.t->dim() == 1 && p.t->size(0) == x.size(-1), p.name, " must have ", x.size(-1), " values, got ", p.t->sizes());
+      TORCH_CHECK(p.t->scalar_type() == x.scalar_type() || p.t->scalar_type() == at::kFloat, p.name, " must be float32 or ", x.scalar_type(), ", got ",
+                  p.t->scalar_type());
+    }
+  TORCH_CHECK(!(weight && bias) || weight->scalar_type() == bias->scalar_type(), "weight and bias dtypes must match");
+  return {x, weight ? *weight : at::Tensor(), bias ? *bias : at::Tensor(), groups, eps};
+}
+const void* data_or_null(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+struct NormResult { at::Tensor y, mean, rstd; };
+NormResult run_norm_forward(const NormArgs& c, bool keep) {
+  NormResult r;
+  fnb_norm_fwd_args a{};
+  a.shape = norm_shape(c.x, norm_param_type(c), c.groups, c.eps);
+  const at::Tensor x = norm_rows(c.x), w = contiguous_or_none(c.weight), b = contiguous_or_none(c.bias);
+  r.y = at::empty(c.x.sizes(), c.x.options());
+  if (keep) {
+    const at::Tensor stats = at::empty({2, a.shape.rows * c.groups}, c.x.options().dtype(at::kFloat));
+    r.mean = stats.select(0, 0);
+    r.rstd = stats.select(0, 1);
+  }
+  a.x = x.data_ptr(); a.x_stride = x.stride(0); a.y = r.y.data_ptr(); a.y_stride = x.size(1);
+  a.weight = data_or_null(w); a.bias = data_or_null(b); a.mean = floats_or_null(r.mean); a.rstd = floats_or_null(r.rstd);
+  a.device = x.device().index();
+  a.stream = c10::cuda::getCurrentCUDAStream(x.device().index()).stream();
+  check(fnb_norm_forward(&a));
+  return r;
+}
+// d_x, d_weight, d_bias, those that are wanted
+variable_list run_norm_backward(const at::Tensor& x_, const at::Tensor& weight, const at::Tensor& mean, const at::Tensor& rstd, const at::Tensor& d_,
+                                int64_t groups, double eps, at::ScalarType param, bool want_x, bool want_w, bool want_b) {
+  fnb_norm_bwd_args a{};
+  a.shape = norm_shape(x_, param, groups, eps);
+  check(fnb_check_norm_shape(&a.shape));
+  const at::Tensor x = norm_rows(x_), d = norm_rows(d_), w = contiguous_or_none(weight);
+  TORCH_CHECK(mean.is_contiguous() && rstd.is_contiguous() && mean.scalar_type() == at::kFloat && rstd.scalar_type() == at::kFloat && mean.device() == x.device() &&
+                  rstd.device() == x.device() && mean.numel() == a.shape.rows * groups && rstd.numel() == a.shape.rows * groups,
+              "the saved statistics do not match x");
+  at::Tensor dx, dw, db, ws;
+  if (want_x) dx = at::empty(x_.sizes(), x_.options());
+  const auto po = x_.options().dtype(param);
+  if (want_w) dw = at::empty({x.size(1)}, po);
+  if (want_b) db = at::empty({x.size(1)}, po);
+  if (want_w || want_b) {
+    ws = bytes(fnb_norm_workspace_bytes(&a.shape), x);
+    a.workspace = ws.data_ptr();
+    a.workspace_bytes = (size_t)ws.numel();
+  }
+  a.x = x.data_ptr(); a.x_stride = x.stride(0); a.d_y = d.data_ptr(); a.d_y_stride = d.stride(0);
+  a.d_x = want_x ? dx.data_ptr() : nullptr; a.d_x_stride = x.size(1); a.weight = data_or_null(w);
+  a.mean = mean.data_ptr<float>(); a.rstd = rstd.data_ptr<float>();
+  a.d_weight = want_w ? dw.data_ptr() : nullptr; a.d_bias = want_b ? db.data_ptr() : nullptr;
+  a.device = x.device().index();
+  a.stream = c10::cuda::getCurrentCUDAStream(x.device().index()).stream();
+  check(fnb_norm_backward(&a));
+  return {dx, dw, db};
+}
+
+struct NormNode : torch::autograd::Function<NormNode> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const OptTensor& weight, const OptTensor& bias, int64_t groups, double eps) {
+    const NormArgs c{x, weight ? *weight : at::Tensor(), bias ? *bias : at::Tensor(), groups, eps};
+    const NormResult r = run_norm_forward(c, true);
+    ctx->save_for_backward({x, c.weight, r.mean, r.rstd});
+    ctx->saved_data["bias"] = bias.has_value();
+    ctx->saved_data["groups"] = groups;
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["param"] = (int64_t)norm_param_type(c);
+    return r.y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list kept = ctx->get_saved_variables();
+    const at::Tensor &x = kept[0], &d = grads[0];
+    c10::cuda::CUDAGuard guard(x.device());
+    TORCH_CHECK(d.is_cuda() && d.device() == x.device() && d.sizes() == x.sizes() && d.scalar_type() == x.scalar_type(),
+                "the gradient of the output does not match x in shape, dtype or device");
+    const bool has_w = kept[1].defined(), has_b = ctx->saved_data["bias"].toBool();      // (what is not given has no place among the inputs)
+    variable_list g;
+    {
+      at::AutoGradMode off(false);
+      g = run_norm_backward(x, kept[1], kept[2], kept[3], d, ctx->saved_data["groups"].toInt(), ctx->saved_data["eps"].toDouble(),
+                            (at::ScalarType)ctx->saved_data["param"].toInt(), ctx->needs_input_grad(0), has_w && ctx->needs_input_grad(1),
+                            has_b && ctx->needs_input_grad(has_w ? 2 : 1));
+    }
+    g.resize(5);
+    return once_differentiable(std::move(g), "layer_norm", {x, kept[1], d});
+  }
+};
+at::Tensor layer_norm(const at::Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps, int64_t groups) {
+  const NormArgs c = norm_args(x, weight, bias, eps, groups);
+  py::gil_scoped_release nogil;
+  c10::cuda::CUDAGuard guard(x.device());
+  if (x.numel() == 0) {      // no rows: gradients of weight and bias are zeros
+    at::Tensor y = x.clone();
+    if (weight) y = y * weight->to(x.scalar_type());
+    return bias ? y + bias->to(x.scalar_type()) : y;
+  }
+  if (at::GradMode::is_enabled() && (x.requires_grad() || (weight && weight->requires_grad()) || (bias && bias->requires_grad())))
+    return NormNode::apply(x, weight, bias, groups, eps);
+  at::AutoGradMode off(false);
+  return run_norm_forward(c, false).y;
+}
+std::tuple<at::Tensor, at::Tensor, at::Tensor> norm_forward(const at::Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps, int64_t groups) {
+  at::AutoGradMode off(false);
+  c10::cuda::CUDAGuard guard(x.device());
+  const NormResult r = run_norm_forward(norm_args(x, weight, bias, eps, groups), true);
+  return {r.y, r.mean.clone(), r.rstd.clone()};
+}
+std::tuple<at::Tensor, at::Tensor, at::Tensor> norm_backward(const at::Tensor& d, const at::Tensor& x, const OptTensor& weight, const at::Tensor& mean,
+                                                             const at::Tensor& rstd, double eps, int64_t groups, bool param_f32) {
+  at::AutoGradMode off(false);
+  c10::cuda::CUDAGuard guard(x.device());
+  norm_args(x, weight, std::nullopt, eps, groups);
+  TORCH_CHECK(d.sizes() == x.sizes() && d.scalar_type() == x.scalar_type() && d.device() == x.device(), "d_y does not match x");
+  const variable_list g = run_norm_backward(x, weight ? *weight : at::Tensor(), mean, rstd, d, groups, eps, param_f32 ? at::kFloat : x.scalar_type(), true, true,
+                                            true);
+  return {g[0], g[1], g[2]};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_native, mod) {
   mod.def("attention", &attention);
   mod.def("module_forward", &module_forward);
+  mod.def("decay_attention", &decay_attention);
+  mod.def("decay_forward", &decay_forward);
+  mod.def("decay_backward", &decay_backward);
+  mod.def("decay_step", &decay_step);
+  mod.def("layer_norm", &layer_norm);
+  mod.def("norm_forward", &norm_forward);
+  mod.def("norm_backward", &norm_backward);
   mod.def("set_flags", [](uint32_t flags) { g_flags = flags; });
   mod.def("set_debug", [](py::object f) { g_debug = f.release().ptr(); });
 }

@@ -1,0 +1,292 @@
+// Layer norm over runs of n columns (a row is `groups` runs), forward and backward.
+//
+// A run is held by LANES threads of a warp (several runs a warp where they are short) or by a whole CTA, EPT elements a thread in
+// registers, so that x is read once: mean first, then the sum of squared distances from it.  A CTA has SPC places, each with a
+// group of its own that it keeps over all its rows: weight and bias stay in registers, and the backward adds up its share
+// of d_weight and d_bias there; places are joined in shared memory in their order, CTAs by a second kernel in theirs.
+// Bound by HBM: x (and d_y) read once, y (d_x) written once.
+#pragma once
+#include "common.cuh"
+
+namespace fnb {
+
+constexpr int kNormThreads = 256;         // of a CTA that holds several runs
+constexpr int kNormMaxCols = 16384;       // of a run: 512 threads with 32 elements each
+
+struct NormParams {
+  const void *x, *dy, *w, *b;
+  void* y;                    // y, or d_x (may be null)
+  int64_t xs, dys, ys;        // row strides, elements
+  float *mean, *rstd;
+  float* part;                // backward: [CTA][2][span] sums of this CTA, or null
+  int64_t rows;
+  int n, groups;
+  float eps;
+  int lanes;                  // threads of a run
+  int places, per_row;        // places a CTA uses; how many of them one row takes
+  int gblocks;                // blocks of groups (more than one where a row has more groups than a CTA places)
+  int span;                   // columns whose sums a CTA has: places of distinct groups x n
+};
+
+// element type of weight and bias: F32 or T
+template <class T, bool PF32> struct NormParam { using type = T; };
+template <class T> struct NormParam<T, true> { using type = float; };
+
+template <class T, int VEC>
+__device__ __forceinline__ void norm_load(const T* p, float* v) {
+  if (VEC == 1) {
+    v[0] = to_f<T>(*p);
+  } else if (VEC * sizeof(T) == 16) {
+    load16<T>(p, v);
+  } else {      // eight floats beside eight 16-bit values
+#pragma unroll
+    for (int j = 0; j < VEC; j += 4) load16<T>(p + j, v + j);
+  }
+}
+template <class T, int VEC>
+__device__ __forceinline__ void norm_store(T* p, const float* v) {
+  if (VEC == 1) {
+    *p = from_f<T>(v[0]);
+  } else {
+    uint4 raw;
+    T* e = reinterpret_cast<T*>(&raw);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) e[j] = from_f<T>(v[j]);
+    *reinterpret_cast<uint4*>(p) = raw;
+  }
+}
+
+// Sum over the threads of a run.  BLOCK: the CTA's warps meet in `red` (two sets of 16 floats, used in turn).
+template <bool BLOCK>
+__device__ __forceinline__ float norm_sum(float v, int lanes, float* red, int& turn) {
+  for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if (BLOCK) {
+    float* r = red + 16 * turn;
+    turn ^= 1;
+    if ((threadIdx.x & 31) == 0) r[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = 0.f;
+    const int warps = blockDim.x >> 5;
+    for (int i = 0; i < warps; ++i) v += r[i];
+  }
+  return v;
+}
+
+struct NormPlace {
+  int lane, place, group;
+  int64_t row, step;
+  bool active;
+};
+template <bool BLOCK>
+__device__ __forceinline__ NormPlace norm_place(const NormParams& p) {
+  NormPlace t;
+  t.lane = BLOCK ? threadIdx.x : threadIdx.x & (p.lanes - 1);
+  t.place = BLOCK ? 0 : threadIdx.x / p.lanes;
+  const int gb = blockIdx.x % p.gblocks, rb = blockIdx.x / p.gblocks, nrb = gridDim.x / p.gblocks;
+  const int rows_at_once = p.places / p.per_row;
+  t.group = gb * p.places + t.place % p.per_row;
+  t.active = t.place < p.places && t.group < p.groups;
+  t.row = (int64_t)rb * rows_at_once + t.place / p.per_row;
+  t.step = (int64_t)nrb * rows_at_once;
+  return t;
+}
+
+template <class T, bool PF32, int VEC, int ITEMS, bool BLOCK>
+__global__ void __launch_bounds__(BLOCK ? 512 : kNormThreads) norm_fwd_kernel(NormParams p) {
+  using P = typename NormParam<T, PF32>::type;
+  constexpr int EPT = VEC * ITEMS;
+  __shared__ float red[32];
+  int turn = 0;
+  const NormPlace t = norm_place<BLOCK>(p);
+  const int threads = BLOCK ? blockDim.x : p.lanes, lanes = BLOCK ? 32 : p.lanes;
+  float w[EPT], b[EPT];
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const int c = (i * threads + t.lane) * VEC;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) { w[i * VEC + j] = 1.f; b[i * VEC + j] = 0.f; }
+    if (t.active && c < p.n) {
+      if (p.w) norm_load<P, VEC>(static_cast<const P*>(p.w) + (int64_t)t.group * p.n + c, w + i * VEC);
+      if (p.b) norm_load<P, VEC>(static_cast<const P*>(p.b) + (int64_t)t.group * p.n + c, b + i * VEC);
+    }
+  }
+  const float inv_n = 1.f / (float)p.n;
+  // (every thread of a warp goes round as often as the others: the sums are shuffles of whole warps)
+  const int64_t first = BLOCK ? t.row : (int64_t)(blockIdx.x / p.gblocks) * (p.places / p.per_row);
+  for (int64_t base = first; base < p.rows; base += t.step) {
+    const int64_t row = BLOCK ? base : base + t.place / p.per_row;
+    const bool on = t.active && row < p.rows;
+    const T* x = static_cast<const T*>(p.x) + row * p.xs + (int64_t)t.group * p.n;
+    float v[EPT];
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int c = (i * threads + t.lane) * VEC;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) v[i * VEC + j] = 0.f;
+      if (on && c < p.n) norm_load<T, VEC>(x + c, v + i * VEC);
+    }
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < EPT; ++j) s += v[j];
+    const float mean = norm_sum<BLOCK>(s, lanes, red, turn) * inv_n;
+    s = 0.f;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const bool in = (i * threads + t.lane) * VEC < p.n;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        v[i * VEC + j] = in ? v[i * VEC + j] - mean : 0.f;
+        s = fmaf(v[i * VEC + j], v[i * VEC + j], s);
+      }
+    }
+    const float r = 1.f / sqrtf(norm_sum<BLOCK>(s, lanes, red, turn) * inv_n + p.eps);
+    if (!on) continue;
+    T* y = static_cast<T*>(p.y) + row * p.ys + (int64_t)t.group * p.n;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int c = (i * threads + t.lane) * VEC;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) v[i * VEC + j] = fmaf(v[i * VEC + j] * r, w[i * VEC + j], b[i * VEC + j]);
+      if (c < p.n) norm_store<T, VEC>(y + c, v + i * VEC);
+    }
+    if (t.lane == 0) {
+      if (p.mean) p.mean[row * p.groups + t.group] = mean;
+      if (p.rstd) p.rstd[row * p.groups + t.group] = r;
+    }
+  }
+}
+
+// With u = d_y w and xh = (x - mean) rstd:  d_x = rstd (u - mean(u) - xh mean(u xh)).
+template <class T, bool PF32, int VEC, int ITEMS, bool BLOCK>
+__global__ void __launch_bounds__(BLOCK ? 512 : kNormThreads) norm_bwd_kernel(NormParams p) {
+  using P = typename NormParam<T, PF32>::type;
+  constexpr int EPT = VEC * ITEMS;
+  __shared__ float red[32];
+  extern __shared__ float sums[];      // [2][span]
+  int turn = 0;
+  const NormPlace t = norm_place<BLOCK>(p);
+  const int threads = BLOCK ? blockDim.x : p.lanes, lanes = BLOCK ? 32 : p.lanes;
+  float w[EPT], dw[EPT], db[EPT];
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const int c = (i * threads + t.lane) * VEC;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) { w[i * VEC + j] = 1.f; dw[i * VEC + j] = db[i * VEC + j] = 0.f; }
+    if (p.w && t.active && c < p.n) norm_load<P, VEC>(static_cast<const P*>(p.w) + (int64_t)t.group * p.n + c, w + i * VEC);
+  }
+  const float inv_n = 1.f / (float)p.n;
+  const int64_t first = BLOCK ? t.row : (int64_t)(blockIdx.x / p.gblocks) * (p.places / p.per_row);
+  for (int64_t base = first; base < p.rows; base += t.step) {
+    const int64_t row = BLOCK ? base : base + t.place / p.per_row;
+    const bool on = t.active && row < p.rows;
+    const T* x = static_cast<const T*>(p.x) + row * p.xs + (int64_t)t.group * p.n;
+    const T* dy = static_cast<const T*>(p.dy) + row * p.dys + (int64_t)t.group * p.n;
+    float v[EPT], d[EPT];
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int c = (i * threads + t.lane) * VEC;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) v[i * VEC + j] = d[i * VEC + j] = 0.f;
+      if (on && c < p.n) {
+        norm_load<T, VEC>(x + c, v + i * VEC);
+        norm_load<T, VEC>(dy + c, d + i * VEC);
+      }
+    }
+    const float mean = on ? p.mean[row * p.groups + t.group] : 0.f, r = on ? p.rstd[row * p.groups + t.group] : 0.f;
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const bool in = on && (i * threads + t.lane) * VEC < p.n;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const int e = i * VEC + j;
+        v[e] = in ? (v[e] - mean) * r : 0.f;
+        dw[e] = fmaf(d[e], v[e], dw[e]);
+        db[e] += d[e];
+        d[e] *= w[e];
+        s1 += d[e];
+        s2 = fmaf(d[e], v[e], s2);
+      }
+    }
+    if (!p.y) continue;      // (the same for all threads)
+    s1 = norm_sum<BLOCK>(s1, lanes, red, turn) * inv_n;
+    s2 = norm_sum<BLOCK>(s2, lanes, red, turn) * inv_n;
+    if (!on) continue;
+    T* dx = static_cast<T*>(p.y) + row * p.ys + (int64_t)t.group * p.n;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int c = (i * threads + t.lane) * VEC;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) d[i * VEC + j] = r * (d[i * VEC + j] - s1 - v[i * VEC + j] * s2);
+      if (c < p.n) norm_store<T, VEC>(dx + c, d + i * VEC);
+    }
+  }
+  if (!p.part) return;
+  float* part = p.part + (size_t)blockIdx.x * 2 * p.span;
+  if constexpr (BLOCK) {
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int c = (i * threads + t.lane) * VEC;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j)
+        if (c + j < p.n) {
+          part[c + j] = dw[i * VEC + j];
+          part[p.span + c + j] = db[i * VEC + j];
+        }
+    }
+  } else {
+    for (int c = threadIdx.x; c < 2 * p.span; c += kNormThreads) sums[c] = 0.f;
+    __syncthreads();
+    // one place after the other: each adds to the columns of its group
+    const int rounds = p.places / p.per_row;
+    for (int k = 0; k < rounds; ++k) {
+      if (t.place < p.places && t.place / p.per_row == k) {
+        float* to = sums + (t.place % p.per_row) * p.n;
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+          const int c = (i * threads + t.lane) * VEC;
+#pragma unroll
+          for (int j = 0; j < VEC; ++j)
+            if (c + j < p.n) {
+              to[c + j] += dw[i * VEC + j];
+              to[p.span + c + j] += db[i * VEC + j];
+            }
+        }
+      }
+      __syncthreads();
+    }
+    for (int c = threadIdx.x; c < 2 * p.span; c += kNormThreads) part[c] = sums[c];
+  }
+}
+
+// d_weight, d_bias: the CTAs' sums of a column.  32 columns a CTA, eight threads a column, each a run of CTAs in ascending order.
+template <class P>
+__global__ void __launch_bounds__(256) norm_reduce_kernel(const float* __restrict__ part, P* __restrict__ dw, P* __restrict__ db, int cols, int n,
+                                                          int places, int gblocks, int ctas, int span) {
+  __shared__ float s[2][8][33];
+  const int c = blockIdx.x * 32 + threadIdx.x % 32, k = threadIdx.x / 32;
+  float a = 0.f, b = 0.f;
+  if (c < cols) {
+    const int gb = gblocks == 1 ? 0 : c / n / places, col = c - gb * places * n, nrb = ctas / gblocks;
+    const int r0 = (int)((int64_t)nrb * k / 8), r1 = (int)((int64_t)nrb * (k + 1) / 8);
+#pragma unroll 4
+    for (int r = r0; r < r1; ++r) {
+      const float* q = part + (size_t)(r * gblocks + gb) * 2 * span + col;
+      a += q[0];
+      b += q[span];
+    }
+  }
+  s[0][k][threadIdx.x % 32] = a;
+  s[1][k][threadIdx.x % 32] = b;
+  __syncthreads();
+  if (threadIdx.x < 64) {
+    const int which = threadIdx.x / 32, l = threadIdx.x % 32;
+    float t = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t += s[which][i][l];
+    P* to = which ? db : dw;
+    if (blockIdx.x * 32 + l < cols && to) to[blockIdx.x * 32 + l] = from_f<P>(t);
+  }
+}
+
+}  // namespace fnb

@@ -2,34 +2,11 @@
 #pragma once
 #include <cuda.h>
 #include <cuda_runtime.h>
-#include <mutex>
+#include "tma_host.cuh"
 #include "tc_stream.cuh"
 
 namespace fnb {
 namespace tc {
-
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
-                                  CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
-                                  CUtensorMapFloatOOBfill);
-
-// The driver entry point is resolved through the runtime, so the library does not link libcuda.
-inline EncodeTiledFn encode_fn() {
-  static EncodeTiledFn fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(p);
-  });
-  return fn;
-}
-
-inline CUtensorMapDataType map_dtype(int dtype) {
-  return dtype == FNB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-}
 
 // Where slice (b, h) of a (B, H, N, D) tensor lives.  FNB_LAYOUT_BHND: contiguous (B, H, N, D).
 // FNB_LAYOUT_BNHD: the head-split view of a contiguous (B, N, H * D) tensor, i.e. rows of one slice

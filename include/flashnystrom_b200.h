@@ -312,6 +312,140 @@ typedef struct fnb_conv_dw_args {
 FNB_API size_t fnb_conv_dweight_workspace_bytes(int64_t batch, int64_t heads, int64_t seq_len, int32_t kernel_size);
 FNB_API int fnb_conv_residual_dweight(const fnb_conv_dw_args* args);
 
+/* ---- causal attention with a decay for each head (no counterpart in the reference) ------------
+ * With g = log_decay[h] and S_0 = initial_state (zeros where it is NULL), for t = 1 .. len of each (b, h):
+ *     S_t = exp(g) S_{t-1} + k_t v_t^T          (D x D, FP32)
+ *     o_t = scale * S_t^T q_t
+ * Each token sees itself and what lies before it; there is no normaliser.  log_decay: FP32 [heads] on the device, <= 0
+ * (0: no decay, -inf: every token sees itself alone; positive values grow and are the caller's affair).
+ *
+ * A (B,H,N,D) tensor is a pointer with the strides of b, h and n in elements; the last dimension is contiguous.  Pointers and
+ * strides of whole 16 bytes let the tensor-core kernels run (fp16 / bf16); anything else that is aligned to its
+ * type takes the CUDA-core kernels.  Rows past the first seq_lens[b] (int32 [B] on the device, NULL: all have seq_len rows; values
+ * are clamped to 0 .. seq_len) do not take part, whatever they hold: outputs and gradients are zero there and
+ * the final state is the one behind the last row that counts.
+ *
+ * segment_states: FP32, fnb_decay_segment_floats() of them (0: may be NULL), written by the forward and read by the backward:
+ * the states at the cuts where the sequence is split over SMs.  workspace: fnb_decay_workspace_bytes(), 256-byte aligned,
+ * for either direction.  Both sizes follow the SM count of the device that is current when they are asked for. */
+typedef struct fnb_decay_shape {
+  int64_t batch, heads, seq_len;
+  int32_t head_dim;       /* 16, 32, 64 or 128 */
+  int32_t dtype;          /* fnb_dtype of q, k, v, out and the gradients; states are FP32 */
+  float scale;            /* finite, not 0 */
+  uint32_t flags;         /* 0 or FNB_FLAG_FORCE_GENERIC */
+} fnb_decay_shape;
+typedef struct fnb_rows {
+  void* data;
+  int64_t stride_b, stride_h, stride_n;
+} fnb_rows;
+typedef struct fnb_decay_fwd_args {
+  fnb_decay_shape shape;
+  fnb_rows q, k, v;             /* read-only */
+  fnb_rows out;
+  const float* log_decay;       /* [H] */
+  const int32_t* seq_lens;      /* [B] or NULL */
+  const float* initial_state;   /* (B,H,D,D) contiguous, S[i][j] = sum k_i v_j, or NULL */
+  float* final_state;           /* (B,H,D,D) or NULL: not wanted; may be initial_state's own memory */
+  float* segment_states;
+  void* workspace;
+  size_t workspace_bytes;
+  int32_t device;
+  void* stream;
+  int32_t* device_status;       /* as in fnb_fwd_args */
+} fnb_decay_fwd_args;
+typedef struct fnb_decay_bwd_args {
+  fnb_decay_shape shape;
+  fnb_rows q, k, v, d_out;      /* read-only */
+  fnb_rows dq, dk, dv;
+  const float* log_decay;
+  const int32_t* seq_lens;
+  const float* initial_state;
+  const float* d_final_state;   /* (B,H,D,D) or NULL: zeros */
+  float* d_initial_state;       /* (B,H,D,D) or NULL: not wanted */
+  const float* segment_states;  /* what the forward wrote */
+  void* workspace;
+  size_t workspace_bytes;
+  int32_t device;
+  void* stream;
+  int32_t* device_status;
+} fnb_decay_bwd_args;
+FNB_API int fnb_check_decay_shape(const fnb_decay_shape* shape);
+FNB_API size_t fnb_decay_segment_floats(const fnb_decay_shape* shape);
+FNB_API size_t fnb_decay_workspace_bytes(const fnb_decay_shape* shape);
+FNB_API int fnb_decay_forward(const fnb_decay_fwd_args* args);
+FNB_API int fnb_decay_backward(const fnb_decay_bwd_args* args);
+
+/* One token of the same recurrence for each row of a batch, the states updated in place:
+ *     S = exp(g) S + k v^T,   out = scale * S^T q
+ * q, k, v, out: (batch, heads, D) with strides of b and h in elements (stride_n is not read), last dimension contiguous.
+ * states: (num_states, heads, D, D) FP32 contiguous, 16-byte aligned.  slots: int32 [batch] on the device, the state of each row; a
+ * row whose slot is not in 0 .. num_states - 1 is idle (its output is zero, no state is touched).  Rows that name one
+ * slot are taken in the order of the batch, as tokens that follow one another.  NULL: row b has state b
+ * (num_states >= batch). */
+typedef struct fnb_decay_step_args {
+  int64_t batch, heads, num_states;
+  int32_t head_dim, dtype;
+  float scale;
+  fnb_rows q, k, v, out;
+  const float* log_decay;
+  float* states;
+  const int32_t* slots;
+  int32_t device;
+  void* stream;
+} fnb_decay_step_args;
+FNB_API int fnb_decay_step(const fnb_decay_step_args* args);
+
+/* ---- layer norm, whole rows or groups of columns (no counterpart in the reference) ------------
+ * Each row of `cols` elements is cut into `groups` equal runs of n columns; every run is brought to mean 0 and variance 1:
+ *     y = (x - mean) * rstd * weight + bias,  rstd = 1 / sqrt(var + eps),  var = sum (x - mean)^2 / n
+ * weight, bias: [cols] of param_dtype (FNB_F32 or x's own), either may be NULL.  Statistics are FP32; mean and rstd
+ * ([rows][groups]) are written where they are not NULL and are what the backward reads.
+ * Backward: dx, and the sums over the rows d_weight, d_bias (each may be NULL: not wanted) in a fixed order; d_weight and d_bias are of
+ * param_dtype and may be wanted without weight and bias being given.  Row strides are in elements.  n <= 16384.
+ * workspace: fnb_norm_workspace_bytes(), 16-byte aligned; it follows the SM count of the current device. */
+typedef struct fnb_norm_shape {
+  int64_t rows;
+  int32_t cols, groups;
+  int32_t dtype, param_dtype;
+  float eps;              /* finite, >= 0 */
+} fnb_norm_shape;
+typedef struct fnb_norm_fwd_args {
+  fnb_norm_shape shape;
+  const void* x;
+  int64_t x_stride;
+  void* y;
+  int64_t y_stride;
+  const void* weight;
+  const void* bias;
+  float* mean;
+  float* rstd;
+  int32_t device;
+  void* stream;
+} fnb_norm_fwd_args;
+typedef struct fnb_norm_bwd_args {
+  fnb_norm_shape shape;
+  const void* x;
+  int64_t x_stride;
+  const void* d_y;
+  int64_t d_y_stride;
+  void* d_x;              /* or NULL: not wanted */
+  int64_t d_x_stride;
+  const void* weight;
+  const float* mean;
+  const float* rstd;
+  void* d_weight;         /* or NULL */
+  void* d_bias;           /* or NULL */
+  void* workspace;
+  size_t workspace_bytes;
+  int32_t device;
+  void* stream;
+} fnb_norm_bwd_args;
+FNB_API int fnb_check_norm_shape(const fnb_norm_shape* shape);
+FNB_API size_t fnb_norm_workspace_bytes(const fnb_norm_shape* shape);
+FNB_API int fnb_norm_forward(const fnb_norm_fwd_args* args);
+FNB_API int fnb_norm_backward(const fnb_norm_bwd_args* args);
+
 /* Tests only: the time limit of every bounded device-side wait on `device` (default 1500 ms),
  * so that a test of the expiry path does not take seconds.  1..10000 ms.  No counterpart in the
  * reference. */
