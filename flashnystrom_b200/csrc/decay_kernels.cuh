@@ -21,8 +21,7 @@ struct DecayParams {
   const float* log_decay;     // [H]
   const int32_t* seq_lens;    // [B] or null
   const float* state_in;      // [BH][ncut][D][D] or null (zeros): the state that enters each run of rows
-  float* state_out;           // chunk kernel with outputs: [BH][D][D] or null, the state that leaves the last run of a slice;
-                              // without: [BH][ncut][D][D], the sum of each run alone
+  float* state_out;           // (without outputs) [BH][ncut][D][D]: the sum of each run alone
   int64_t N;
   int H, ncut;                // runs of rows per slice
   int cut0, nrun;             // the runs of this launch: nrun of them from cut0 on
@@ -303,12 +302,8 @@ __global__ void __launch_bounds__(kThreads, D <= 64 ? 2 : 1) decay_chunk_kernel(
 #pragma unroll
           for (int j = 0; j < CW; ++j) S[a][i][c][j] = decay_by(by_nv, S[a][i][c][j]) + U[a][i][c][j];
   }
-  if (!p.state_out) return;
-  if (OUT) {
-    const int64_t last = len > 0 ? (len - 1) / p.seg_rows : 0;      // (with outputs a run is a segment)
-    if (cut != (REV ? 0 : (int)last)) return;
-  }
-  float* to = p.state_out + (OUT ? (size_t)bh : (size_t)bh * p.ncut + cut) * D * D;
+  if (OUT) return;
+  float* to = p.state_out + ((size_t)bh * p.ncut + cut) * D * D;
 #pragma unroll
   for (int a = 0; a < CG; ++a)
 #pragma unroll
@@ -337,6 +332,8 @@ struct DecayJoinParams {
 template <bool REV>
 __global__ void __launch_bounds__(kThreads) decay_join_kernel(DecayJoinParams p) {
   const int bh = blockIdx.y, e = blockIdx.x * kThreads + threadIdx.x, DD = p.D * p.D, ncut = p.nseg * p.sub;
+  pdl_trigger();
+  pdl_wait();
   if (e >= DD) return;
   const double g = decay_log(p.log_decay[bh % p.H]);
   const int64_t len = decay_len(p.seq_lens, bh / p.H, p.N);

@@ -1,0 +1,656 @@
+// Causal attention with a decay on the tensor cores (fp16 / bf16): out = A(x, y, z) of decay_kernels.cuh, C rows at a time, and the
+// sums of y z^T over runs of rows that join the segments of a sequence.
+//
+// Per chunk, with S the state that enters it (FP32, in registers):
+//     P = x y^T (C x C)             -> times exp(g |s - t|) and the mask, rounded to 16 bits
+//     out = P z + exp(g (s + 1)) x S
+//     S = exp(g C) S + y'^T z,      y' = exp(g (C - 1 - t)) y, as the sum of two or three 16-bit terms
+// S takes part in x S as the sum of two 16-bit terms.  So each term of an output is rounded once on its way (its score, to 16 bits)
+// and the output once; the state keeps 16 to 24 bits.
+#pragma once
+#include "common.cuh"
+#include "decay_kernels.cuh"
+#include "tc_common.cuh"
+
+namespace fnb {
+namespace dtc {
+
+using namespace tc;
+
+constexpr int kGroup = 256;                                   // threads of a group of eight warps
+__device__ __forceinline__ uint8_t* at1024(uint8_t* p) {
+  return reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(p) + 1023) & ~(uintptr_t)1023);
+}
+// operands staged as blocks of [rows x 64] with the 128-byte swizzle: K along the rows' 128 bytes, or K along the rows
+__device__ __forceinline__ uint64_t along_row(uint32_t base, int k, int rows) {
+  return smem_desc_sw128(base + (k >> 2) * (rows * 128) + (k & 3) * 32, 16, 1024);
+}
+__device__ __forceinline__ uint64_t along_rows(uint32_t base, int k, int rows) {
+  return smem_desc_sw128(base + k * 2048, rows * 128, 1024);
+}
+template <int NC> __device__ __forceinline__ void ld_cols(uint32_t taddr, float* v) {
+  if (NC == 16) {
+    tmem_ld16(taddr, v);
+  } else {
+#pragma unroll
+    for (int c = 0; c < NC; c += 32) tmem_ld32(taddr + c, v + c);
+  }
+}
+
+struct DecayTcParams {
+  const float* log_decay;
+  const int32_t* seq_lens;
+  const float* state_in;      // main kernel: [BH][nseg][Dr][Dr] or null
+  float* sums;                // sums kernel: [BH][ncut][Dr][Dr]
+  void* out;                  // rows that do not count are cleared by plain stores
+  int64_t ob, oh, on;
+  int64_t N, seg_rows, sub_rows;
+  int H, Dr, sub, ncut, cut0, nrun;
+  float scale, inter, sum_scale;
+  int transposed;
+  int* status;
+};
+
+// y' for 16 bytes (eight elements) of one row, as TERMS 16-bit terms
+template <class T, int TERMS>
+__device__ __forceinline__ void scaled_terms(uint4 raw, float w, uint4* terms) {
+  const T* e = reinterpret_cast<const T*>(&raw);
+  float f[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] = to_f<T>(e[j]) * w;
+#pragma unroll
+  for (int t = 0; t < TERMS; ++t) {
+    uint32_t u[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      u[j] = pack2<T>(f[2 * j], f[2 * j + 1]);
+      if (t + 1 < TERMS) {
+        const T* h = reinterpret_cast<const T*>(&u[j]);
+        f[2 * j] -= to_f<T>(h[0]);
+        f[2 * j + 1] -= to_f<T>(h[1]);
+      }
+    }
+    terms[t] = make_uint4(u[0], u[1], u[2], u[3]);
+  }
+}
+
+// ---- sums over runs ------------------------------------------------------------------------------------------
+// One CTA a run, two CTAs an SM: a group of eight warps forms the terms of y', double-buffered, one thread issues the products, which add up in
+// tensor memory over kSpan rows (weights reach back that far) before the group takes them out and decays what it has.
+// Two terms of fp16 and three of bf16 are 22 and 24 bits: the sums are FP32 sums.  Bound by HBM (y and z once).
+template <class T, int D> struct SumsCfg {
+  static constexpr int C = D == 64 ? 64 : 32, kStages = 3, kTerms = sizeof(T) == 2 && UmmaFmt<T>::v == 0 ? 2 : 3;
+  static constexpr int kSpan = 256;
+  static constexpr int kTile = C * D * 2;
+  static constexpr int kThreads = kGroup + 64;
+  static constexpr int kBytes = 1024 + kStages * 2 * kTile + 2 * kTerms * kTile + (kSpan + 1) * 4 + 256;
+};
+
+template <class T, int D, bool REV>
+__global__ void __launch_bounds__((SumsCfg<T, D>::kThreads), 2)
+decay_tc_sums_kernel(const __grid_constant__ CUtensorMap tm_y, const __grid_constant__ CUtensorMap tm_z, DecayTcParams p) {
+  using L = SumsCfg<T, D>;
+  constexpr int C = L::C, NST = L::kStages, KB = D / 64, PER = L::kSpan / C;
+  extern __shared__ uint8_t smem_raw[];
+  pdl_trigger();
+  uint8_t* s_in = at1024(smem_raw);                      // stages of [y | z]
+  uint8_t* s_y = s_in + NST * 2 * L::kTile;               // two buffers of kTerms tiles
+  float* pw = reinterpret_cast<float*>(s_y + 2 * L::kTerms * L::kTile);
+  uint64_t* bars = reinterpret_cast<uint64_t*>((reinterpret_cast<uintptr_t>(pw + L::kSpan + 1) + 15) & ~(uintptr_t)15);
+  uint64_t* full = bars;             // [3]
+  uint64_t* empty = bars + 3;        // [3]
+  uint64_t* y_ready = bars + 6;      // [2]
+  uint64_t* y_free = bars + 8;       // [2]
+  uint64_t* u_full = bars + 10;
+  uint64_t* u_free = bars + 11;
+  uint64_t* fin = bars + 12;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 13);
+  int* abort_word = reinterpret_cast<int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int bh = blockIdx.x / p.nrun, cut = p.cut0 + blockIdx.x % p.nrun, b = bh / p.H, h = bh % p.H;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < NST; ++i) { mbar_init(full + i, 1); mbar_init(empty + i, 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(y_ready + i, kGroup / 32); mbar_init(y_free + i, 1); }
+    mbar_init(u_full, 1); mbar_init(u_free, kGroup / 32); mbar_init(fin, 1);
+    *abort_word = 0;
+    fence_mbar_init();
+  }
+  if (warp == 0) { tmem_alloc(tmem_slot, D); tmem_relinquish(); }
+  tc_fence_before();
+  pdl_wait();
+  const int64_t len = decay_len(p.seq_lens, b, p.N);
+  const int64_t r0 = decay_cut_begin(p.seg_rows, p.sub, p.sub_rows, cut);
+  const int64_t r1 = decay_cut_end(p.seg_rows, p.sub, p.sub_rows, p.N, cut);
+  const int64_t end = r1 < len ? r1 : len;
+  const double g = decay_log(p.log_decay[h]);
+  for (int i = threadIdx.x; i <= L::kSpan; i += L::kThreads) pw[i] = (float)exp(g * i);
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  Abort ab{abort_word, p.status};
+  const int count = r0 < end ? (int)((end - r0 + C - 1) / C) : 0;
+  // Chunks are taken in the order of time; a span is PER chunks of it, the last one (backwards: the first) may be shorter.
+  const auto row_of = [&](int i) { return r0 + (int64_t)(REV ? count - 1 - i : i) * C; };
+  // spans are aligned to the end of the run in time, so that each but the first is whole
+  const int first_span = count % PER == 0 ? PER : count % PER;
+  const auto last_of_span = [&](int i) { return (i + 1 - first_span) % PER == 0 && i + 1 >= first_span; };
+  const auto first_of_span = [&](int i) { return i == 0 || last_of_span(i - 1); };
+
+  if (warp == 8) {
+    if (lane == 0 && count > 0) {
+      tma_prefetch_desc(&tm_y);
+      tma_prefetch_desc(&tm_z);
+      int armed = 0;
+      for (int i = 0; i < count; ++i) {
+        const int st = i % NST;
+        if (!mbar_wait(empty + st, ((i / NST) & 1) ^ 1, ab, 0x7100 + i)) break;
+        mbar_expect_tx(full + st, 2 * L::kTile);
+        uint8_t* to = s_in + st * 2 * L::kTile;
+        for (int kb = 0; kb < KB; ++kb) {
+          tma_load_4d_h(to + kb * (C * 128), &tm_y, full + st, kb * 64, (int)row_of(i), h, b, 0);
+          tma_load_4d_h(to + L::kTile + kb * (C * 128), &tm_z, full + st, kb * 64, (int)row_of(i), h, b, 0);
+        }
+        armed = i + 1;
+      }
+      if (ab.raised())
+        for (int i = max(0, armed - NST); i < armed; ++i) mbar_drain(full + i % NST, (i / NST) & 1);
+    }
+  } else if (warp == 9) {
+    if (lane == 0 && count > 0) {
+      constexpr uint32_t idesc = make_idesc<T>(D, D, true, true);
+      int spans = 0;
+      for (int i = 0; i < count; ++i) {
+        const int st = i % NST, u = i & 1;
+        if (!mbar_wait(y_ready + u, (i >> 1) & 1, ab, 0x7200 + i)) break;
+        const bool fresh = first_of_span(i);
+        if (fresh && spans > 0 && !mbar_wait(u_free, (spans - 1) & 1, ab, 0x7300 + i)) break;
+        tc_fence_after();
+        const uint32_t a_z = smem_u32(s_in + st * 2 * L::kTile + L::kTile), a_y = smem_u32(s_y + u * L::kTerms * L::kTile);
+#pragma unroll
+        for (int t = L::kTerms - 1; t >= 0; --t)
+#pragma unroll
+          for (int k = 0; k < C / 16; ++k)
+            umma(tmem, along_rows(a_y + t * L::kTile, k, C), along_rows(a_z, k, C), idesc, !(fresh && t == L::kTerms - 1 && k == 0));
+        umma_commit(empty + st);
+        umma_commit(y_free + u);
+        if (last_of_span(i)) { umma_commit(u_full); ++spans; }
+      }
+      umma_commit(fin);          // nothing of the CTA is given back while a product runs
+      mbar_drain(fin, 0);
+    }
+  } else {
+    const int quarter = warp & 3, half = warp >> 2;
+    const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
+    const int row = D == 64 ? quarter * 16 + lane : quarter * 32 + lane;
+    float S[D / 2];
+#pragma unroll
+    for (int j = 0; j < D / 2; ++j) S[j] = 0.f;
+    // (a wait that gave up does not leave the loop: the lanes of a warp, and the warps of a group, stay together to its end)
+    bool alive = true;
+    int spans = 0, in_span = 0;
+    // forwards the last span may end with the sequence; backwards that one is the first
+    const DecayPair whole = decay_pair(g, L::kSpan), last = decay_pair(g, count > 0 ? (end - r0) - (int64_t)(count - PER) * C : 0);
+    int64_t span_end = 0;        // forwards: the row behind the span; backwards: its first row
+    for (int i = 0; i < count; ++i) {
+      const int st = i % NST, u = i & 1;
+      if (first_of_span(i)) {
+        const int n = i == 0 ? first_span : PER;
+        span_end = REV ? row_of(i + n - 1) : row_of(i + n - 1) + C;
+        if (!REV && span_end > end) span_end = end;
+        in_span = REV ? (int)((i == 0 ? end : row_of(i) + C) - span_end) : (int)(span_end - row_of(i));
+      }
+      alive &= mbar_wait(full + st, (i / NST) & 1, ab, 0x7400 + i);
+      if (i >= 2) alive &= mbar_wait(y_free + u, ((i >> 1) & 1) ^ 1, ab, 0x7500 + i);
+      __syncwarp();
+      uint8_t* src = s_in + st * 2 * L::kTile;
+      uint8_t* dst = s_y + u * L::kTerms * L::kTile;
+      const int64_t c0 = row_of(i);
+      const int nv = end - c0 < C ? (int)(end - c0) : C;
+#pragma unroll
+      for (int q = 0; q < L::kTile / 16 / kGroup; ++q) {
+        const int idx = threadIdx.x + q * kGroup, r = (idx >> 3) & (C - 1);
+        uint4 terms[L::kTerms];
+#pragma unroll
+        for (int t = 0; t < L::kTerms; ++t) terms[t] = make_uint4(0, 0, 0, 0);
+        // weights: forwards exp(g (rows of the span behind this one)), backwards exp(g (rows of the span up to and with this one))
+        if (r < nv) scaled_terms<T, L::kTerms>(*reinterpret_cast<const uint4*>(src + idx * 16), pw[REV ? (int)(c0 + r - span_end) + 1 : (int)(span_end - 1 - c0 - r)], terms);
+        else *reinterpret_cast<uint4*>(src + L::kTile + idx * 16) = make_uint4(0, 0, 0, 0);      // (z's row too: it may hold anything)
+#pragma unroll
+        for (int t = 0; t < L::kTerms; ++t) *reinterpret_cast<uint4*>(dst + t * L::kTile + idx * 16) = terms[t];
+      }
+      fence_proxy_async();
+      mbar_arrive_warp(y_ready + u);
+      if (last_of_span(i)) {
+        alive &= mbar_wait(u_full, spans & 1, ab, 0x7600 + i);
+        __syncwarp();
+        tc_fence_after();
+        const DecayPair w = in_span == L::kSpan ? whole : last;      // (the first one's multiplies zeros)
+#pragma unroll
+        for (int q = 0; q < D / 32; ++q) {
+          float U[16];
+          tmem_ld16(tmem + lane_base + half * (D / 2) + q * 16, U);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) S[q * 16 + j] = decay_by(w, S[q * 16 + j]) + p.sum_scale * U[j];
+        }
+        tc_fence_before();
+        mbar_arrive_warp(u_free);
+        ++spans;
+      }
+    }
+    if (alive && count > 0 && (D == 128 || lane < 16) && row < p.Dr) {
+      float* to = p.sums + ((size_t)bh * p.ncut + cut) * p.Dr * p.Dr + row * p.Dr;
+#pragma unroll
+      for (int j = 0; j < D / 2; j += 4)
+        if (half * (D / 2) + j < p.Dr) *reinterpret_cast<float4*>(to + half * (D / 2) + j) = make_float4(S[j], S[j + 1], S[j + 2], S[j + 3]);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) tmem_dealloc(tmem, D);
+}
+
+// ---- outputs -------------------------------------------------------------------------------------------------
+// One CTA a segment, one CTA an SM, 18 warps: group A (warps 0-7) turns P into its 16-bit operand and takes the output tile out, group B (8-15) forms
+// y' and carries the state, warp 16 loads, warp 17 issues.  The two groups meet only in what the products need: while A works on the scores of a
+// chunk, B is at the state behind it.  C = 128 rows for heads of up to 64 and 64 for 128: what the state's operands leave room for.
+template <int D> struct MainCfg {
+  static constexpr int C = D == 64 ? 128 : 64, kStages = D == 64 ? 3 : 2;
+  static constexpr int kTile = C * D * 2;                                // 16 KB
+  static constexpr int kP = C * C * 2 > kTile ? C * C * 2 : kTile;      // scores, then the output tile
+  static constexpr int kS = D * D * 2;
+  static constexpr int kThreads = 2 * kGroup + 64;
+  static constexpr int kBytes = 1024 + kStages * 3 * kTile + kP + 2 * kTile + 2 * kS + (C + 1) * 4 + 80 + 256;
+  static constexpr int kPcol = 0, kIntra = C, kInter = C + D, kU = C + 2 * D;      // tensor-memory columns
+};
+
+template <class T, int D, bool REV>
+__global__ void __launch_bounds__(MainCfg<D>::kThreads, 1)
+decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_y, const __grid_constant__ CUtensorMap tm_z,
+                const __grid_constant__ CUtensorMap tm_o, DecayTcParams p) {
+  using L = MainCfg<D>;
+  constexpr int C = L::C, NST = L::kStages, KB = D / 64, RPW = C / 4;      // rows of a tile that one warp's lanes hold
+  constexpr bool F16 = UmmaFmt<T>::v == 0;
+  extern __shared__ uint8_t smem_raw[];
+  pdl_trigger();
+  uint8_t* s_in = at1024(smem_raw);                   // stages of [x | y | z]
+  uint8_t* s_p = s_in + NST * 3 * L::kTile;
+  uint8_t* s_y = s_p + L::kP;                         // two terms of y'
+  uint8_t* s_s = s_y + 2 * L::kTile;                  // two terms of S
+  float* pw = reinterpret_cast<float*>(s_s + 2 * L::kS);
+  float* s_mul = pw + C + 1;                          // [2]: what x S is to be multiplied by, by chunk parity
+  float* s_max = s_mul + 2;                           // [16]
+  uint64_t* bars = reinterpret_cast<uint64_t*>((reinterpret_cast<uintptr_t>(s_max + 16) + 15) & ~(uintptr_t)15);
+  uint64_t* full = bars;             // [3]
+  uint64_t* empty = bars + 3;        // [3]
+  uint64_t* p_full = bars + 6;
+  uint64_t* p_free = bars + 7;
+  uint64_t* p_ready = bars + 8;
+  uint64_t* o_full = bars + 9;
+  uint64_t* o_free = bars + 10;
+  uint64_t* y_ready = bars + 11;
+  uint64_t* u_full = bars + 12;
+  uint64_t* s_ready = bars + 13;
+  uint64_t* s_done = bars + 14;
+  uint64_t* clean = bars + 15;
+  uint64_t* fin = bars + 16;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 17);
+  int* abort_word = reinterpret_cast<int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int bh = blockIdx.x / p.ncut, cut = blockIdx.x % p.ncut, b = bh / p.H, h = bh % p.H;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < NST; ++i) { mbar_init(full + i, 1); mbar_init(empty + i, 1); }
+    mbar_init(p_full, 1); mbar_init(p_free, kGroup / 32); mbar_init(p_ready, kGroup / 32); mbar_init(o_full, 1); mbar_init(o_free, kGroup / 32);
+    mbar_init(y_ready, kGroup / 32); mbar_init(u_full, 1); mbar_init(s_ready, kGroup / 32); mbar_init(s_done, 1);
+    mbar_init(clean, kGroup / 32); mbar_init(fin, 1);
+    *abort_word = 0;
+    fence_mbar_init();
+  }
+  if (warp == 0) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
+  tc_fence_before();
+  pdl_wait();
+  const int64_t len = decay_len(p.seq_lens, b, p.N);
+  const int64_t r0 = (int64_t)cut * p.seg_rows;
+  const int64_t r1 = r0 + p.seg_rows < p.N ? r0 + p.seg_rows : p.N;
+  const int64_t end = r1 < len ? r1 : len;
+  const double g = decay_log(p.log_decay[h]);
+  for (int i = threadIdx.x; i <= C; i += L::kThreads) pw[i] = (float)exp(g * i);
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  Abort ab{abort_word, p.status};
+  const int count = r0 < end ? (int)((end - r0 + C - 1) / C) : 0;
+  const auto row_of = [&](int i) { return r0 + (int64_t)(REV ? count - 1 - i : i) * C; };
+  // The last rows of a tile lie past the sequence's length, but not past the tensor: they hold anything, and are cleared.
+  const int dirty = end == len && len < p.N && (end - r0) % C != 0 ? (REV ? 0 : count - 1) : -1;
+
+  if (warp == 16) {
+    if (lane == 0 && count > 0) {
+      tma_prefetch_desc(&tm_x);
+      tma_prefetch_desc(&tm_y);
+      tma_prefetch_desc(&tm_z);
+      tma_prefetch_desc(&tm_o);
+      int armed = 0;
+      for (int i = 0; i < count; ++i) {
+        const int st = i % NST;
+        if (!mbar_wait(empty + st, ((i / NST) & 1) ^ 1, ab, 0x8100 + i)) break;
+        mbar_expect_tx(full + st, 3 * L::kTile);
+        uint8_t* to = s_in + st * 3 * L::kTile;
+        for (int kb = 0; kb < KB; ++kb) {
+          tma_load_4d_h(to + kb * (C * 128), &tm_x, full + st, kb * 64, (int)row_of(i), h, b, 0);
+          tma_load_4d_h(to + L::kTile + kb * (C * 128), &tm_y, full + st, kb * 64, (int)row_of(i), h, b, 0);
+        }
+        for (int kb = 0; kb < KB; ++kb)
+          tma_load_4d_h(to + 2 * L::kTile + kb * (C * 128), &tm_z, full + st, kb * 64, (int)row_of(i), h, b, 0);
+        armed = i + 1;
+      }
+      if (ab.raised())
+        for (int i = max(0, armed - NST); i < armed; ++i) mbar_drain(full + i % NST, (i / NST) & 1);
+    }
+  } else if (warp == 17) {
+    if (lane == 0 && count > 0) {
+      constexpr uint32_t i_p = make_idesc<T>(C, C, false, false);       // x y^T
+      constexpr uint32_t i_o = make_idesc<T>(C, D, false, true);        // P z, x S
+      constexpr uint32_t i_u = make_idesc<T>(D, D, true, true);         // y'^T z
+      uint32_t a_p = smem_u32(s_p), a_y = smem_u32(s_y), a_s = smem_u32(s_s);
+      const auto scores = [&](int i) -> bool {
+        const int st = i % NST;
+        if (!mbar_wait(full + st, (i / NST) & 1, ab, 0x8200 + i)) return false;
+        if (i == dirty && !mbar_wait(clean, 0, ab, 0x8300 + i)) return false;
+        if (i > 0 && !mbar_wait(p_free, (i - 1) & 1, ab, 0x8400 + i)) return false;
+        tc_fence_after();
+        const uint32_t a_x = smem_u32(s_in + st * 3 * L::kTile);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) umma(tmem + L::kPcol, along_row(a_x, k, C), along_row(a_x + L::kTile, k, C), i_p, k > 0);
+        umma_commit(p_full);
+        return true;
+      };
+      bool ok = scores(0);
+      for (int i = 0; ok && i < count; ++i) {
+        asm volatile("" : "+r"(a_p), "+r"(a_y), "+r"(a_s));      // (descriptors are formed here, not kept over the loop in registers there are not)
+        const uint32_t a_x = smem_u32(s_in + (i % NST) * 3 * L::kTile), a_z = a_x + 2 * L::kTile;
+        if (i + 1 < count) {
+          if (!mbar_wait(y_ready, i & 1, ab, 0x8500 + i)) break;
+          tc_fence_after();
+#pragma unroll
+          for (int t = 1; t >= 0; --t)
+#pragma unroll
+            for (int k = 0; k < C / 16; ++k)
+              umma(tmem + L::kU, along_rows(a_y + t * L::kTile, k, C), along_rows(a_z, k, C), i_u, !(t == 1 && k == 0));
+          umma_commit(u_full);
+        }
+        if (!mbar_wait(s_ready, i & 1, ab, 0x8600 + i)) break;
+        if (i > 0 && !mbar_wait(o_free, (i - 1) & 1, ab, 0x8700 + i)) break;
+        tc_fence_after();
+#pragma unroll
+        for (int t = 1; t >= 0; --t)
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k)
+            umma(tmem + L::kInter, along_row(a_x, k, C), along_rows(a_s + t * L::kS, k, D), i_o, !(t == 1 && k == 0));
+        umma_commit(s_done);
+        if (i + 1 < count) ok = scores(i + 1);
+        if (!ok || !mbar_wait(p_ready, i & 1, ab, 0x8800 + i)) break;
+        tc_fence_after();
+#pragma unroll
+        for (int k = 0; k < C / 16; ++k) umma(tmem + L::kIntra, along_row(a_p, k, C), along_rows(a_z, k, C), i_o, k > 0);
+        umma_commit(o_full);
+        umma_commit(empty + i % NST);
+      }
+      umma_commit(fin);          // nothing of the CTA is given back while a product runs
+      mbar_drain(fin, 0);
+    }
+  } else if (warp < 8) {
+    // ---- group A: scores and outputs
+    // (here and in group B a wait that gave up does not leave the loop: the warps meet at barriers, and the status word has it)
+    const int quarter = warp & 3, half = warp >> 2;
+    const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
+    const int w0 = quarter * RPW, s = w0 + (lane & (RPW - 1));
+    const bool owner = lane < RPW;
+    constexpr int NB = C / 32;                     // 16-column blocks of a thread: every other one
+    // rows of the segment past the sequence's length
+    {
+      const int64_t z0 = r0 + (int64_t)count * C;
+      T* out = static_cast<T*>(p.out) + b * p.ob + h * p.oh;
+      const int per = p.Dr / 8;
+      for (int64_t i = threadIdx.x; i < (r1 - z0) * per; i += kGroup)
+        *reinterpret_cast<uint4*>(out + (z0 + i / per) * p.on + (i % per) * 8) = make_uint4(0, 0, 0, 0);
+    }
+    for (int i = 0; i < count; ++i) {
+      const int64_t c0 = row_of(i);
+      const int nv = end - c0 < C ? (int)(end - c0) : C;
+      mbar_wait(p_full, i & 1, ab, 0x8900 + i);
+      __syncwarp();
+      tc_fence_after();
+      float v[NB][16];
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        const int t0 = (2 * n + half) * 16;
+        if (REV ? t0 + 15 >= w0 : t0 <= w0 + RPW - 1) ld_cols<16>(tmem + L::kPcol + lane_base + t0, v[n]);
+      }
+      tmem_ld_wait();
+      tc_fence_before();
+      mbar_arrive_warp(p_free);
+      float most = 0.f;
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        const int t0 = (2 * n + half) * 16;
+        if (REV ? t0 + 15 < w0 : t0 > w0 + RPW - 1) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) v[n][j] = 0.f;
+        } else if (REV ? t0 >= w0 + RPW - 1 : t0 + 15 <= w0) {
+          // the whole block lies behind the rows: exp(g d) as a row's factor times a column's
+          const float row = p.scale * pw[REV ? t0 - s : s - t0 - 15];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const float4 c = *reinterpret_cast<const float4*>(pw + 4 * q);
+            v[n][REV ? 4 * q : 15 - 4 * q] *= row * c.x;
+            v[n][REV ? 4 * q + 1 : 14 - 4 * q] *= row * c.y;
+            v[n][REV ? 4 * q + 2 : 13 - 4 * q] *= row * c.z;
+            v[n][REV ? 4 * q + 3 : 12 - 4 * q] *= row * c.w;
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const int d = REV ? t0 + j - s : s - t0 - j;
+            v[n][j] = d >= 0 ? v[n][j] * (p.scale * pw[d < 0 ? 0 : d]) : 0.f;
+          }
+        }
+        if (F16)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) most = fmaxf(most, fabsf(v[n][j]));
+      }
+      // the output tile of the chunk before has left the buffer that the scores go to
+      float up = 1.f;
+      if (threadIdx.x == 0) tma_store_wait_read();
+      if (F16) {
+        // scores past the range of fp16 (rare): the tile goes in divided by a power of two
+        if (named_barrier_or(1, kGroup, owner && most > 32768.f)) {
+          float m = owner && most < INFINITY ? most : 0.f;
+          for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+          if (lane == 0) s_max[warp] = m;
+          named_barrier(1, kGroup);
+          for (int k = 0; k < 8; ++k) m = fmaxf(m, s_max[k]);
+          int e = 0;
+          frexpf(m, &e);
+          up = ldexpf(1.f, max(0, e - 15));
+          const float down = 1.f / up;
+#pragma unroll
+          for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[n][j] *= down;
+          named_barrier(1, kGroup);
+        }
+      } else {
+        named_barrier(1, kGroup);
+      }
+      if (owner) {
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          const int cc = (2 * n + half) * 2;
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            const float* e = v[n] + 8 * q;
+            *reinterpret_cast<uint4*>(s_p + ((cc + q) >> 3) * (C * 128) + sw128_offset(s, (cc + q) & 7)) =
+                make_uint4(pack2<T>(e[0], e[1]), pack2<T>(e[2], e[3]), pack2<T>(e[4], e[5]), pack2<T>(e[6], e[7]));
+          }
+        }
+      }
+      fence_proxy_async();
+      mbar_arrive_warp(p_ready);
+      float wi = 0.f;
+      if (REV ? s < nv : true) wi = p.inter * pw[REV ? nv - 1 - s : s + 1];
+      mbar_wait(o_full, i & 1, ab, 0x8a00 + i);
+      __syncwarp();
+      tc_fence_after();
+      if (F16) wi *= s_mul[i & 1];
+#pragma unroll
+      for (int q = 0; q < D / 64; ++q) {
+        const int col = half * (D / 2) + q * 32;
+        float a[32], e[32];
+        tmem_ld32(tmem + L::kIntra + lane_base + col, a);
+        tmem_ld32(tmem + L::kInter + lane_base + col, e);
+        tmem_ld_wait();
+        if (q == D / 64 - 1) {
+          tc_fence_before();
+          mbar_arrive_warp(o_free);
+        }
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          if (F16) a[j] *= up;
+          a[j] = wi == 0.f ? a[j] : fmaf(wi, e[j], a[j]);
+        }
+        if (owner) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int cc = (col >> 3) + k;
+            *reinterpret_cast<uint4*>(s_p + (cc >> 3) * (C * 128) + sw128_offset(s, cc & 7)) =
+                make_uint4(pack2<T>(a[8 * k], a[8 * k + 1]), pack2<T>(a[8 * k + 2], a[8 * k + 3]), pack2<T>(a[8 * k + 4], a[8 * k + 5]),
+                           pack2<T>(a[8 * k + 6], a[8 * k + 7]));
+          }
+        }
+      }
+      fence_proxy_async();
+      named_barrier(1, kGroup);
+      if (threadIdx.x == 0) {
+        for (int kb = 0; kb < KB; ++kb) tma_store_4d_h(&tm_o, s_p + kb * (C * 128), kb * 64, (int)c0, h, b, 0);
+        tma_store_commit();
+      }
+    }
+    if (threadIdx.x == 0) tma_store_wait_all();
+  } else {
+    // ---- group B: the state
+    const int tid = threadIdx.x - kGroup, quarter = warp & 3, half = (warp - 8) >> 2;
+    const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
+    const int row = D == 64 ? quarter * 16 + lane : quarter * 32 + lane;
+    const bool owner = D == 128 || lane < 16;
+    constexpr int HC = D / 2;
+    // (only the last chunk in space is not whole: backwards in time the first, forwards one whose state nobody needs)
+    const DecayPair full_chunk = decay_pair(g, C), first_chunk = REV && count > 0 ? decay_pair(g, end - row_of(0)) : full_chunk;
+    float S[HC];
+#pragma unroll
+    for (int j = 0; j < HC; ++j) {
+      const int col = half * HC + j;
+      S[j] = 0.f;
+      if (p.state_in && owner && row < p.Dr && col < p.Dr)
+        S[j] = p.state_in[((size_t)bh * p.ncut + cut) * p.Dr * p.Dr + (p.transposed ? col * p.Dr + row : row * p.Dr + col)];
+    }
+    // S as two 16-bit terms; in fp16 divided by a power of two where it would leave the range
+    const auto put_state = [&](int i) {
+      float down = 1.f;
+      if (F16) {
+        float most = 0.f;
+#pragma unroll
+        for (int j = 0; j < HC; ++j) most = fmaxf(most, fabsf(S[j]));
+        float up = 1.f;
+        if (named_barrier_or(2, kGroup, owner && most > 32768.f)) {
+          float m = owner && most < INFINITY ? most : 0.f;
+          for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+          if (lane == 0) s_max[warp] = m;
+          named_barrier(2, kGroup);
+          for (int k = 0; k < 8; ++k) m = fmaxf(m, s_max[8 + k]);
+          int e = 0;
+          frexpf(m, &e);
+          up = ldexpf(1.f, max(0, e - 15));
+          down = 1.f / up;
+          named_barrier(2, kGroup);
+        }
+        if (tid == 0) s_mul[i & 1] = up;
+      }
+      if (owner) {
+#pragma unroll
+        for (int k = 0; k < HC / 8; ++k) {
+          float f[8];
+          uint32_t hi[4], lo[4];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) f[j] = F16 ? S[8 * k + j] * down : S[8 * k + j];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            hi[j] = pack2<T>(f[2 * j], f[2 * j + 1]);
+            const T* e = reinterpret_cast<const T*>(&hi[j]);
+            lo[j] = pack2<T>(f[2 * j] - to_f<T>(e[0]), f[2 * j + 1] - to_f<T>(e[1]));
+          }
+          const int cc = (half * HC >> 3) + k;
+          const uint32_t off = (cc >> 3) * (D * 128) + sw128_offset(row, cc & 7);
+          *reinterpret_cast<uint4*>(s_s + off) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          *reinterpret_cast<uint4*>(s_s + L::kS + off) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        }
+      }
+      fence_proxy_async();
+      mbar_arrive_warp(s_ready);
+    };
+    if (count > 0) put_state(0);
+    for (int i = 0; i < count; ++i) {
+      const int st = i % NST;
+      const int64_t c0 = row_of(i);
+      const int nv = end - c0 < C ? (int)(end - c0) : C;
+      uint8_t* src = s_in + st * 3 * L::kTile;
+      if (i == dirty) {
+        mbar_wait(full + st, (i / NST) & 1, ab, 0x8b00 + i);
+        __syncwarp();
+        for (int idx = tid; idx < 3 * L::kTile / 16; idx += kGroup)
+          if (((idx >> 3) & (C - 1)) >= nv) *reinterpret_cast<uint4*>(src + idx * 16) = make_uint4(0, 0, 0, 0);
+        fence_proxy_async();
+        mbar_arrive_warp(clean);
+        named_barrier(2, kGroup);
+      }
+      if (i + 1 == count) break;
+      mbar_wait(full + st, (i / NST) & 1, ab, 0x8c00 + i);
+      __syncwarp();
+      // (the products that read the terms before are done: u_full of the chunk before has been waited for)
+#pragma unroll
+      for (int q = 0; q < L::kTile / 16 / kGroup; ++q) {
+        const int idx = tid + q * kGroup, r = (idx >> 3) & (C - 1);
+        uint4 terms[2];
+        scaled_terms<T, 2>(*reinterpret_cast<const uint4*>(src + L::kTile + idx * 16), r < nv ? pw[REV ? r + 1 : nv - 1 - r] : 0.f, terms);
+        *reinterpret_cast<uint4*>(s_y + idx * 16) = terms[0];
+        *reinterpret_cast<uint4*>(s_y + L::kTile + idx * 16) = terms[1];
+      }
+      fence_proxy_async();
+      mbar_arrive_warp(y_ready);
+      mbar_wait(u_full, i & 1, ab, 0x8d00 + i);
+      __syncwarp();
+      tc_fence_after();
+      const DecayPair w = i == 0 ? first_chunk : full_chunk;
+#pragma unroll
+      for (int q = 0; q < HC / 16; ++q) {
+        float U[16];
+        tmem_ld16(tmem + L::kU + lane_base + half * HC + q * 16, U);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) S[q * 16 + j] = decay_by(w, S[q * 16 + j]) + p.sum_scale * U[j];
+      }
+      tc_fence_before();
+      mbar_wait(s_done, i & 1, ab, 0x8e00 + i);
+      __syncwarp();
+      put_state(i + 1);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) tmem_dealloc(tmem, 512);
+}
+
+}  // namespace dtc
+}  // namespace fnb

@@ -1476,6 +1476,7 @@ int fnb_debug_set_wait_limit_ms(int device, int ms) {
   if (!g.ok) return fail(FNB_ERR_CUDA, "cannot select CUDA device %d", device);
   const unsigned long long ns = (unsigned long long)ms * 1000000ull;
   FNB_CUDA(cudaMemcpyToSymbol(tc::g_wait_limit_ns, &ns, sizeof(ns)));
+  FNB_CUDA(set_operators_wait_limit(ns));
   return 0;
 }
 

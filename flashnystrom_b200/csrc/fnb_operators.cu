@@ -7,9 +7,13 @@
 #include "common.cuh"
 #include "host.cuh"
 #include "decay_kernels.cuh"
+#include "decay_tc.cuh"
 #include "norm_kernels.cuh"
+#include "tma_host.cuh"
 
 namespace fnb {
+
+cudaError_t set_operators_wait_limit(unsigned long long ns) { return cudaMemcpyToSymbol(tc::g_wait_limit_ns, &ns, sizeof(ns)); }
 
 // ---- how a sequence is split ----------------------------------------------------------------------------------
 // A slice (b, h) is cut into segments of whole 128-row units, one CTA each; the states that enter the segments come from a pass over
@@ -26,22 +30,24 @@ static DecayPlan decay_plan(const fnb_decay_shape& s) {
   const int64_t BH = s.batch * s.heads, units = (s.seq_len + kDecayUnit - 1) / kDecayUnit;
   const int sms = current_sm_count();
   // Estimated time of a split, in units that one CTA takes in turn: rounds of CTAs x units of the longest, and, where there is more
-  // than one segment, 0.6 of that for the pass over the states and about four units' time for two more launches.
-  const int slots = s.head_dim <= 64 ? 2 * sms : sms;
+  // than one segment, half of that for the pass over the states and about four units' time for two more launches.
+  const int slots = s.dtype == FNB_F32 && s.head_dim <= 64 ? 2 * sms : sms;
   int64_t best = 1;
   double least = 1e300;
-  const int64_t most = std::min<int64_t>(units, std::max<int64_t>(1, slots / std::max<int64_t>(1, std::min<int64_t>(BH, slots))));
+  const int64_t most = std::min<int64_t>(units, std::max<int64_t>(1, 2 * slots / std::min<int64_t>(BH, 2 * slots)));
   for (int64_t n = 1; n <= most; ++n) {
     const double per = (double)((units + n - 1) / n);
     double t = (double)((BH * n + slots - 1) / slots) * per;
-    if (n > 1) t += 0.6 * (double)((BH * (n - 1) + slots - 1) / slots) * per + 4.0;
+    if (n > 1) t += 0.5 * (double)(BH * (n - 1)) / slots * per + 4.0;
     if (t < least) { least = t; best = n; }
   }
   DecayPlan p;
   p.seg_rows = (units + best - 1) / best * kDecayUnit;
   p.nseg = (int)((s.seq_len + p.seg_rows - 1) / p.seg_rows);
-  p.sub = 1;
-  p.sub_rows = p.seg_rows;
+  // two CTAs of the pass over the states fit on an SM
+  int64_t sub = std::max<int64_t>(1, std::min<int64_t>(2 * (int64_t)sms / std::max<int64_t>(1, BH * p.nseg), p.seg_rows / kDecayUnit));
+  p.sub_rows = (p.seg_rows / kDecayUnit + sub - 1) / sub * kDecayUnit;
+  p.sub = (int)((p.seg_rows + p.sub_rows - 1) / p.sub_rows);
   return p;
 }
 
@@ -141,34 +147,114 @@ static int launch_chunks(const DecayCall& c, const DecayParams& p, Launcher& L, 
   });
 }
 
-// The states that enter the segments of a slice -> seg_states (nothing to do with one segment).  state_in: what enters the slice.
+// ---- tensor cores ---------------------------------------------------------------------------------------------
+// 16-bit rows that TMA can address: whole 16 bytes everywhere, no dimension spread out of one element.
+static bool tma_rows(const fnb_rows& t, const fnb_decay_shape& s) {
+  const int64_t size[3] = {s.batch, s.heads, s.seq_len}, stride[3] = {t.stride_b, t.stride_h, t.stride_n};
+  for (int i = 0; i < 3; ++i)
+    if (size[i] > 1 && (stride[i] <= 0 || stride[i] >= ((int64_t)1 << 38))) return false;
+  return vec_rows(t, s.dtype);
+}
+// (D, N, H, B) map of it, box 64 columns x `rows` rows of one slice: rows past N and columns past D read as zero and are not stored.
+static bool make_rows_map(CUtensorMap* map, const fnb_rows& t, const fnb_decay_shape& s, int rows) {
+  tc::EncodeTiledFn fn = tc::encode_fn();
+  if (!fn) return false;
+  const auto stride = [](int64_t size, int64_t st) { return (cuuint64_t)(size > 1 ? st : 128) * 2; };
+  cuuint64_t dims[4] = {(cuuint64_t)s.head_dim, (cuuint64_t)s.seq_len, (cuuint64_t)s.heads, (cuuint64_t)s.batch};
+  cuuint64_t strides[3] = {stride(s.seq_len, t.stride_n), stride(s.heads, t.stride_h), stride(s.batch, t.stride_b)};
+  cuuint32_t box[4] = {64, (cuuint32_t)rows, 1, 1}, each[4] = {1, 1, 1, 1};
+  return fn(map, tc::map_dtype(s.dtype), 4, t.data, dims, strides, box, each, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// f(T{}, D of the kernel): heads narrower than 64 are padded by the maps
+template <class F>
+static int dispatch_decay_tc(const fnb_decay_shape& s, F&& f) {
+  const auto by_d = [&](auto tag) -> int {
+    return s.head_dim <= 64 ? f(tag, std::integral_constant<int, 64>{}) : f(tag, std::integral_constant<int, 128>{});
+  };
+  return s.dtype == FNB_F16 ? by_d(__half{}) : by_d(__nv_bfloat16{});
+}
+static dtc::DecayTcParams decay_tc_params(const DecayCall& c, bool reversed) {
+  dtc::DecayTcParams p{};
+  p.log_decay = c.log_decay; p.seq_lens = c.seq_lens; p.N = c.s.seq_len; p.H = (int)c.s.heads; p.Dr = c.s.head_dim;
+  p.seg_rows = c.plan.seg_rows; p.scale = c.s.scale; p.inter = reversed ? 1.f : c.s.scale; p.sum_scale = reversed ? c.s.scale : 1.f;
+  p.status = c.status;
+  return p;
+}
+template <bool REV>
+static int launch_tc_sums(const DecayCall& c, const fnb_rows& y, const fnb_rows& z, int cut0, int nrun, Launcher& L) {
+  return dispatch_decay_tc(c.s, [&](auto tag, auto d) -> int {
+    using T = decltype(tag);
+    constexpr int D = decltype(d)::value;
+    using Cfg = dtc::SumsCfg<T, D>;
+    CUtensorMap my, mz;
+    if (!make_rows_map(&my, y, c.s, Cfg::C) || !make_rows_map(&mz, z, c.s, Cfg::C)) return fail(FNB_ERR_CUDA, "cuTensorMapEncodeTiled failed");
+    dtc::DecayTcParams p = decay_tc_params(c, REV);
+    p.sums = c.sums; p.sub = c.plan.sub; p.sub_rows = c.plan.sub_rows; p.ncut = c.plan.runs(); p.cut0 = cut0; p.nrun = nrun;
+    auto kern = dtc::decay_tc_sums_kernel<T, D, REV>;
+    if (int rc = set_smem(kern, Cfg::kBytes, c.max_smem, "decay_sums")) return rc;
+    L.begin();
+    FNB_CUDA(launch_pdl(kern, dim3((unsigned)(c.BH * nrun)), dim3(Cfg::kThreads), Cfg::kBytes, c.stream, my, mz, p));
+    return L.end("decay_sums");
+  });
+}
+template <bool REV>
+static int launch_tc_form(const DecayCall& c, const DecayForm& f, const float* state_in, Launcher& L, const char* name) {
+  return dispatch_decay_tc(c.s, [&](auto tag, auto d) -> int {
+    using T = decltype(tag);
+    constexpr int D = decltype(d)::value;
+    using Cfg = dtc::MainCfg<D>;
+    CUtensorMap mx, my, mz, mo;
+    if (!make_rows_map(&mx, f.x, c.s, Cfg::C) || !make_rows_map(&my, f.y, c.s, Cfg::C) || !make_rows_map(&mz, f.z, c.s, Cfg::C) ||
+        !make_rows_map(&mo, f.out, c.s, Cfg::C))
+      return fail(FNB_ERR_CUDA, "cuTensorMapEncodeTiled failed");
+    dtc::DecayTcParams p = decay_tc_params(c, REV);
+    p.state_in = state_in; p.transposed = f.transposed; p.ncut = c.plan.nseg;
+    p.out = f.out.data; p.ob = f.out.stride_b; p.oh = f.out.stride_h; p.on = f.out.stride_n;
+    auto kern = dtc::decay_tc_kernel<T, D, REV>;
+    if (int rc = set_smem(kern, Cfg::kBytes, c.max_smem, name)) return rc;
+    L.begin();
+    FNB_CUDA(launch_pdl(kern, dim3((unsigned)(c.BH * c.plan.nseg)), dim3(Cfg::kThreads), Cfg::kBytes, c.stream, mx, my, mz, mo, p));
+    return L.end(name);
+  });
+}
+static bool decay_on_tensor_cores(const fnb_decay_shape& s) { return s.dtype != FNB_F32 && !(s.flags & FNB_FLAG_FORCE_GENERIC); }
+
+// The states that enter the segments of a slice -> seg_states (none with one segment), and what leaves the slice -> state_out, where
+// that is wanted of this pass.  state_in: what enters the slice.
 static int decay_states(const DecayCall& c, const fnb_rows& y, const fnb_rows& z, bool reversed, const float* state_in, float* seg_states,
-                        Launcher& L) {
-  if (c.plan.nseg == 1) return 0;
-  DecayParams p = decay_params(c, y, z);
-  p.sum_scale = reversed ? c.s.scale : 1.f;
-  p.state_out = c.sums;
-  p.ncut = c.plan.runs(); p.sub = c.plan.sub; p.sub_rows = c.plan.sub_rows;
-  p.nrun = p.ncut - p.sub; p.cut0 = reversed ? p.sub : 0;      // (nothing needs the sums of the last segment in time)
-  if (int rc = reversed ? launch_chunks<true, false>(c, p, L, "decay_sums") : launch_chunks<false, false>(c, p, L, "decay_sums")) return rc;
+                        float* state_out, Launcher& L) {
+  const bool cut = c.plan.nseg > 1;
+  if (!cut && !state_out) return 0;
+  // (without state_out nothing needs the sums of the last segment in time)
+  const int runs = c.plan.runs(), nrun = state_out ? runs : runs - c.plan.sub, cut0 = state_out || !reversed ? 0 : c.plan.sub;
+  if (decay_on_tensor_cores(c.s) && tma_rows(y, c.s) && tma_rows(z, c.s)) {
+    if (int rc = reversed ? launch_tc_sums<true>(c, y, z, cut0, nrun, L) : launch_tc_sums<false>(c, y, z, cut0, nrun, L)) return rc;
+  } else {
+    DecayParams p = decay_params(c, y, z);
+    p.sum_scale = reversed ? c.s.scale : 1.f;
+    p.state_out = c.sums;
+    p.ncut = runs; p.sub = c.plan.sub; p.sub_rows = c.plan.sub_rows; p.nrun = nrun; p.cut0 = cut0;
+    if (int rc = reversed ? launch_chunks<true, false>(c, p, L, "decay_sums") : launch_chunks<false, false>(c, p, L, "decay_sums")) return rc;
+  }
   DecayJoinParams j{};
-  j.sums = c.sums; j.state_in = state_in; j.seg_states = seg_states; j.log_decay = c.log_decay; j.seq_lens = c.seq_lens;
-  j.N = c.s.seq_len; j.H = (int)c.s.heads; j.D = c.s.head_dim; j.nseg = c.plan.nseg; j.sub = c.plan.sub;
-  j.seg_rows = c.plan.seg_rows; j.sub_rows = c.plan.sub_rows; j.count = p.nrun;
+  j.sums = c.sums; j.state_in = state_in; j.seg_states = cut ? seg_states : nullptr; j.state_out = state_out; j.log_decay = c.log_decay;
+  j.seq_lens = c.seq_lens; j.N = c.s.seq_len; j.H = (int)c.s.heads; j.D = c.s.head_dim; j.nseg = c.plan.nseg; j.sub = c.plan.sub;
+  j.seg_rows = c.plan.seg_rows; j.sub_rows = c.plan.sub_rows; j.count = nrun;
   const dim3 grid((unsigned)((j.D * j.D + kThreads - 1) / kThreads), (unsigned)c.BH);
   L.begin();
-  if (reversed) decay_join_kernel<true><<<grid, kThreads, 0, c.stream>>>(j);
-  else decay_join_kernel<false><<<grid, kThreads, 0, c.stream>>>(j);
+  FNB_CUDA(launch_pdl(reversed ? decay_join_kernel<true> : decay_join_kernel<false>, grid, dim3(kThreads), 0, c.stream, j));
   return L.end("decay_join");
 }
 
-// out = scale A(x, y, z) with the states that enter each segment; state_out: what leaves the slice.  Backwards in time the state is
-// dL/dS, which has the scale in it.
-static int decay_form(const DecayCall& c, const DecayForm& f, const float* state_in, float* state_out, Launcher& L, const char* name) {
+// out = scale A(x, y, z) with the states that enter each segment.  Backwards in time the state is dL/dS, which has the scale in it.
+static int decay_form(const DecayCall& c, const DecayForm& f, const float* state_in, Launcher& L, const char* name) {
+  if (decay_on_tensor_cores(c.s) && tma_rows(f.x, c.s) && tma_rows(f.y, c.s) && tma_rows(f.z, c.s) && tma_rows(f.out, c.s))
+    return f.reversed ? launch_tc_form<true>(c, f, state_in, L, name) : launch_tc_form<false>(c, f, state_in, L, name);
   DecayParams p = decay_params(c, f.y, f.z);
   p.x = rows_of(f.x); p.out = rows_of(f.out);
   p.vec = p.vec && vec_rows(f.x, c.s.dtype) && vec_rows(f.out, c.s.dtype);
-  p.state_in = state_in; p.state_out = state_out;
+  p.state_in = state_in;
   p.inter = f.reversed ? 1.f : c.s.scale;
   p.sum_scale = f.reversed ? c.s.scale : 1.f;
   p.ncut = p.nrun = c.plan.nseg; p.sub = 1; p.sub_rows = p.seg_rows; p.transposed = f.transposed;
@@ -311,8 +397,8 @@ int fnb_decay_forward(const fnb_decay_fwd_args* a) {
               (cudaStream_t)a->stream, a->device_status};
   if (int rc = check_decay_common(c, a->segment_states, a->workspace, a->workspace_bytes)) return rc;
   Launcher L(c.stream, a->device);
-  if (int rc = decay_states(c, a->k, a->v, false, a->initial_state, a->segment_states, L)) return rc;
-  return decay_form(c, {a->q, a->k, a->v, a->out, false, false}, c.plan.nseg > 1 ? a->segment_states : a->initial_state, a->final_state, L, "decay_fwd");
+  if (int rc = decay_states(c, a->k, a->v, false, a->initial_state, a->segment_states, a->final_state, L)) return rc;
+  return decay_form(c, {a->q, a->k, a->v, a->out, false, false}, c.plan.nseg > 1 ? a->segment_states : a->initial_state, L, "decay_fwd");
 }
 
 int fnb_decay_backward(const fnb_decay_bwd_args* a) {
@@ -333,11 +419,11 @@ int fnb_decay_backward(const fnb_decay_bwd_args* a) {
   const bool cut = c.plan.nseg > 1;
   // E = dL/dS runs backwards in time; its states at the cuts lie behind the sums in the workspace
   float* e_states = (float*)((char*)a->workspace + align256(slice_floats(c.s) * c.plan.runs() * sizeof(float)));
-  if (int rc = decay_states(c, a->q, a->d_out, true, a->d_final_state, e_states, L)) return rc;
+  if (int rc = decay_states(c, a->q, a->d_out, true, a->d_final_state, e_states, a->d_initial_state, L)) return rc;
   const float* e_in = cut ? e_states : a->d_final_state;
-  if (int rc = decay_form(c, {a->d_out, a->v, a->k, a->dq, false, true}, cut ? a->segment_states : a->initial_state, nullptr, L, "decay_dq")) return rc;
-  if (int rc = decay_form(c, {a->k, a->q, a->d_out, a->dv, true, false}, e_in, a->d_initial_state, L, "decay_dv")) return rc;
-  return decay_form(c, {a->v, a->d_out, a->q, a->dk, true, true}, e_in, nullptr, L, "decay_dk");
+  if (int rc = decay_form(c, {a->d_out, a->v, a->k, a->dq, false, true}, cut ? a->segment_states : a->initial_state, L, "decay_dq")) return rc;
+  if (int rc = decay_form(c, {a->k, a->q, a->d_out, a->dv, true, false}, e_in, L, "decay_dv")) return rc;
+  return decay_form(c, {a->v, a->d_out, a->q, a->dk, true, true}, e_in, L, "decay_dk");
 }
 
 int fnb_decay_step(const fnb_decay_step_args* a) {

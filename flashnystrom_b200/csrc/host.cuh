@@ -160,6 +160,9 @@ inline int device_limits(int device, int* max_smem, int* cc_major, int* sm_count
   return 0;
 }
 
+// The limit of the bounded waits is a device variable of each translation unit with kernels that wait: that of fnb_operators.cu.
+cudaError_t set_operators_wait_limit(unsigned long long ns);
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // Launch with programmatic stream serialization: the kernel may be scheduled while its

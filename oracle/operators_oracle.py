@@ -66,28 +66,66 @@ def half_step(dtype):
     return torch.finfo(dtype).eps / 2
 
 
+def _small_steps(x, y, z, log_decay, scale, seq_lens, backwards):
+    """What fp16's smallest step adds to the bound of A(x, y, z).  A pair's score, or the pair's part of y' in the state, is off by up to
+    2^-25 (half that step) where it lies below the normal numbers, and never by more than it is: min(pair, 2^-25 (1 + scale |x|_1)) |z|
+    summed over the pairs; the state's own 16-bit terms are off by 2^-25 an element: 2^-25 |x|_1 (1 or scale)."""
+    u = 2.0 ** -25
+    out = torch.zeros_like(x)
+    for b in range(x.shape[0]):
+        n = x.shape[2] if seq_lens is None else max(0, min(x.shape[2], int(seq_lens[b])))
+        xb, yb, zb = x[b, :, :n].abs(), y[b, :, :n].abs(), z[b, :, :n].abs()
+        w = _weights(log_decay, n, x.device)
+        w = w.transpose(-1, -2) if backwards else w
+        length = xb.sum(-1, keepdim=True)
+        pair = scale * (xb @ yb.transpose(-1, -2)) * w
+        out[b, :, :n] = torch.minimum(pair, u * (1 + scale * length)) @ zb + u * max(1.0, scale) * length
+    return out
+
+
+def _small_state_steps(y, z, log_decay, scale, seq_lens, backwards):
+    """The same of the sum of weight * y z^T: min(weight |y|, 2^-25) |z|."""
+    out = []
+    for b in range(y.shape[0]):
+        n = y.shape[2] if seq_lens is None else max(0, min(y.shape[2], int(seq_lens[b])))
+        at = torch.arange(n, dtype=torch.float64, device=y.device)
+        w = torch.exp(log_decay.double().clamp(min=-1e30)[:, None] * (at + 1 if backwards else n - 1 - at)[None]).unsqueeze(-1)
+        out.append(scale * (y[b, :, :n].abs() * w).clamp(max=2.0 ** -25).transpose(-1, -2) @ z[b, :, :n].abs())
+    return torch.stack(out)
+
+
 def decay_bounds(q, k, v, d, log_decay, scale, initial_state, d_state, seq_lens, dtype):
     """How far the kernels' (out, state, dq, dk, dv, d_initial) may be off, element by element, given the float64 inputs.
 
     Every output is a sum of products of three factors (a pair of rows) or four (with a weight); `mass` is the same sum of absolute values.
     A float32 sum of n terms in any order is off by at most n 2^-24 mass; the tensor cores cut off where others round, two half
     steps.  n is at most the head size, the rows of a chunk and the number of chunks, as a sum of sums.  16-bit calls round each
-    pair's score, or the key's part of the state, once to their type (half a step of mass), and the result once."""
+    pair's score, or the key's part of the state, once to their type (half a step of mass), and the result once; fp16 has a smallest step
+    on top (_small_steps)."""
     a = lambda t: None if t is None else t.abs()  # noqa: E731
     D, N = q.shape[-1], q.shape[2]
     n = 2 * (D + 128 + N / 64 + 8) * 2.0 ** -24
     qa, ka, va = (a(t).requires_grad_(True) for t in (q, k, v))
     ia = None if initial_state is None else a(initial_state).requires_grad_(True)
-    out, state = decay_attention(qa, ka, va, log_decay, abs(scale), ia, seq_lens)
+    scale = abs(scale)
+    out, state = decay_attention(qa, ka, va, log_decay, scale, ia, seq_lens)
     grads = [None] * 4
     if d is not None:
         wanted = [qa, ka, va] + ([ia] if ia is not None else [])
         top = (out * a(d)).sum() + (0 if d_state is None else (state * a(d_state)).sum())
         grads = list(torch.autograd.grad(top, wanted, allow_unused=True)) + [None] * (4 - len(wanted))
     u = half_step(dtype) if dtype != torch.float32 else 0.0
-    big = lambda t: None if t is None else (n + 1.01 * u) * t.detach() + 2.0 ** -24 * (dtype == torch.float16)  # noqa: E731
+    big = lambda t: None if t is None else (n + 1.01 * u) * t.detach()  # noqa: E731
     small = lambda t: None if t is None else n * t.detach()  # noqa: E731
-    return big(out), small(state), big(grads[0]), big(grads[1]), big(grads[2]), small(grads[3])
+    bounds = [big(out), small(state), big(grads[0]), big(grads[1]), big(grads[2]), small(grads[3])]
+    if dtype == torch.float16:
+        forms = [(0, (q, k, v), False)] + ([(2, (d, v, k), False), (3, (v, d, q), True), (4, (k, q, d), True)] if d is not None else [])
+        for i, f, backwards in forms:
+            bounds[i] = bounds[i] + _small_steps(*f, log_decay, scale, seq_lens, backwards)
+        bounds[1] = bounds[1] + _small_state_steps(k, v, log_decay, 1.0, seq_lens, False)
+        if bounds[5] is not None:
+            bounds[5] = bounds[5] + _small_state_steps(q, d, log_decay, scale, seq_lens, True)
+    return bounds
 
 
 def within(got, ref, bound, dtype):
