@@ -1,7 +1,7 @@
 // Causal attention with a decay on the tensor cores (fp16 / bf16): out = A(x, y, z) of decay_kernels.cuh, C rows at a time, and the
 // sums of y z^T over runs of rows that join the segments of a sequence.
 //
-// Per chunk, with S the state that enters it (FP32, in registers):
+// Per chunk, with S the state that enters it (FP32):
 //     P = x y^T (C x C)             -> times exp(g |s - t|) and the mask, rounded to 16 bits
 //     out = P z + exp(g (s + 1)) x S
 //     S = exp(g C) S + y'^T z,      y' = exp(g (C - 1 - t)) y, as the sum of two or three 16-bit terms
@@ -51,27 +51,52 @@ struct DecayTcParams {
   int* status;
 };
 
+// two FP32 values in one instruction
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
+  return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)), "l"(*reinterpret_cast<uint64_t*>(&c)));
+  return *reinterpret_cast<float2*>(&d);
+}
+template <class T> __device__ __forceinline__ float2 unpack2(uint32_t u);
+template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t u) { return __half22float2(*reinterpret_cast<__half2*>(&u)); }
+template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t u) {
+  return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
+// 16 values, TERMS of them 16-bit: term t holds what the terms before it leave
+template <class T, int TERMS, int N>
+__device__ __forceinline__ void split_terms(float2* f, uint32_t (*terms)[N]) {
+#pragma unroll
+  for (int t = 0; t < TERMS; ++t)
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      terms[t][j] = pack2<T>(f[j].x, f[j].y);
+      if (t + 1 < TERMS) f[j] = fma2(unpack2<T>(terms[t][j]), make_float2(-1.f, -1.f), f[j]);
+    }
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const float* v) {
+  const uint32_t* r = reinterpret_cast<const uint32_t*>(v);
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+               ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+               "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+               : "memory");
+}
+
 // y' for 16 bytes (eight elements) of one row, as TERMS 16-bit terms
 template <class T, int TERMS>
 __device__ __forceinline__ void scaled_terms(uint4 raw, float w, uint4* terms) {
-  const T* e = reinterpret_cast<const T*>(&raw);
-  float f[8];
+  const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
+  float2 f[4];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) f[j] = to_f<T>(e[j]) * w;
+  for (int j = 0; j < 4; ++j) f[j] = mul2(unpack2<T>(u[j]), make_float2(w, w));
+  uint32_t t[TERMS][4];
+  split_terms<T, TERMS, 4>(f, t);
 #pragma unroll
-  for (int t = 0; t < TERMS; ++t) {
-    uint32_t u[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      u[j] = pack2<T>(f[2 * j], f[2 * j + 1]);
-      if (t + 1 < TERMS) {
-        const T* h = reinterpret_cast<const T*>(&u[j]);
-        f[2 * j] -= to_f<T>(h[0]);
-        f[2 * j + 1] -= to_f<T>(h[1]);
-      }
-    }
-    terms[t] = make_uint4(u[0], u[1], u[2], u[3]);
-  }
+  for (int k = 0; k < TERMS; ++k) terms[k] = make_uint4(t[k][0], t[k][1], t[k][2], t[k][3]);
 }
 
 // ---- sums over runs ------------------------------------------------------------------------------------------
@@ -261,8 +286,8 @@ template <int D> struct MainCfg {
   static constexpr int kP = C * C * 2 > kTile ? C * C * 2 : kTile;      // scores, then the output tile
   static constexpr int kS = D * D * 2;
   static constexpr int kThreads = 2 * kGroup + 64;
-  static constexpr int kBytes = 1024 + kStages * 3 * kTile + kP + 2 * kTile + 2 * kS + (C + 1) * 4 + 80 + 256;
-  static constexpr int kPcol = 0, kIntra = C, kInter = C + D, kU = C + 2 * D;      // tensor-memory columns
+  static constexpr int kBytes = 1024 + kStages * 3 * kTile + kP + 2 * kTile + 2 * kS + (C + 8) * 4 + 64 + 80 + 256;
+  static constexpr int kPcol = 0, kIntra = C, kInter = C + D, kState = C + 2 * D;      // tensor-memory columns
 };
 
 template <class T, int D, bool REV>
@@ -279,7 +304,8 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
   uint8_t* s_y = s_p + L::kP;                         // two terms of y'
   uint8_t* s_s = s_y + 2 * L::kTile;                  // two terms of S
   float* pw = reinterpret_cast<float*>(s_s + 2 * L::kS);
-  float* s_mul = pw + C + 1;                          // [2]: what x S is to be multiplied by, by chunk parity
+  float* rpw = pw + C + 4;                            // [16]: exp(g (15 - j))
+  float* s_mul = rpw + 16;                            // [2]: what x S is to be multiplied by, by chunk parity
   float* s_max = s_mul + 2;                           // [16]
   uint64_t* bars = reinterpret_cast<uint64_t*>((reinterpret_cast<uintptr_t>(s_max + 16) + 15) & ~(uintptr_t)15);
   uint64_t* full = bars;             // [3]
@@ -316,7 +342,10 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
   const int64_t r1 = r0 + p.seg_rows < p.N ? r0 + p.seg_rows : p.N;
   const int64_t end = r1 < len ? r1 : len;
   const double g = decay_log(p.log_decay[h]);
-  for (int i = threadIdx.x; i <= C; i += L::kThreads) pw[i] = (float)exp(g * i);
+  for (int i = threadIdx.x; i <= C; i += L::kThreads) {
+    pw[i] = (float)exp(g * i);
+    if (i < 16) rpw[15 - i] = pw[i];
+  }
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
@@ -371,16 +400,6 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
       for (int i = 0; ok && i < count; ++i) {
         asm volatile("" : "+r"(a_p), "+r"(a_y), "+r"(a_s));      // (descriptors are formed here, not kept over the loop in registers there are not)
         const uint32_t a_x = smem_u32(s_in + (i % NST) * 3 * L::kTile), a_z = a_x + 2 * L::kTile;
-        if (i + 1 < count) {
-          if (!mbar_wait(y_ready, i & 1, ab, 0x8500 + i)) break;
-          tc_fence_after();
-#pragma unroll
-          for (int t = 1; t >= 0; --t)
-#pragma unroll
-            for (int k = 0; k < C / 16; ++k)
-              umma(tmem + L::kU, along_rows(a_y + t * L::kTile, k, C), along_rows(a_z, k, C), i_u, !(t == 1 && k == 0));
-          umma_commit(u_full);
-        }
         if (!mbar_wait(s_ready, i & 1, ab, 0x8600 + i)) break;
         if (i > 0 && !mbar_wait(o_free, (i - 1) & 1, ab, 0x8700 + i)) break;
         tc_fence_after();
@@ -390,6 +409,16 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
           for (int k = 0; k < D / 16; ++k)
             umma(tmem + L::kInter, along_row(a_x, k, C), along_rows(a_s + t * L::kS, k, D), i_o, !(t == 1 && k == 0));
         umma_commit(s_done);
+        if (i + 1 < count) {
+          // the state in tensor memory has been decayed by the time its 16-bit terms are ready
+          if (!mbar_wait(y_ready, i & 1, ab, 0x8500 + i)) break;
+          tc_fence_after();
+#pragma unroll
+          for (int t = 1; t >= 0; --t)
+#pragma unroll
+            for (int k = 0; k < C / 16; ++k) umma(tmem + L::kState, along_rows(a_y + t * L::kTile, k, C), along_rows(a_z, k, C), i_u, 1);
+          umma_commit(u_full);
+        }
         if (i + 1 < count) ok = scores(i + 1);
         if (!ok || !mbar_wait(p_ready, i & 1, ab, 0x8800 + i)) break;
         tc_fence_after();
@@ -423,111 +452,104 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
       mbar_wait(p_full, i & 1, ab, 0x8900 + i);
       __syncwarp();
       tc_fence_after();
-      float v[NB][16];
-#pragma unroll
-      for (int n = 0; n < NB; ++n) {
-        const int t0 = (2 * n + half) * 16;
-        if (REV ? t0 + 15 >= w0 : t0 <= w0 + RPW - 1) ld_cols<16>(tmem + L::kPcol + lane_base + t0, v[n]);
-      }
-      tmem_ld_wait();
-      tc_fence_before();
-      mbar_arrive_warp(p_free);
-      float most = 0.f;
-#pragma unroll
-      for (int n = 0; n < NB; ++n) {
-        const int t0 = (2 * n + half) * 16;
-        if (REV ? t0 + 15 < w0 : t0 > w0 + RPW - 1) {
-#pragma unroll
-          for (int j = 0; j < 16; ++j) v[n][j] = 0.f;
-        } else if (REV ? t0 >= w0 + RPW - 1 : t0 + 15 <= w0) {
-          // the whole block lies behind the rows: exp(g d) as a row's factor times a column's
-          const float row = p.scale * pw[REV ? t0 - s : s - t0 - 15];
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const float4 c = *reinterpret_cast<const float4*>(pw + 4 * q);
-            v[n][REV ? 4 * q : 15 - 4 * q] *= row * c.x;
-            v[n][REV ? 4 * q + 1 : 14 - 4 * q] *= row * c.y;
-            v[n][REV ? 4 * q + 2 : 13 - 4 * q] *= row * c.z;
-            v[n][REV ? 4 * q + 3 : 12 - 4 * q] *= row * c.w;
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const int d = REV ? t0 + j - s : s - t0 - j;
-            v[n][j] = d >= 0 ? v[n][j] * (p.scale * pw[d < 0 ? 0 : d]) : 0.f;
-          }
-        }
-        if (F16)
-#pragma unroll
-          for (int j = 0; j < 16; ++j) most = fmaxf(most, fabsf(v[n][j]));
-      }
-      // the output tile of the chunk before has left the buffer that the scores go to
-      float up = 1.f;
-      if (threadIdx.x == 0) tma_store_wait_read();
-      if (F16) {
-        // scores past the range of fp16 (rare): the tile goes in divided by a power of two
-        if (named_barrier_or(1, kGroup, owner && most > 32768.f)) {
-          float m = owner && most < INFINITY ? most : 0.f;
-          for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-          if (lane == 0) s_max[warp] = m;
-          named_barrier(1, kGroup);
-          for (int k = 0; k < 8; ++k) m = fmaxf(m, s_max[k]);
-          int e = 0;
-          frexpf(m, &e);
-          up = ldexpf(1.f, max(0, e - 15));
-          const float down = 1.f / up;
-#pragma unroll
-          for (int n = 0; n < NB; ++n)
-#pragma unroll
-            for (int j = 0; j < 16; ++j) v[n][j] *= down;
-          named_barrier(1, kGroup);
-        }
-      } else {
-        named_barrier(1, kGroup);
-      }
-      if (owner) {
+      // scores, weighted and packed; in fp16 again, divided by a power of two, where some leave that type's range (rare)
+      uint32_t pk[NB][8];
+      float up = 1.f, factor = p.scale;
+      for (bool again = false;; again = true) {
+        float most = 0.f;
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
-          const int cc = (2 * n + half) * 2;
+          const int t0 = (2 * n + half) * 16;
+          if (REV ? t0 + 15 < w0 : t0 > w0 + RPW - 1) {
 #pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            const float* e = v[n] + 8 * q;
-            *reinterpret_cast<uint4*>(s_p + ((cc + q) >> 3) * (C * 128) + sw128_offset(s, (cc + q) & 7)) =
-                make_uint4(pack2<T>(e[0], e[1]), pack2<T>(e[2], e[3]), pack2<T>(e[4], e[5]), pack2<T>(e[6], e[7]));
+            for (int j = 0; j < 8; ++j) pk[n][j] = 0u;
+            continue;
+          }
+          float2 v[8];
+          tmem_ld16(tmem + L::kPcol + lane_base + t0, reinterpret_cast<float*>(v));
+          tmem_ld_wait();
+          if (REV ? t0 >= w0 + RPW - 1 : t0 + 15 <= w0) {
+            // the whole block lies behind the rows: exp(g d) as a row's factor times a column's
+            const float row = factor * pw[REV ? t0 - s : s - t0 - 15];
+            const float2* c = reinterpret_cast<const float2*>(REV ? pw : rpw);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = mul2(mul2(v[j], make_float2(row, row)), c[j]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const int d = REV ? t0 + 2 * j - s : s - t0 - 2 * j, e = REV ? d + 1 : d - 1;
+              v[j].x = d >= 0 ? v[j].x * (factor * pw[max(d, 0)]) : 0.f;
+              v[j].y = e >= 0 ? v[j].y * (factor * pw[max(e, 0)]) : 0.f;
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            if (F16) most = fmaxf(most, fmaxf(fabsf(v[j].x), fabsf(v[j].y)));
+            pk[n][j] = pack2<T>(v[j].x, v[j].y);
           }
         }
+        if (again) break;
+        // the output tile of the chunk before has left the buffer that the scores go to
+        if (threadIdx.x == 0) tma_store_wait_read();
+        if (!F16) {
+          named_barrier(1, kGroup);
+          break;
+        }
+        if (!named_barrier_or(1, kGroup, owner && most > 32768.f)) break;
+        float m = owner && most < INFINITY ? most : 0.f;
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if (lane == 0) s_max[warp] = m;
+        named_barrier(1, kGroup);
+        for (int k = 0; k < 8; ++k) m = fmaxf(m, s_max[k]);
+        int e = 0;
+        frexpf(m, &e);
+        up = ldexpf(1.f, max(0, e - 15));
+        factor = p.scale / up;
+        named_barrier(1, kGroup);
+      }
+      tc_fence_before();
+      mbar_arrive_warp(p_free);
+      if (owner) {
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            const int cc = (2 * n + half) * 2 + q;
+            *reinterpret_cast<uint4*>(s_p + (cc >> 3) * (C * 128) + sw128_offset(s, cc & 7)) =
+                make_uint4(pk[n][4 * q], pk[n][4 * q + 1], pk[n][4 * q + 2], pk[n][4 * q + 3]);
+          }
       }
       fence_proxy_async();
       mbar_arrive_warp(p_ready);
       float wi = 0.f;
-      if (REV ? s < nv : true) wi = p.inter * pw[REV ? nv - 1 - s : s + 1];
+      if (REV ? s < nv : true) wi = p.inter * p.sum_scale * pw[REV ? nv - 1 - s : s + 1];
       mbar_wait(o_full, i & 1, ab, 0x8a00 + i);
       __syncwarp();
       tc_fence_after();
       if (F16) wi *= s_mul[i & 1];
 #pragma unroll
-      for (int q = 0; q < D / 64; ++q) {
-        const int col = half * (D / 2) + q * 32;
-        float a[32], e[32];
-        tmem_ld32(tmem + L::kIntra + lane_base + col, a);
-        tmem_ld32(tmem + L::kInter + lane_base + col, e);
+      for (int q = 0; q < D / 32; ++q) {
+        const int col = half * (D / 2) + q * 16;
+        float2 a[8], e[8];
+        tmem_ld16(tmem + L::kIntra + lane_base + col, reinterpret_cast<float*>(a));
+        tmem_ld16(tmem + L::kInter + lane_base + col, reinterpret_cast<float*>(e));
         tmem_ld_wait();
-        if (q == D / 64 - 1) {
+        if (q == D / 32 - 1) {
           tc_fence_before();
           mbar_arrive_warp(o_free);
         }
+        uint32_t u[8];
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          if (F16) a[j] *= up;
-          a[j] = wi == 0.f ? a[j] : fmaf(wi, e[j], a[j]);
+        for (int j = 0; j < 8; ++j) {
+          if (F16) a[j] = mul2(a[j], make_float2(up, up));
+          if (wi != 0.f) a[j] = fma2(e[j], make_float2(wi, wi), a[j]);
+          u[j] = pack2<T>(a[j].x, a[j].y);
         }
         if (owner) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
+          for (int k = 0; k < 2; ++k) {
             const int cc = (col >> 3) + k;
-            *reinterpret_cast<uint4*>(s_p + (cc >> 3) * (C * 128) + sw128_offset(s, cc & 7)) =
-                make_uint4(pack2<T>(a[8 * k], a[8 * k + 1]), pack2<T>(a[8 * k + 2], a[8 * k + 3]), pack2<T>(a[8 * k + 4], a[8 * k + 5]),
-                           pack2<T>(a[8 * k + 6], a[8 * k + 7]));
+            *reinterpret_cast<uint4*>(s_p + (cc >> 3) * (C * 128) + sw128_offset(s, cc & 7)) = make_uint4(u[4 * k], u[4 * k + 1], u[4 * k + 2], u[4 * k + 3]);
           }
         }
       }
@@ -548,22 +570,36 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
     constexpr int HC = D / 2;
     // (only the last chunk in space is not whole: backwards in time the first, forwards one whose state nobody needs)
     const DecayPair full_chunk = decay_pair(g, C), first_chunk = REV && count > 0 ? decay_pair(g, end - row_of(0)) : full_chunk;
-    float S[HC];
+    const uint32_t t_state = tmem + L::kState + lane_base + half * HC;
+    // 16 columns of the state that enters chunk i, as the products have left it (the first: as it enters the segment; without the factor of the sums)
+    const auto piece = [&](int i, int q, float* f) {
+      if (i > 0) {
+        tmem_ld16(t_state + q * 16, f);
+        tmem_ld_wait();
+        return;
+      }
+      const float mul = 1.f / p.sum_scale;
 #pragma unroll
-    for (int j = 0; j < HC; ++j) {
-      const int col = half * HC + j;
-      S[j] = 0.f;
-      if (p.state_in && owner && row < p.Dr && col < p.Dr)
-        S[j] = p.state_in[((size_t)bh * p.ncut + cut) * p.Dr * p.Dr + (p.transposed ? col * p.Dr + row : row * p.Dr + col)];
-    }
-    // S as two 16-bit terms; in fp16 divided by a power of two where it would leave the range
+      for (int j = 0; j < 16; ++j) {
+        const int col = half * HC + q * 16 + j;
+        f[j] = 0.f;
+        if (p.state_in && owner && row < p.Dr && col < p.Dr)
+          f[j] = mul * p.state_in[((size_t)bh * p.ncut + cut) * p.Dr * p.Dr + (p.transposed ? col * p.Dr + row : row * p.Dr + col)];
+      }
+    };
+    // The state as two 16-bit terms for x S (in fp16 divided by a power of two where it would leave the range), and, decayed by the chunk's
+    // rows, back to tensor memory, where y'^T z is added to it.
     const auto put_state = [&](int i) {
       float down = 1.f;
       if (F16) {
-        float most = 0.f;
+        float most = 0.f, up = 1.f;
+#pragma unroll 1
+        for (int q = 0; q < HC / 16; ++q) {
+          float f[16];
+          piece(i, q, f);
 #pragma unroll
-        for (int j = 0; j < HC; ++j) most = fmaxf(most, fabsf(S[j]));
-        float up = 1.f;
+          for (int j = 0; j < 16; ++j) most = fmaxf(most, fabsf(f[j]));
+        }
         if (named_barrier_or(2, kGroup, owner && most > 32768.f)) {
           float m = owner && most < INFINITY ? most : 0.f;
           for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -578,25 +614,34 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
         }
         if (tid == 0) s_mul[i & 1] = up;
       }
-      if (owner) {
+      const DecayPair w = i == 0 ? first_chunk : full_chunk;
 #pragma unroll
-        for (int k = 0; k < HC / 8; ++k) {
-          float f[8];
-          uint32_t hi[4], lo[4];
+      for (int q = 0; q < HC / 16; ++q) {
+        float2 f[8];
+        piece(i, q, reinterpret_cast<float*>(f));
+        if (i + 1 < count) {
+          float d[16];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) f[j] = F16 ? S[8 * k + j] * down : S[8 * k + j];
+          for (int j = 0; j < 8; ++j) { d[2 * j] = decay_by(w, f[j].x); d[2 * j + 1] = decay_by(w, f[j].y); }
+          tmem_st16(t_state + q * 16, d);
+        }
+        if (F16)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            hi[j] = pack2<T>(f[2 * j], f[2 * j + 1]);
-            const T* e = reinterpret_cast<const T*>(&hi[j]);
-            lo[j] = pack2<T>(f[2 * j] - to_f<T>(e[0]), f[2 * j + 1] - to_f<T>(e[1]));
+          for (int j = 0; j < 8; ++j) f[j] = mul2(f[j], make_float2(down, down));
+        uint32_t t[2][8];
+        split_terms<T, 2, 8>(f, t);
+        if (owner) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const int cc = (half * HC >> 3) + 2 * q + k;
+            const uint32_t off = (cc >> 3) * (D * 128) + sw128_offset(row, cc & 7);
+            *reinterpret_cast<uint4*>(s_s + off) = make_uint4(t[0][4 * k], t[0][4 * k + 1], t[0][4 * k + 2], t[0][4 * k + 3]);
+            *reinterpret_cast<uint4*>(s_s + L::kS + off) = make_uint4(t[1][4 * k], t[1][4 * k + 1], t[1][4 * k + 2], t[1][4 * k + 3]);
           }
-          const int cc = (half * HC >> 3) + k;
-          const uint32_t off = (cc >> 3) * (D * 128) + sw128_offset(row, cc & 7);
-          *reinterpret_cast<uint4*>(s_s + off) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-          *reinterpret_cast<uint4*>(s_s + L::kS + off) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
       }
+      tmem_st_wait();
+      tc_fence_before();
       fence_proxy_async();
       mbar_arrive_warp(s_ready);
     };
@@ -630,20 +675,9 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
       fence_proxy_async();
       mbar_arrive_warp(y_ready);
       mbar_wait(u_full, i & 1, ab, 0x8d00 + i);
-      __syncwarp();
-      tc_fence_after();
-      const DecayPair w = i == 0 ? first_chunk : full_chunk;
-#pragma unroll
-      for (int q = 0; q < HC / 16; ++q) {
-        float U[16];
-        tmem_ld16(tmem + L::kU + lane_base + half * HC + q * 16, U);
-        tmem_ld_wait();
-#pragma unroll
-        for (int j = 0; j < 16; ++j) S[q * 16 + j] = decay_by(w, S[q * 16 + j]) + p.sum_scale * U[j];
-      }
-      tc_fence_before();
       mbar_wait(s_done, i & 1, ab, 0x8e00 + i);
       __syncwarp();
+      tc_fence_after();
       put_state(i + 1);
     }
   }
