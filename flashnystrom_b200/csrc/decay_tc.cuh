@@ -4,9 +4,10 @@
 // Per chunk, with S the state that enters it (FP32):
 //     P = x y^T (C x C)             -> times exp(g |s - t|) and the mask, rounded to 16 bits
 //     out = P z + exp(g (s + 1)) x S
-//     S = exp(g C) S + y'^T z,      y' = exp(g (C - 1 - t)) y, as the sum of two or three 16-bit terms
-// S takes part in x S as the sum of two 16-bit terms.  So each term of an output is rounded once on its way (its score, to 16 bits)
-// and the output once; the state keeps 16 to 24 bits.
+//     S = exp(g C) S + y'^T z,      y' = exp(g (C - 1 - t)) y, as one 16-bit term for the outputs, as two or three
+//                                                                 for the sums that join segments and for the state that is handed out
+// S takes part in x S as the sum of two 16-bit terms.  So each term of an output is rounded once on its way to 16 bits (its score inside a chunk, its y'
+// outside), and the output once.
 #pragma once
 #include "common.cuh"
 #include "decay_kernels.cuh"
@@ -277,60 +278,78 @@ decay_tc_sums_kernel(const __grid_constant__ CUtensorMap tm_y, const __grid_cons
 }
 
 // ---- outputs -------------------------------------------------------------------------------------------------
-// One CTA a segment, one CTA an SM, 18 warps: group A (warps 0-7) turns P into its 16-bit operand and takes the output tile out, group B (8-15) forms
-// y' and carries the state, warp 16 loads, warp 17 issues.  The two groups meet only in what the products need: while A works on the scores of a
-// chunk, B is at the state behind it.  C = 128 rows for heads of up to 64 and 64 for 128: what the state's operands leave room for.
+// One CTA a segment, one CTA an SM, 19 warps, chunks of 128 rows: group A (warps 0-7) turns P into its 16-bit operand and takes the output
+// tile out, group B (8-15) forms y' and carries the state, one warp loads, one issues the products of A and one those of B.  The two groups meet
+// only in what the products need: while A works on the scores of a chunk, B is at the state behind it.
+//
+// Shared memory's bandwidth is what there is least of (every operand of a product passes it), so P goes to its product through tensor memory, y' takes
+// y's own place, and the output tile x's.  The state stays in tensor memory: B takes it out to form its two 16-bit terms, puts it back decayed, and the
+// products add y'^T z to it.
+constexpr int kC = 128;      // rows of a chunk
 template <int D> struct MainCfg {
-  static constexpr int C = D == 64 ? 128 : 64, kStages = D == 64 ? 3 : 2;
-  static constexpr int kTile = C * D * 2;                                // 16 KB
-  static constexpr int kP = C * C * 2 > kTile ? C * C * 2 : kTile;      // scores, then the output tile
-  static constexpr int kS = D * D * 2;
-  static constexpr int kThreads = 2 * kGroup + 64;
-  static constexpr int kBytes = 1024 + kStages * 3 * kTile + kP + 2 * kTile + 2 * kS + (C + 8) * 4 + 64 + 80 + 256;
-  static constexpr int kPcol = 0, kIntra = C, kInter = C + D, kState = C + 2 * D;      // tensor-memory columns
+  static constexpr int kTile = kC * D * 2;
+  static constexpr int kS = D * D * 2;                                   // one term of the state
+  static constexpr int kSlots = D == 64 ? 12 : 5;                        // tiles in flight, in the order y, x, z of the chunks
+  static constexpr int kInters = D == 64 ? 2 : 1;                        // accumulators of x S
+  static constexpr int kThreads = 2 * kGroup + 96;
+  static constexpr int kBytes = 1024 + kSlots * kTile + 2 * kS + (kC + 4) * 4 + 64 + 80 + 512;
+  // Tensor-memory columns.  The packed scores of columns 0-63 begin at kPacked, those of 64-127 kPackedHalf behind; with heads of 128 they take the place
+  // of the scores that they come from, a thread's own.
+  static constexpr int kScores = 0, kPacked = D == 64 ? 128 : 0, kPackedHalf = D == 64 ? 32 : 64, kIntra = D == 64 ? 192 : 128, kInter = 256, kState = 384;
 };
+// D[tmem] (+)= A[tmem] * B[smem]
+__device__ __forceinline__ void umma_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
 
 template <class T, int D, bool REV>
 __global__ void __launch_bounds__(MainCfg<D>::kThreads, 1)
 decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_y, const __grid_constant__ CUtensorMap tm_z,
                 const __grid_constant__ CUtensorMap tm_o, DecayTcParams p) {
   using L = MainCfg<D>;
-  constexpr int C = L::C, NST = L::kStages, KB = D / 64, RPW = C / 4;      // rows of a tile that one warp's lanes hold
+  constexpr int C = kC, NS = L::kSlots, KB = D / 64, NI = L::kInters;
   constexpr bool F16 = UmmaFmt<T>::v == 0;
   extern __shared__ uint8_t smem_raw[];
   pdl_trigger();
-  uint8_t* s_in = at1024(smem_raw);                   // stages of [x | y | z]
-  uint8_t* s_p = s_in + NST * 3 * L::kTile;
-  uint8_t* s_y = s_p + L::kP;                         // two terms of y'
-  uint8_t* s_s = s_y + 2 * L::kTile;                  // two terms of S
+  uint8_t* s_in = at1024(smem_raw);
+  uint8_t* s_s = s_in + NS * L::kTile;                // two terms of S
   float* pw = reinterpret_cast<float*>(s_s + 2 * L::kS);
   float* rpw = pw + C + 4;                            // [16]: exp(g (15 - j))
-  float* s_mul = rpw + 16;                            // [2]: what x S is to be multiplied by, by chunk parity
-  float* s_max = s_mul + 2;                           // [16]
+  float* s_mul = rpw + 16;                            // [4]: what x S of chunk i is to be multiplied by, in s_mul[i & 3] (B may be two ahead)
+  float* s_max = s_mul + 4;                           // [16]
   uint64_t* bars = reinterpret_cast<uint64_t*>((reinterpret_cast<uintptr_t>(s_max + 16) + 15) & ~(uintptr_t)15);
-  uint64_t* full = bars;             // [3]
-  uint64_t* empty = bars + 3;        // [3]
-  uint64_t* p_full = bars + 6;
-  uint64_t* p_free = bars + 7;
-  uint64_t* p_ready = bars + 8;
-  uint64_t* o_full = bars + 9;
-  uint64_t* o_free = bars + 10;
-  uint64_t* y_ready = bars + 11;
-  uint64_t* u_full = bars + 12;
-  uint64_t* s_ready = bars + 13;
-  uint64_t* s_done = bars + 14;
-  uint64_t* clean = bars + 15;
-  uint64_t* fin = bars + 16;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 17);
+  uint64_t* full = bars;             // [NS]
+  uint64_t* empty = full + NS;       // [NS]
+  uint64_t* p_full = empty + NS;     // [4]: scores of chunk i in p_full[i & 3]; B waits for them too and may be two chunks behind
+  uint64_t* p_free = p_full + 4;
+  uint64_t* p_ready = p_free + 1;
+  uint64_t* o_full = p_free + 2;
+  uint64_t* o_free = p_free + 3;
+  uint64_t* y_ready = p_free + 4;
+  uint64_t* u_full = p_free + 5;
+  uint64_t* s_ready = p_free + 6;
+  uint64_t* s_done = p_free + 7;
+  uint64_t* clean = p_free + 8;
+  uint64_t* fin = p_free + 9;        // [2]
+  uint64_t* i_full = p_free + 11;    // [2], by accumulator
+  uint64_t* i_free = p_free + 13;    // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(p_free + 15);
   int* abort_word = reinterpret_cast<int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int bh = blockIdx.x / p.ncut, cut = blockIdx.x % p.ncut, b = bh / p.H, h = bh % p.H;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < NST; ++i) { mbar_init(full + i, 1); mbar_init(empty + i, 1); }
-    mbar_init(p_full, 1); mbar_init(p_free, kGroup / 32); mbar_init(p_ready, kGroup / 32); mbar_init(o_full, 1); mbar_init(o_free, kGroup / 32);
+    for (int i = 0; i < NS; ++i) { mbar_init(full + i, 1); mbar_init(empty + i, 2); }
+    for (int i = 0; i < 4; ++i) mbar_init(p_full + i, 1);
+    mbar_init(p_free, kGroup / 32); mbar_init(p_ready, kGroup / 32); mbar_init(o_full, 1); mbar_init(o_free, kGroup / 32);
     mbar_init(y_ready, kGroup / 32); mbar_init(u_full, 1); mbar_init(s_ready, kGroup / 32); mbar_init(s_done, 1);
-    mbar_init(clean, kGroup / 32); mbar_init(fin, 1);
+    mbar_init(clean, kGroup / 32);
+    for (int i = 0; i < 2; ++i) { mbar_init(fin + i, 1); mbar_init(i_full + i, 1); mbar_init(i_free + i, kGroup / 32); }
     *abort_word = 0;
     fence_mbar_init();
   }
@@ -354,6 +373,8 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
   const auto row_of = [&](int i) { return r0 + (int64_t)(REV ? count - 1 - i : i) * C; };
   // The last rows of a tile lie past the sequence's length, but not past the tensor: they hold anything, and are cleared.
   const int dirty = end == len && len < p.N && (end - r0) % C != 0 ? (REV ? 0 : count - 1) : -1;
+  const auto tile = [&](int n) { return s_in + (n % NS) * L::kTile; };      // n = 3 i + 0, 1, 2: y, x, z of chunk i
+  const auto landed = [&](int n, int where) { return mbar_wait(full + n % NS, (n / NS) & 1, ab, where + n); };
 
   if (warp == 16) {
     if (lane == 0 && count > 0) {
@@ -362,82 +383,93 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
       tma_prefetch_desc(&tm_z);
       tma_prefetch_desc(&tm_o);
       int armed = 0;
-      for (int i = 0; i < count; ++i) {
-        const int st = i % NST;
-        if (!mbar_wait(empty + st, ((i / NST) & 1) ^ 1, ab, 0x8100 + i)) break;
-        mbar_expect_tx(full + st, 3 * L::kTile);
-        uint8_t* to = s_in + st * 3 * L::kTile;
-        for (int kb = 0; kb < KB; ++kb) {
-          tma_load_4d_h(to + kb * (C * 128), &tm_x, full + st, kb * 64, (int)row_of(i), h, b, 0);
-          tma_load_4d_h(to + L::kTile + kb * (C * 128), &tm_y, full + st, kb * 64, (int)row_of(i), h, b, 0);
-        }
-        for (int kb = 0; kb < KB; ++kb)
-          tma_load_4d_h(to + 2 * L::kTile + kb * (C * 128), &tm_z, full + st, kb * 64, (int)row_of(i), h, b, 0);
-        armed = i + 1;
+      for (int n = 0; n < 3 * count; ++n) {
+        if (!mbar_wait(empty + n % NS, ((n / NS) & 1) ^ 1, ab, 0x8100 + n)) break;
+        mbar_expect_tx(full + n % NS, L::kTile);
+        const CUtensorMap* m = n % 3 == 0 ? &tm_y : n % 3 == 1 ? &tm_x : &tm_z;
+        for (int kb = 0; kb < KB; ++kb) tma_load_4d_h(tile(n) + kb * (C * 128), m, full + n % NS, kb * 64, (int)row_of(n / 3), h, b, 0);
+        armed = n + 1;
       }
       if (ab.raised())
-        for (int i = max(0, armed - NST); i < armed; ++i) mbar_drain(full + i % NST, (i / NST) & 1);
+        for (int n = max(0, armed - NS); n < armed; ++n) mbar_drain(full + n % NS, (n / NS) & 1);
     }
   } else if (warp == 17) {
+    // ---- products of group A: scores a chunk ahead, then P z
     if (lane == 0 && count > 0) {
-      constexpr uint32_t i_p = make_idesc<T>(C, C, false, false);       // x y^T
-      constexpr uint32_t i_o = make_idesc<T>(C, D, false, true);        // P z, x S
-      constexpr uint32_t i_u = make_idesc<T>(D, D, true, true);         // y'^T z
-      uint32_t a_p = smem_u32(s_p), a_y = smem_u32(s_y), a_s = smem_u32(s_s);
+      constexpr uint32_t i_p = make_idesc<T>(C, C, false, false), i_o = make_idesc<T>(C, D, false, true);
       const auto scores = [&](int i) -> bool {
-        const int st = i % NST;
-        if (!mbar_wait(full + st, (i / NST) & 1, ab, 0x8200 + i)) return false;
+        if (!landed(3 * i, 0x8200) || !landed(3 * i + 1, 0x8200)) return false;
         if (i == dirty && !mbar_wait(clean, 0, ab, 0x8300 + i)) return false;
-        if (i > 0 && !mbar_wait(p_free, (i - 1) & 1, ab, 0x8400 + i)) return false;
+        if (i > 0) {
+          // (where the packed scores lie among them, the product that reads these has to be done)
+          if (!(D == 64 ? mbar_wait(p_free, (i - 1) & 1, ab, 0x8400 + i) : mbar_wait(o_full, (i - 1) & 1, ab, 0x8400 + i))) return false;
+        }
         tc_fence_after();
-        const uint32_t a_x = smem_u32(s_in + st * 3 * L::kTile);
+        const uint32_t a_y = smem_u32(tile(3 * i)), a_x = smem_u32(tile(3 * i + 1));
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) umma(tmem + L::kPcol, along_row(a_x, k, C), along_row(a_x + L::kTile, k, C), i_p, k > 0);
-        umma_commit(p_full);
+        for (int k = 0; k < D / 16; ++k) umma(tmem + L::kScores, along_row(a_x, k, C), along_row(a_y, k, C), i_p, k > 0);
+        umma_commit(p_full + (i & 3));
         return true;
       };
       bool ok = scores(0);
       for (int i = 0; ok && i < count; ++i) {
-        asm volatile("" : "+r"(a_p), "+r"(a_y), "+r"(a_s));      // (descriptors are formed here, not kept over the loop in registers there are not)
-        const uint32_t a_x = smem_u32(s_in + (i % NST) * 3 * L::kTile), a_z = a_x + 2 * L::kTile;
-        if (!mbar_wait(s_ready, i & 1, ab, 0x8600 + i)) break;
+        if (D == 64 && i + 1 < count) ok = scores(i + 1);
+        if (!ok || !landed(3 * i + 2, 0x8880) || !mbar_wait(p_ready, i & 1, ab, 0x8800 + i)) break;
         if (i > 0 && !mbar_wait(o_free, (i - 1) & 1, ab, 0x8700 + i)) break;
         tc_fence_after();
+        const uint32_t a_z = smem_u32(tile(3 * i + 2));
+#pragma unroll
+        for (int k = 0; k < C / 16; ++k) umma_ta(tmem + L::kIntra, tmem + L::kPacked + (k >> 2) * L::kPackedHalf + 8 * (k & 3), along_rows(a_z, k, C), i_o, k > 0);
+        umma_commit(o_full);
+        umma_commit(empty + (3 * i + 2) % NS);
+        if (D == 128 && i + 1 < count) ok = scores(i + 1);
+      }
+      umma_commit(fin);          // nothing of the CTA is given back while a product runs
+      mbar_drain(fin, 0);
+    }
+  } else if (warp == 18) {
+    // ---- products of group B: the state's own, and x S
+    if (lane == 0 && count > 0) {
+      constexpr uint32_t i_o = make_idesc<T>(C, D, false, true), i_u = make_idesc<T>(D, D, true, true);
+      uint32_t a_s = smem_u32(s_s);
+      for (int i = 0; i < count; ++i) {
+        asm volatile("" : "+r"(a_s));      // (descriptors are formed here, not kept over the loop in registers there are not)
+        const int ia = i % NI;
+        if (!landed(3 * i + 1, 0x8580)) break;
+        if (i == dirty && !mbar_wait(clean, 0, ab, 0x8590 + i)) break;
+        if (!mbar_wait(s_ready, i & 1, ab, 0x8600 + i)) break;
+        if (i + 1 < count) {
+          // the state in tensor memory has been decayed by the time its 16-bit terms are ready
+          if (!landed(3 * i + 2, 0x8590) || !mbar_wait(y_ready, i & 1, ab, 0x8500 + i)) break;
+          tc_fence_after();
+          const uint32_t a_y = smem_u32(tile(3 * i)), a_z = smem_u32(tile(3 * i + 2));
+#pragma unroll
+          for (int k = 0; k < C / 16; ++k) umma(tmem + L::kState, along_rows(a_y, k, C), along_rows(a_z, k, C), i_u, 1);
+          umma_commit(u_full);
+          umma_commit(empty + (3 * i) % NS);
+          umma_commit(empty + (3 * i) % NS);
+          umma_commit(empty + (3 * i + 2) % NS);
+        }
+        if (i >= NI && !mbar_wait(i_free + ia, (i / NI - 1) & 1, ab, 0x8780 + i)) break;
+        tc_fence_after();
+        const uint32_t a_x = smem_u32(tile(3 * i + 1));
 #pragma unroll
         for (int t = 1; t >= 0; --t)
 #pragma unroll
           for (int k = 0; k < D / 16; ++k)
-            umma(tmem + L::kInter, along_row(a_x, k, C), along_rows(a_s + t * L::kS, k, D), i_o, !(t == 1 && k == 0));
+            umma(tmem + L::kInter + ia * D, along_row(a_x, k, C), along_rows(a_s + t * L::kS, k, D), i_o, !(t == 1 && k == 0));
         umma_commit(s_done);
-        if (i + 1 < count) {
-          // the state in tensor memory has been decayed by the time its 16-bit terms are ready
-          if (!mbar_wait(y_ready, i & 1, ab, 0x8500 + i)) break;
-          tc_fence_after();
-#pragma unroll
-          for (int t = 1; t >= 0; --t)
-#pragma unroll
-            for (int k = 0; k < C / 16; ++k) umma(tmem + L::kState, along_rows(a_y + t * L::kTile, k, C), along_rows(a_z, k, C), i_u, 1);
-          umma_commit(u_full);
-        }
-        if (i + 1 < count) ok = scores(i + 1);
-        if (!ok || !mbar_wait(p_ready, i & 1, ab, 0x8800 + i)) break;
-        tc_fence_after();
-#pragma unroll
-        for (int k = 0; k < C / 16; ++k) umma(tmem + L::kIntra, along_row(a_p, k, C), along_rows(a_z, k, C), i_o, k > 0);
-        umma_commit(o_full);
-        umma_commit(empty + i % NST);
+        umma_commit(i_full + ia);
       }
-      umma_commit(fin);          // nothing of the CTA is given back while a product runs
-      mbar_drain(fin, 0);
+      umma_commit(fin + 1);
+      mbar_drain(fin + 1, 0);
     }
   } else if (warp < 8) {
     // ---- group A: scores and outputs
     // (here and in group B a wait that gave up does not leave the loop: the warps meet at barriers, and the status word has it)
     const int quarter = warp & 3, half = warp >> 2;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
-    const int w0 = quarter * RPW, s = w0 + (lane & (RPW - 1));
-    const bool owner = lane < RPW;
-    constexpr int NB = C / 32;                     // 16-column blocks of a thread: every other one
+    const int w0 = quarter * 32, s = w0 + lane;
     // rows of the segment past the sequence's length
     {
       const int64_t z0 = r0 + (int64_t)count * C;
@@ -449,94 +481,102 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
     for (int i = 0; i < count; ++i) {
       const int64_t c0 = row_of(i);
       const int nv = end - c0 < C ? (int)(end - c0) : C;
-      mbar_wait(p_full, i & 1, ab, 0x8900 + i);
+      mbar_wait(p_full + (i & 3), (i >> 2) & 1, ab, 0x8900 + i);
       __syncwarp();
       tc_fence_after();
-      // scores, weighted and packed; in fp16 again, divided by a power of two, where some leave that type's range (rare)
-      uint32_t pk[NB][8];
-      float up = 1.f, factor = p.scale;
-      for (bool again = false;; again = true) {
-        float most = 0.f;
+      // Scores, weighted and packed, 16 columns at a time.  In fp16 the largest is looked at first: where some leave that type's range (rare), all go in
+      // divided by a power of two.  (Loops are not unrolled: the warps' ways through this kernel have to share the instruction cache.)
+      const uint32_t t_scores = tmem + L::kScores + lane_base + half * 64, t_packed = tmem + L::kPacked + lane_base + half * L::kPackedHalf;
+      const auto block = [&](int n, float factor, float2* v) {
+        const int t0 = half * 64 + n * 16;
+        tmem_ld16(t_scores + n * 16, reinterpret_cast<float*>(v));
+        tmem_ld_wait();
+        if (REV ? t0 >= w0 + 31 : t0 + 15 <= w0) {
+          // the whole block lies behind the rows: exp(g d) as a row's factor times a column's
+          const float row = factor * pw[REV ? t0 - s : s - t0 - 15];
+          const float4* c = reinterpret_cast<const float4*>(REV ? pw : rpw);
 #pragma unroll
-        for (int n = 0; n < NB; ++n) {
-          const int t0 = (2 * n + half) * 16;
-          if (REV ? t0 + 15 < w0 : t0 > w0 + RPW - 1) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) pk[n][j] = 0u;
-            continue;
+          for (int j = 0; j < 4; ++j) {
+            const float4 f = c[j];
+            v[2 * j] = mul2(mul2(v[2 * j], make_float2(row, row)), make_float2(f.x, f.y));
+            v[2 * j + 1] = mul2(mul2(v[2 * j + 1], make_float2(row, row)), make_float2(f.z, f.w));
           }
-          float2 v[8];
-          tmem_ld16(tmem + L::kPcol + lane_base + t0, reinterpret_cast<float*>(v));
-          tmem_ld_wait();
-          if (REV ? t0 >= w0 + RPW - 1 : t0 + 15 <= w0) {
-            // the whole block lies behind the rows: exp(g d) as a row's factor times a column's
-            const float row = factor * pw[REV ? t0 - s : s - t0 - 15];
-            const float2* c = reinterpret_cast<const float2*>(REV ? pw : rpw);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = mul2(mul2(v[j], make_float2(row, row)), c[j]);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const int d = REV ? t0 + 2 * j - s : s - t0 - 2 * j, e = REV ? d + 1 : d - 1;
-              v[j].x = d >= 0 ? v[j].x * (factor * pw[max(d, 0)]) : 0.f;
-              v[j].y = e >= 0 ? v[j].y * (factor * pw[max(e, 0)]) : 0.f;
-            }
-          }
+        } else {
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            if (F16) most = fmaxf(most, fmaxf(fabsf(v[j].x), fabsf(v[j].y)));
-            pk[n][j] = pack2<T>(v[j].x, v[j].y);
+            const int d = REV ? t0 + 2 * j - s : s - t0 - 2 * j, e = REV ? d + 1 : d - 1;
+            v[j].x = d >= 0 ? v[j].x * (factor * pw[max(d, 0)]) : 0.f;
+            v[j].y = e >= 0 ? v[j].y * (factor * pw[max(e, 0)]) : 0.f;
           }
         }
-        if (again) break;
-        // the output tile of the chunk before has left the buffer that the scores go to
-        if (threadIdx.x == 0) tma_store_wait_read();
-        if (!F16) {
+      };
+      const auto behind = [&](int n) { const int t0 = half * 64 + n * 16; return REV ? t0 + 15 >= w0 : t0 <= w0 + 31; };      // (some of it)
+      float up = 1.f, factor = p.scale;
+      if (F16) {
+        float most = 0.f;
+#pragma unroll 1
+        for (int n = 0; n < 4; ++n)
+          if (behind(n)) {
+            float2 v[8];
+            block(n, factor, v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) most = fmaxf(most, fmaxf(fabsf(v[j].x), fabsf(v[j].y)));
+          }
+        if (named_barrier_or(1, kGroup, most > 32768.f)) {
+          float m = most < INFINITY ? most : 0.f;
+          for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+          if (lane == 0) s_max[warp] = m;
           named_barrier(1, kGroup);
-          break;
+          for (int k = 0; k < 8; ++k) m = fmaxf(m, s_max[k]);
+          int e = 0;
+          frexpf(m, &e);
+          up = ldexpf(1.f, max(0, e - 15));
+          factor = p.scale / up;
+          named_barrier(1, kGroup);
         }
-        if (!named_barrier_or(1, kGroup, owner && most > 32768.f)) break;
-        float m = owner && most < INFINITY ? most : 0.f;
-        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        if (lane == 0) s_max[warp] = m;
-        named_barrier(1, kGroup);
-        for (int k = 0; k < 8; ++k) m = fmaxf(m, s_max[k]);
-        int e = 0;
-        frexpf(m, &e);
-        up = ldexpf(1.f, max(0, e - 15));
-        factor = p.scale / up;
-        named_barrier(1, kGroup);
       }
+#pragma unroll 1
+      for (int n = 0; n < 4; ++n) {
+        uint32_t pk[8];
+        if (behind(n)) {
+          float2 v[8];
+          block(n, factor, v);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) pk[j] = pack2<T>(v[j].x, v[j].y);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) pk[j] = 0u;
+        }
+        tmem_st8(t_packed + n * 8, reinterpret_cast<const float*>(pk));
+      }
+      tmem_st_wait();
       tc_fence_before();
-      mbar_arrive_warp(p_free);
-      if (owner) {
-#pragma unroll
-        for (int n = 0; n < NB; ++n)
-#pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            const int cc = (2 * n + half) * 2 + q;
-            *reinterpret_cast<uint4*>(s_p + (cc >> 3) * (C * 128) + sw128_offset(s, cc & 7)) =
-                make_uint4(pk[n][4 * q], pk[n][4 * q + 1], pk[n][4 * q + 2], pk[n][4 * q + 3]);
-          }
-      }
-      fence_proxy_async();
+      if (D == 64) mbar_arrive_warp(p_free);
       mbar_arrive_warp(p_ready);
+      if (threadIdx.x == 0 && i > 0) {
+        tma_store_wait_read();                         // the output tile of the chunk before has left its place, x's
+        mbar_arrive(empty + (3 * i - 2) % NS);
+        mbar_arrive(empty + (3 * i - 2) % NS);
+      }
       float wi = 0.f;
       if (REV ? s < nv : true) wi = p.inter * p.sum_scale * pw[REV ? nv - 1 - s : s + 1];
+      mbar_wait(i_full + i % NI, (i / NI) & 1, ab, 0x8a80 + i);
       mbar_wait(o_full, i & 1, ab, 0x8a00 + i);
       __syncwarp();
       tc_fence_after();
-      if (F16) wi *= s_mul[i & 1];
-#pragma unroll
+      if (F16) wi *= s_mul[i & 3];
+      uint8_t* to = tile(3 * i + 1);
+#pragma unroll 1
       for (int q = 0; q < D / 32; ++q) {
         const int col = half * (D / 2) + q * 16;
         float2 a[8], e[8];
         tmem_ld16(tmem + L::kIntra + lane_base + col, reinterpret_cast<float*>(a));
-        tmem_ld16(tmem + L::kInter + lane_base + col, reinterpret_cast<float*>(e));
+        tmem_ld16(tmem + L::kInter + (i % NI) * D + lane_base + col, reinterpret_cast<float*>(e));
         tmem_ld_wait();
         if (q == D / 32 - 1) {
           tc_fence_before();
           mbar_arrive_warp(o_free);
+          mbar_arrive_warp(i_free + i % NI);
         }
         uint32_t u[8];
 #pragma unroll
@@ -545,18 +585,16 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
           if (wi != 0.f) a[j] = fma2(e[j], make_float2(wi, wi), a[j]);
           u[j] = pack2<T>(a[j].x, a[j].y);
         }
-        if (owner) {
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const int cc = (col >> 3) + k;
-            *reinterpret_cast<uint4*>(s_p + (cc >> 3) * (C * 128) + sw128_offset(s, cc & 7)) = make_uint4(u[4 * k], u[4 * k + 1], u[4 * k + 2], u[4 * k + 3]);
-          }
+        for (int k = 0; k < 2; ++k) {
+          const int cc = (col >> 3) + k;
+          *reinterpret_cast<uint4*>(to + (cc >> 3) * (C * 128) + sw128_offset(s, cc & 7)) = make_uint4(u[4 * k], u[4 * k + 1], u[4 * k + 2], u[4 * k + 3]);
         }
       }
       fence_proxy_async();
       named_barrier(1, kGroup);
       if (threadIdx.x == 0) {
-        for (int kb = 0; kb < KB; ++kb) tma_store_4d_h(&tm_o, s_p + kb * (C * 128), kb * 64, (int)c0, h, b, 0);
+        for (int kb = 0; kb < KB; ++kb) tma_store_4d_h(&tm_o, to + kb * (C * 128), kb * 64, (int)c0, h, b, 0);
         tma_store_commit();
       }
     }
@@ -571,21 +609,26 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
     // (only the last chunk in space is not whole: backwards in time the first, forwards one whose state nobody needs)
     const DecayPair full_chunk = decay_pair(g, C), first_chunk = REV && count > 0 ? decay_pair(g, end - row_of(0)) : full_chunk;
     const uint32_t t_state = tmem + L::kState + lane_base + half * HC;
-    // 16 columns of the state that enters chunk i, as the products have left it (the first: as it enters the segment; without the factor of the sums)
-    const auto piece = [&](int i, int q, float* f) {
-      if (i > 0) {
-        tmem_ld16(t_state + q * 16, f);
-        tmem_ld_wait();
-        return;
-      }
+    // the state that enters the segment, without the factor of the sums, to tensor memory
+    if (count > 0) {
       const float mul = 1.f / p.sum_scale;
+      const float* from = p.state_in ? p.state_in + ((size_t)bh * p.ncut + cut) * p.Dr * p.Dr + (p.transposed ? row : row * p.Dr) : nullptr;
+      const int step = p.transposed ? p.Dr : 1;
+#pragma unroll 1
+      for (int q = 0; q < HC / 16; ++q) {
+        float f[16];
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const int col = half * HC + q * 16 + j;
-        f[j] = 0.f;
-        if (p.state_in && owner && row < p.Dr && col < p.Dr)
-          f[j] = mul * p.state_in[((size_t)bh * p.ncut + cut) * p.Dr * p.Dr + (p.transposed ? col * p.Dr + row : row * p.Dr + col)];
+        for (int j = 0; j < 16; ++j) {
+          const int col = half * HC + q * 16 + j;
+          f[j] = from && owner && row < p.Dr && col < p.Dr ? mul * from[col * step] : 0.f;
+        }
+        tmem_st16(t_state + q * 16, f);
       }
+      tmem_st_wait();
+    }
+    const auto piece = [&](int q, float* f) {
+      tmem_ld16(t_state + q * 16, f);
+      tmem_ld_wait();
     };
     // The state as two 16-bit terms for x S (in fp16 divided by a power of two where it would leave the range), and, decayed by the chunk's
     // rows, back to tensor memory, where y'^T z is added to it.
@@ -596,7 +639,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
 #pragma unroll 1
         for (int q = 0; q < HC / 16; ++q) {
           float f[16];
-          piece(i, q, f);
+          piece(q, f);
 #pragma unroll
           for (int j = 0; j < 16; ++j) most = fmaxf(most, fabsf(f[j]));
         }
@@ -612,13 +655,13 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
           down = 1.f / up;
           named_barrier(2, kGroup);
         }
-        if (tid == 0) s_mul[i & 1] = up;
+        if (tid == 0) s_mul[i & 3] = up;
       }
       const DecayPair w = i == 0 ? first_chunk : full_chunk;
-#pragma unroll
+#pragma unroll 1
       for (int q = 0; q < HC / 16; ++q) {
         float2 f[8];
-        piece(i, q, reinterpret_cast<float*>(f));
+        piece(q, reinterpret_cast<float*>(f));
         if (i + 1 < count) {
           float d[16];
 #pragma unroll
@@ -647,30 +690,30 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
     };
     if (count > 0) put_state(0);
     for (int i = 0; i < count; ++i) {
-      const int st = i % NST;
       const int64_t c0 = row_of(i);
       const int nv = end - c0 < C ? (int)(end - c0) : C;
-      uint8_t* src = s_in + st * 3 * L::kTile;
       if (i == dirty) {
-        mbar_wait(full + st, (i / NST) & 1, ab, 0x8b00 + i);
-        __syncwarp();
-        for (int idx = tid; idx < 3 * L::kTile / 16; idx += kGroup)
-          if (((idx >> 3) & (C - 1)) >= nv) *reinterpret_cast<uint4*>(src + idx * 16) = make_uint4(0, 0, 0, 0);
+        for (int j = 0; j < 3; ++j) {
+          landed(3 * i + j, 0x8b00);
+          for (int idx = tid; idx < L::kTile / 16; idx += kGroup)
+            if (((idx >> 3) & (C - 1)) >= nv) *reinterpret_cast<uint4*>(tile(3 * i + j) + idx * 16) = make_uint4(0, 0, 0, 0);
+        }
         fence_proxy_async();
         mbar_arrive_warp(clean);
         named_barrier(2, kGroup);
       }
       if (i + 1 == count) break;
-      mbar_wait(full + st, (i / NST) & 1, ab, 0x8c00 + i);
+      // y' takes y's place once the scores have been formed from it
+      landed(3 * i, 0x8c80);
+      mbar_wait(p_full + (i & 3), (i >> 2) & 1, ab, 0x8c00 + i);
       __syncwarp();
-      // (the products that read the terms before are done: u_full of the chunk before has been waited for)
-#pragma unroll
+      uint8_t* src = tile(3 * i);
+#pragma unroll 2
       for (int q = 0; q < L::kTile / 16 / kGroup; ++q) {
         const int idx = tid + q * kGroup, r = (idx >> 3) & (C - 1);
-        uint4 terms[2];
-        scaled_terms<T, 2>(*reinterpret_cast<const uint4*>(src + L::kTile + idx * 16), r < nv ? pw[REV ? r + 1 : nv - 1 - r] : 0.f, terms);
-        *reinterpret_cast<uint4*>(s_y + idx * 16) = terms[0];
-        *reinterpret_cast<uint4*>(s_y + L::kTile + idx * 16) = terms[1];
+        uint4 term;
+        scaled_terms<T, 1>(*reinterpret_cast<const uint4*>(src + idx * 16), r < nv ? pw[REV ? r + 1 : nv - 1 - r] : 0.f, &term);
+        *reinterpret_cast<uint4*>(src + idx * 16) = term;
       }
       fence_proxy_async();
       mbar_arrive_warp(y_ready);

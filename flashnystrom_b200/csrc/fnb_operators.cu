@@ -205,8 +205,8 @@ static int launch_tc_form(const DecayCall& c, const DecayForm& f, const float* s
     constexpr int D = decltype(d)::value;
     using Cfg = dtc::MainCfg<D>;
     CUtensorMap mx, my, mz, mo;
-    if (!make_rows_map(&mx, f.x, c.s, Cfg::C) || !make_rows_map(&my, f.y, c.s, Cfg::C) || !make_rows_map(&mz, f.z, c.s, Cfg::C) ||
-        !make_rows_map(&mo, f.out, c.s, Cfg::C))
+    if (!make_rows_map(&mx, f.x, c.s, dtc::kC) || !make_rows_map(&my, f.y, c.s, dtc::kC) || !make_rows_map(&mz, f.z, c.s, dtc::kC) ||
+        !make_rows_map(&mo, f.out, c.s, dtc::kC))
       return fail(FNB_ERR_CUDA, "cuTensorMapEncodeTiled failed");
     dtc::DecayTcParams p = decay_tc_params(c, REV);
     p.state_in = state_in; p.transposed = f.transposed; p.ncut = c.plan.nseg;
