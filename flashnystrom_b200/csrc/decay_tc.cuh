@@ -297,12 +297,13 @@ template <int D> struct MainCfg {
   // of the scores that they come from, a thread's own.
   static constexpr int kScores = 0, kPacked = D == 64 ? 128 : 0, kPackedHalf = D == 64 ? 32 : 64, kIntra = D == 64 ? 192 : 128, kInter = 256, kState = 384;
 };
-// D[tmem] (+)= A[tmem] * B[smem]
-__device__ __forceinline__ void umma_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+// D[tmem] (+)= A[tmem] * B[smem], from warp-uniform code as umma_elect
+__device__ __forceinline__ void umma_ta_elect(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
       ::"r"(d_tmem), "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
@@ -326,19 +327,18 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
   uint64_t* full = bars;             // [NS]
   uint64_t* empty = full + NS;       // [NS]
   uint64_t* p_full = empty + NS;     // [4]: scores of chunk i in p_full[i & 3]; B waits for them too and may be two chunks behind
-  uint64_t* p_free = p_full + 4;
-  uint64_t* p_ready = p_free + 1;
-  uint64_t* o_full = p_free + 2;
-  uint64_t* o_free = p_free + 3;
-  uint64_t* y_ready = p_free + 4;
-  uint64_t* u_full = p_free + 5;
-  uint64_t* s_ready = p_free + 6;
-  uint64_t* s_done = p_free + 7;
-  uint64_t* clean = p_free + 8;
-  uint64_t* fin = p_free + 9;        // [2]
-  uint64_t* i_full = p_free + 11;    // [2], by accumulator
-  uint64_t* i_free = p_free + 13;    // [2]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(p_free + 15);
+  uint64_t* p_ready = p_full + 4;
+  uint64_t* o_full = p_ready + 1;
+  uint64_t* o_free = p_ready + 2;
+  uint64_t* u_full = p_ready + 3;
+  uint64_t* s_ready = p_ready + 4;
+  uint64_t* s_done = p_ready + 5;
+  uint64_t* clean = p_ready + 6;
+  uint64_t* y_ready = p_ready + 7;    // [2], by chunk parity: B is a chunk ahead with it
+  uint64_t* fin = p_ready + 9;       // [2]
+  uint64_t* i_full = p_ready + 11;    // [2], by accumulator
+  uint64_t* i_free = p_ready + 13;    // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(p_ready + 15);
   int* abort_word = reinterpret_cast<int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -346,10 +346,10 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
   if (threadIdx.x == 0) {
     for (int i = 0; i < NS; ++i) { mbar_init(full + i, 1); mbar_init(empty + i, 2); }
     for (int i = 0; i < 4; ++i) mbar_init(p_full + i, 1);
-    mbar_init(p_free, kGroup / 32); mbar_init(p_ready, kGroup / 32); mbar_init(o_full, 1); mbar_init(o_free, kGroup / 32);
-    mbar_init(y_ready, kGroup / 32); mbar_init(u_full, 1); mbar_init(s_ready, kGroup / 32); mbar_init(s_done, 1);
+    mbar_init(p_ready, kGroup / 32); mbar_init(o_full, 1); mbar_init(o_free, kGroup / 32);
+    mbar_init(u_full, 1); mbar_init(s_ready, kGroup / 32); mbar_init(s_done, 1);
     mbar_init(clean, kGroup / 32);
-    for (int i = 0; i < 2; ++i) { mbar_init(fin + i, 1); mbar_init(i_full + i, 1); mbar_init(i_free + i, kGroup / 32); }
+    for (int i = 0; i < 2; ++i) { mbar_init(fin + i, 1); mbar_init(y_ready + i, kGroup / 32); mbar_init(i_full + i, 1); mbar_init(i_free + i, kGroup / 32); }
     *abort_word = 0;
     fence_mbar_init();
   }
@@ -394,74 +394,76 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
         for (int n = max(0, armed - NS); n < armed; ++n) mbar_drain(full + n % NS, (n / NS) & 1);
     }
   } else if (warp == 17) {
-    // ---- products of group A: scores a chunk ahead, then P z
-    if (lane == 0 && count > 0) {
+    // ---- products of group A: P z, then the scores of the next chunk
+    // (the whole warp walks this code and the next branch's, and one lane issues: descriptors stay in uniform registers, 70 to 100 cycles a product less)
+    if (count > 0) {
       constexpr uint32_t i_p = make_idesc<T>(C, C, false, false), i_o = make_idesc<T>(C, D, false, true);
       const auto scores = [&](int i) -> bool {
-        if (!landed(3 * i, 0x8200) || !landed(3 * i + 1, 0x8200)) return false;
-        if (i == dirty && !mbar_wait(clean, 0, ab, 0x8300 + i)) return false;
-        if (i > 0) {
-          // (where the packed scores lie among them, the product that reads these has to be done)
-          if (!(D == 64 ? mbar_wait(p_free, (i - 1) & 1, ab, 0x8400 + i) : mbar_wait(o_full, (i - 1) & 1, ab, 0x8400 + i))) return false;
-        }
+        bool ok = landed(3 * i, 0x8200) && landed(3 * i + 1, 0x8280);
+        if (i == dirty) ok = ok && mbar_wait(clean, 0, ab, 0x8300 + i);
+        // (where packed scores lie among the scores, the product that reads them has to be done)
+        if (D == 128 && i > 0) ok = ok && mbar_wait(o_full, (i - 1) & 1, ab, 0x8400 + i);
+        if (!__all_sync(0xffffffffu, ok)) return false;
         tc_fence_after();
         const uint32_t a_y = smem_u32(tile(3 * i)), a_x = smem_u32(tile(3 * i + 1));
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) umma(tmem + L::kScores, along_row(a_x, k, C), along_row(a_y, k, C), i_p, k > 0);
-        umma_commit(p_full + (i & 3));
+        for (int k = 0; k < D / 16; ++k) umma_elect(tmem + L::kScores, along_row(a_x, k, C), along_row(a_y, k, C), i_p, k > 0);
+        umma_commit_elect(p_full + (i & 3));
         return true;
       };
-      bool ok = scores(0);
-      for (int i = 0; ok && i < count; ++i) {
-        if (D == 64 && i + 1 < count) ok = scores(i + 1);
-        if (!ok || !landed(3 * i + 2, 0x8880) || !mbar_wait(p_ready, i & 1, ab, 0x8800 + i)) break;
-        if (i > 0 && !mbar_wait(o_free, (i - 1) & 1, ab, 0x8700 + i)) break;
+      bool go = scores(0);
+      for (int i = 0; go && i < count; ++i) {
+        bool ok = landed(3 * i + 2, 0x8880) && mbar_wait(p_ready, i & 1, ab, 0x8800 + i);
+        if (i > 0) ok = ok && mbar_wait(o_free, (i - 1) & 1, ab, 0x8700 + i);
+        if (!__all_sync(0xffffffffu, ok)) break;
         tc_fence_after();
         const uint32_t a_z = smem_u32(tile(3 * i + 2));
 #pragma unroll
-        for (int k = 0; k < C / 16; ++k) umma_ta(tmem + L::kIntra, tmem + L::kPacked + (k >> 2) * L::kPackedHalf + 8 * (k & 3), along_rows(a_z, k, C), i_o, k > 0);
-        umma_commit(o_full);
-        umma_commit(empty + (3 * i + 2) % NS);
-        if (D == 128 && i + 1 < count) ok = scores(i + 1);
+        for (int k = 0; k < C / 16; ++k)
+          umma_ta_elect(tmem + L::kIntra, tmem + L::kPacked + (k >> 2) * L::kPackedHalf + 8 * (k & 3), along_rows(a_z, k, C), i_o, k > 0);
+        umma_commit_elect(o_full);
+        umma_commit_elect(empty + (3 * i + 2) % NS);
+        if (i + 1 < count) go = scores(i + 1);      // (A has read the scores before: p_ready)
       }
-      umma_commit(fin);          // nothing of the CTA is given back while a product runs
+      umma_commit_elect(fin);          // nothing of the CTA is given back while a product runs
       mbar_drain(fin, 0);
     }
   } else if (warp == 18) {
-    // ---- products of group B: the state's own, and x S
-    if (lane == 0 && count > 0) {
+    // ---- products of group B: x S, then the state's own
+    if (count > 0) {
       constexpr uint32_t i_o = make_idesc<T>(C, D, false, true), i_u = make_idesc<T>(D, D, true, true);
-      uint32_t a_s = smem_u32(s_s);
+      const uint32_t a_s = smem_u32(s_s);
       for (int i = 0; i < count; ++i) {
-        asm volatile("" : "+r"(a_s));      // (descriptors are formed here, not kept over the loop in registers there are not)
         const int ia = i % NI;
-        if (!landed(3 * i + 1, 0x8580)) break;
-        if (i == dirty && !mbar_wait(clean, 0, ab, 0x8590 + i)) break;
-        if (!mbar_wait(s_ready, i & 1, ab, 0x8600 + i)) break;
-        if (i + 1 < count) {
-          // the state in tensor memory has been decayed by the time its 16-bit terms are ready
-          if (!landed(3 * i + 2, 0x8590) || !mbar_wait(y_ready, i & 1, ab, 0x8500 + i)) break;
-          tc_fence_after();
-          const uint32_t a_y = smem_u32(tile(3 * i)), a_z = smem_u32(tile(3 * i + 2));
-#pragma unroll
-          for (int k = 0; k < C / 16; ++k) umma(tmem + L::kState, along_rows(a_y, k, C), along_rows(a_z, k, C), i_u, 1);
-          umma_commit(u_full);
-          umma_commit(empty + (3 * i) % NS);
-          umma_commit(empty + (3 * i) % NS);
-          umma_commit(empty + (3 * i + 2) % NS);
-        }
-        if (i >= NI && !mbar_wait(i_free + ia, (i / NI - 1) & 1, ab, 0x8780 + i)) break;
+        bool ok = landed(3 * i + 1, 0x8580);
+        if (i == dirty) ok = ok && mbar_wait(clean, 0, ab, 0x8590 + i);
+        ok = ok && mbar_wait(s_ready, i & 1, ab, 0x8600 + i);
+        if (i >= NI) ok = ok && mbar_wait(i_free + ia, (i / NI - 1) & 1, ab, 0x8780 + i);
+        if (!__all_sync(0xffffffffu, ok)) break;
         tc_fence_after();
         const uint32_t a_x = smem_u32(tile(3 * i + 1));
 #pragma unroll
         for (int t = 1; t >= 0; --t)
 #pragma unroll
           for (int k = 0; k < D / 16; ++k)
-            umma(tmem + L::kInter + ia * D, along_row(a_x, k, C), along_rows(a_s + t * L::kS, k, D), i_o, !(t == 1 && k == 0));
-        umma_commit(s_done);
-        umma_commit(i_full + ia);
+            umma_elect(tmem + L::kInter + ia * D, along_row(a_x, k, C), along_rows(a_s + t * L::kS, k, D), i_o, !(t == 1 && k == 0));
+        umma_commit_elect(s_done);
+        umma_commit_elect(i_full + ia);
+        if (i + 1 < count) {
+          // (the state in tensor memory has been decayed by the time its 16-bit terms are ready)
+          ok = landed(3 * i + 2, 0x8590) && mbar_wait(y_ready + (i & 1), (i >> 1) & 1, ab, 0x8500 + i);
+          if (!__all_sync(0xffffffffu, ok)) break;
+          tc_fence_after();
+          const uint32_t a_y = smem_u32(tile(3 * i)), a_z = smem_u32(tile(3 * i + 2));
+#pragma unroll
+          for (int k = 0; k < C / 16; ++k) umma_elect(tmem + L::kState, along_rows(a_y, k, C), along_rows(a_z, k, C), i_u, 1);
+          umma_commit_elect(u_full);
+          umma_commit_elect(empty + (3 * i) % NS);
+          umma_commit_elect(empty + (3 * i) % NS);
+          umma_commit_elect(empty + (3 * i + 2) % NS);
+        }
       }
-      umma_commit(fin + 1);
+      umma_commit_elect(fin + 1);
       mbar_drain(fin + 1, 0);
     }
   } else if (warp < 8) {
@@ -470,6 +472,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
     const int quarter = warp & 3, half = warp >> 2;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
     const int w0 = quarter * 32, s = w0 + lane;
+    const float largest = fabsf(p.scale) * fmaxf(1.f, pw[C - 1]);      // of a score's factors
     // rows of the segment past the sequence's length
     {
       const int64_t z0 = r0 + (int64_t)count * C;
@@ -484,8 +487,8 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
       mbar_wait(p_full + (i & 3), (i >> 2) & 1, ab, 0x8900 + i);
       __syncwarp();
       tc_fence_after();
-      // Scores, weighted and packed, 16 columns at a time.  In fp16 the largest is looked at first: where some leave that type's range (rare), all go in
-      // divided by a power of two.  (Loops are not unrolled: the warps' ways through this kernel have to share the instruction cache.)
+      // Scores, weighted and packed, 16 columns at a time.  In fp16 the largest is looked at first: where some might leave that type's range
+      // (rare), all go in divided by a power of two.  (Loops are not unrolled: the warps' ways through this kernel have to share the instruction cache.)
       const uint32_t t_scores = tmem + L::kScores + lane_base + half * 64, t_packed = tmem + L::kPacked + lane_base + half * L::kPackedHalf;
       const auto block = [&](int n, float factor, float2* v) {
         const int t0 = half * 64 + n * 16;
@@ -511,17 +514,18 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
         }
       };
       const auto behind = [&](int n) { const int t0 = half * 64 + n * 16; return REV ? t0 + 15 >= w0 : t0 <= w0 + 31; };      // (some of it)
-      float up = 1.f, factor = p.scale;
+      float up = 1.f, factor = p.scale;      // (unweighted scores, masked ones among them: what is too large of them costs a factor that does no harm)
       if (F16) {
         float most = 0.f;
 #pragma unroll 1
-        for (int n = 0; n < 4; ++n)
-          if (behind(n)) {
-            float2 v[8];
-            block(n, factor, v);
+        for (int n = 0; n < 2; ++n) {
+          float v[32];
+          tmem_ld32(t_scores + n * 32, v);
+          tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 8; ++j) most = fmaxf(most, fmaxf(fabsf(v[j].x), fabsf(v[j].y)));
-          }
+          for (int j = 0; j < 32; ++j) most = fmaxf(most, fabsf(v[j]));
+        }
+        most *= largest;
         if (named_barrier_or(1, kGroup, most > 32768.f)) {
           float m = most < INFINITY ? most : 0.f;
           for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -551,7 +555,6 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
       }
       tmem_st_wait();
       tc_fence_before();
-      if (D == 64) mbar_arrive_warp(p_free);
       mbar_arrive_warp(p_ready);
       if (threadIdx.x == 0 && i > 0) {
         tma_store_wait_read();                         // the output tile of the chunk before has left its place, x's
@@ -637,11 +640,12 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
       if (F16) {
         float most = 0.f, up = 1.f;
 #pragma unroll 1
-        for (int q = 0; q < HC / 16; ++q) {
-          float f[16];
-          piece(q, f);
+        for (int q = 0; q < HC / 32; ++q) {
+          float f[32];
+          tmem_ld32(t_state + q * 32, f);
+          tmem_ld_wait();
 #pragma unroll
-          for (int j = 0; j < 16; ++j) most = fmaxf(most, fabsf(f[j]));
+          for (int j = 0; j < 32; ++j) most = fmaxf(most, fabsf(f[j]));
         }
         if (named_barrier_or(2, kGroup, owner && most > 32768.f)) {
           float m = owner && most < INFINITY ? most : 0.f;
@@ -688,8 +692,8 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
       fence_proxy_async();
       mbar_arrive_warp(s_ready);
     };
-    if (count > 0) put_state(0);
-    for (int i = 0; i < count; ++i) {
+    // y' of chunk i, in y's place once the scores have been formed from it; rows that do not count are cleared before these
+    const auto put_y = [&](int i) {
       const int64_t c0 = row_of(i);
       const int nv = end - c0 < C ? (int)(end - c0) : C;
       if (i == dirty) {
@@ -702,8 +706,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
         mbar_arrive_warp(clean);
         named_barrier(2, kGroup);
       }
-      if (i + 1 == count) break;
-      // y' takes y's place once the scores have been formed from it
+      if (i + 1 >= count) return;
       landed(3 * i, 0x8c80);
       mbar_wait(p_full + (i & 3), (i >> 2) & 1, ab, 0x8c00 + i);
       __syncwarp();
@@ -716,9 +719,16 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
         *reinterpret_cast<uint4*>(src + idx * 16) = term;
       }
       fence_proxy_async();
-      mbar_arrive_warp(y_ready);
-      mbar_wait(u_full, i & 1, ab, 0x8d00 + i);
+      mbar_arrive_warp(y_ready + (i & 1));
+    };
+    if (count > 0) {
+      put_state(0);
+      put_y(0);
+    }
+    for (int i = 0; i + 1 < count; ++i) {
+      put_y(i + 1);
       mbar_wait(s_done, i & 1, ab, 0x8e00 + i);
+      mbar_wait(u_full, i & 1, ab, 0x8d00 + i);
       __syncwarp();
       tc_fence_after();
       put_state(i + 1);
