@@ -278,21 +278,24 @@ decay_tc_sums_kernel(const __grid_constant__ CUtensorMap tm_y, const __grid_cons
 }
 
 // ---- outputs -------------------------------------------------------------------------------------------------
-// One CTA a segment, one CTA an SM, 19 warps, chunks of 128 rows: group A (warps 0-7) turns P into its 16-bit operand and takes the output
-// tile out, group B (8-15) forms y' and carries the state, one warp loads, one issues the products of A and one those of B.  The two groups meet
-// only in what the products need: while A works on the scores of a chunk, B is at the state behind it.
+// One CTA a segment, one CTA an SM, 20 warps, chunks of 128 rows: group A (warps 0-7) turns P into its 16-bit operand and takes the output
+// tile out, group B (8-15) forms y' and carries the state, one warp loads, one issues the products of A, one those of B, one
+// stores.  The two groups meet only in what the products need: while A works on the scores of a chunk, B is at the state behind it.
 //
-// Shared memory's bandwidth is what there is least of (every operand of a product passes it), so P goes to its product through tensor memory, y' takes
-// y's own place, and the output tile x's.  The state stays in tensor memory: B takes it out to form its two 16-bit terms, puts it back decayed, and the
-// products add y'^T z to it.
+// Shared memory is what there is least of, its bandwidth (every operand of a product passes it) and, with heads of 128, its room: so P goes to its product
+// through tensor memory, the output tile takes x's place, and with heads of 128 y' takes y's.  The state stays in tensor memory: B takes it out to form
+// its two 16-bit terms, puts it back decayed, and the products add y'^T z to it.
 constexpr int kC = 128;      // rows of a chunk
 template <int D> struct MainCfg {
   static constexpr int kTile = kC * D * 2;
   static constexpr int kS = D * D * 2;                                   // one term of the state
-  static constexpr int kSlots = D == 64 ? 12 : 5;                        // tiles in flight, in the order y, x, z of the chunks
+  static constexpr int kSlots = D == 64 ? 10 : 5;                        // tiles in flight, in the order y, x, z of the chunks
+  static constexpr int kTerms = D == 64 ? 2 : 0;                         // tiles for y' (none: in y's place)
   static constexpr int kInters = D == 64 ? 2 : 1;                        // accumulators of x S
-  static constexpr int kThreads = 2 * kGroup + 96;
-  static constexpr int kBytes = 1024 + kSlots * kTile + 2 * kS + (kC + 4) * 4 + 64 + 80 + 512;
+  static constexpr int kThreads = 2 * kGroup + 128;
+  // (relies on the dynamic shared window being 1024-byte aligned, which is checked)
+  static constexpr int kBytes = (kSlots + kTerms) * kTile + 2 * kS + 32 * 16 * 4 + (kC + 4) * 4 + 80 + (2 * kSlots + 24) * 8 + 16;
+  static_assert(kBytes <= 232448, "shared memory of one CTA");
   // Tensor-memory columns.  The packed scores of columns 0-63 begin at kPacked, those of 64-127 kPackedHalf behind; with heads of 128 they take the place
   // of the scores that they come from, a thread's own.
   static constexpr int kScores = 0, kPacked = D == 64 ? 128 : 0, kPackedHalf = D == 64 ? 32 : 64, kIntra = D == 64 ? 192 : 128, kInter = 256, kState = 384;
@@ -317,13 +320,18 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
   constexpr bool F16 = UmmaFmt<T>::v == 0;
   extern __shared__ uint8_t smem_raw[];
   pdl_trigger();
-  uint8_t* s_in = at1024(smem_raw);
-  uint8_t* s_s = s_in + NS * L::kTile;                // two terms of S
-  float* pw = reinterpret_cast<float*>(s_s + 2 * L::kS);
-  float* rpw = pw + C + 4;                            // [16]: exp(g (15 - j))
-  float* s_mul = rpw + 16;                            // [4]: what x S of chunk i is to be multiplied by, in s_mul[i & 3] (B may be two ahead)
+  if (smem_u32(smem_raw) & 1023u) {
+    if (threadIdx.x == 0 && p.status) atomicCAS(p.status, 0, (kStatusSmemAlign << 24) | 0x8000);
+    return;
+  }
+  uint8_t* s_in = smem_raw;
+  uint8_t* s_y = s_in + NS * L::kTile;                // y' of even and odd chunks
+  uint8_t* s_s = s_y + L::kTerms * L::kTile;          // two terms of S
+  float* s_diag = reinterpret_cast<float*>(s_s + 2 * L::kS);      // [32][16]: weights beside the diagonal, see below
+  float* s_pow = s_diag + 32 * 16;                    // powers of exp(g): forwards that of C - k at k, backwards that of k
+  float* s_mul = s_pow + C + 4;                       // [4]: what x S of chunk i is to be multiplied by, in s_mul[i & 3] (B may be two ahead)
   float* s_max = s_mul + 4;                           // [16]
-  uint64_t* bars = reinterpret_cast<uint64_t*>((reinterpret_cast<uintptr_t>(s_max + 16) + 15) & ~(uintptr_t)15);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(s_max + 16);
   uint64_t* full = bars;             // [NS]
   uint64_t* empty = full + NS;       // [NS]
   uint64_t* p_full = empty + NS;     // [4]: scores of chunk i in p_full[i & 3]; B waits for them too and may be two chunks behind
@@ -338,14 +346,15 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
   uint64_t* fin = p_ready + 9;       // [2]
   uint64_t* i_full = p_ready + 11;    // [2], by accumulator
   uint64_t* i_free = p_ready + 13;    // [2]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(p_ready + 15);
+  uint64_t* t_ready = p_ready + 15;  // [4]: the output tile of chunk i in t_ready[i & 3]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(p_ready + 19);
   int* abort_word = reinterpret_cast<int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int bh = blockIdx.x / p.ncut, cut = blockIdx.x % p.ncut, b = bh / p.H, h = bh % p.H;
   if (threadIdx.x == 0) {
     for (int i = 0; i < NS; ++i) { mbar_init(full + i, 1); mbar_init(empty + i, 2); }
-    for (int i = 0; i < 4; ++i) mbar_init(p_full + i, 1);
+    for (int i = 0; i < 4; ++i) { mbar_init(p_full + i, 1); mbar_init(t_ready + i, kGroup / 32); }
     mbar_init(p_ready, kGroup / 32); mbar_init(o_full, 1); mbar_init(o_free, kGroup / 32);
     mbar_init(u_full, 1); mbar_init(s_ready, kGroup / 32); mbar_init(s_done, 1);
     mbar_init(clean, kGroup / 32);
@@ -361,10 +370,15 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
   const int64_t r1 = r0 + p.seg_rows < p.N ? r0 + p.seg_rows : p.N;
   const int64_t end = r1 < len ? r1 : len;
   const double g = decay_log(p.log_decay[h]);
-  for (int i = threadIdx.x; i <= C; i += L::kThreads) {
-    pw[i] = (float)exp(g * i);
-    if (i < 16) rpw[15 - i] = pw[i];
+  for (int i = threadIdx.x; i <= C; i += L::kThreads) s_pow[REV ? i : C - i] = (float)exp(g * i);
+  // Row r of a 32 x 32 block on the diagonal: forwards the weight of column j < 16 is s_diag[r][j], of column 16 + j s_diag[r - 16][j]; backwards of
+  // column 16 + j s_diag[r][j], of column j < 16 s_diag[r + 16][j]; what such an index would leave the table with is behind the mask.
+  // (16-byte pieces of a row are stored at piece ^ (row / 2) % 4: eight rows read at once fall on different banks)
+  for (int i = threadIdx.x; i < 32 * 16; i += L::kThreads) {
+    const int row = i / 16, j = i % 16, d = REV ? 16 + j - row : row - j;
+    s_diag[row * 16 + ((j / 4) ^ (row / 2 % 4)) * 4 + j % 4] = d >= 0 ? p.scale * (float)exp(g * d) : 0.f;
   }
+  const auto power = [&](int n) { return s_pow[REV ? n : C - n]; };
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
@@ -376,12 +390,25 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
   const auto tile = [&](int n) { return s_in + (n % NS) * L::kTile; };      // n = 3 i + 0, 1, 2: y, x, z of chunk i
   const auto landed = [&](int n, int where) { return mbar_wait(full + n % NS, (n / NS) & 1, ab, where + n); };
 
-  if (warp == 16) {
+  if (warp == 19) {
+    // ---- output tiles, from x's place to their rows; the place is then free
+    if (lane == 0 && count > 0) {
+      tma_prefetch_desc(&tm_o);
+      for (int i = 0; i < count; ++i) {
+        if (!mbar_wait(t_ready + (i & 3), (i >> 2) & 1, ab, 0x8080 + i)) break;
+        for (int kb = 0; kb < KB; ++kb) tma_store_4d_h(&tm_o, tile(3 * i + 1) + kb * (C * 128), kb * 64, (int)row_of(i), h, b, 0);
+        tma_store_commit();
+        tma_store_wait_read();
+        mbar_arrive(empty + (3 * i + 1) % NS);
+        mbar_arrive(empty + (3 * i + 1) % NS);
+      }
+      tma_store_wait_all();
+    }
+  } else if (warp == 16) {
     if (lane == 0 && count > 0) {
       tma_prefetch_desc(&tm_x);
       tma_prefetch_desc(&tm_y);
       tma_prefetch_desc(&tm_z);
-      tma_prefetch_desc(&tm_o);
       int armed = 0;
       for (int n = 0; n < 3 * count; ++n) {
         if (!mbar_wait(empty + n % NS, ((n / NS) & 1) ^ 1, ab, 0x8100 + n)) break;
@@ -409,6 +436,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) umma_elect(tmem + L::kScores, along_row(a_x, k, C), along_row(a_y, k, C), i_p, k > 0);
         umma_commit_elect(p_full + (i & 3));
+        if (D == 64) umma_commit_elect(empty + (3 * i) % NS);
         return true;
       };
       bool go = scores(0);
@@ -454,12 +482,12 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
           ok = landed(3 * i + 2, 0x8590) && mbar_wait(y_ready + (i & 1), (i >> 1) & 1, ab, 0x8500 + i);
           if (!__all_sync(0xffffffffu, ok)) break;
           tc_fence_after();
-          const uint32_t a_y = smem_u32(tile(3 * i)), a_z = smem_u32(tile(3 * i + 2));
+          const uint32_t a_y = smem_u32(D == 64 ? s_y + (i & 1) * L::kTile : tile(3 * i)), a_z = smem_u32(tile(3 * i + 2));
 #pragma unroll
           for (int k = 0; k < C / 16; ++k) umma_elect(tmem + L::kState, along_rows(a_y, k, C), along_rows(a_z, k, C), i_u, 1);
           umma_commit_elect(u_full);
-          umma_commit_elect(empty + (3 * i) % NS);
-          umma_commit_elect(empty + (3 * i) % NS);
+          umma_commit_elect(empty + (3 * i) % NS);      // (with heads of 64 y' has been formed: y_ready)
+          if (D == 128) umma_commit_elect(empty + (3 * i) % NS);
           umma_commit_elect(empty + (3 * i + 2) % NS);
         }
       }
@@ -472,7 +500,8 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
     const int quarter = warp & 3, half = warp >> 2;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
     const int w0 = quarter * 32, s = w0 + lane;
-    const float largest = fabsf(p.scale) * fmaxf(1.f, pw[C - 1]);      // of a score's factors
+    const float largest = fabsf(p.scale) * fmaxf(1.f, power(C - 1));      // of a score's factors
+    const float row_factor = p.scale * power(REV ? 32 - lane : lane);
     // rows of the segment past the sequence's length
     {
       const int64_t z0 = r0 + (int64_t)count * C;
@@ -482,39 +511,14 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
         *reinterpret_cast<uint4*>(out + (z0 + i / per) * p.on + (i % per) * 8) = make_uint4(0, 0, 0, 0);
     }
     for (int i = 0; i < count; ++i) {
-      const int64_t c0 = row_of(i);
-      const int nv = end - c0 < C ? (int)(end - c0) : C;
+      const int nv = end - row_of(i) < C ? (int)(end - row_of(i)) : C;
       mbar_wait(p_full + (i & 3), (i >> 2) & 1, ab, 0x8900 + i);
       __syncwarp();
       tc_fence_after();
       // Scores, weighted and packed, 16 columns at a time.  In fp16 the largest is looked at first: where some might leave that type's range
       // (rare), all go in divided by a power of two.  (Loops are not unrolled: the warps' ways through this kernel have to share the instruction cache.)
       const uint32_t t_scores = tmem + L::kScores + lane_base + half * 64, t_packed = tmem + L::kPacked + lane_base + half * L::kPackedHalf;
-      const auto block = [&](int n, float factor, float2* v) {
-        const int t0 = half * 64 + n * 16;
-        tmem_ld16(t_scores + n * 16, reinterpret_cast<float*>(v));
-        tmem_ld_wait();
-        if (REV ? t0 >= w0 + 31 : t0 + 15 <= w0) {
-          // the whole block lies behind the rows: exp(g d) as a row's factor times a column's
-          const float row = factor * pw[REV ? t0 - s : s - t0 - 15];
-          const float4* c = reinterpret_cast<const float4*>(REV ? pw : rpw);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float4 f = c[j];
-            v[2 * j] = mul2(mul2(v[2 * j], make_float2(row, row)), make_float2(f.x, f.y));
-            v[2 * j + 1] = mul2(mul2(v[2 * j + 1], make_float2(row, row)), make_float2(f.z, f.w));
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const int d = REV ? t0 + 2 * j - s : s - t0 - 2 * j, e = REV ? d + 1 : d - 1;
-            v[j].x = d >= 0 ? v[j].x * (factor * pw[max(d, 0)]) : 0.f;
-            v[j].y = e >= 0 ? v[j].y * (factor * pw[max(e, 0)]) : 0.f;
-          }
-        }
-      };
-      const auto behind = [&](int n) { const int t0 = half * 64 + n * 16; return REV ? t0 + 15 >= w0 : t0 <= w0 + 31; };      // (some of it)
-      float up = 1.f, factor = p.scale;      // (unweighted scores, masked ones among them: what is too large of them costs a factor that does no harm)
+      float up = 1.f;      // (unweighted scores, masked ones among them: what is too large of them costs a factor that does no harm)
       if (F16) {
         float most = 0.f;
 #pragma unroll 1
@@ -535,34 +539,61 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
           int e = 0;
           frexpf(m, &e);
           up = ldexpf(1.f, max(0, e - 15));
-          factor = p.scale / up;
           named_barrier(1, kGroup);
         }
       }
 #pragma unroll 1
-      for (int n = 0; n < 4; ++n) {
-        uint32_t pk[8];
-        if (behind(n)) {
-          float2 v[8];
-          block(n, factor, v);
+      for (int n = 0; n < 2; ++n) {
+        const int t0 = half * 64 + n * 32;
+        float2 v[16];
+        if (REV ? t0 < w0 : t0 > w0) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) pk[j] = pack2<T>(v[j].x, v[j].y);
+          for (int j = 0; j < 16; ++j) v[j] = make_float2(0.f, 0.f);
         } else {
+          tmem_ld32(t_scores + n * 32, reinterpret_cast<float*>(v));
+          tmem_ld_wait();
+          if (t0 == w0) {
+            // the block on the diagonal
 #pragma unroll
-          for (int j = 0; j < 8; ++j) pk[j] = 0u;
+            for (int part = 0; part < 2; ++part) {
+              const int from = REV ? (part == 0 ? lane + 16 : lane) : (part == 0 ? lane : lane - 16);
+              const bool none = REV ? part == 0 && lane >= 16 : part == 1 && lane < 16;
+              const float* row = s_diag + (from & 31) * 16;
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const float4 f = *reinterpret_cast<const float4*>(row + (j ^ (from / 2 & 3)) * 4);
+                float2 *a = v + 8 * part + 2 * j, *e = a + 1;
+                *a = mul2(*a, make_float2(f.x, f.y));
+                *e = mul2(*e, make_float2(f.z, f.w));
+                if (none) *a = *e = make_float2(0.f, 0.f);
+              }
+            }
+          } else {
+            // one that lies behind it: exp(g |s - t|) as the row's distance to a block's edge, and the column's
+            const float4* c = reinterpret_cast<const float4*>(s_pow + (REV ? t0 - w0 - 32 : C - w0 + t0));
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const float4 f = c[j];
+              v[2 * j] = mul2(mul2(v[2 * j], make_float2(row_factor, row_factor)), make_float2(f.x, f.y));
+              v[2 * j + 1] = mul2(mul2(v[2 * j + 1], make_float2(row_factor, row_factor)), make_float2(f.z, f.w));
+            }
+          }
+          if (F16 && up != 1.f) {
+            const float down = 1.f / up;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = mul2(v[j], make_float2(down, down));
+          }
         }
-        tmem_st8(t_packed + n * 8, reinterpret_cast<const float*>(pk));
+        uint32_t pk[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) pk[j] = pack2<T>(v[j].x, v[j].y);
+        tmem_st16(t_packed + n * 16, reinterpret_cast<const float*>(pk));
       }
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive_warp(p_ready);
-      if (threadIdx.x == 0 && i > 0) {
-        tma_store_wait_read();                         // the output tile of the chunk before has left its place, x's
-        mbar_arrive(empty + (3 * i - 2) % NS);
-        mbar_arrive(empty + (3 * i - 2) % NS);
-      }
       float wi = 0.f;
-      if (REV ? s < nv : true) wi = p.inter * p.sum_scale * pw[REV ? nv - 1 - s : s + 1];
+      if (REV ? s < nv : true) wi = p.inter * p.sum_scale * power(REV ? nv - 1 - s : s + 1);
       mbar_wait(i_full + i % NI, (i / NI) & 1, ab, 0x8a80 + i);
       mbar_wait(o_full, i & 1, ab, 0x8a00 + i);
       __syncwarp();
@@ -570,38 +601,37 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
       if (F16) wi *= s_mul[i & 3];
       uint8_t* to = tile(3 * i + 1);
 #pragma unroll 1
-      for (int q = 0; q < D / 32; ++q) {
-        const int col = half * (D / 2) + q * 16;
-        float2 a[8], e[8];
-        tmem_ld16(tmem + L::kIntra + lane_base + col, reinterpret_cast<float*>(a));
-        tmem_ld16(tmem + L::kInter + (i % NI) * D + lane_base + col, reinterpret_cast<float*>(e));
+      for (int q = 0; q < D / 64; ++q) {
+        const int col = half * (D / 2) + q * 32;
+        float2 a[16], e[16];
+        tmem_ld32(tmem + L::kIntra + lane_base + col, reinterpret_cast<float*>(a));
+        tmem_ld32(tmem + L::kInter + (i % NI) * D + lane_base + col, reinterpret_cast<float*>(e));
         tmem_ld_wait();
-        if (q == D / 32 - 1) {
+        if (q == D / 64 - 1) {
           tc_fence_before();
           mbar_arrive_warp(o_free);
           mbar_arrive_warp(i_free + i % NI);
         }
-        uint32_t u[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if (F16) a[j] = mul2(a[j], make_float2(up, up));
-          if (wi != 0.f) a[j] = fma2(e[j], make_float2(wi, wi), a[j]);
-          u[j] = pack2<T>(a[j].x, a[j].y);
-        }
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const int cc = (col >> 3) + k;
-          *reinterpret_cast<uint4*>(to + (cc >> 3) * (C * 128) + sw128_offset(s, cc & 7)) = make_uint4(u[4 * k], u[4 * k + 1], u[4 * k + 2], u[4 * k + 3]);
+          uint32_t u[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            float2 f = a[8 * k + j];
+            if (F16) f = mul2(f, make_float2(up, up));
+            if (wi != 0.f) f = fma2(e[8 * k + j], make_float2(wi, wi), f);
+            u[j] = pack2<T>(f.x, f.y);
+          }
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int cc = (col >> 3) + 2 * k + j;
+            *reinterpret_cast<uint4*>(to + (cc >> 3) * (C * 128) + sw128_offset(s, cc & 7)) = make_uint4(u[4 * j], u[4 * j + 1], u[4 * j + 2], u[4 * j + 3]);
+          }
         }
       }
       fence_proxy_async();
-      named_barrier(1, kGroup);
-      if (threadIdx.x == 0) {
-        for (int kb = 0; kb < KB; ++kb) tma_store_4d_h(&tm_o, to + kb * (C * 128), kb * 64, (int)c0, h, b, 0);
-        tma_store_commit();
-      }
+      mbar_arrive_warp(t_ready + (i & 3));
     }
-    if (threadIdx.x == 0) tma_store_wait_all();
   } else {
     // ---- group B: the state
     const int tid = threadIdx.x - kGroup, quarter = warp & 3, half = (warp - 8) >> 2;
@@ -629,10 +659,6 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
       }
       tmem_st_wait();
     }
-    const auto piece = [&](int q, float* f) {
-      tmem_ld16(t_state + q * 16, f);
-      tmem_ld_wait();
-    };
     // The state as two 16-bit terms for x S (in fp16 divided by a power of two where it would leave the range), and, decayed by the chunk's
     // rows, back to tensor memory, where y'^T z is added to it.
     const auto put_state = [&](int i) {
@@ -663,14 +689,19 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
       }
       const DecayPair w = i == 0 ? first_chunk : full_chunk;
 #pragma unroll 1
-      for (int q = 0; q < HC / 16; ++q) {
-        float2 f[8];
-        piece(q, reinterpret_cast<float*>(f));
-        if (i + 1 < count) {
-          float d[16];
+      for (int q2 = 0; q2 < HC / 32; ++q2) {
+       float2 both[16];
+       tmem_ld32(t_state + q2 * 32, reinterpret_cast<float*>(both));
+       tmem_ld_wait();
 #pragma unroll
-          for (int j = 0; j < 8; ++j) { d[2 * j] = decay_by(w, f[j].x); d[2 * j + 1] = decay_by(w, f[j].y); }
-          tmem_st16(t_state + q * 16, d);
+       for (int k2 = 0; k2 < 2; ++k2) {
+        const int q = 2 * q2 + k2;
+        float2* f = both + 8 * k2;
+        if (i + 1 < count) {
+          float2 d[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) d[j] = fma2(f[j], make_float2(w.hi, w.hi), mul2(f[j], make_float2(w.lo, w.lo)));
+          tmem_st16(t_state + q * 16, reinterpret_cast<const float*>(d));
         }
         if (F16)
 #pragma unroll
@@ -686,13 +717,14 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
             *reinterpret_cast<uint4*>(s_s + L::kS + off) = make_uint4(t[1][4 * k], t[1][4 * k + 1], t[1][4 * k + 2], t[1][4 * k + 3]);
           }
         }
+       }
       }
       tmem_st_wait();
       tc_fence_before();
       fence_proxy_async();
       mbar_arrive_warp(s_ready);
     };
-    // y' of chunk i, in y's place once the scores have been formed from it; rows that do not count are cleared before these
+    // y' of chunk i (in y's place: once the scores have been formed from it); rows that do not count are cleared before these
     const auto put_y = [&](int i) {
       const int64_t c0 = row_of(i);
       const int nv = end - c0 < C ? (int)(end - c0) : C;
@@ -708,15 +740,16 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
       }
       if (i + 1 >= count) return;
       landed(3 * i, 0x8c80);
-      mbar_wait(p_full + (i & 3), (i >> 2) & 1, ab, 0x8c00 + i);
+      if (D == 128) mbar_wait(p_full + (i & 3), (i >> 2) & 1, ab, 0x8c00 + i);
       __syncwarp();
-      uint8_t* src = tile(3 * i);
+      const uint8_t* src = tile(3 * i);
+      uint8_t* dst = D == 64 ? s_y + (i & 1) * L::kTile : tile(3 * i);
 #pragma unroll 2
       for (int q = 0; q < L::kTile / 16 / kGroup; ++q) {
         const int idx = tid + q * kGroup, r = (idx >> 3) & (C - 1);
         uint4 term;
-        scaled_terms<T, 1>(*reinterpret_cast<const uint4*>(src + idx * 16), r < nv ? pw[REV ? r + 1 : nv - 1 - r] : 0.f, &term);
-        *reinterpret_cast<uint4*>(src + idx * 16) = term;
+        scaled_terms<T, 1>(*reinterpret_cast<const uint4*>(src + idx * 16), r < nv ? power(REV ? r + 1 : nv - 1 - r) : 0.f, &term);
+        *reinterpret_cast<uint4*>(dst + idx * 16) = term;
       }
       fence_proxy_async();
       mbar_arrive_warp(y_ready + (i & 1));
@@ -725,13 +758,15 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
       put_state(0);
       put_y(0);
     }
+    // (heads of 64: y' a chunk ahead, while the products that end this one run; its tile is free since u_full of the chunk before)
     for (int i = 0; i + 1 < count; ++i) {
-      put_y(i + 1);
+      if (D == 64) put_y(i + 1);
       mbar_wait(s_done, i & 1, ab, 0x8e00 + i);
       mbar_wait(u_full, i & 1, ab, 0x8d00 + i);
       __syncwarp();
       tc_fence_after();
       put_state(i + 1);
+      if (D == 128) put_y(i + 1);
     }
   }
   tc_fence_before();
