@@ -433,7 +433,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
         if (!__all_sync(0xffffffffu, ok)) return false;
         tc_fence_after();
         const uint32_t a_y = smem_u32(tile(3 * i)), a_x = smem_u32(tile(3 * i + 1));
-#pragma unroll
+#pragma unroll 2
         for (int k = 0; k < D / 16; ++k) umma_elect(tmem + L::kScores, along_row(a_x, k, C), along_row(a_y, k, C), i_p, k > 0);
         umma_commit_elect(p_full + (i & 3));
         if (D == 64) umma_commit_elect(empty + (3 * i) % NS);
@@ -446,7 +446,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
         if (!__all_sync(0xffffffffu, ok)) break;
         tc_fence_after();
         const uint32_t a_z = smem_u32(tile(3 * i + 2));
-#pragma unroll
+#pragma unroll 2
         for (int k = 0; k < C / 16; ++k)
           umma_ta_elect(tmem + L::kIntra, tmem + L::kPacked + (k >> 2) * L::kPackedHalf + 8 * (k & 3), along_rows(a_z, k, C), i_o, k > 0);
         umma_commit_elect(o_full);
@@ -470,9 +470,9 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
         if (!__all_sync(0xffffffffu, ok)) break;
         tc_fence_after();
         const uint32_t a_x = smem_u32(tile(3 * i + 1));
-#pragma unroll
+#pragma unroll 1
         for (int t = 1; t >= 0; --t)
-#pragma unroll
+#pragma unroll 2
           for (int k = 0; k < D / 16; ++k)
             umma_elect(tmem + L::kInter + ia * D, along_row(a_x, k, C), along_rows(a_s + t * L::kS, k, D), i_o, !(t == 1 && k == 0));
         umma_commit_elect(s_done);
@@ -483,7 +483,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
           if (!__all_sync(0xffffffffu, ok)) break;
           tc_fence_after();
           const uint32_t a_y = smem_u32(D == 64 ? s_y + (i & 1) * L::kTile : tile(3 * i)), a_z = smem_u32(tile(3 * i + 2));
-#pragma unroll
+#pragma unroll 2
           for (int k = 0; k < C / 16; ++k) umma_elect(tmem + L::kState, along_rows(a_y, k, C), along_rows(a_z, k, C), i_u, 1);
           umma_commit_elect(u_full);
           umma_commit_elect(empty + (3 * i) % NS);      // (with heads of 64 y' has been formed: y_ready)
@@ -518,7 +518,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
       // Scores, weighted and packed, 16 columns at a time.  In fp16 the largest is looked at first: where some might leave that type's range
       // (rare), all go in divided by a power of two.  (Loops are not unrolled: the warps' ways through this kernel have to share the instruction cache.)
       const uint32_t t_scores = tmem + L::kScores + lane_base + half * 64, t_packed = tmem + L::kPacked + lane_base + half * L::kPackedHalf;
-      float up = 1.f;      // (unweighted scores, masked ones among them: what is too large of them costs a factor that does no harm)
+      float up = 1.f, down = 1.f;      // (unweighted scores, masked ones among them: what is too large of them costs a factor that does no harm)
       if (F16) {
         float most = 0.f;
 #pragma unroll 1
@@ -539,55 +539,38 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
           int e = 0;
           frexpf(m, &e);
           up = ldexpf(1.f, max(0, e - 15));
+          down = 1.f / up;
           named_barrier(1, kGroup);
         }
       }
 #pragma unroll 1
-      for (int n = 0; n < 2; ++n) {
-        const int t0 = half * 64 + n * 32;
-        float2 v[16];
-        if (REV ? t0 < w0 : t0 > w0) {
+      for (int n = 0; n < 4; ++n) {
+        const int t0 = half * 64 + n * 16, part = n & 1, d0 = t0 - 16 * part - w0;      // d0: of the 32-column block, from the diagonal
+        float2 v[8];
+        uint32_t pk[8];
+        if (REV ? d0 < 0 : d0 > 0) {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) v[j] = make_float2(0.f, 0.f);
+          for (int j = 0; j < 8; ++j) pk[j] = 0u;
         } else {
-          tmem_ld32(t_scores + n * 32, reinterpret_cast<float*>(v));
+          tmem_ld16(t_scores + n * 16, reinterpret_cast<float*>(v));
+          const int from = REV ? lane + 16 - 16 * part : lane - 16 * part;
+          const float4* c = reinterpret_cast<const float4*>(d0 == 0 ? s_diag + (from & 31) * 16 : s_pow + (REV ? d0 - 32 : C + d0) + 16 * part);
+          const int turn = d0 == 0 ? from / 2 & 3 : 0;
+          // on the diagonal the table has it all; behind it exp(g |s - t|) is the row's distance to a block's edge, and the column's
+          float row = d0 == 0 ? 1.f : row_factor;
+          if (F16) row *= down;
+          const bool none = d0 == 0 && (REV ? from >= 32 : from < 0);
           tmem_ld_wait();
-          if (t0 == w0) {
-            // the block on the diagonal
 #pragma unroll
-            for (int part = 0; part < 2; ++part) {
-              const int from = REV ? (part == 0 ? lane + 16 : lane) : (part == 0 ? lane : lane - 16);
-              const bool none = REV ? part == 0 && lane >= 16 : part == 1 && lane < 16;
-              const float* row = s_diag + (from & 31) * 16;
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const float4 f = *reinterpret_cast<const float4*>(row + (j ^ (from / 2 & 3)) * 4);
-                float2 *a = v + 8 * part + 2 * j, *e = a + 1;
-                *a = mul2(*a, make_float2(f.x, f.y));
-                *e = mul2(*e, make_float2(f.z, f.w));
-                if (none) *a = *e = make_float2(0.f, 0.f);
-              }
-            }
-          } else {
-            // one that lies behind it: exp(g |s - t|) as the row's distance to a block's edge, and the column's
-            const float4* c = reinterpret_cast<const float4*>(s_pow + (REV ? t0 - w0 - 32 : C - w0 + t0));
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const float4 f = c[j];
-              v[2 * j] = mul2(mul2(v[2 * j], make_float2(row_factor, row_factor)), make_float2(f.x, f.y));
-              v[2 * j + 1] = mul2(mul2(v[2 * j + 1], make_float2(row_factor, row_factor)), make_float2(f.z, f.w));
-            }
+          for (int j = 0; j < 4; ++j) {
+            const float4 f = c[j ^ turn];
+            v[2 * j] = mul2(mul2(v[2 * j], make_float2(row, row)), make_float2(f.x, f.y));
+            v[2 * j + 1] = mul2(mul2(v[2 * j + 1], make_float2(row, row)), make_float2(f.z, f.w));
           }
-          if (F16 && up != 1.f) {
-            const float down = 1.f / up;
 #pragma unroll
-            for (int j = 0; j < 16; ++j) v[j] = mul2(v[j], make_float2(down, down));
-          }
+          for (int j = 0; j < 8; ++j) pk[j] = none ? 0u : pack2<T>(v[j].x, v[j].y);
         }
-        uint32_t pk[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) pk[j] = pack2<T>(v[j].x, v[j].y);
-        tmem_st16(t_packed + n * 16, reinterpret_cast<const float*>(pk));
+        tmem_st8(t_packed + n * 8, reinterpret_cast<const float*>(pk));
       }
       tmem_st_wait();
       tc_fence_before();
@@ -601,32 +584,28 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
       if (F16) wi *= s_mul[i & 3];
       uint8_t* to = tile(3 * i + 1);
 #pragma unroll 1
-      for (int q = 0; q < D / 64; ++q) {
-        const int col = half * (D / 2) + q * 32;
-        float2 a[16], e[16];
-        tmem_ld32(tmem + L::kIntra + lane_base + col, reinterpret_cast<float*>(a));
-        tmem_ld32(tmem + L::kInter + (i % NI) * D + lane_base + col, reinterpret_cast<float*>(e));
+      for (int q = 0; q < D / 32; ++q) {
+        const int col = half * (D / 2) + q * 16;
+        float2 a[8], e[8];
+        tmem_ld16(tmem + L::kIntra + lane_base + col, reinterpret_cast<float*>(a));
+        tmem_ld16(tmem + L::kInter + (i % NI) * D + lane_base + col, reinterpret_cast<float*>(e));
         tmem_ld_wait();
-        if (q == D / 64 - 1) {
+        if (q == D / 32 - 1) {
           tc_fence_before();
           mbar_arrive_warp(o_free);
           mbar_arrive_warp(i_free + i % NI);
         }
+        uint32_t u[8];
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          uint32_t u[8];
+        for (int j = 0; j < 8; ++j) {
+          if (F16) a[j] = mul2(a[j], make_float2(up, up));
+          if (wi != 0.f) a[j] = fma2(e[j], make_float2(wi, wi), a[j]);
+          u[j] = pack2<T>(a[j].x, a[j].y);
+        }
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            float2 f = a[8 * k + j];
-            if (F16) f = mul2(f, make_float2(up, up));
-            if (wi != 0.f) f = fma2(e[8 * k + j], make_float2(wi, wi), f);
-            u[j] = pack2<T>(f.x, f.y);
-          }
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int cc = (col >> 3) + 2 * k + j;
-            *reinterpret_cast<uint4*>(to + (cc >> 3) * (C * 128) + sw128_offset(s, cc & 7)) = make_uint4(u[4 * j], u[4 * j + 1], u[4 * j + 2], u[4 * j + 3]);
-          }
+        for (int j = 0; j < 2; ++j) {
+          const int cc = (col >> 3) + j;
+          *reinterpret_cast<uint4*>(to + (cc >> 3) * (C * 128) + sw128_offset(s, cc & 7)) = make_uint4(u[4 * j], u[4 * j + 1], u[4 * j + 2], u[4 * j + 3]);
         }
       }
       fence_proxy_async();
@@ -689,14 +668,10 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
       }
       const DecayPair w = i == 0 ? first_chunk : full_chunk;
 #pragma unroll 1
-      for (int q2 = 0; q2 < HC / 32; ++q2) {
-       float2 both[16];
-       tmem_ld32(t_state + q2 * 32, reinterpret_cast<float*>(both));
-       tmem_ld_wait();
-#pragma unroll
-       for (int k2 = 0; k2 < 2; ++k2) {
-        const int q = 2 * q2 + k2;
-        float2* f = both + 8 * k2;
+      for (int q = 0; q < HC / 16; ++q) {
+        float2 f[8];
+        tmem_ld16(t_state + q * 16, reinterpret_cast<float*>(f));
+        tmem_ld_wait();
         if (i + 1 < count) {
           float2 d[8];
 #pragma unroll
@@ -717,7 +692,6 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
             *reinterpret_cast<uint4*>(s_s + L::kS + off) = make_uint4(t[1][4 * k], t[1][4 * k + 1], t[1][4 * k + 2], t[1][4 * k + 3]);
           }
         }
-       }
       }
       tmem_st_wait();
       tc_fence_before();
@@ -744,7 +718,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
       __syncwarp();
       const uint8_t* src = tile(3 * i);
       uint8_t* dst = D == 64 ? s_y + (i & 1) * L::kTile : tile(3 * i);
-#pragma unroll 2
+#pragma unroll 1
       for (int q = 0; q < L::kTile / 16 / kGroup; ++q) {
         const int idx = tid + q * kGroup, r = (idx >> 3) & (C - 1);
         uint4 term;
