@@ -496,7 +496,8 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
     }
   } else if (warp < 8) {
     // ---- group A: scores and outputs
-    // (here and in group B a wait that gave up does not leave the loop: the warps meet at barriers, and the status word has it)
+    // (Here and in group B one warp asks the mbarriers for all, the others wait at a barrier, which takes no issue slots: twenty warps that ask took 40 % of
+    // them.  A wait that gave up does not leave the loop: the warps meet at barriers, and the status word has it.)
     const int quarter = warp & 3, half = warp >> 2;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
     const int w0 = quarter * 32, s = w0 + lane;
@@ -512,8 +513,8 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
     }
     for (int i = 0; i < count; ++i) {
       const int nv = end - row_of(i) < C ? (int)(end - row_of(i)) : C;
-      mbar_wait(p_full + (i & 3), (i >> 2) & 1, ab, 0x8900 + i);
-      __syncwarp();
+      if (warp == 0) mbar_wait(p_full + (i & 3), (i >> 2) & 1, ab, 0x8900 + i);
+      named_barrier(1, kGroup);
       tc_fence_after();
       // Scores, weighted and packed, 16 columns at a time.  In fp16 the largest is looked at first: where some might leave that type's range
       // (rare), all go in divided by a power of two.  (Loops are not unrolled: the warps' ways through this kernel have to share the instruction cache.)
@@ -577,9 +578,11 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
       mbar_arrive_warp(p_ready);
       float wi = 0.f;
       if (REV ? s < nv : true) wi = p.inter * p.sum_scale * power(REV ? nv - 1 - s : s + 1);
-      mbar_wait(i_full + i % NI, (i / NI) & 1, ab, 0x8a80 + i);
-      mbar_wait(o_full, i & 1, ab, 0x8a00 + i);
-      __syncwarp();
+      if (warp == 0) {
+        mbar_wait(i_full + i % NI, (i / NI) & 1, ab, 0x8a80 + i);
+        mbar_wait(o_full, i & 1, ab, 0x8a00 + i);
+      }
+      named_barrier(1, kGroup);
       tc_fence_after();
       if (F16) wi *= s_mul[i & 3];
       uint8_t* to = tile(3 * i + 1);
@@ -713,9 +716,11 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
         named_barrier(2, kGroup);
       }
       if (i + 1 >= count) return;
-      landed(3 * i, 0x8c80);
-      if (D == 128) mbar_wait(p_full + (i & 3), (i >> 2) & 1, ab, 0x8c00 + i);
-      __syncwarp();
+      if (warp == 8) {
+        landed(3 * i, 0x8c80);
+        if (D == 128) mbar_wait(p_full + (i & 3), (i >> 2) & 1, ab, 0x8c00 + i);
+      }
+      named_barrier(2, kGroup);
       const uint8_t* src = tile(3 * i);
       uint8_t* dst = D == 64 ? s_y + (i & 1) * L::kTile : tile(3 * i);
 #pragma unroll 1
@@ -735,9 +740,11 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
     // (heads of 64: y' a chunk ahead, while the products that end this one run; its tile is free since u_full of the chunk before)
     for (int i = 0; i + 1 < count; ++i) {
       if (D == 64) put_y(i + 1);
-      mbar_wait(s_done, i & 1, ab, 0x8e00 + i);
-      mbar_wait(u_full, i & 1, ab, 0x8d00 + i);
-      __syncwarp();
+      if (warp == 8) {
+        mbar_wait(s_done, i & 1, ab, 0x8e00 + i);
+        mbar_wait(u_full, i & 1, ab, 0x8d00 + i);
+      }
+      named_barrier(2, kGroup);
       tc_fence_after();
       put_state(i + 1);
       if (D == 128) put_y(i + 1);
