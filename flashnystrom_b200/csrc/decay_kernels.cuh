@@ -316,7 +316,7 @@ __global__ void __launch_bounds__(kThreads, D <= 64 ? 2 : 1) decay_chunk_kernel(
 
 // ---- the runs of a slice joined -----------------------------------------------------------------------------
 // One thread per element of the state of a slice goes through the runs in the order of time: before the first run of a segment
-// the state so far is what enters that segment.
+// the state so far is what enters that segment.  What depends on the run alone is formed once a CTA.
 struct DecayJoinParams {
   const float* sums;          // [BH][ncut][D][D]: each run alone
   const float* state_in;      // [BH][D][D] or null
@@ -329,40 +329,43 @@ struct DecayJoinParams {
   int64_t seg_rows, sub_rows;
   int count;                  // runs with a sum, in the order of time; with fewer than all of them there is no state_out
 };
+struct DecayJoinRun { float hi, lo; int rows, seg; };      // exp(g rows); rows that count; the segment that begins (in time) with it, or -1
 template <bool REV>
 __global__ void __launch_bounds__(kThreads) decay_join_kernel(DecayJoinParams p) {
-  const int bh = blockIdx.y, e = blockIdx.x * kThreads + threadIdx.x, DD = p.D * p.D, ncut = p.nseg * p.sub;
+  extern __shared__ float4 smem4[];
+  DecayJoinRun* runs = reinterpret_cast<DecayJoinRun*>(smem4);
   pdl_trigger();
   pdl_wait();
-  if (e >= DD) return;
+  const int bh = blockIdx.y, e = blockIdx.x * kThreads + threadIdx.x, DD = p.D * p.D, ncut = p.nseg * p.sub;
+  const int walk = min(ncut, p.count + 1);
   const double g = decay_log(p.log_decay[bh % p.H]);
   const int64_t len = decay_len(p.seq_lens, bh / p.H, p.N);
+  for (int k = threadIdx.x; k < walk; k += kThreads) {
+    const int i = REV ? ncut - 1 - k : k;
+    int64_t n = decay_cut_end(p.seg_rows, p.sub, p.sub_rows, p.N, i);
+    n = (n < len ? n : len) - decay_cut_begin(p.seg_rows, p.sub, p.sub_rows, i);
+    if (n < 0 || k >= p.count) n = 0;
+    const DecayPair w = decay_pair(g, n);
+    runs[k] = {w.hi, w.lo, (int)n, i % p.sub == (REV ? p.sub - 1 : 0) ? i / p.sub : -1};
+  }
+  __syncthreads();
+  if (e >= DD) return;
   float s = p.state_in ? p.state_in[(size_t)bh * DD + e] : 0.f;
-  int64_t known = -1;
-  DecayPair w{1.f, 0.f};
+  const float* from = p.sums + (size_t)bh * ncut * DD + e;
+  float* to = p.seg_states ? p.seg_states + (size_t)bh * p.nseg * DD + e : nullptr;
   constexpr int kAhead = 8;      // sums fetched ahead: the walk is a chain, its loads are not
-  const int walk = min(ncut, p.count + 1);
-  for (int i0 = 0; i0 < walk; i0 += kAhead) {
+  for (int k0 = 0; k0 < walk; k0 += kAhead) {
     float u[kAhead];
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      const int i = REV ? ncut - 1 - (i0 + k) : i0 + k;
-      u[k] = 0.f;
-      if (i0 + k < p.count && decay_cut_begin(p.seg_rows, p.sub, p.sub_rows, i) < len &&
-          decay_cut_begin(p.seg_rows, p.sub, p.sub_rows, i) < decay_cut_end(p.seg_rows, p.sub, p.sub_rows, p.N, i))
-        u[k] = p.sums[((size_t)bh * ncut + i) * DD + e];
-    }
+    for (int k = 0; k < kAhead; ++k)
+      u[k] = k0 + k < walk && runs[k0 + k].rows > 0 ? from[(size_t)(REV ? ncut - 1 - (k0 + k) : k0 + k) * DD] : 0.f;
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      if (i0 + k >= walk) break;
-      const int i = REV ? ncut - 1 - (i0 + k) : i0 + k;
-      if (p.seg_states && i % p.sub == (REV ? p.sub - 1 : 0)) p.seg_states[((size_t)bh * p.nseg + i / p.sub) * DD + e] = s;
-      int64_t n = decay_cut_end(p.seg_rows, p.sub, p.sub_rows, p.N, i);
-      n = (n < len ? n : len) - decay_cut_begin(p.seg_rows, p.sub, p.sub_rows, i);
-      if (n <= 0) continue;
-      if (n != known) { w = decay_pair(g, n); known = n; }
-      s = decay_by(w, s) + u[k];
-    }
+    for (int k = 0; k < kAhead; ++k)
+      if (k0 + k < walk) {
+        const DecayJoinRun run = runs[k0 + k];
+        if (to && run.seg >= 0) to[(size_t)run.seg * DD] = s;
+        if (run.rows > 0) s = decay_by({run.hi, run.lo}, s) + u[k];
+      }
   }
   if (p.state_out) p.state_out[(size_t)bh * DD + e] = s;
 }

@@ -183,26 +183,28 @@ decay_tc_sums_kernel(const __grid_constant__ CUtensorMap tm_y, const __grid_cons
         for (int i = max(0, armed - NST); i < armed; ++i) mbar_drain(full + i % NST, (i / NST) & 1);
     }
   } else if (warp == 9) {
-    if (lane == 0 && count > 0) {
+    // (the whole warp walks this code and one lane issues: descriptors stay in uniform registers)
+    if (count > 0) {
       constexpr uint32_t idesc = make_idesc<T>(D, D, true, true);
       int spans = 0;
       for (int i = 0; i < count; ++i) {
         const int st = i % NST, u = i & 1;
-        if (!mbar_wait(y_ready + u, (i >> 1) & 1, ab, 0x7200 + i)) break;
+        bool ok = mbar_wait(full + st, (i / NST) & 1, ab, 0x7280 + i) && mbar_wait(y_ready + u, (i >> 1) & 1, ab, 0x7200 + i);
         const bool fresh = first_of_span(i);
-        if (fresh && spans > 0 && !mbar_wait(u_free, (spans - 1) & 1, ab, 0x7300 + i)) break;
+        if (fresh && spans > 0) ok = ok && mbar_wait(u_free, (spans - 1) & 1, ab, 0x7300 + i);
+        if (!__all_sync(0xffffffffu, ok)) break;
         tc_fence_after();
         const uint32_t a_z = smem_u32(s_in + st * 2 * L::kTile + L::kTile), a_y = smem_u32(s_y + u * L::kTerms * L::kTile);
-#pragma unroll
+#pragma unroll 1
         for (int t = L::kTerms - 1; t >= 0; --t)
-#pragma unroll
+#pragma unroll 2
           for (int k = 0; k < C / 16; ++k)
-            umma(tmem, along_rows(a_y + t * L::kTile, k, C), along_rows(a_z, k, C), idesc, !(fresh && t == L::kTerms - 1 && k == 0));
-        umma_commit(empty + st);
-        umma_commit(y_free + u);
-        if (last_of_span(i)) { umma_commit(u_full); ++spans; }
+            umma_elect(tmem, along_rows(a_y + t * L::kTile, k, C), along_rows(a_z, k, C), idesc, !(fresh && t == L::kTerms - 1 && k == 0));
+        umma_commit_elect(empty + st);
+        umma_commit_elect(y_free + u);
+        if (last_of_span(i)) { umma_commit_elect(u_full); ++spans; }
       }
-      umma_commit(fin);          // nothing of the CTA is given back while a product runs
+      umma_commit_elect(fin);          // nothing of the CTA is given back while a product runs
       mbar_drain(fin, 0);
     }
   } else {
@@ -212,8 +214,7 @@ decay_tc_sums_kernel(const __grid_constant__ CUtensorMap tm_y, const __grid_cons
     float S[D / 2];
 #pragma unroll
     for (int j = 0; j < D / 2; ++j) S[j] = 0.f;
-    // (a wait that gave up does not leave the loop: the lanes of a warp, and the warps of a group, stay together to its end)
-    bool alive = true;
+    // (a wait that gave up does not leave the loop: the warps meet at barriers, and the status word has it)
     int spans = 0, in_span = 0;
     // forwards the last span may end with the sequence; backwards that one is the first
     const DecayPair whole = decay_pair(g, L::kSpan), last = decay_pair(g, count > 0 ? (end - r0) - (int64_t)(count - PER) * C : 0);
@@ -226,14 +227,16 @@ decay_tc_sums_kernel(const __grid_constant__ CUtensorMap tm_y, const __grid_cons
         if (!REV && span_end > end) span_end = end;
         in_span = REV ? (int)((i == 0 ? end : row_of(i) + C) - span_end) : (int)(span_end - row_of(i));
       }
-      alive &= mbar_wait(full + st, (i / NST) & 1, ab, 0x7400 + i);
-      if (i >= 2) alive &= mbar_wait(y_free + u, ((i >> 1) & 1) ^ 1, ab, 0x7500 + i);
-      __syncwarp();
+      if (warp == 0) {      // (one warp asks for all)
+        mbar_wait(full + st, (i / NST) & 1, ab, 0x7400 + i);
+        if (i >= 2) mbar_wait(y_free + u, ((i >> 1) & 1) ^ 1, ab, 0x7500 + i);
+      }
+      named_barrier(1, kGroup);
       uint8_t* src = s_in + st * 2 * L::kTile;
       uint8_t* dst = s_y + u * L::kTerms * L::kTile;
       const int64_t c0 = row_of(i);
       const int nv = end - c0 < C ? (int)(end - c0) : C;
-#pragma unroll
+#pragma unroll 1
       for (int q = 0; q < L::kTile / 16 / kGroup; ++q) {
         const int idx = threadIdx.x + q * kGroup, r = (idx >> 3) & (C - 1);
         uint4 terms[L::kTerms];
@@ -248,8 +251,8 @@ decay_tc_sums_kernel(const __grid_constant__ CUtensorMap tm_y, const __grid_cons
       fence_proxy_async();
       mbar_arrive_warp(y_ready + u);
       if (last_of_span(i)) {
-        alive &= mbar_wait(u_full, spans & 1, ab, 0x7600 + i);
-        __syncwarp();
+        if (warp == 0) mbar_wait(u_full, spans & 1, ab, 0x7600 + i);
+        named_barrier(1, kGroup);
         tc_fence_after();
         const DecayPair w = in_span == L::kSpan ? whole : last;      // (the first one's multiplies zeros)
 #pragma unroll
@@ -265,7 +268,7 @@ decay_tc_sums_kernel(const __grid_constant__ CUtensorMap tm_y, const __grid_cons
         ++spans;
       }
     }
-    if (alive && count > 0 && (D == 128 || lane < 16) && row < p.Dr) {
+    if (count > 0 && (D == 128 || lane < 16) && row < p.Dr) {
       float* to = p.sums + ((size_t)bh * p.ncut + cut) * p.Dr * p.Dr + row * p.Dr;
 #pragma unroll
       for (int j = 0; j < D / 2; j += 4)

@@ -45,7 +45,7 @@ static DecayPlan decay_plan(const fnb_decay_shape& s) {
   p.seg_rows = (units + best - 1) / best * kDecayUnit;
   p.nseg = (int)((s.seq_len + p.seg_rows - 1) / p.seg_rows);
   // two CTAs of the pass over the states fit on an SM
-  int64_t sub = std::max<int64_t>(1, std::min<int64_t>(2 * (int64_t)sms / std::max<int64_t>(1, BH * p.nseg), p.seg_rows / kDecayUnit));
+  int64_t sub = std::max<int64_t>(1, std::min<int64_t>(2 * (int64_t)sms / std::max<int64_t>(1, BH * std::max(1, p.nseg - 1)), p.seg_rows / kDecayUnit));
   p.sub_rows = (p.seg_rows / kDecayUnit + sub - 1) / sub * kDecayUnit;
   p.sub = (int)((p.seg_rows + p.sub_rows - 1) / p.sub_rows);
   return p;
@@ -243,7 +243,7 @@ static int decay_states(const DecayCall& c, const fnb_rows& y, const fnb_rows& z
   j.seg_rows = c.plan.seg_rows; j.sub_rows = c.plan.sub_rows; j.count = nrun;
   const dim3 grid((unsigned)((j.D * j.D + kThreads - 1) / kThreads), (unsigned)c.BH);
   L.begin();
-  FNB_CUDA(launch_pdl(reversed ? decay_join_kernel<true> : decay_join_kernel<false>, grid, dim3(kThreads), 0, c.stream, j));
+  FNB_CUDA(launch_pdl(reversed ? decay_join_kernel<true> : decay_join_kernel<false>, grid, dim3(kThreads), runs * sizeof(DecayJoinRun), c.stream, j));
   return L.end("decay_join");
 }
 
