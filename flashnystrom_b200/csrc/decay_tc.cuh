@@ -142,7 +142,7 @@ decay_tc_sums_kernel(const __grid_constant__ CUtensorMap tm_y, const __grid_cons
     *abort_word = 0;
     fence_mbar_init();
   }
-  if (warp == 0) { tmem_alloc(tmem_slot, D); tmem_relinquish(); }
+  if (warp == 0) { tmem_alloc(tmem_slot, 2 * D); tmem_relinquish(); }      // the products' sums, and what was taken out of them so far
   tc_fence_before();
   pdl_wait();
   const int64_t len = decay_len(p.seq_lens, b, p.N);
@@ -211,9 +211,7 @@ decay_tc_sums_kernel(const __grid_constant__ CUtensorMap tm_y, const __grid_cons
     const int quarter = warp & 3, half = warp >> 2;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
     const int row = D == 64 ? quarter * 16 + lane : quarter * 32 + lane;
-    float S[D / 2];
-#pragma unroll
-    for (int j = 0; j < D / 2; ++j) S[j] = 0.f;
+    const uint32_t t_sum = tmem + lane_base + half * (D / 2), t_state = t_sum + D;
     // (a wait that gave up does not leave the loop: the warps meet at barriers, and the status word has it)
     int spans = 0, in_span = 0;
     // forwards the last span may end with the sequence; backwards that one is the first
@@ -236,7 +234,7 @@ decay_tc_sums_kernel(const __grid_constant__ CUtensorMap tm_y, const __grid_cons
       uint8_t* dst = s_y + u * L::kTerms * L::kTile;
       const int64_t c0 = row_of(i);
       const int nv = end - c0 < C ? (int)(end - c0) : C;
-#pragma unroll 1
+#pragma unroll
       for (int q = 0; q < L::kTile / 16 / kGroup; ++q) {
         const int idx = threadIdx.x + q * kGroup, r = (idx >> 3) & (C - 1);
         uint4 terms[L::kTerms];
@@ -254,30 +252,40 @@ decay_tc_sums_kernel(const __grid_constant__ CUtensorMap tm_y, const __grid_cons
         if (warp == 0) mbar_wait(u_full, spans & 1, ab, 0x7600 + i);
         named_barrier(1, kGroup);
         tc_fence_after();
-        const DecayPair w = in_span == L::kSpan ? whole : last;      // (the first one's multiplies zeros)
-#pragma unroll
+        const DecayPair w = in_span == L::kSpan ? whole : last;      // (the first one has nothing to decay)
+#pragma unroll 1
         for (int q = 0; q < D / 32; ++q) {
-          float U[16];
-          tmem_ld16(tmem + lane_base + half * (D / 2) + q * 16, U);
+          float U[16], S[16];
+          tmem_ld16(t_sum + q * 16, U);
+          if (spans > 0) tmem_ld16(t_state + q * 16, S);
           tmem_ld_wait();
 #pragma unroll
-          for (int j = 0; j < 16; ++j) S[q * 16 + j] = decay_by(w, S[q * 16 + j]) + p.sum_scale * U[j];
+          for (int j = 0; j < 16; ++j) S[j] = (spans > 0 ? decay_by(w, S[j]) : 0.f) + p.sum_scale * U[j];
+          tmem_st16(t_state + q * 16, S);
         }
+        tmem_st_wait();
         tc_fence_before();
         mbar_arrive_warp(u_free);
         ++spans;
       }
     }
-    if (count > 0 && (D == 128 || lane < 16) && row < p.Dr) {
+    if (count > 0) {
       float* to = p.sums + ((size_t)bh * p.ncut + cut) * p.Dr * p.Dr + row * p.Dr;
+#pragma unroll 1
+      for (int q = 0; q < D / 32; ++q) {
+        float S[16];
+        const int col = half * (D / 2) + q * 16;
+        tmem_ld16(t_state + q * 16, S);
+        tmem_ld_wait();
+        if ((D == 128 || lane < 16) && row < p.Dr && col < p.Dr)
 #pragma unroll
-      for (int j = 0; j < D / 2; j += 4)
-        if (half * (D / 2) + j < p.Dr) *reinterpret_cast<float4*>(to + half * (D / 2) + j) = make_float4(S[j], S[j + 1], S[j + 2], S[j + 3]);
+          for (int j = 0; j < 16; j += 4) *reinterpret_cast<float4*>(to + col + j) = make_float4(S[j], S[j + 1], S[j + 2], S[j + 3]);
+      }
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 0) tmem_dealloc(tmem, D);
+  if (warp == 0) tmem_dealloc(tmem, 2 * D);
 }
 
 // ---- outputs -------------------------------------------------------------------------------------------------
