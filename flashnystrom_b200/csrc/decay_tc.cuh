@@ -103,19 +103,20 @@ __device__ __forceinline__ void scaled_terms(uint4 raw, float w, uint4* terms) {
 // ---- sums over runs ------------------------------------------------------------------------------------------
 // One CTA a run, two CTAs an SM: a group of eight warps forms the terms of y', double-buffered, one thread issues the products, which add up in
 // tensor memory over kSpan rows (weights reach back that far) before the group takes them out and decays what it has.
-// Two terms of fp16 and three of bf16 are 22 and 24 bits: the sums are FP32 sums.  Bound by HBM (y and z once).
-template <class T, int D> struct SumsCfg {
-  static constexpr int C = D == 64 ? 64 : 32, kStages = 3, kTerms = sizeof(T) == 2 && UmmaFmt<T>::v == 0 ? 2 : 3;
+// EXACT: two terms of fp16, three of bf16, 22 and 24 bits: the sums are FP32 sums, as a state that is handed out has to be.  Where the sums only join
+// segments, one term, as the chunks inside a segment have it: what an output gets from before its segment is then rounded once, like the rest.
+template <class T, int D, bool EXACT> struct SumsCfg {
+  static constexpr int C = D == 64 ? 64 : 32, kStages = 3, kTerms = !EXACT ? 1 : UmmaFmt<T>::v == 0 ? 2 : 3;
   static constexpr int kSpan = 256;
   static constexpr int kTile = C * D * 2;
   static constexpr int kThreads = kGroup + 64;
   static constexpr int kBytes = 1024 + kStages * 2 * kTile + 2 * kTerms * kTile + (kSpan + 1) * 4 + 256;
 };
 
-template <class T, int D, bool REV>
-__global__ void __launch_bounds__((SumsCfg<T, D>::kThreads), 2)
+template <class T, int D, bool EXACT, bool REV>
+__global__ void __launch_bounds__((SumsCfg<T, D, EXACT>::kThreads), 2)
 decay_tc_sums_kernel(const __grid_constant__ CUtensorMap tm_y, const __grid_constant__ CUtensorMap tm_z, DecayTcParams p) {
-  using L = SumsCfg<T, D>;
+  using L = SumsCfg<T, D, EXACT>;
   constexpr int C = L::C, NST = L::kStages, KB = D / 64, PER = L::kSpan / C;
   extern __shared__ uint8_t smem_raw[];
   pdl_trigger();

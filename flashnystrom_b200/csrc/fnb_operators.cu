@@ -182,21 +182,23 @@ static dtc::DecayTcParams decay_tc_params(const DecayCall& c, bool reversed) {
   return p;
 }
 template <bool REV>
-static int launch_tc_sums(const DecayCall& c, const fnb_rows& y, const fnb_rows& z, int cut0, int nrun, Launcher& L) {
-  return dispatch_decay_tc(c.s, [&](auto tag, auto d) -> int {
+static int launch_tc_sums(const DecayCall& c, const fnb_rows& y, const fnb_rows& z, int cut0, int nrun, bool exact, Launcher& L) {
+  const auto go = [&](auto tag, auto d, auto ex) -> int {
     using T = decltype(tag);
     constexpr int D = decltype(d)::value;
-    using Cfg = dtc::SumsCfg<T, D>;
+    constexpr bool EXACT = decltype(ex)::value;
+    using Cfg = dtc::SumsCfg<T, D, EXACT>;
     CUtensorMap my, mz;
     if (!make_rows_map(&my, y, c.s, Cfg::C) || !make_rows_map(&mz, z, c.s, Cfg::C)) return fail(FNB_ERR_CUDA, "cuTensorMapEncodeTiled failed");
     dtc::DecayTcParams p = decay_tc_params(c, REV);
     p.sums = c.sums; p.sub = c.plan.sub; p.sub_rows = c.plan.sub_rows; p.ncut = c.plan.runs(); p.cut0 = cut0; p.nrun = nrun;
-    auto kern = dtc::decay_tc_sums_kernel<T, D, REV>;
+    auto kern = dtc::decay_tc_sums_kernel<T, D, EXACT, REV>;
     if (int rc = set_smem(kern, Cfg::kBytes, c.max_smem, "decay_sums")) return rc;
     L.begin();
     FNB_CUDA(launch_pdl(kern, dim3((unsigned)(c.BH * nrun)), dim3(Cfg::kThreads), Cfg::kBytes, c.stream, my, mz, p));
     return L.end("decay_sums");
-  });
+  };
+  return dispatch_decay_tc(c.s, [&](auto tag, auto d) -> int { return exact ? go(tag, d, std::true_type{}) : go(tag, d, std::false_type{}); });
 }
 template <bool REV>
 static int launch_tc_form(const DecayCall& c, const DecayForm& f, const float* state_in, Launcher& L, const char* name) {
@@ -229,7 +231,7 @@ static int decay_states(const DecayCall& c, const fnb_rows& y, const fnb_rows& z
   // (without state_out nothing needs the sums of the last segment in time)
   const int runs = c.plan.runs(), nrun = state_out ? runs : runs - c.plan.sub, cut0 = state_out || !reversed ? 0 : c.plan.sub;
   if (decay_on_tensor_cores(c.s) && tma_rows(y, c.s) && tma_rows(z, c.s)) {
-    if (int rc = reversed ? launch_tc_sums<true>(c, y, z, cut0, nrun, L) : launch_tc_sums<false>(c, y, z, cut0, nrun, L)) return rc;
+    if (int rc = reversed ? launch_tc_sums<true>(c, y, z, cut0, nrun, state_out, L) : launch_tc_sums<false>(c, y, z, cut0, nrun, state_out, L)) return rc;
   } else {
     DecayParams p = decay_params(c, y, z);
     p.sum_scale = reversed ? c.s.scale : 1.f;
