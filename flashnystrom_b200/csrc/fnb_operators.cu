@@ -324,7 +324,9 @@ static NormPlan norm_plan(const fnb_norm_shape& s, bool wide, int sms) {
   p.span = p.per_row * n;
   const int64_t at_once = p.places / p.per_row;
   const int64_t row_blocks = (s.rows + at_once - 1) / at_once;
-  const int64_t slots = (int64_t)sms * std::max(1, 512 / p.threads);
+  // as many threads on an SM as their registers allow: up to 8, 16 and 32 elements a thread
+  const int per_thread = p.vec * p.items, resident = per_thread <= 8 ? 1024 : 768;
+  const int64_t slots = (int64_t)sms * std::max(1, resident / p.threads);
   p.ctas = p.gblocks * (int)std::max<int64_t>(1, std::min<int64_t>(row_blocks, slots / p.gblocks));
   return p;
 }
@@ -529,7 +531,7 @@ int fnb_norm_backward(const fnb_norm_bwd_args* a) {
   auto reduce = [&](auto tag) -> int {
     using P = decltype(tag);
     L.begin();
-    norm_reduce_kernel<P><<<(unsigned)((s.cols + 31) / 32), 256, 0, L.stream>>>(p.part, (P*)a->d_weight, (P*)a->d_bias, s.cols, p.n, n.per_row, n.gblocks,
+    norm_reduce_kernel<P><<<(unsigned)((s.cols + 31) / 32), 1024, 0, L.stream>>>(p.part, (P*)a->d_weight, (P*)a->d_bias, s.cols, p.n, n.per_row, n.gblocks,
                                                                                 n.ctas, n.span);
     return L.end("norm_reduce");
   };

@@ -56,6 +56,22 @@ __device__ __forceinline__ void norm_store(T* p, const float* v) {
   }
 }
 
+// VEC elements as they lie in memory
+template <class T, int VEC> struct NormRaw { uint4 v; };
+template <class T> struct NormRaw<T, 1> { T v; };
+template <class T, int VEC> __device__ __forceinline__ NormRaw<T, VEC> norm_raw(const T* p) { return *reinterpret_cast<const NormRaw<T, VEC>*>(p); }
+template <class T, int VEC> __device__ __forceinline__ NormRaw<T, VEC> norm_nothing() {
+  NormRaw<T, VEC> r;
+  if constexpr (VEC == 1) r.v = from_f<T>(0.f);
+  else r.v = make_uint4(0u, 0u, 0u, 0u);
+  return r;
+}
+template <class T, int VEC> __device__ __forceinline__ void norm_floats(const NormRaw<T, VEC>& r, float* v) {
+  const T* e = reinterpret_cast<const T*>(&r);
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) v[j] = to_f<T>(e[j]);
+}
+
 // Sum over the threads of a run.  BLOCK: the CTA's warps meet in `red` (two sets of 16 floats, used in turn).
 template <bool BLOCK>
 __device__ __forceinline__ float norm_sum(float v, int lanes, float* red, int& turn) {
@@ -113,18 +129,25 @@ __global__ void __launch_bounds__(BLOCK ? 512 : kNormThreads) norm_fwd_kernel(No
   const float inv_n = 1.f / (float)p.n;
   // (every thread of a warp goes round as often as the others: the sums are shuffles of whole warps)
   const int64_t first = BLOCK ? t.row : (int64_t)(blockIdx.x / p.gblocks) * (p.places / p.per_row);
-  for (int64_t base = first; base < p.rows; base += t.step) {
-    const int64_t row = BLOCK ? base : base + t.place / p.per_row;
-    const bool on = t.active && row < p.rows;
+  const int apart = BLOCK ? 0 : t.place / p.per_row;
+  // the next row's loads are under way while one is worked on
+  NormRaw<T, VEC> next[ITEMS];
+  const auto fetch = [&](int64_t row) {
     const T* x = static_cast<const T*>(p.x) + row * p.xs + (int64_t)t.group * p.n;
-    float v[EPT];
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
       const int c = (i * threads + t.lane) * VEC;
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) v[i * VEC + j] = 0.f;
-      if (on && c < p.n) norm_load<T, VEC>(x + c, v + i * VEC);
+      next[i] = t.active && row < p.rows && c < p.n ? norm_raw<T, VEC>(x + c) : norm_nothing<T, VEC>();
     }
+  };
+  fetch(first + apart);
+  for (int64_t base = first; base < p.rows; base += t.step) {
+    const int64_t row = base + apart;
+    const bool on = t.active && row < p.rows;
+    float v[EPT];
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) norm_floats<T, VEC>(next[i], v + i * VEC);
+    fetch(row + t.step);
     float s = 0.f;
 #pragma unroll
     for (int j = 0; j < EPT; ++j) s += v[j];
@@ -176,23 +199,34 @@ __global__ void __launch_bounds__(BLOCK ? 512 : kNormThreads) norm_bwd_kernel(No
   }
   const float inv_n = 1.f / (float)p.n;
   const int64_t first = BLOCK ? t.row : (int64_t)(blockIdx.x / p.gblocks) * (p.places / p.per_row);
-  for (int64_t base = first; base < p.rows; base += t.step) {
-    const int64_t row = BLOCK ? base : base + t.place / p.per_row;
+  const int apart = BLOCK ? 0 : t.place / p.per_row;
+  NormRaw<T, VEC> next_x[ITEMS], next_d[ITEMS];
+  float next_mean, next_r;
+  const auto fetch = [&](int64_t row) {
     const bool on = t.active && row < p.rows;
     const T* x = static_cast<const T*>(p.x) + row * p.xs + (int64_t)t.group * p.n;
     const T* dy = static_cast<const T*>(p.dy) + row * p.dys + (int64_t)t.group * p.n;
-    float v[EPT], d[EPT];
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
       const int c = (i * threads + t.lane) * VEC;
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) v[i * VEC + j] = d[i * VEC + j] = 0.f;
-      if (on && c < p.n) {
-        norm_load<T, VEC>(x + c, v + i * VEC);
-        norm_load<T, VEC>(dy + c, d + i * VEC);
-      }
+      next_x[i] = on && c < p.n ? norm_raw<T, VEC>(x + c) : norm_nothing<T, VEC>();
+      next_d[i] = on && c < p.n ? norm_raw<T, VEC>(dy + c) : norm_nothing<T, VEC>();
     }
-    const float mean = on ? p.mean[row * p.groups + t.group] : 0.f, r = on ? p.rstd[row * p.groups + t.group] : 0.f;
+    next_mean = on ? p.mean[row * p.groups + t.group] : 0.f;
+    next_r = on ? p.rstd[row * p.groups + t.group] : 0.f;
+  };
+  fetch(first + apart);
+  for (int64_t base = first; base < p.rows; base += t.step) {
+    const int64_t row = base + apart;
+    const bool on = t.active && row < p.rows;
+    float v[EPT], d[EPT];
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      norm_floats<T, VEC>(next_x[i], v + i * VEC);
+      norm_floats<T, VEC>(next_d[i], d + i * VEC);
+    }
+    const float mean = next_mean, r = next_r;
+    fetch(row + t.step);
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
@@ -259,17 +293,17 @@ __global__ void __launch_bounds__(BLOCK ? 512 : kNormThreads) norm_bwd_kernel(No
   }
 }
 
-// d_weight, d_bias: the CTAs' sums of a column.  32 columns a CTA, eight threads a column, each a run of CTAs in ascending order.
+// d_weight, d_bias: the CTAs' sums of a column.  32 columns a CTA, 32 threads a column, each a run of CTAs in ascending order.
 template <class P>
-__global__ void __launch_bounds__(256) norm_reduce_kernel(const float* __restrict__ part, P* __restrict__ dw, P* __restrict__ db, int cols, int n,
+__global__ void __launch_bounds__(1024) norm_reduce_kernel(const float* __restrict__ part, P* __restrict__ dw, P* __restrict__ db, int cols, int n,
                                                           int places, int gblocks, int ctas, int span) {
-  __shared__ float s[2][8][33];
+  __shared__ float s[2][32][33];
   const int c = blockIdx.x * 32 + threadIdx.x % 32, k = threadIdx.x / 32;
   float a = 0.f, b = 0.f;
   if (c < cols) {
     const int gb = gblocks == 1 ? 0 : c / n / places, col = c - gb * places * n, nrb = ctas / gblocks;
-    const int r0 = (int)((int64_t)nrb * k / 8), r1 = (int)((int64_t)nrb * (k + 1) / 8);
-#pragma unroll 4
+    const int r0 = (int)((int64_t)nrb * k / 32), r1 = (int)((int64_t)nrb * (k + 1) / 32);
+#pragma unroll 8
     for (int r = r0; r < r1; ++r) {
       const float* q = part + (size_t)(r * gblocks + gb) * 2 * span + col;
       a += q[0];
@@ -283,7 +317,7 @@ __global__ void __launch_bounds__(256) norm_reduce_kernel(const float* __restric
     const int which = threadIdx.x / 32, l = threadIdx.x % 32;
     float t = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) t += s[which][i][l];
+    for (int i = 0; i < 32; ++i) t += s[which][i][l];
     P* to = which ? db : dw;
     if (blockIdx.x * 32 + l < cols && to) to[blockIdx.x * 32 + l] = from_f<P>(t);
   }
