@@ -72,20 +72,32 @@ template <class T, int VEC> __device__ __forceinline__ void norm_floats(const No
   for (int j = 0; j < VEC; ++j) v[j] = to_f<T>(e[j]);
 }
 
-// Sum over the threads of a run.  BLOCK: the CTA's warps meet in `red` (two sets of 16 floats, used in turn).
-template <bool BLOCK>
-__device__ __forceinline__ float norm_sum(float v, int lanes, float* red, int& turn) {
+// Sum over `lanes` neighbouring threads of a warp.
+__device__ __forceinline__ float norm_lanes(float v, int lanes) {
   for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if (BLOCK) {
-    float* r = red + 16 * turn;
-    turn ^= 1;
-    if ((threadIdx.x & 31) == 0) r[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = 0.f;
-    const int warps = blockDim.x >> 5;
-    for (int i = 0; i < warps; ++i) v += r[i];
-  }
   return v;
+}
+// Two values of every warp of the CTA to all its threads, added up by f(first, second) in the warps' order.  `red`: two sets of 32 floats, used in turn, so
+// that one barrier is enough.
+template <class F>
+__device__ __forceinline__ void norm_block(float a, float b, float* red, int& turn, F&& f) {
+  float* r = red + 32 * turn;
+  turn ^= 1;
+  if ((threadIdx.x & 31) == 0) {
+    r[threadIdx.x >> 5] = a;
+    r[16 + (threadIdx.x >> 5)] = b;
+  }
+  __syncthreads();
+  const int warps = blockDim.x >> 5;
+  for (int i = 0; i < warps; ++i) f(r[i], r[16 + i], i);
+}
+// Columns that a warp of a CTA-wide run holds.
+template <int VEC, int ITEMS>
+__device__ __forceinline__ int norm_warp_cols(int n, int warp, int threads) {
+  int cols = 0;
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) cols += max(0, min(32 * VEC, n - (i * threads + 32 * warp) * VEC));
+  return cols;
 }
 
 struct NormPlace {
@@ -107,11 +119,15 @@ __device__ __forceinline__ NormPlace norm_place(const NormParams& p) {
   return t;
 }
 
+// threads that an SM should hold at once, by elements a thread: what keeps enough loads under way, and what their registers allow
+__host__ __device__ constexpr int norm_resident(bool backward, int elements) {
+  return elements <= 8 ? 1024 : elements <= 16 && !backward ? 768 : 512;
+}
 template <class T, bool PF32, int VEC, int ITEMS, bool BLOCK>
-__global__ void __launch_bounds__(BLOCK ? 512 : kNormThreads) norm_fwd_kernel(NormParams p) {
+__global__ void __launch_bounds__(BLOCK ? 512 : kNormThreads, BLOCK ? norm_resident(false, VEC * ITEMS) / 512 : norm_resident(false, VEC * ITEMS) / kNormThreads) norm_fwd_kernel(NormParams p) {
   using P = typename NormParam<T, PF32>::type;
   constexpr int EPT = VEC * ITEMS;
-  __shared__ float red[32];
+  __shared__ float red[64];
   int turn = 0;
   const NormPlace t = norm_place<BLOCK>(p);
   const int threads = BLOCK ? blockDim.x : p.lanes, lanes = BLOCK ? 32 : p.lanes;
@@ -125,6 +141,15 @@ __global__ void __launch_bounds__(BLOCK ? 512 : kNormThreads) norm_fwd_kernel(No
       if (p.w) norm_load<P, VEC>(static_cast<const P*>(p.w) + (int64_t)t.group * p.n + c, w + i * VEC);
       if (p.b) norm_load<P, VEC>(static_cast<const P*>(p.b) + (int64_t)t.group * p.n + c, b + i * VEC);
     }
+  }
+  __shared__ float warp_cols[16], warp_inv[16];
+  if (BLOCK) {
+    if (threadIdx.x < (blockDim.x >> 5)) {
+      const int cols = norm_warp_cols<VEC, ITEMS>(p.n, threadIdx.x, threads);
+      warp_cols[threadIdx.x] = (float)cols;
+      warp_inv[threadIdx.x] = cols ? 1.f / (float)cols : 0.f;
+    }
+    __syncthreads();
   }
   const float inv_n = 1.f / (float)p.n;
   // (every thread of a warp goes round as often as the others: the sums are shuffles of whole warps)
@@ -151,18 +176,34 @@ __global__ void __launch_bounds__(BLOCK ? 512 : kNormThreads) norm_fwd_kernel(No
     float s = 0.f;
 #pragma unroll
     for (int j = 0; j < EPT; ++j) s += v[j];
-    const float mean = norm_sum<BLOCK>(s, lanes, red, turn) * inv_n;
-    s = 0.f;
+    s = norm_lanes(s, lanes);
+    // (a warp of a CTA-wide run: about its own mean first; the warps' sums of squares are then moved to the mean of all)
+    float mean = s * (BLOCK ? warp_inv[threadIdx.x >> 5] : inv_n), q = 0.f;
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
       const bool in = (i * threads + t.lane) * VEC < p.n;
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
         v[i * VEC + j] = in ? v[i * VEC + j] - mean : 0.f;
-        s = fmaf(v[i * VEC + j], v[i * VEC + j], s);
+        q = fmaf(v[i * VEC + j], v[i * VEC + j], q);
       }
     }
-    const float r = 1.f / sqrtf(norm_sum<BLOCK>(s, lanes, red, turn) * inv_n + p.eps);
+    q = norm_lanes(q, lanes);
+    if (BLOCK) {
+      const float own = mean;
+      float all = 0.f, squares = 0.f;
+      norm_block(s, q, red, turn, [&](float a, float b, int) { all += a; squares += b; });
+      mean = all * inv_n;
+      const float* r = red + 32 * (turn ^ 1);
+      for (int w = 0; w < (int)(blockDim.x >> 5); ++w) {
+        const float off = r[w] * warp_inv[w] - mean;
+        squares = fmaf(warp_cols[w] * off, off, squares);
+      }
+      q = squares;
+#pragma unroll
+      for (int j = 0; j < EPT; ++j) v[j] += own - mean;
+    }
+    const float r = 1.f / sqrtf(q * inv_n + p.eps);
     if (!on) continue;
     T* y = static_cast<T*>(p.y) + row * p.ys + (int64_t)t.group * p.n;
 #pragma unroll
@@ -181,14 +222,15 @@ __global__ void __launch_bounds__(BLOCK ? 512 : kNormThreads) norm_fwd_kernel(No
 
 // With u = d_y w and xh = (x - mean) rstd:  d_x = rstd (u - mean(u) - xh mean(u xh)).
 template <class T, bool PF32, int VEC, int ITEMS, bool BLOCK>
-__global__ void __launch_bounds__(BLOCK ? 512 : kNormThreads) norm_bwd_kernel(NormParams p) {
+__global__ void __launch_bounds__(BLOCK ? 512 : kNormThreads, BLOCK ? norm_resident(true, VEC * ITEMS) / 512 : norm_resident(true, VEC * ITEMS) / kNormThreads) norm_bwd_kernel(NormParams p) {
   using P = typename NormParam<T, PF32>::type;
   constexpr int EPT = VEC * ITEMS;
-  __shared__ float red[32];
+  __shared__ float red[64];
   extern __shared__ float sums[];      // [2][span]
   int turn = 0;
   const NormPlace t = norm_place<BLOCK>(p);
   const int threads = BLOCK ? blockDim.x : p.lanes, lanes = BLOCK ? 32 : p.lanes;
+  pdl_trigger();
   float w[EPT], dw[EPT], db[EPT];
 #pragma unroll
   for (int i = 0; i < ITEMS; ++i) {
@@ -243,8 +285,16 @@ __global__ void __launch_bounds__(BLOCK ? 512 : kNormThreads) norm_bwd_kernel(No
       }
     }
     if (!p.y) continue;      // (the same for all threads)
-    s1 = norm_sum<BLOCK>(s1, lanes, red, turn) * inv_n;
-    s2 = norm_sum<BLOCK>(s2, lanes, red, turn) * inv_n;
+    s1 = norm_lanes(s1, lanes);
+    s2 = norm_lanes(s2, lanes);
+    if (BLOCK) {
+      float a1 = 0.f, a2 = 0.f;
+      norm_block(s1, s2, red, turn, [&](float a, float b, int) { a1 += a; a2 += b; });
+      s1 = a1;
+      s2 = a2;
+    }
+    s1 *= inv_n;
+    s2 *= inv_n;
     if (!on) continue;
     T* dx = static_cast<T*>(p.y) + row * p.ys + (int64_t)t.group * p.n;
 #pragma unroll
@@ -293,33 +343,29 @@ __global__ void __launch_bounds__(BLOCK ? 512 : kNormThreads) norm_bwd_kernel(No
   }
 }
 
-// d_weight, d_bias: the CTAs' sums of a column.  32 columns a CTA, 32 threads a column, each a run of CTAs in ascending order.
+// d_weight (blockIdx.y 0) or d_bias (1): the CTAs' sums of a column.  32 columns a CTA, 32 threads a column, each a run of CTAs in ascending order.
 template <class P>
 __global__ void __launch_bounds__(1024) norm_reduce_kernel(const float* __restrict__ part, P* __restrict__ dw, P* __restrict__ db, int cols, int n,
-                                                          int places, int gblocks, int ctas, int span) {
-  __shared__ float s[2][32][33];
-  const int c = blockIdx.x * 32 + threadIdx.x % 32, k = threadIdx.x / 32;
-  float a = 0.f, b = 0.f;
+                                                           int places, int gblocks, int ctas, int span) {
+  __shared__ float s[32][33];
+  pdl_wait();
+  const int l = threadIdx.x % 32, k = threadIdx.x / 32, c = blockIdx.x * 32 + l;
+  P* to = blockIdx.y ? db : dw;
+  if (!to) return;
+  float a = 0.f;
   if (c < cols) {
     const int gb = gblocks == 1 ? 0 : c / n / places, col = c - gb * places * n, nrb = ctas / gblocks;
     const int r0 = (int)((int64_t)nrb * k / 32), r1 = (int)((int64_t)nrb * (k + 1) / 32);
 #pragma unroll 8
-    for (int r = r0; r < r1; ++r) {
-      const float* q = part + (size_t)(r * gblocks + gb) * 2 * span + col;
-      a += q[0];
-      b += q[span];
-    }
+    for (int r = r0; r < r1; ++r) a += part[((size_t)(r * gblocks + gb) * 2 + blockIdx.y) * span + col];
   }
-  s[0][k][threadIdx.x % 32] = a;
-  s[1][k][threadIdx.x % 32] = b;
+  s[k][l] = a;
   __syncthreads();
-  if (threadIdx.x < 64) {
-    const int which = threadIdx.x / 32, l = threadIdx.x % 32;
+  if (k == 0 && c < cols) {
     float t = 0.f;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) t += s[which][i][l];
-    P* to = which ? db : dw;
-    if (blockIdx.x * 32 + l < cols && to) to[blockIdx.x * 32 + l] = from_f<P>(t);
+    for (int i = 0; i < 32; ++i) t += s[i][l];
+    to[c] = from_f<P>(t);
   }
 }
 
