@@ -65,6 +65,18 @@ __device__ __forceinline__ DecayPair decay_pair(double g, int64_t n) {
 }
 __device__ __forceinline__ float decay_by(const DecayPair& p, float s) { return s == 0.f ? 0.f : fmaf(s, p.hi, s * p.lo); }
 
+// two FP32 values in one instruction
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
+  return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)), "l"(*reinterpret_cast<uint64_t*>(&c)));
+  return *reinterpret_cast<float2*>(&d);
+}
+
 // ---- chunked form ------------------------------------------------------------------------------------------
 // A CTA walks one run of rows, C at a time; tiles in shared memory as FP32.  Thread (ty, tx) of a 16 x 16 grid holds rows
 // ty + 16 i of the score and output tiles and a (D / 16)^2 piece of the state.  Bound by the shared-memory loads of its FP32 products.
@@ -109,6 +121,16 @@ template <int CW> __device__ __forceinline__ void decay_lds(const float* p, floa
   }
 }
 
+// o += a z, CW values
+template <int CW> __device__ __forceinline__ void decay_axpy(float a, const float* z, float* o) {
+  if (CW == 1) {
+    o[0] = fmaf(a, z[0], o[0]);
+  } else {
+#pragma unroll
+    for (int j = 0; j + 1 < CW; j += 2)
+      *reinterpret_cast<float2*>(o + j) = fma2(make_float2(a, a), *reinterpret_cast<const float2*>(z + j), *reinterpret_cast<const float2*>(o + j));
+  }
+}
 template <class T, int D, bool REV, bool OUT>
 __global__ void __launch_bounds__(kThreads, D <= 64 ? 2 : 1) decay_chunk_kernel(DecayParams p) {
   using L = DecaySmem<D>;
@@ -139,7 +161,7 @@ __global__ void __launch_bounds__(kThreads, D <= 64 ? 2 : 1) decay_chunk_kernel(
     const int64_t z0 = r0 > end ? r0 : end;
     for (int64_t i = threadIdx.x; i < (r1 - z0) * D; i += kThreads) out[(z0 + i / D) * p.out.sn + i % D] = from_f<T>(0.f);
   }
-  float S[CG][CW][CG][CW];
+  __align__(8) float S[CG][CW][CG][CW];
 #pragma unroll
   for (int a = 0; a < CG; ++a)
 #pragma unroll
@@ -174,7 +196,12 @@ __global__ void __launch_bounds__(kThreads, D <= 64 ? 2 : 1) decay_chunk_kernel(
 #pragma unroll
             for (int j = 0; j < CW; ++j) ss[(a * 64 + ty * CW + i) * LD + c * 64 + tx * CW + j] = S[a][i][c][j];
       __syncthreads();
-      float acc[4][4] = {};
+      float2 acc[4][4];      // even and odd columns
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = make_float2(0.f, 0.f);
+#pragma unroll 2
       for (int k = 0; k < D; k += 4) {
         float4 xv[4], yv[4];
 #pragma unroll
@@ -185,18 +212,20 @@ __global__ void __launch_bounds__(kThreads, D <= 64 ? 2 : 1) decay_chunk_kernel(
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            acc[i][j] = fmaf(xv[i].w, yv[j].w, fmaf(xv[i].z, yv[j].z, fmaf(xv[i].y, yv[j].y, fmaf(xv[i].x, yv[j].x, acc[i][j]))));
+          for (int j = 0; j < 4; ++j) {
+            acc[i][j] = fma2(make_float2(xv[i].x, xv[i].y), make_float2(yv[j].x, yv[j].y), acc[i][j]);
+            acc[i][j] = fma2(make_float2(xv[i].z, xv[i].w), make_float2(yv[j].z, yv[j].w), acc[i][j]);
+          }
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int s = ty + 16 * i, t = tx + 16 * j, d = REV ? t - s : s - t;
-          ps[s * LP + t] = d >= 0 ? acc[i][j] * pw[d] : 0.f;
+          ps[s * LP + t] = d >= 0 ? (acc[i][j].x + acc[i][j].y) * pw[d] : 0.f;
         }
       __syncthreads();
-      float o[4][CG][CW], q[4][CG][CW];
+      __align__(8) float o[4][CG][CW], q[4][CG][CW];
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -214,13 +243,11 @@ __global__ void __launch_bounds__(kThreads, D <= 64 ? 2 : 1) decay_chunk_kernel(
           for (int u = 0; u < 4; ++u)
 #pragma unroll
             for (int c = 0; c < CG; ++c) {
-              float zv[CW];
+              __align__(8) float zv[CW];
               decay_lds<CW>(zs + (t + u) * LD + c * 64 + tx * CW, zv);
 #pragma unroll
               for (int i = 0; i < 4; ++i)
-                if (REV ? i <= tb : i >= tb)
-#pragma unroll
-                  for (int j = 0; j < CW; ++j) o[i][c][j] = fmaf(pv[i][u], zv[j], o[i][c][j]);
+                if (REV ? i <= tb : i >= tb) decay_axpy<CW>(pv[i][u], zv, o[i][c]);
             }
         }
       for (int k = 0; k < D; k += 4) {
@@ -231,12 +258,10 @@ __global__ void __launch_bounds__(kThreads, D <= 64 ? 2 : 1) decay_chunk_kernel(
         for (int u = 0; u < 4; ++u)
 #pragma unroll
           for (int c = 0; c < CG; ++c) {
-            float sv[CW];
+            __align__(8) float sv[CW];
             decay_lds<CW>(ss + (k + u) * LD + c * 64 + tx * CW, sv);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-              for (int j = 0; j < CW; ++j) q[i][c][j] = fmaf(xv[i][u], sv[j], q[i][c][j]);
+            for (int i = 0; i < 4; ++i) decay_axpy<CW>(xv[i][u], sv, q[i][c]);
           }
       }
 #pragma unroll
@@ -262,8 +287,9 @@ __global__ void __launch_bounds__(kThreads, D <= 64 ? 2 : 1) decay_chunk_kernel(
     } else {
       __syncthreads();
     }
+    if (OUT && ci + 1 == chunks) break;      // (nothing needs the state behind the last)
     // the state: U = sum over the chunk's rows, then S = exp(g nv) S + U
-    float U[CG][CW][CG][CW];
+    __align__(8) float U[CG][CW][CG][CW];
 #pragma unroll
     for (int a = 0; a < CG; ++a)
 #pragma unroll
@@ -275,7 +301,7 @@ __global__ void __launch_bounds__(kThreads, D <= 64 ? 2 : 1) decay_chunk_kernel(
 #pragma unroll 4
     for (int t = 0; t < nv; ++t) {
       const float w = p.sum_scale * pw[REV ? t + 1 : nv - 1 - t];
-      float yv[CG][CW], zv[CG][CW];
+      __align__(8) float yv[CG][CW], zv[CG][CW];
 #pragma unroll
       for (int a = 0; a < CG; ++a) {
         decay_lds<CW>(ys + t * LD + a * 64 + ty * CW, yv[a]);
@@ -288,9 +314,7 @@ __global__ void __launch_bounds__(kThreads, D <= 64 ? 2 : 1) decay_chunk_kernel(
 #pragma unroll
         for (int i = 0; i < CW; ++i)
 #pragma unroll
-          for (int c = 0; c < CG; ++c)
-#pragma unroll
-            for (int j = 0; j < CW; ++j) U[a][i][c][j] = fmaf(yv[a][i], zv[c][j], U[a][i][c][j]);
+          for (int c = 0; c < CG; ++c) decay_axpy<CW>(yv[a][i], zv[c], U[a][i][c]);
     }
     const DecayPair by_nv = nv == C ? full : decay_pair(g, nv);
 #pragma unroll

@@ -52,17 +52,6 @@ struct DecayTcParams {
   int* status;
 };
 
-// two FP32 values in one instruction
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
-  return *reinterpret_cast<float2*>(&d);
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)), "l"(*reinterpret_cast<uint64_t*>(&c)));
-  return *reinterpret_cast<float2*>(&d);
-}
 template <class T> __device__ __forceinline__ float2 unpack2(uint32_t u);
 template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t u) { return __half22float2(*reinterpret_cast<__half2*>(&u)); }
 template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t u) {
@@ -110,7 +99,7 @@ template <class T, int D, bool EXACT> struct SumsCfg {
   static constexpr int kSpan = 256;
   static constexpr int kTile = C * D * 2;
   static constexpr int kThreads = kGroup + 64;
-  static constexpr int kBytes = 1024 + kStages * 2 * kTile + 2 * kTerms * kTile + (kSpan + 1) * 4 + 256;
+  static constexpr int kBytes = 1024 + kStages * 2 * kTile + 2 * kTerms * kTile + (kSpan + 1) * 4 + 16 + 256;
 };
 
 template <class T, int D, bool EXACT, bool REV>
@@ -123,7 +112,7 @@ decay_tc_sums_kernel(const __grid_constant__ CUtensorMap tm_y, const __grid_cons
   uint8_t* s_in = at1024(smem_raw);                      // stages of [y | z]
   uint8_t* s_y = s_in + NST * 2 * L::kTile;               // two buffers of kTerms tiles
   float* pw = reinterpret_cast<float*>(s_y + 2 * L::kTerms * L::kTile);
-  uint64_t* bars = reinterpret_cast<uint64_t*>((reinterpret_cast<uintptr_t>(pw + L::kSpan + 1) + 15) & ~(uintptr_t)15);
+  uint64_t* bars = reinterpret_cast<uint64_t*>((reinterpret_cast<uintptr_t>(pw + L::kSpan + 1 + 4) + 15) & ~(uintptr_t)15);
   uint64_t* full = bars;             // [3]
   uint64_t* empty = bars + 3;        // [3]
   uint64_t* y_ready = bars + 6;      // [2]
@@ -151,12 +140,16 @@ decay_tc_sums_kernel(const __grid_constant__ CUtensorMap tm_y, const __grid_cons
   const int64_t r1 = decay_cut_end(p.seg_rows, p.sub, p.sub_rows, p.N, cut);
   const int64_t end = r1 < len ? r1 : len;
   const double g = decay_log(p.log_decay[h]);
+  const int count = r0 < end ? (int)((end - r0 + C - 1) / C) : 0;
   for (int i = threadIdx.x; i <= L::kSpan; i += L::kThreads) pw[i] = (float)exp(g * i);
+  // what a span decays the sums before it by: a whole one, and (forwards) the last, which may end with the sequence; backwards that one is the first
+  DecayPair* s_pair = reinterpret_cast<DecayPair*>(pw + L::kSpan + 1);
+  if (threadIdx.x >= L::kThreads - 2)
+    s_pair[threadIdx.x - (L::kThreads - 2)] = decay_pair(g, threadIdx.x == L::kThreads - 2 ? L::kSpan : count > 0 ? (end - r0) - (int64_t)(count - PER) * C : 0);
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   Abort ab{abort_word, p.status};
-  const int count = r0 < end ? (int)((end - r0 + C - 1) / C) : 0;
   // Chunks are taken in the order of time; a span is PER chunks of it, the last one (backwards: the first) may be shorter.
   const auto row_of = [&](int i) { return r0 + (int64_t)(REV ? count - 1 - i : i) * C; };
   // spans are aligned to the end of the run in time, so that each but the first is whole
@@ -215,8 +208,7 @@ decay_tc_sums_kernel(const __grid_constant__ CUtensorMap tm_y, const __grid_cons
     const uint32_t t_sum = tmem + lane_base + half * (D / 2), t_state = t_sum + D;
     // (a wait that gave up does not leave the loop: the warps meet at barriers, and the status word has it)
     int spans = 0, in_span = 0;
-    // forwards the last span may end with the sequence; backwards that one is the first
-    const DecayPair whole = decay_pair(g, L::kSpan), last = decay_pair(g, count > 0 ? (end - r0) - (int64_t)(count - PER) * C : 0);
+    const DecayPair whole = s_pair[0], last = s_pair[1];
     int64_t span_end = 0;        // forwards: the row behind the span; backwards: its first row
     for (int i = 0; i < count; ++i) {
       const int st = i % NST, u = i & 1;
@@ -306,7 +298,7 @@ template <int D> struct MainCfg {
   static constexpr int kInters = D == 64 ? 2 : 1;                        // accumulators of x S
   static constexpr int kThreads = 2 * kGroup + 128;
   // (relies on the dynamic shared window being 1024-byte aligned, which is checked)
-  static constexpr int kBytes = (kSlots + kTerms) * kTile + 2 * kS + 32 * 16 * 4 + (kC + 4) * 4 + 80 + (2 * kSlots + 24) * 8 + 16;
+  static constexpr int kBytes = (kSlots + kTerms) * kTile + 2 * kS + 32 * 16 * 4 + (kC + 4) * 4 + 96 + (2 * kSlots + 24) * 8 + 16;
   static_assert(kBytes <= 232448, "shared memory of one CTA");
   // Tensor-memory columns.  The packed scores of columns 0-63 begin at kPacked, those of 64-127 kPackedHalf behind; with heads of 128 they take the place
   // of the scores that they come from, a thread's own.
@@ -343,7 +335,8 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
   float* s_pow = s_diag + 32 * 16;                    // powers of exp(g): forwards that of C - k at k, backwards that of k
   float* s_mul = s_pow + C + 4;                       // [4]: what x S of chunk i is to be multiplied by, in s_mul[i & 3] (B may be two ahead)
   float* s_max = s_mul + 4;                           // [16]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(s_max + 16);
+  DecayPair* s_pair = reinterpret_cast<DecayPair*>(s_max + 16);      // [2]: what a chunk decays the state by, a whole one and the first
+  uint64_t* bars = reinterpret_cast<uint64_t*>(s_pair + 2);
   uint64_t* full = bars;             // [NS]
   uint64_t* empty = full + NS;       // [NS]
   uint64_t* p_full = empty + NS;     // [4]: scores of chunk i in p_full[i & 3]; B waits for them too and may be two chunks behind
@@ -382,21 +375,25 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
   const int64_t r1 = r0 + p.seg_rows < p.N ? r0 + p.seg_rows : p.N;
   const int64_t end = r1 < len ? r1 : len;
   const double g = decay_log(p.log_decay[h]);
-  for (int i = threadIdx.x; i <= C; i += L::kThreads) s_pow[REV ? i : C - i] = (float)exp(g * i);
-  // Row r of a 32 x 32 block on the diagonal: forwards the weight of column j < 16 is s_diag[r][j], of column 16 + j s_diag[r - 16][j]; backwards of
-  // column 16 + j s_diag[r][j], of column j < 16 s_diag[r + 16][j]; what such an index would leave the table with is behind the mask.
-  // (16-byte pieces of a row are stored at piece ^ (row / 2) % 4: eight rows read at once fall on different banks)
-  for (int i = threadIdx.x; i < 32 * 16; i += L::kThreads) {
-    const int row = i / 16, j = i % 16, d = REV ? 16 + j - row : row - j;
-    s_diag[row * 16 + ((j / 4) ^ (row / 2 % 4)) * 4 + j % 4] = d >= 0 ? p.scale * (float)exp(g * d) : 0.f;
-  }
+  const int count = r0 < end ? (int)((end - r0 + C - 1) / C) : 0;
+  const auto row_of = [&](int i) { return r0 + (int64_t)(REV ? count - 1 - i : i) * C; };
+  if (threadIdx.x <= C) s_pow[REV ? threadIdx.x : C - threadIdx.x] = (float)exp(g * threadIdx.x);
+  // (only the last chunk in space is not whole: backwards in time the first, forwards one whose state nobody needs)
+  if (threadIdx.x >= L::kThreads - 2) s_pair[threadIdx.x - (L::kThreads - 2)] = decay_pair(g, REV && count > 0 && threadIdx.x == L::kThreads - 1 ? end - row_of(0) : C);
   const auto power = [&](int n) { return s_pow[REV ? n : C - n]; };
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   Abort ab{abort_word, p.status};
-  const int count = r0 < end ? (int)((end - r0 + C - 1) / C) : 0;
-  const auto row_of = [&](int i) { return r0 + (int64_t)(REV ? count - 1 - i : i) * C; };
+  // Row r of a 32 x 32 block on the diagonal: forwards the weight of column j < 16 is s_diag[r][j], of column 16 + j s_diag[r - 16][j]; backwards of
+  // column 16 + j s_diag[r][j], of column j < 16 s_diag[r + 16][j]; what such an index would leave the table with is behind the mask.
+  // (16-byte pieces of a row are stored at piece ^ (row / 2) % 4: eight rows read at once fall on different banks)
+  if (warp < 8) {
+    for (int i = threadIdx.x; i < 32 * 16; i += kGroup) {
+      const int row = i / 16, j = i % 16, d = REV ? 16 + j - row : row - j;
+      s_diag[row * 16 + ((j / 4) ^ (row / 2 % 4)) * 4 + j % 4] = d >= 0 ? p.scale * power(d) : 0.f;
+    }
+  }
   // The last rows of a tile lie past the sequence's length, but not past the tensor: they hold anything, and are cleared.
   const int dirty = end == len && len < p.N && (end - r0) % C != 0 ? (REV ? 0 : count - 1) : -1;
   const auto tile = [&](int n) { return s_in + (n % NS) * L::kTile; };      // n = 3 i + 0, 1, 2: y, x, z of chunk i
@@ -633,8 +630,7 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
     const int row = D == 64 ? quarter * 16 + lane : quarter * 32 + lane;
     const bool owner = D == 128 || lane < 16;
     constexpr int HC = D / 2;
-    // (only the last chunk in space is not whole: backwards in time the first, forwards one whose state nobody needs)
-    const DecayPair full_chunk = decay_pair(g, C), first_chunk = REV && count > 0 ? decay_pair(g, end - row_of(0)) : full_chunk;
+    const DecayPair full_chunk = s_pair[0], first_chunk = s_pair[1];
     const uint32_t t_state = tmem + L::kState + lane_base + half * HC;
     // the state that enters the segment, without the factor of the sums, to tensor memory
     if (count > 0) {
