@@ -43,14 +43,21 @@ struct DecayTcParams {
   const int32_t* seq_lens;
   const float* state_in;      // main kernel: [BH][nseg][Dr][Dr] or null
   float* sums;                // sums kernel: [BH][ncut][Dr][Dr]
-  void* out;                  // rows that do not count are cleared by plain stores
-  int64_t ob, oh, on;
   int64_t N, seg_rows, sub_rows;
   int H, Dr, sub, ncut, cut0, nrun;
   float scale, inter, sum_scale;
-  int transposed;
   int* status;
 };
+// One form of a launch of the main kernel.
+struct DecayTcForm {
+  CUtensorMap x, y, z, o;
+  void* out;                  // rows that do not count are cleared by plain stores
+  int64_t ob, oh, on;
+  int transposed;             // the state is read as its transpose
+};
+// Two forms that read mostly the same rows (dv and dk: q and do in both, k or v) run side by side, the same segment of both in neighbouring CTAs: what one
+// reads the other finds in L2 (B=4, H=16, N=16384, D=128: 425 us one after the other, see kForms below for both together).
+template <int FORMS> struct DecayTcForms { DecayTcForm f[FORMS]; };
 
 template <class T> __device__ __forceinline__ float2 unpack2(uint32_t u);
 template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t u) { return __half22float2(*reinterpret_cast<__half2*>(&u)); }
@@ -315,10 +322,8 @@ __device__ __forceinline__ void umma_ta_elect(uint32_t d_tmem, uint32_t a_tmem, 
       : "memory");
 }
 
-template <class T, int D, bool REV>
-__global__ void __launch_bounds__(MainCfg<D>::kThreads, 1)
-decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_y, const __grid_constant__ CUtensorMap tm_z,
-                const __grid_constant__ CUtensorMap tm_o, DecayTcParams p) {
+template <class T, int D, bool REV, int FORMS>
+__global__ void __launch_bounds__(MainCfg<D>::kThreads, 1) decay_tc_kernel(const __grid_constant__ DecayTcForms<FORMS> forms, DecayTcParams p) {
   using L = MainCfg<D>;
   constexpr int C = kC, NS = L::kSlots, KB = D / 64, NI = L::kInters;
   constexpr bool F16 = UmmaFmt<T>::v == 0;
@@ -356,7 +361,8 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
   int* abort_word = reinterpret_cast<int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int bh = blockIdx.x / p.ncut, cut = blockIdx.x % p.ncut, b = bh / p.H, h = bh % p.H;
+  const DecayTcForm& form = forms.f[FORMS == 1 ? 0 : blockIdx.x % FORMS];
+  const int segment = blockIdx.x / FORMS, bh = segment / p.ncut, cut = segment % p.ncut, b = bh / p.H, h = bh % p.H;
   if (threadIdx.x == 0) {
     for (int i = 0; i < NS; ++i) { mbar_init(full + i, 1); mbar_init(empty + i, 2); }
     for (int i = 0; i < 4; ++i) { mbar_init(p_full + i, 1); mbar_init(t_ready + i, kGroup / 32); }
@@ -402,10 +408,10 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
   if (warp == 19) {
     // ---- output tiles, from x's place to their rows; the place is then free
     if (lane == 0 && count > 0) {
-      tma_prefetch_desc(&tm_o);
+      tma_prefetch_desc(&form.o);
       for (int i = 0; i < count; ++i) {
         if (!mbar_wait(t_ready + (i & 3), (i >> 2) & 1, ab, 0x8080 + i)) break;
-        for (int kb = 0; kb < KB; ++kb) tma_store_4d_h(&tm_o, tile(3 * i + 1) + kb * (C * 128), kb * 64, (int)row_of(i), h, b, 0);
+        for (int kb = 0; kb < KB; ++kb) tma_store_4d_h(&form.o, tile(3 * i + 1) + kb * (C * 128), kb * 64, (int)row_of(i), h, b, 0);
         tma_store_commit();
         tma_store_wait_read();
         mbar_arrive(empty + (3 * i + 1) % NS);
@@ -415,14 +421,14 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
     }
   } else if (warp == 16) {
     if (lane == 0 && count > 0) {
-      tma_prefetch_desc(&tm_x);
-      tma_prefetch_desc(&tm_y);
-      tma_prefetch_desc(&tm_z);
+      tma_prefetch_desc(&form.x);
+      tma_prefetch_desc(&form.y);
+      tma_prefetch_desc(&form.z);
       int armed = 0;
       for (int n = 0; n < 3 * count; ++n) {
         if (!mbar_wait(empty + n % NS, ((n / NS) & 1) ^ 1, ab, 0x8100 + n)) break;
         mbar_expect_tx(full + n % NS, L::kTile);
-        const CUtensorMap* m = n % 3 == 0 ? &tm_y : n % 3 == 1 ? &tm_x : &tm_z;
+        const CUtensorMap* m = n % 3 == 0 ? &form.y : n % 3 == 1 ? &form.x : &form.z;
         for (int kb = 0; kb < KB; ++kb) tma_load_4d_h(tile(n) + kb * (C * 128), m, full + n % NS, kb * 64, (int)row_of(n / 3), h, b, 0);
         armed = n + 1;
       }
@@ -515,10 +521,10 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
     // rows of the segment past the sequence's length
     {
       const int64_t z0 = r0 + (int64_t)count * C;
-      T* out = static_cast<T*>(p.out) + b * p.ob + h * p.oh;
+      T* out = static_cast<T*>(form.out) + b * form.ob + h * form.oh;
       const int per = p.Dr / 8;
       for (int64_t i = threadIdx.x; i < (r1 - z0) * per; i += kGroup)
-        *reinterpret_cast<uint4*>(out + (z0 + i / per) * p.on + (i % per) * 8) = make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(out + (z0 + i / per) * form.on + (i % per) * 8) = make_uint4(0, 0, 0, 0);
     }
     for (int i = 0; i < count; ++i) {
       const int nv = end - row_of(i) < C ? (int)(end - row_of(i)) : C;
@@ -635,8 +641,8 @@ decay_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
     // the state that enters the segment, without the factor of the sums, to tensor memory
     if (count > 0) {
       const float mul = 1.f / p.sum_scale;
-      const float* from = p.state_in ? p.state_in + ((size_t)bh * p.ncut + cut) * p.Dr * p.Dr + (p.transposed ? row : row * p.Dr) : nullptr;
-      const int step = p.transposed ? p.Dr : 1;
+      const float* from = p.state_in ? p.state_in + ((size_t)bh * p.ncut + cut) * p.Dr * p.Dr + (form.transposed ? row : row * p.Dr) : nullptr;
+      const int step = form.transposed ? p.Dr : 1;
 #pragma unroll 1
       for (int q = 0; q < HC / 16; ++q) {
         float f[16];

@@ -200,23 +200,27 @@ static int launch_tc_sums(const DecayCall& c, const fnb_rows& y, const fnb_rows&
   };
   return dispatch_decay_tc(c.s, [&](auto tag, auto d) -> int { return exact ? go(tag, d, std::true_type{}) : go(tag, d, std::false_type{}); });
 }
-template <bool REV>
-static int launch_tc_form(const DecayCall& c, const DecayForm& f, const float* state_in, Launcher& L, const char* name) {
+template <bool REV, int FORMS>
+static int launch_tc_forms(const DecayCall& c, const DecayForm* const (&f)[FORMS], const float* state_in, Launcher& L, const char* name) {
   return dispatch_decay_tc(c.s, [&](auto tag, auto d) -> int {
     using T = decltype(tag);
     constexpr int D = decltype(d)::value;
     using Cfg = dtc::MainCfg<D>;
-    CUtensorMap mx, my, mz, mo;
-    if (!make_rows_map(&mx, f.x, c.s, dtc::kC) || !make_rows_map(&my, f.y, c.s, dtc::kC) || !make_rows_map(&mz, f.z, c.s, dtc::kC) ||
-        !make_rows_map(&mo, f.out, c.s, dtc::kC))
-      return fail(FNB_ERR_CUDA, "cuTensorMapEncodeTiled failed");
+    dtc::DecayTcForms<FORMS> forms;
+    for (int i = 0; i < FORMS; ++i) {
+      dtc::DecayTcForm& t = forms.f[i];
+      if (!make_rows_map(&t.x, f[i]->x, c.s, dtc::kC) || !make_rows_map(&t.y, f[i]->y, c.s, dtc::kC) || !make_rows_map(&t.z, f[i]->z, c.s, dtc::kC) ||
+          !make_rows_map(&t.o, f[i]->out, c.s, dtc::kC))
+        return fail(FNB_ERR_CUDA, "cuTensorMapEncodeTiled failed");
+      t.out = f[i]->out.data; t.ob = f[i]->out.stride_b; t.oh = f[i]->out.stride_h; t.on = f[i]->out.stride_n;
+      t.transposed = f[i]->transposed;
+    }
     dtc::DecayTcParams p = decay_tc_params(c, REV);
-    p.state_in = state_in; p.transposed = f.transposed; p.ncut = c.plan.nseg;
-    p.out = f.out.data; p.ob = f.out.stride_b; p.oh = f.out.stride_h; p.on = f.out.stride_n;
-    auto kern = dtc::decay_tc_kernel<T, D, REV>;
+    p.state_in = state_in; p.ncut = c.plan.nseg;
+    auto kern = dtc::decay_tc_kernel<T, D, REV, FORMS>;
     if (int rc = set_smem(kern, Cfg::kBytes, c.max_smem, name)) return rc;
     L.begin();
-    FNB_CUDA(launch_pdl(kern, dim3((unsigned)(c.BH * c.plan.nseg)), dim3(Cfg::kThreads), Cfg::kBytes, c.stream, mx, my, mz, mo, p));
+    FNB_CUDA(launch_pdl(kern, dim3((unsigned)(c.BH * c.plan.nseg * FORMS)), dim3(Cfg::kThreads), Cfg::kBytes, c.stream, forms, p));
     return L.end(name);
   });
 }
@@ -249,10 +253,12 @@ static int decay_states(const DecayCall& c, const fnb_rows& y, const fnb_rows& z
   return L.end("decay_join");
 }
 
+static bool tma_form(const DecayCall& c, const DecayForm& f) {
+  return decay_on_tensor_cores(c.s) && tma_rows(f.x, c.s) && tma_rows(f.y, c.s) && tma_rows(f.z, c.s) && tma_rows(f.out, c.s);
+}
 // out = scale A(x, y, z) with the states that enter each segment.  Backwards in time the state is dL/dS, which has the scale in it.
 static int decay_form(const DecayCall& c, const DecayForm& f, const float* state_in, Launcher& L, const char* name) {
-  if (decay_on_tensor_cores(c.s) && tma_rows(f.x, c.s) && tma_rows(f.y, c.s) && tma_rows(f.z, c.s) && tma_rows(f.out, c.s))
-    return f.reversed ? launch_tc_form<true>(c, f, state_in, L, name) : launch_tc_form<false>(c, f, state_in, L, name);
+  if (tma_form(c, f)) return f.reversed ? launch_tc_forms<true, 1>(c, {&f}, state_in, L, name) : launch_tc_forms<false, 1>(c, {&f}, state_in, L, name);
   DecayParams p = decay_params(c, f.y, f.z);
   p.x = rows_of(f.x); p.out = rows_of(f.out);
   p.vec = p.vec && vec_rows(f.x, c.s.dtype) && vec_rows(f.out, c.s.dtype);
@@ -428,8 +434,10 @@ int fnb_decay_backward(const fnb_decay_bwd_args* a) {
   if (int rc = decay_states(c, a->q, a->d_out, true, a->d_final_state, e_states, a->d_initial_state, L)) return rc;
   const float* e_in = cut ? e_states : a->d_final_state;
   if (int rc = decay_form(c, {a->d_out, a->v, a->k, a->dq, false, true}, cut ? a->segment_states : a->initial_state, L, "decay_dq")) return rc;
-  if (int rc = decay_form(c, {a->k, a->q, a->d_out, a->dv, true, false}, e_in, L, "decay_dv")) return rc;
-  return decay_form(c, {a->v, a->d_out, a->q, a->dk, true, true}, e_in, L, "decay_dk");
+  const DecayForm dv{a->k, a->q, a->d_out, a->dv, true, false}, dk{a->v, a->d_out, a->q, a->dk, true, true};
+  if (tma_form(c, dv) && tma_form(c, dk)) return launch_tc_forms<true, 2>(c, {&dv, &dk}, e_in, L, "decay_dv_dk");
+  if (int rc = decay_form(c, dv, e_in, L, "decay_dv")) return rc;
+  return decay_form(c, dk, e_in, L, "decay_dk");
 }
 
 int fnb_decay_step(const fnb_decay_step_args* a) {

@@ -459,7 +459,8 @@ DecayResult run_decay_forward(const DecayArgs& c, bool want_state) {
   const auto f32 = q.options().dtype(at::kFloat);
   r.out = empty_rows_like(q);
   if (want_state) r.final = at::empty({q.size(0), q.size(1), q.size(3), q.size(3)}, f32);
-  r.segments = at::empty({(int64_t)fnb_decay_segment_floats(&a.shape)}, f32);
+  const int64_t cuts = (int64_t)fnb_decay_segment_floats(&a.shape);
+  r.segments = at::empty({cuts}, f32);
   const at::Tensor ws = bytes(fnb_decay_workspace_bytes(&a.shape), q);
   a.q = rows_arg(q); a.k = rows_arg(k); a.v = rows_arg(v); a.out = rows_arg(r.out);
   a.log_decay = g.data_ptr<float>(); a.seq_lens = lens_or_null(lens);
