@@ -289,8 +289,9 @@ decay_tc_sums_kernel(const __grid_constant__ CUtensorMap tm_y, const __grid_cons
 }
 
 // ---- outputs -------------------------------------------------------------------------------------------------
-// One CTA a segment, one CTA an SM, 20 warps, chunks of 128 rows: group A (warps 0-7) turns P into its 16-bit operand and takes the output
-// tile out, group B (8-15) forms y' and carries the state, one warp loads, one issues the products of A, one those of B, one
+// One CTA a segment, one CTA an SM, 20 or 28 warps, chunks of 128 rows: group A (eight warps, with heads of 64 two groups that
+// take the chunks in turn) turns P into its 16-bit operand and takes the output
+// tile out, group B (eight) forms y' and carries the state, one warp loads, one issues the products of A, one those of B, one
 // stores.  The two groups meet only in what the products need: while A works on the scores of a chunk, B is at the state behind it.
 //
 // Shared memory is what there is least of, its bandwidth (every operand of a product passes it) and, with heads of 128, its room: so P goes to its product
@@ -302,14 +303,17 @@ template <int D> struct MainCfg {
   static constexpr int kS = D * D * 2;                                   // one term of the state
   static constexpr int kSlots = D == 64 ? 10 : 5;                        // tiles in flight, in the order y, x, z of the chunks
   static constexpr int kTerms = D == 64 ? 2 : 0;                         // tiles for y' (none: in y's place)
-  static constexpr int kInters = D == 64 ? 2 : 1;                        // accumulators of x S
-  static constexpr int kThreads = 2 * kGroup + 128;
+  static constexpr int kGroupsA = D == 64 ? 2 : 1;                       // groups A, which take the chunks in turn: as many as there is tensor memory for
+  static constexpr int kWarpB = 8 * kGroupsA;                            // first warp of group B, then single warps
+  static constexpr int kLoad = kWarpB + 8, kProductsA = kLoad + 1, kProductsB = kLoad + 2, kStore = kLoad + 3;
+  static constexpr int kThreads = (kGroupsA + 1) * kGroup + 128;
   // (relies on the dynamic shared window being 1024-byte aligned, which is checked)
-  static constexpr int kBytes = (kSlots + kTerms) * kTile + 2 * kS + 32 * 16 * 4 + (kC + 4) * 4 + 96 + (2 * kSlots + 24) * 8 + 16;
+  static constexpr int kBytes = (kSlots + kTerms) * kTile + 2 * kS + 32 * 16 * 4 + (kC + 4) * 4 + 128 + (2 * kSlots + 26) * 8 + 16;
   static_assert(kBytes <= 232448, "shared memory of one CTA");
-  // Tensor-memory columns.  The packed scores of columns 0-63 begin at kPacked, those of 64-127 kPackedHalf behind; with heads of 128 they take the place
-  // of the scores that they come from, a thread's own.
-  static constexpr int kScores = 0, kPacked = D == 64 ? 128 : 0, kPackedHalf = D == 64 ? 32 : 64, kIntra = D == 64 ? 192 : 128, kInter = 256, kState = 384;
+  // Tensor-memory columns.  Packed scores take the place of the scores that they come from, each half of a row in its own: of columns 0-63 from kScores on,
+  // of 64-127 from kPackedHalf on behind.  Scores and P z are there for each group A.
+  static constexpr int kScores = 0, kPackedHalf = 64, kIntra = kGroupsA * 128, kInter = kIntra + kGroupsA * D, kState = kInter + D;
+  static_assert(kState + D <= 512, "tensor memory");
 };
 // D[tmem] (+)= A[tmem] * B[smem], from warp-uniform code as umma_elect
 __device__ __forceinline__ void umma_ta_elect(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
@@ -325,7 +329,7 @@ __device__ __forceinline__ void umma_ta_elect(uint32_t d_tmem, uint32_t a_tmem, 
 template <class T, int D, bool REV, int FORMS>
 __global__ void __launch_bounds__(MainCfg<D>::kThreads, 1) decay_tc_kernel(const __grid_constant__ DecayTcForms<FORMS> forms, DecayTcParams p) {
   using L = MainCfg<D>;
-  constexpr int C = kC, NS = L::kSlots, KB = D / 64, NI = L::kInters;
+  constexpr int C = kC, NS = L::kSlots, KB = D / 64, NA = L::kGroupsA;
   constexpr bool F16 = UmmaFmt<T>::v == 0;
   extern __shared__ uint8_t smem_raw[];
   pdl_trigger();
@@ -338,26 +342,26 @@ __global__ void __launch_bounds__(MainCfg<D>::kThreads, 1) decay_tc_kernel(const
   uint8_t* s_s = s_y + L::kTerms * L::kTile;          // two terms of S
   float* s_diag = reinterpret_cast<float*>(s_s + 2 * L::kS);      // [32][16]: weights beside the diagonal, see below
   float* s_pow = s_diag + 32 * 16;                    // powers of exp(g): forwards that of C - k at k, backwards that of k
-  float* s_mul = s_pow + C + 4;                       // [4]: what x S of chunk i is to be multiplied by, in s_mul[i & 3] (B may be two ahead)
-  float* s_max = s_mul + 4;                           // [16]
-  DecayPair* s_pair = reinterpret_cast<DecayPair*>(s_max + 16);      // [2]: what a chunk decays the state by, a whole one and the first
+  float* s_mul = s_pow + C + 4;                       // [4]: what x S of chunk i is to be multiplied by, in s_mul[i & 3] (B may be ahead)
+  float* s_max = s_mul + 4;                           // [24]
+  DecayPair* s_pair = reinterpret_cast<DecayPair*>(s_max + 24);      // [2]: what a chunk decays the state by, a whole one and the first
   uint64_t* bars = reinterpret_cast<uint64_t*>(s_pair + 2);
   uint64_t* full = bars;             // [NS]
   uint64_t* empty = full + NS;       // [NS]
   uint64_t* p_full = empty + NS;     // [4]: scores of chunk i in p_full[i & 3]; B waits for them too and may be two chunks behind
-  uint64_t* p_ready = p_full + 4;
-  uint64_t* o_full = p_ready + 1;
-  uint64_t* o_free = p_ready + 2;
-  uint64_t* u_full = p_ready + 3;
-  uint64_t* s_ready = p_ready + 4;
-  uint64_t* s_done = p_ready + 5;
-  uint64_t* clean = p_ready + 6;
-  uint64_t* y_ready = p_ready + 7;    // [2], by chunk parity: B is a chunk ahead with it
-  uint64_t* fin = p_ready + 9;       // [2]
-  uint64_t* i_full = p_ready + 11;    // [2], by accumulator
-  uint64_t* i_free = p_ready + 13;    // [2]
-  uint64_t* t_ready = p_ready + 15;  // [4]: the output tile of chunk i in t_ready[i & 3]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(p_ready + 19);
+  uint64_t* u_full = p_full + 4;
+  uint64_t* s_ready = u_full + 1;
+  uint64_t* s_done = u_full + 2;
+  uint64_t* clean = u_full + 3;
+  uint64_t* i_free = u_full + 4;
+  uint64_t* y_ready = u_full + 5;    // [2], by chunk parity: B is a chunk ahead with it
+  uint64_t* fin = u_full + 7;        // [2]
+  uint64_t* p_ready = u_full + 9;   // [2], by group A
+  uint64_t* o_full = u_full + 11;    // [2]
+  uint64_t* o_free = u_full + 13;    // [2]
+  uint64_t* i_full = u_full + 15;    // [2]
+  uint64_t* t_ready = u_full + 17;   // [4]: the output tile of chunk i in t_ready[i & 3]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(u_full + 21);
   int* abort_word = reinterpret_cast<int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -366,10 +370,12 @@ __global__ void __launch_bounds__(MainCfg<D>::kThreads, 1) decay_tc_kernel(const
   if (threadIdx.x == 0) {
     for (int i = 0; i < NS; ++i) { mbar_init(full + i, 1); mbar_init(empty + i, 2); }
     for (int i = 0; i < 4; ++i) { mbar_init(p_full + i, 1); mbar_init(t_ready + i, kGroup / 32); }
-    mbar_init(p_ready, kGroup / 32); mbar_init(o_full, 1); mbar_init(o_free, kGroup / 32);
-    mbar_init(u_full, 1); mbar_init(s_ready, kGroup / 32); mbar_init(s_done, 1);
-    mbar_init(clean, kGroup / 32);
-    for (int i = 0; i < 2; ++i) { mbar_init(fin + i, 1); mbar_init(y_ready + i, kGroup / 32); mbar_init(i_full + i, 1); mbar_init(i_free + i, kGroup / 32); }
+    mbar_init(u_full, 1); mbar_init(s_ready, kGroup / 32); mbar_init(s_done, 1); mbar_init(clean, kGroup / 32);
+    mbar_init(i_free, kGroup / 32);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(fin + i, 1); mbar_init(y_ready + i, kGroup / 32); mbar_init(p_ready + i, kGroup / 32); mbar_init(o_full + i, 1);
+      mbar_init(o_free + i, kGroup / 32); mbar_init(i_full + i, 1);
+    }
     *abort_word = 0;
     fence_mbar_init();
   }
@@ -394,8 +400,8 @@ __global__ void __launch_bounds__(MainCfg<D>::kThreads, 1) decay_tc_kernel(const
   // Row r of a 32 x 32 block on the diagonal: forwards the weight of column j < 16 is s_diag[r][j], of column 16 + j s_diag[r - 16][j]; backwards of
   // column 16 + j s_diag[r][j], of column j < 16 s_diag[r + 16][j]; what such an index would leave the table with is behind the mask.
   // (16-byte pieces of a row are stored at piece ^ (row / 2) % 4: eight rows read at once fall on different banks)
-  if (warp < 8) {
-    for (int i = threadIdx.x; i < 32 * 16; i += kGroup) {
+  if (warp < L::kWarpB) {
+    for (int i = threadIdx.x & (kGroup - 1); i < 32 * 16; i += kGroup) {      // (both groups A the same)
       const int row = i / 16, j = i % 16, d = REV ? 16 + j - row : row - j;
       s_diag[row * 16 + ((j / 4) ^ (row / 2 % 4)) * 4 + j % 4] = d >= 0 ? p.scale * power(d) : 0.f;
     }
@@ -405,7 +411,7 @@ __global__ void __launch_bounds__(MainCfg<D>::kThreads, 1) decay_tc_kernel(const
   const auto tile = [&](int n) { return s_in + (n % NS) * L::kTile; };      // n = 3 i + 0, 1, 2: y, x, z of chunk i
   const auto landed = [&](int n, int where) { return mbar_wait(full + n % NS, (n / NS) & 1, ab, where + n); };
 
-  if (warp == 19) {
+  if (warp == L::kStore) {
     // ---- output tiles, from x's place to their rows; the place is then free
     if (lane == 0 && count > 0) {
       tma_prefetch_desc(&form.o);
@@ -419,7 +425,7 @@ __global__ void __launch_bounds__(MainCfg<D>::kThreads, 1) decay_tc_kernel(const
       }
       tma_store_wait_all();
     }
-  } else if (warp == 16) {
+  } else if (warp == L::kLoad) {
     if (lane == 0 && count > 0) {
       tma_prefetch_desc(&form.x);
       tma_prefetch_desc(&form.y);
@@ -435,53 +441,55 @@ __global__ void __launch_bounds__(MainCfg<D>::kThreads, 1) decay_tc_kernel(const
       if (ab.raised())
         for (int n = max(0, armed - NS); n < armed; ++n) mbar_drain(full + n % NS, (n / NS) & 1);
     }
-  } else if (warp == 17) {
-    // ---- products of group A: P z, then the scores of the next chunk
+  } else if (warp == L::kProductsA) {
+    // ---- products of the groups A: the scores of a chunk, and P z of the one before
     // (the whole warp walks this code and the next branch's, and one lane issues: descriptors stay in uniform registers, 70 to 100 cycles a product less)
     if (count > 0) {
       constexpr uint32_t i_p = make_idesc<T>(C, C, false, false), i_o = make_idesc<T>(C, D, false, true);
       const auto scores = [&](int i) -> bool {
         bool ok = landed(3 * i, 0x8200) && landed(3 * i + 1, 0x8280);
         if (i == dirty) ok = ok && mbar_wait(clean, 0, ab, 0x8300 + i);
-        // (where packed scores lie among the scores, the product that reads them has to be done)
-        if (D == 128 && i > 0) ok = ok && mbar_wait(o_full, (i - 1) & 1, ab, 0x8400 + i);
+        // (the product that reads the packed scores among those of NA chunks before has to be done)
+        if (i >= NA) ok = ok && mbar_wait(o_full + i % NA, (i / NA - 1) & 1, ab, 0x8400 + i);
         if (!__all_sync(0xffffffffu, ok)) return false;
         tc_fence_after();
         const uint32_t a_y = smem_u32(tile(3 * i)), a_x = smem_u32(tile(3 * i + 1));
 #pragma unroll 2
-        for (int k = 0; k < D / 16; ++k) umma_elect(tmem + L::kScores, along_row(a_x, k, C), along_row(a_y, k, C), i_p, k > 0);
+        for (int k = 0; k < D / 16; ++k) umma_elect(tmem + L::kScores + i % NA * 128, along_row(a_x, k, C), along_row(a_y, k, C), i_p, k > 0);
         umma_commit_elect(p_full + (i & 3));
         if (D == 64) umma_commit_elect(empty + (3 * i) % NS);
         return true;
       };
       bool go = scores(0);
       for (int i = 0; go && i < count; ++i) {
-        bool ok = landed(3 * i + 2, 0x8880) && mbar_wait(p_ready, i & 1, ab, 0x8800 + i);
-        if (i > 0) ok = ok && mbar_wait(o_free, (i - 1) & 1, ab, 0x8700 + i);
+        const int ga = i % NA;
+        if (NA == 2 && i + 1 < count) go = scores(i + 1);
+        if (!go) break;
+        bool ok = landed(3 * i + 2, 0x8880) && mbar_wait(p_ready + ga, (i / NA) & 1, ab, 0x8800 + i);
+        if (i >= NA) ok = ok && mbar_wait(o_free + ga, (i / NA - 1) & 1, ab, 0x8700 + i);
         if (!__all_sync(0xffffffffu, ok)) break;
         tc_fence_after();
         const uint32_t a_z = smem_u32(tile(3 * i + 2));
 #pragma unroll 2
         for (int k = 0; k < C / 16; ++k)
-          umma_ta_elect(tmem + L::kIntra, tmem + L::kPacked + (k >> 2) * L::kPackedHalf + 8 * (k & 3), along_rows(a_z, k, C), i_o, k > 0);
-        umma_commit_elect(o_full);
+          umma_ta_elect(tmem + L::kIntra + ga * D, tmem + L::kScores + ga * 128 + (k >> 2) * L::kPackedHalf + 8 * (k & 3), along_rows(a_z, k, C), i_o, k > 0);
+        umma_commit_elect(o_full + ga);
         umma_commit_elect(empty + (3 * i + 2) % NS);
-        if (i + 1 < count) go = scores(i + 1);      // (A has read the scores before: p_ready)
+        if (NA == 1 && i + 1 < count) go = scores(i + 1);
       }
       umma_commit_elect(fin);          // nothing of the CTA is given back while a product runs
       mbar_drain(fin, 0);
     }
-  } else if (warp == 18) {
+  } else if (warp == L::kProductsB) {
     // ---- products of group B: x S, then the state's own
     if (count > 0) {
       constexpr uint32_t i_o = make_idesc<T>(C, D, false, true), i_u = make_idesc<T>(D, D, true, true);
       const uint32_t a_s = smem_u32(s_s);
       for (int i = 0; i < count; ++i) {
-        const int ia = i % NI;
         bool ok = landed(3 * i + 1, 0x8580);
         if (i == dirty) ok = ok && mbar_wait(clean, 0, ab, 0x8590 + i);
         ok = ok && mbar_wait(s_ready, i & 1, ab, 0x8600 + i);
-        if (i >= NI) ok = ok && mbar_wait(i_free + ia, (i / NI - 1) & 1, ab, 0x8780 + i);
+        if (i > 0) ok = ok && mbar_wait(i_free, (i - 1) & 1, ab, 0x8780 + i);
         if (!__all_sync(0xffffffffu, ok)) break;
         tc_fence_after();
         const uint32_t a_x = smem_u32(tile(3 * i + 1));
@@ -489,9 +497,9 @@ __global__ void __launch_bounds__(MainCfg<D>::kThreads, 1) decay_tc_kernel(const
         for (int t = 1; t >= 0; --t)
 #pragma unroll 2
           for (int k = 0; k < D / 16; ++k)
-            umma_elect(tmem + L::kInter + ia * D, along_row(a_x, k, C), along_rows(a_s + t * L::kS, k, D), i_o, !(t == 1 && k == 0));
+            umma_elect(tmem + L::kInter, along_row(a_x, k, C), along_rows(a_s + t * L::kS, k, D), i_o, !(t == 1 && k == 0));
         umma_commit_elect(s_done);
-        umma_commit_elect(i_full + ia);
+        umma_commit_elect(i_full + i % NA);
         if (i + 1 < count) {
           // (the state in tensor memory has been decayed by the time its 16-bit terms are ready)
           ok = landed(3 * i + 2, 0x8590) && mbar_wait(y_ready + (i & 1), (i >> 1) & 1, ab, 0x8500 + i);
@@ -509,11 +517,12 @@ __global__ void __launch_bounds__(MainCfg<D>::kThreads, 1) decay_tc_kernel(const
       umma_commit_elect(fin + 1);
       mbar_drain(fin + 1, 0);
     }
-  } else if (warp < 8) {
-    // ---- group A: scores and outputs
+  } else if (warp < L::kWarpB) {
+    // ---- group A: scores and outputs of every NA-th chunk
     // (Here and in group B one warp asks the mbarriers for all, the others wait at a barrier, which takes no issue slots: twenty warps that ask took 40 % of
     // them.  A wait that gave up does not leave the loop: the warps meet at barriers, and the status word has it.)
-    const int quarter = warp & 3, half = warp >> 2;
+    const int ga = warp >> 3, quarter = warp & 3, half = warp >> 2 & 1, bar = 1 + 2 * ga;
+    const bool asks = (warp & 7) == 0;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
     const int w0 = quarter * 32, s = w0 + lane;
     const float largest = fabsf(p.scale) * fmaxf(1.f, power(C - 1));      // of a score's factors
@@ -523,17 +532,17 @@ __global__ void __launch_bounds__(MainCfg<D>::kThreads, 1) decay_tc_kernel(const
       const int64_t z0 = r0 + (int64_t)count * C;
       T* out = static_cast<T*>(form.out) + b * form.ob + h * form.oh;
       const int per = p.Dr / 8;
-      for (int64_t i = threadIdx.x; i < (r1 - z0) * per; i += kGroup)
+      for (int64_t i = threadIdx.x; i < (r1 - z0) * per; i += NA * kGroup)
         *reinterpret_cast<uint4*>(out + (z0 + i / per) * form.on + (i % per) * 8) = make_uint4(0, 0, 0, 0);
     }
-    for (int i = 0; i < count; ++i) {
+    for (int i = ga; i < count; i += NA) {
       const int nv = end - row_of(i) < C ? (int)(end - row_of(i)) : C;
-      if (warp == 0) mbar_wait(p_full + (i & 3), (i >> 2) & 1, ab, 0x8900 + i);
-      named_barrier(1, kGroup);
+      if (asks) mbar_wait(p_full + (i & 3), (i >> 2) & 1, ab, 0x8900 + i);
+      named_barrier(bar, kGroup);
       tc_fence_after();
       // Scores, weighted and packed, 16 columns at a time.  In fp16 the largest is looked at first: where some might leave that type's range
       // (rare), all go in divided by a power of two.  (Loops are not unrolled: the warps' ways through this kernel have to share the instruction cache.)
-      const uint32_t t_scores = tmem + L::kScores + lane_base + half * 64, t_packed = tmem + L::kPacked + lane_base + half * L::kPackedHalf;
+      const uint32_t t_scores = tmem + L::kScores + ga * 128 + lane_base + half * 64, t_packed = t_scores;
       float up = 1.f, down = 1.f;      // (unweighted scores, masked ones among them: what is too large of them costs a factor that does no harm)
       if (F16) {
         float most = 0.f;
@@ -546,17 +555,17 @@ __global__ void __launch_bounds__(MainCfg<D>::kThreads, 1) decay_tc_kernel(const
           for (int j = 0; j < 32; ++j) most = fmaxf(most, fabsf(v[j]));
         }
         most *= largest;
-        if (named_barrier_or(1, kGroup, most > 32768.f)) {
+        if (named_barrier_or(bar, kGroup, most > 32768.f)) {
           float m = most < INFINITY ? most : 0.f;
           for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
           if (lane == 0) s_max[warp] = m;
-          named_barrier(1, kGroup);
-          for (int k = 0; k < 8; ++k) m = fmaxf(m, s_max[k]);
+          named_barrier(bar, kGroup);
+          for (int k = 0; k < 8; ++k) m = fmaxf(m, s_max[8 * ga + k]);
           int e = 0;
           frexpf(m, &e);
           up = ldexpf(1.f, max(0, e - 15));
           down = 1.f / up;
-          named_barrier(1, kGroup);
+          named_barrier(bar, kGroup);
         }
       }
 #pragma unroll 1
@@ -590,14 +599,14 @@ __global__ void __launch_bounds__(MainCfg<D>::kThreads, 1) decay_tc_kernel(const
       }
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive_warp(p_ready);
+      mbar_arrive_warp(p_ready + ga);
       float wi = 0.f;
       if (REV ? s < nv : true) wi = p.inter * p.sum_scale * power(REV ? nv - 1 - s : s + 1);
-      if (warp == 0) {
-        mbar_wait(i_full + i % NI, (i / NI) & 1, ab, 0x8a80 + i);
-        mbar_wait(o_full, i & 1, ab, 0x8a00 + i);
+      if (asks) {
+        mbar_wait(o_full + ga, (i / NA) & 1, ab, 0x8a00 + i);
+        mbar_wait(i_full + ga, (i / NA) & 1, ab, 0x8a80 + i);
       }
-      named_barrier(1, kGroup);
+      named_barrier(bar, kGroup);
       tc_fence_after();
       if (F16) wi *= s_mul[i & 3];
       uint8_t* to = tile(3 * i + 1);
@@ -605,13 +614,13 @@ __global__ void __launch_bounds__(MainCfg<D>::kThreads, 1) decay_tc_kernel(const
       for (int q = 0; q < D / 32; ++q) {
         const int col = half * (D / 2) + q * 16;
         float2 a[8], e[8];
-        tmem_ld16(tmem + L::kIntra + lane_base + col, reinterpret_cast<float*>(a));
-        tmem_ld16(tmem + L::kInter + (i % NI) * D + lane_base + col, reinterpret_cast<float*>(e));
+        tmem_ld16(tmem + L::kIntra + ga * D + lane_base + col, reinterpret_cast<float*>(a));
+        tmem_ld16(tmem + L::kInter + lane_base + col, reinterpret_cast<float*>(e));
         tmem_ld_wait();
         if (q == D / 32 - 1) {
           tc_fence_before();
-          mbar_arrive_warp(o_free);
-          mbar_arrive_warp(i_free + i % NI);
+          mbar_arrive_warp(o_free + ga);
+          mbar_arrive_warp(i_free);
         }
         uint32_t u[8];
 #pragma unroll
@@ -631,7 +640,7 @@ __global__ void __launch_bounds__(MainCfg<D>::kThreads, 1) decay_tc_kernel(const
     }
   } else {
     // ---- group B: the state
-    const int tid = threadIdx.x - kGroup, quarter = warp & 3, half = (warp - 8) >> 2;
+    const int tid = threadIdx.x - 32 * L::kWarpB, quarter = warp & 3, half = (warp - L::kWarpB) >> 2;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
     const int row = D == 64 ? quarter * 16 + lane : quarter * 32 + lane;
     const bool owner = D == 128 || lane < 16;
@@ -674,7 +683,7 @@ __global__ void __launch_bounds__(MainCfg<D>::kThreads, 1) decay_tc_kernel(const
           for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
           if (lane == 0) s_max[warp] = m;
           named_barrier(2, kGroup);
-          for (int k = 0; k < 8; ++k) m = fmaxf(m, s_max[8 + k]);
+          for (int k = 0; k < 8; ++k) m = fmaxf(m, s_max[L::kWarpB + k]);
           int e = 0;
           frexpf(m, &e);
           up = ldexpf(1.f, max(0, e - 15));
@@ -730,7 +739,7 @@ __global__ void __launch_bounds__(MainCfg<D>::kThreads, 1) decay_tc_kernel(const
         named_barrier(2, kGroup);
       }
       if (i + 1 >= count) return;
-      if (warp == 8) {
+      if (warp == L::kWarpB) {
         landed(3 * i, 0x8c80);
         if (D == 128) mbar_wait(p_full + (i & 3), (i >> 2) & 1, ab, 0x8c00 + i);
       }
@@ -754,7 +763,7 @@ __global__ void __launch_bounds__(MainCfg<D>::kThreads, 1) decay_tc_kernel(const
     // (heads of 64: y' a chunk ahead, while the products that end this one run; its tile is free since u_full of the chunk before)
     for (int i = 0; i + 1 < count; ++i) {
       if (D == 64) put_y(i + 1);
-      if (warp == 8) {
+      if (warp == L::kWarpB) {
         mbar_wait(s_done, i & 1, ab, 0x8e00 + i);
         mbar_wait(u_full, i & 1, ab, 0x8d00 + i);
       }
