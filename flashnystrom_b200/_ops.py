@@ -10,6 +10,7 @@ graph).
 
     torch.ops.flashnystrom_b200.decay_fwd(q, k, v, log_decay, scale, initial_state, seq_lens) -> (out, final_state, states at the cuts)
     torch.ops.flashnystrom_b200.decay_bwd(...) -> (dq, dk, dv, d_initial_state)
+    torch.ops.flashnystrom_b200.decay_step(q, k, v, state, log_decay, scale, slots) -> out, with state written
     torch.ops.flashnystrom_b200.norm_fwd(x, weight, bias, eps, num_groups) -> (y, mean, rstd)
     torch.ops.flashnystrom_b200.norm_bwd(...) -> (dx, d_weight, d_bias)
 
@@ -148,6 +149,17 @@ def decay_attention_via_ops(q, k, v, log_decay, scale, initial_state, seq_lens):
         raise RuntimeError("log_decay is a constant here: it has no gradient")
     out, state, _ = decay_fwd(q, k, v, log_decay, scale, initial_state, seq_lens)
     return out, state
+
+
+@torch.library.custom_op(f"{_LIB}::decay_step", mutates_args=("state",), device_types="cuda")
+def decay_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, state: torch.Tensor, log_decay: torch.Tensor, scale: float,
+               slots: Optional[torch.Tensor]) -> torch.Tensor:
+    return _C.native().decay_step(q, k, v, state, log_decay, scale, slots)
+
+
+@decay_step.register_fake
+def _(q, k, v, state, log_decay, scale, slots):
+    return torch.empty_like(q, memory_format=torch.contiguous_format)
 
 
 # ---- layer norm -------------------------------------------------------------------------------------------

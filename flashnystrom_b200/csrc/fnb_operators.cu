@@ -444,6 +444,8 @@ int fnb_decay_step(const fnb_decay_step_args* a) {
   if (!a) return fail(FNB_ERR_INVALID_ARGUMENT, "args is NULL");
   fnb_decay_shape s{a->batch, a->heads, 1, a->head_dim, a->dtype, a->scale, 0};
   if (s.batch > 65535) return fail(FNB_ERR_INVALID_ARGUMENT, "batch (%lld) exceeds 65535", (long long)s.batch);
+  if (s.heads > 0 && s.heads <= 65535 && s.batch * s.heads > INT32_MAX)
+    return fail(FNB_ERR_INVALID_ARGUMENT, "batch * heads (%lld * %lld) exceeds 2^31 - 1", (long long)s.batch, (long long)s.heads);
   if (s.heads > 0 && s.heads <= 65535 && s.batch * s.heads > 65535) s.batch = 1;      // (one CTA a head: more of them are taken here)
   if (int rc = check_decay_shape(&s)) return rc;
   const struct { const fnb_rows* t; const char* name; } big[] = {{&a->q, "q"}, {&a->k, "k"}, {&a->v, "v"}, {&a->out, "out"}};

@@ -42,9 +42,10 @@ def decay_attention(q, k, v, log_decay, scale=None, initial_state=None, seq_lens
     return_state: also return the state behind each sequence's last row (B, H, D, D), float32, differentiable: what the next
         call takes as initial_state, or decay_attention_step as its state.
 
-    A row of k or v that holds an infinity or NaN may reach rows up to 127 before it as NaN, too; later rows it reaches by definition.  In fp16
-    the score q . k * scale and the state must stay in that type's range only as far as the output does; sums and states are float32.
-    There is no second derivative, and no CPU path."""
+    Sums and states are float32.  fp16 and bf16 calls round each pair's score, or the key's share of the state, once to their type on the way;
+    a state that is handed out does not have that rounding, and asking for it may change the last bit of the output of long sequences.  Scores
+    and states may leave fp16's range as long as the output does not.  A row of q, k or v that counts and holds an infinity or NaN reaches
+    the rows after it by definition, and may reach up to 127 rows before it.  There is no second derivative, and no CPU path."""
     _check_tensors("decay_attention", q=q, k=k, v=v, log_decay=log_decay)
     scale = _scale(scale, q.shape[-1] if q.dim() else 0)
     if torch.compiler.is_compiling() or _C.being_transformed():
@@ -64,7 +65,11 @@ def decay_attention_step(q, k, v, state, log_decay, scale=None, slots=None):
         None: row b has state b, and S is B.
     Returns (B, H, D).  No gradient: with one wanted the call is refused (decay_attention has one)."""
     _check_tensors("decay_attention_step", q=q, k=k, v=v, state=state, log_decay=log_decay)
-    return _C.native().decay_step(q, k, v, state, log_decay, _scale(scale, q.shape[-1] if q.dim() else 0), slots)
+    scale = _scale(scale, q.shape[-1] if q.dim() else 0)
+    if torch.compiler.is_compiling():
+        from . import _ops
+        return _ops.decay_step(q, k, v, state, log_decay, scale, slots)
+    return _C.native().decay_step(q, k, v, state, log_decay, scale, slots)
 
 
 def default_log_decay(heads):

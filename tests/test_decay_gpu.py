@@ -351,7 +351,7 @@ def test_c_abi_writes_nothing_but_its_rows(cuda_device):
     """Output rows inside a larger tensor: what lies between and behind them is left as it was."""
     from flashnystrom_b200 import _C, _lib
     lib = _lib.load()
-    for D in (64, 128):
+    for D in (64, 128, 16):
         B, H, N = 2, 2, 200
         q, k, v, _, _, _, log_decay = _inputs(B, H, N, D, torch.bfloat16, 3, state=False)
         room = torch.full((B, H, N + 7, D + 64), 7.0, dtype=torch.bfloat16, device="cuda")
@@ -419,6 +419,58 @@ def test_compiled(cuda_device):
         return [y, state, *torch.autograd.grad((y, state), leaves, (torch.ones_like(y) * 0.5 + y.detach(), ds))]
     for a, b in zip(run(f), run(torch.compile(f, fullgraph=True, backend="aot_eager"))):
         assert torch.allclose(a, b, rtol=1e-5, atol=1e-5)
+
+
+def test_compiled_step(cuda_device):
+    from flashnystrom_b200 import decay_attention_step
+    q, k, v, _, s0, _, log_decay = _inputs(3, 2, 1, 64, torch.float16, 33)
+    q, k, v = (t[:, :, 0] for t in (q, k, v))
+    a, b = s0.clone(), s0.clone()
+
+    def f(state):
+        return decay_attention_step(q, k, v, state, log_decay) * 2
+    assert torch.equal(torch.compile(f, fullgraph=True, backend="aot_eager")(a), f(b)) and torch.equal(a, b)
+
+
+@pytest.mark.parametrize("D", [64, 128, 32])
+@pytest.mark.parametrize("N", [300, 6000])
+def test_scores_and_states_past_the_range_of_fp16(cuda_device, D, N):
+    """Scores of up to several hundred thousand and states of several million, with outputs of order one; the range is left in some tiles only."""
+    q, k, v, d, s0, ds, log_decay = _inputs(1, 2, N, D, torch.float16, 41)
+    q, k, v, d = (t.float() for t in (q, k, v, d))
+    q, k, v, d = q * 100, k * 100, v * 1e-4, d * 1e-4                    # scores
+    q[:, :, N // 2:] *= 1e-3
+    _check(*(t.half() for t in (q, k, v, d)), s0 * 1e-6, ds * 1e-6, log_decay, scale=1.0)
+    g = torch.Generator().manual_seed(5)
+    k, v = (torch.randn(1, 2, N, D, generator=g).cuda() * 5 + 200 for _ in range(2))      # states: sums of one sign
+    q, d = (torch.randn(1, 2, N, D, generator=g).cuda() * 1e-5 for _ in range(2))
+    log_decay[:] = -1e-3
+    _check(*(t.half() for t in (q, k, v, d)), s0 * 1e6, ds, log_decay)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_segments_of_odd_lengths(cuda_device, dtype):
+    """Sequences that are split over many SMs: lengths that end in the first, a middle and the last segment, whole and partial chunks, from states and to them."""
+    for N, D, lens in ((9000, 64, [9000, 1, 4500, 0, 8999, 128]), (7001, 128, [7001, 3000, 6999]), (5000, 16, [4999, 100])):
+        q, k, v, d, s0, ds, log_decay = _inputs(len(lens), 1, N, D, dtype, N, split=True)
+        _check(q, k, v, d, s0, ds, log_decay, torch.tensor(lens, dtype=torch.int32).cuda())
+        _check(q, k, v, d, None, None, log_decay, torch.tensor(lens, dtype=torch.int32).cuda())
+
+
+def test_calls_side_by_side(cuda_device):
+    """Different shapes on two streams at once, each with workspaces of its own."""
+    from flashnystrom_b200 import decay_attention
+    sets = [_inputs(1, 4, 3000, 64, torch.bfloat16, 1), _inputs(2, 2, 2500, 128, torch.float16, 2)]
+    alone = [decay_attention(s[0], s[1], s[2], s[6], initial_state=s[4], return_state=True) for s in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        together = []
+        for s, stream in zip(sets, streams):
+            with torch.cuda.stream(stream):
+                together.append(decay_attention(s[0], s[1], s[2], s[6], initial_state=s[4], return_state=True))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for x, y in zip(alone, together) for a, b in zip(x, y))
 
 
 def test_refusals(cuda_device):

@@ -54,6 +54,8 @@ def test_decay_pointers(lib):
     assert lib.fnb_decay_step(C.byref(s)) == -1 and "16-byte aligned" in _lib.last_error()
     s = _lib.DecayStepArgs(3, 2, 3, 64, _lib.FNB_F32, 1.0, rows, rows, rows, rows, None, 64, None, 0, None)
     assert lib.fnb_decay_step(C.byref(s)) == -1 and "must not be NULL" in _lib.last_error()
+    s = _lib.DecayStepArgs(65535, 65535, 65535, 64, _lib.FNB_F32, 1.0, rows, rows, rows, rows, 64, 64, 64, 0, None)
+    assert lib.fnb_decay_step(C.byref(s)) == -1 and "exceeds 2^31" in _lib.last_error()
     s = _lib.DecayStepArgs(2 ** 33, 2, 3, 64, _lib.FNB_F32, 1.0, rows, rows, rows, rows, 64, 64, 64, 0, None)
     assert lib.fnb_decay_step(C.byref(s)) == -1 and "exceeds 65535" in _lib.last_error()
 
