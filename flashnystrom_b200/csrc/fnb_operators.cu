@@ -297,19 +297,24 @@ static int check_norm_shape(const fnb_norm_shape* s) {
 // How a norm is spread over threads and CTAs.  The grid follows the shape and the SM count alone, whatever the alignment: it sizes the
 // workspace.
 struct NormPlan {
+  int how;                   // NormLoads
   int vec, items;            // elements of a load; loads of a thread
   bool block;                // a run is a CTA's
   int threads, lanes, places, per_row, gblocks, span, ctas;
 };
-static NormPlan norm_plan(const fnb_norm_shape& s, bool wide, bool backward, int sms) {
+// How rows are read: loads of 16 bytes that their starts and lengths are multiples of; such loads with the rows' ends picked out of them, where x, y (and the gradients)
+// lie alike; one element at a time.
+enum NormLoads { kNormWhole, kNormShifted, kNormSingle };
+static NormPlan norm_plan(const fnb_norm_shape& s, NormLoads how, bool backward, int sms) {
   NormPlan p;
   const int n = s.cols / s.groups, V = 16 / (int)elem_bytes(s.dtype);
-  p.vec = wide && n % V == 0 ? V : 1;
+  p.how = how;
+  p.vec = how == kNormSingle ? 1 : V;
   // Up to 512 columns a warp (or a part of one) holds a run, 16 elements a thread and two loads where there are as many; above that a CTA, 16 elements a
   // thread while it has threads (65536 x 1024 fp16, backward: 95 us, with a warp a run 168).  The forward keeps to warps up to 1024 columns of 16 bits
   // (56 us, a CTA a run 76).
-  p.block = n > (!backward && p.vec == 8 ? 1024 : 512);
-  const int loads = (n + p.vec - 1) / p.vec;
+  p.block = n > (!backward && how == kNormWhole && V == 8 ? 1024 : 512);
+  const int loads = how == kNormShifted ? (n + 2 * V - 2) / V : (n + p.vec - 1) / p.vec;
   if (!p.block) {
     p.lanes = 1;
     while (p.lanes < 32 && p.lanes * (p.vec > 1 ? 2 : 1) < loads) p.lanes *= 2;
@@ -333,32 +338,39 @@ static NormPlan norm_plan(const fnb_norm_shape& s, bool wide, bool backward, int
   const int64_t at_once = p.places / p.per_row;
   const int64_t row_blocks = (s.rows + at_once - 1) / at_once;
   const int64_t slots = (int64_t)sms * std::max(1, norm_resident(backward, p.vec * p.items) / p.threads);
-  p.ctas = p.gblocks * (int)std::max<int64_t>(1, std::min<int64_t>(row_blocks, slots / p.gblocks));
+  int64_t nrb = std::max<int64_t>(1, std::min<int64_t>(row_blocks, slots / p.gblocks));
+  if (how == kNormShifted && nrb < row_blocks) nrb = std::min<int64_t>(row_blocks, std::max<int64_t>(1, nrb / V) * V);      // (see norm_shift)
+  p.ctas = p.gblocks * (int)nrb;
   return p;
 }
 static size_t norm_ws_bytes(const fnb_norm_shape& s) {
   const int sms = current_sm_count();
-  const NormPlan a = norm_plan(s, true, true, sms), b = norm_plan(s, false, true, sms);
-  return align256(std::max((size_t)a.ctas * 2 * a.span, (size_t)b.ctas * 2 * b.span) * sizeof(float));
+  size_t most = 0;
+  for (NormLoads how : {kNormWhole, kNormShifted, kNormSingle}) {
+    const NormPlan p = norm_plan(s, how, true, sms);
+    most = std::max(most, (size_t)p.ctas * 2 * p.span);
+  }
+  return align256(most * sizeof(float));
 }
 
-// f(T{}, PF32, VEC, ITEMS, BLOCK)
+// f(T{}, PF32, VEC, ITEMS, BLOCK, SHIFT)
 template <class F>
 static int dispatch_norm(const fnb_norm_shape& s, const NormPlan& p, F&& f) {
   auto by_items = [&](auto tag, auto pf, auto block) -> int {
     constexpr int V = 16 / sizeof(tag);
     using I = std::integral_constant<int, V>;
     using One = std::integral_constant<int, 1>;
-    if (p.vec > 1) {
-      if (p.items <= 1) return f(tag, pf, I{}, std::integral_constant<int, 1>{}, block);
-      if (p.items <= 2) return f(tag, pf, I{}, std::integral_constant<int, 2>{}, block);
-      if (V == 8 || p.items <= 4) return f(tag, pf, I{}, std::integral_constant<int, 4>{}, block);
-      return f(tag, pf, I{}, std::integral_constant<int, 32 / V>{}, block);
-    }
-    if (p.items <= 4) return f(tag, pf, One{}, std::integral_constant<int, 4>{}, block);
-    if (p.items <= 8) return f(tag, pf, One{}, std::integral_constant<int, 8>{}, block);
-    if (p.items <= 16) return f(tag, pf, One{}, std::integral_constant<int, 16>{}, block);
-    return f(tag, pf, One{}, std::integral_constant<int, 32>{}, block);
+    const auto vectors = [&](auto shift) -> int {
+      if (p.items <= 1) return f(tag, pf, I{}, std::integral_constant<int, 1>{}, block, shift);
+      if (p.items <= 2) return f(tag, pf, I{}, std::integral_constant<int, 2>{}, block, shift);
+      if (V == 8 || p.items <= 4) return f(tag, pf, I{}, std::integral_constant<int, 4>{}, block, shift);
+      return f(tag, pf, I{}, std::integral_constant<int, 32 / V>{}, block, shift);
+    };
+    if (p.how == kNormWhole) return vectors(std::false_type{});
+    if (p.how == kNormShifted) return vectors(std::true_type{});
+    if (p.items <= 8) return f(tag, pf, One{}, std::integral_constant<int, 8>{}, block, std::false_type{});
+    if (p.items <= 16) return f(tag, pf, One{}, std::integral_constant<int, 16>{}, block, std::false_type{});
+    return f(tag, pf, One{}, std::integral_constant<int, 32>{}, block, std::false_type{});
   };
   auto by_block = [&](auto tag, auto pf) -> int {
     return p.block ? by_items(tag, pf, std::true_type{}) : by_items(tag, pf, std::false_type{});
@@ -379,7 +391,20 @@ static NormParams norm_params(const fnb_norm_shape& s, const NormPlan& n) {
   return p;
 }
 static bool typed(const void* p, int dtype) { return reinterpret_cast<uintptr_t>(p) % elem_bytes(dtype) == 0; }
-static bool wide_rows(const void* p, int64_t stride, int dtype) { return aligned16(p) && stride * (int64_t)elem_bytes(dtype) % 16 == 0; }
+// How far into 16 bytes a tensor's first row begins, and rows lie apart past whole ones, in elements.
+struct NormAlign { int base, stride; };
+static NormAlign norm_align(const void* p, int64_t stride, int dtype) {
+  const int64_t e = (int64_t)elem_bytes(dtype), V = 16 / e;
+  return {(int)(reinterpret_cast<uintptr_t>(p) / e % V), (int)((stride % V + V) % V)};
+}
+static NormLoads norm_loads(const fnb_norm_shape& s, const NormAlign* t, int count, bool params_wide) {
+  const int V = 16 / (int)elem_bytes(s.dtype);
+  bool alike = true;
+  for (int i = 1; i < count; ++i) alike = alike && t[i].base == t[0].base && t[i].stride == t[0].stride;
+  const int n = s.cols / s.groups;
+  if (alike && t[0].base == 0 && t[0].stride == 0 && n % V == 0 && params_wide) return kNormWhole;
+  return alike && n + V - 1 <= kNormMaxCols ? kNormShifted : kNormSingle;
+}
 
 }  // namespace fnb
 
@@ -492,14 +517,15 @@ int fnb_norm_forward(const fnb_norm_fwd_args* a) {
   if (!g.ok) return fail(FNB_ERR_CUDA, "cannot select CUDA device %d", a->device);
   int max_smem = 0, cc = 0, sms = 0;
   if (int rc = device_limits(a->device, &max_smem, &cc, &sms)) return rc;
-  const bool wide = wide_rows(a->x, a->x_stride, s.dtype) && wide_rows(a->y, a->y_stride, s.dtype) && aligned16(a->weight) && aligned16(a->bias);
-  const NormPlan n = norm_plan(s, wide, false, sms);
+  const NormAlign at[2] = {norm_align(a->x, a->x_stride, s.dtype), norm_align(a->y, a->y_stride, s.dtype)};
+  const NormPlan n = norm_plan(s, norm_loads(s, at, 2, aligned16(a->weight) && aligned16(a->bias)), false, sms);
   NormParams p = norm_params(s, n);
+  p.base_left = at[0].base; p.stride_left = at[0].stride;
   p.x = a->x; p.xs = a->x_stride; p.y = a->y; p.ys = a->y_stride; p.w = a->weight; p.b = a->bias; p.mean = a->mean; p.rstd = a->rstd;
   Launcher L((cudaStream_t)a->stream, a->device);
-  return dispatch_norm(s, n, [&](auto tag, auto pf, auto vec, auto items, auto block) -> int {
+  return dispatch_norm(s, n, [&](auto tag, auto pf, auto vec, auto items, auto block, auto shift) -> int {
     L.begin();
-    norm_fwd_kernel<decltype(tag), decltype(pf)::value, decltype(vec)::value, decltype(items)::value, decltype(block)::value>
+    norm_fwd_kernel<decltype(tag), decltype(pf)::value, decltype(vec)::value, decltype(items)::value, decltype(block)::value, decltype(shift)::value>
         <<<n.ctas, n.threads, 0, L.stream>>>(p);
     return L.end("norm_fwd");
   });
@@ -522,17 +548,17 @@ int fnb_norm_backward(const fnb_norm_bwd_args* a) {
   const size_t need = norm_ws_bytes(s);
   if (sums && (!a->workspace || a->workspace_bytes < need || !aligned16(a->workspace)))
     return fail(FNB_ERR_WORKSPACE, "workspace must be 16-byte aligned and >= %zu bytes (got %zu)", need, a->workspace_bytes);
-  const bool wide = wide_rows(a->x, a->x_stride, s.dtype) && wide_rows(a->d_y, a->d_y_stride, s.dtype) &&
-                    (!a->d_x || wide_rows(a->d_x, a->d_x_stride, s.dtype)) && aligned16(a->weight);
-  const NormPlan n = norm_plan(s, wide, true, sms);
+  const NormAlign at[3] = {norm_align(a->x, a->x_stride, s.dtype), norm_align(a->d_y, a->d_y_stride, s.dtype), norm_align(a->d_x, a->d_x_stride, s.dtype)};
+  const NormPlan n = norm_plan(s, norm_loads(s, at, a->d_x ? 3 : 2, aligned16(a->weight)), true, sms);
   NormParams p = norm_params(s, n);
+  p.base_left = at[0].base; p.stride_left = at[0].stride;
   p.x = a->x; p.xs = a->x_stride; p.dy = a->d_y; p.dys = a->d_y_stride; p.y = a->d_x; p.ys = a->d_x_stride; p.w = a->weight;
   p.mean = const_cast<float*>(a->mean); p.rstd = const_cast<float*>(a->rstd);
   p.part = sums ? (float*)a->workspace : nullptr;
-  const size_t smem = sums && !n.block ? (size_t)2 * n.span * sizeof(float) : 0;
+  const size_t smem = sums && !n.block ? (size_t)2 * n.span * norm_copies(n.lanes, n.per_row) * sizeof(float) : 0;
   Launcher L((cudaStream_t)a->stream, a->device);
-  int rc = dispatch_norm(s, n, [&](auto tag, auto pf, auto vec, auto items, auto block) -> int {
-    auto kern = norm_bwd_kernel<decltype(tag), decltype(pf)::value, decltype(vec)::value, decltype(items)::value, decltype(block)::value>;
+  int rc = dispatch_norm(s, n, [&](auto tag, auto pf, auto vec, auto items, auto block, auto shift) -> int {
+    auto kern = norm_bwd_kernel<decltype(tag), decltype(pf)::value, decltype(vec)::value, decltype(items)::value, decltype(block)::value, decltype(shift)::value>;
     if (smem > 32768)
       if (int e = set_smem(kern, smem, max_smem, "norm_bwd")) return e;
     L.begin();

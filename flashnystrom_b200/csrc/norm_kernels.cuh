@@ -26,7 +26,19 @@ struct NormParams {
   int places, per_row;        // places a CTA uses; how many of them one row takes
   int gblocks;                // blocks of groups (more than one where a row has more groups than a CTA places)
   int span;                   // columns whose sums a CTA has: places of distinct groups x n
+  int stride_left, base_left; // SHIFT: elements by which rows lie apart and the first begins, past whole loads
 };
+
+// SHIFT, rows of a length that whole loads do not divide: a run's first load is the one that its first element lies in, `off` elements into it.  The rows of a
+// place lie a multiple of VEC rows apart (the host sees to it), so that this is the same for all of them.
+struct NormPlace {
+  int lane, place, group;
+  int64_t row, step;
+  bool active;
+};
+template <int VEC> __device__ __forceinline__ int norm_shift(const NormParams& p, const NormPlace& t) {
+  return (int)((p.base_left + t.row % VEC * p.stride_left + (int64_t)t.group * p.n) % VEC);
+}
 
 // element type of weight and bias: F32 or T
 template <class T, bool PF32> struct NormParam { using type = T; };
@@ -43,10 +55,24 @@ __device__ __forceinline__ void norm_load(const T* p, float* v) {
     for (int j = 0; j < VEC; j += 4) load16<T>(p + j, v + j);
   }
 }
-template <class T, int VEC>
-__device__ __forceinline__ void norm_store(T* p, const float* v) {
+template <class P, int VEC, bool SHIFT>
+__device__ __forceinline__ void norm_param(const P* p, int c, int n, float* v) {
+  if (!SHIFT) {
+    norm_load<P, VEC>(p + c, v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j)
+      if (c + j >= 0 && c + j < n) v[j] = to_f<P>(p[c + j]);
+  }
+}
+template <class T, int VEC, bool SHIFT>
+__device__ __forceinline__ void norm_store(T* p, const float* v, int c, int n) {
   if (VEC == 1) {
     *p = from_f<T>(v[0]);
+  } else if (SHIFT && (c < 0 || c + VEC > n)) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j)
+      if (c + j >= 0 && c + j < n) p[j] = from_f<T>(v[j]);
   } else {
     uint4 raw;
     T* e = reinterpret_cast<T*>(&raw);
@@ -59,12 +85,22 @@ __device__ __forceinline__ void norm_store(T* p, const float* v) {
 // VEC elements as they lie in memory
 template <class T, int VEC> struct NormRaw { uint4 v; };
 template <class T> struct NormRaw<T, 1> { T v; };
-template <class T, int VEC> __device__ __forceinline__ NormRaw<T, VEC> norm_raw(const T* p) { return *reinterpret_cast<const NormRaw<T, VEC>*>(p); }
 template <class T, int VEC> __device__ __forceinline__ NormRaw<T, VEC> norm_nothing() {
   NormRaw<T, VEC> r;
   if constexpr (VEC == 1) r.v = from_f<T>(0.f);
   else r.v = make_uint4(0u, 0u, 0u, 0u);
   return r;
+}
+// Columns c .. c + VEC - 1 of a run.  At a run's ends a load has elements beside it, which norm_inside takes out again: a load of 16 bytes from a multiple of 16 that
+// has one of the tensor's elements lies in the tensor's allocation.
+template <class T, int VEC> __device__ __forceinline__ NormRaw<T, VEC> norm_raw(const T* run, int c, int n) {
+  return c < n ? *reinterpret_cast<const NormRaw<T, VEC>*>(run + c) : norm_nothing<T, VEC>();
+}
+template <int VEC, bool SHIFT> __device__ __forceinline__ void norm_inside(float* v, int c, int n) {
+  if (SHIFT) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) v[j] = c + j >= 0 && c + j < n ? v[j] : 0.f;
+  }
 }
 template <class T, int VEC> __device__ __forceinline__ void norm_floats(const NormRaw<T, VEC>& r, float* v) {
   const T* e = reinterpret_cast<const T*>(&r);
@@ -93,18 +129,16 @@ __device__ __forceinline__ void norm_block(float a, float b, float* red, int& tu
 }
 // Columns that a warp of a CTA-wide run holds.
 template <int VEC, int ITEMS>
-__device__ __forceinline__ int norm_warp_cols(int n, int warp, int threads) {
+__device__ __forceinline__ int norm_warp_cols(int n, int off, int warp, int threads) {
   int cols = 0;
 #pragma unroll
-  for (int i = 0; i < ITEMS; ++i) cols += max(0, min(32 * VEC, n - (i * threads + 32 * warp) * VEC));
+  for (int i = 0; i < ITEMS; ++i) {
+    const int c = (i * threads + 32 * warp) * VEC - off;
+    cols += max(0, min(c + 32 * VEC, n) - max(c, 0));
+  }
   return cols;
 }
 
-struct NormPlace {
-  int lane, place, group;
-  int64_t row, step;
-  bool active;
-};
 template <bool BLOCK>
 __device__ __forceinline__ NormPlace norm_place(const NormParams& p) {
   NormPlace t;
@@ -119,11 +153,13 @@ __device__ __forceinline__ NormPlace norm_place(const NormParams& p) {
   return t;
 }
 
+// copies of the sums in a CTA of several runs, each of 2 x span <= 2 x 512 floats where there are several
+__host__ __device__ constexpr int norm_copies(int lanes, int per_row) { return per_row <= 32 / lanes ? kNormThreads / 32 : 1; }
 // threads that an SM should hold at once, by elements a thread: what keeps enough loads under way, and what their registers allow
 __host__ __device__ constexpr int norm_resident(bool backward, int elements) {
   return elements <= 8 ? 1024 : elements <= 16 && !backward ? 768 : 512;
 }
-template <class T, bool PF32, int VEC, int ITEMS, bool BLOCK>
+template <class T, bool PF32, int VEC, int ITEMS, bool BLOCK, bool SHIFT>
 __global__ void __launch_bounds__(BLOCK ? 512 : kNormThreads, BLOCK ? norm_resident(false, VEC * ITEMS) / 512 : norm_resident(false, VEC * ITEMS) / kNormThreads) norm_fwd_kernel(NormParams p) {
   using P = typename NormParam<T, PF32>::type;
   constexpr int EPT = VEC * ITEMS;
@@ -131,21 +167,22 @@ __global__ void __launch_bounds__(BLOCK ? 512 : kNormThreads, BLOCK ? norm_resid
   int turn = 0;
   const NormPlace t = norm_place<BLOCK>(p);
   const int threads = BLOCK ? blockDim.x : p.lanes, lanes = BLOCK ? 32 : p.lanes;
+  const int off = SHIFT ? norm_shift<VEC>(p, t) : 0;
   float w[EPT], b[EPT];
 #pragma unroll
   for (int i = 0; i < ITEMS; ++i) {
-    const int c = (i * threads + t.lane) * VEC;
+    const int c = (i * threads + t.lane) * VEC - off;
 #pragma unroll
     for (int j = 0; j < VEC; ++j) { w[i * VEC + j] = 1.f; b[i * VEC + j] = 0.f; }
     if (t.active && c < p.n) {
-      if (p.w) norm_load<P, VEC>(static_cast<const P*>(p.w) + (int64_t)t.group * p.n + c, w + i * VEC);
-      if (p.b) norm_load<P, VEC>(static_cast<const P*>(p.b) + (int64_t)t.group * p.n + c, b + i * VEC);
+      if (p.w) norm_param<P, VEC, SHIFT>(static_cast<const P*>(p.w) + (int64_t)t.group * p.n, c, p.n, w + i * VEC);
+      if (p.b) norm_param<P, VEC, SHIFT>(static_cast<const P*>(p.b) + (int64_t)t.group * p.n, c, p.n, b + i * VEC);
     }
   }
   __shared__ float warp_cols[16], warp_inv[16];
   if (BLOCK) {
     if (threadIdx.x < (blockDim.x >> 5)) {
-      const int cols = norm_warp_cols<VEC, ITEMS>(p.n, threadIdx.x, threads);
+      const int cols = norm_warp_cols<VEC, ITEMS>(p.n, off, threadIdx.x, threads);
       warp_cols[threadIdx.x] = (float)cols;
       warp_inv[threadIdx.x] = cols ? 1.f / (float)cols : 0.f;
     }
@@ -161,8 +198,8 @@ __global__ void __launch_bounds__(BLOCK ? 512 : kNormThreads, BLOCK ? norm_resid
     const T* x = static_cast<const T*>(p.x) + row * p.xs + (int64_t)t.group * p.n;
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-      const int c = (i * threads + t.lane) * VEC;
-      next[i] = t.active && row < p.rows && c < p.n ? norm_raw<T, VEC>(x + c) : norm_nothing<T, VEC>();
+      const int c = (i * threads + t.lane) * VEC - off;
+      next[i] = t.active && row < p.rows ? norm_raw<T, VEC>(x, c, p.n) : norm_nothing<T, VEC>();
     }
   };
   fetch(first + apart);
@@ -171,7 +208,10 @@ __global__ void __launch_bounds__(BLOCK ? 512 : kNormThreads, BLOCK ? norm_resid
     const bool on = t.active && row < p.rows;
     float v[EPT];
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i) norm_floats<T, VEC>(next[i], v + i * VEC);
+    for (int i = 0; i < ITEMS; ++i) {
+      norm_floats<T, VEC>(next[i], v + i * VEC);
+      norm_inside<VEC, SHIFT>(v + i * VEC, (i * threads + t.lane) * VEC - off, p.n);
+    }
     fetch(row + t.step);
     float s = 0.f;
 #pragma unroll
@@ -181,9 +221,10 @@ __global__ void __launch_bounds__(BLOCK ? 512 : kNormThreads, BLOCK ? norm_resid
     float mean = s * (BLOCK ? warp_inv[threadIdx.x >> 5] : inv_n), q = 0.f;
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-      const bool in = (i * threads + t.lane) * VEC < p.n;
+      const int c = (i * threads + t.lane) * VEC - off;
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
+        const bool in = SHIFT ? c + j >= 0 && c + j < p.n : c < p.n;
         v[i * VEC + j] = in ? v[i * VEC + j] - mean : 0.f;
         q = fmaf(v[i * VEC + j], v[i * VEC + j], q);
       }
@@ -208,10 +249,10 @@ __global__ void __launch_bounds__(BLOCK ? 512 : kNormThreads, BLOCK ? norm_resid
     T* y = static_cast<T*>(p.y) + row * p.ys + (int64_t)t.group * p.n;
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-      const int c = (i * threads + t.lane) * VEC;
+      const int c = (i * threads + t.lane) * VEC - off;
 #pragma unroll
       for (int j = 0; j < VEC; ++j) v[i * VEC + j] = fmaf(v[i * VEC + j] * r, w[i * VEC + j], b[i * VEC + j]);
-      if (c < p.n) norm_store<T, VEC>(y + c, v + i * VEC);
+      if (c < p.n) norm_store<T, VEC, SHIFT>(y + c, v + i * VEC, c, p.n);
     }
     if (t.lane == 0) {
       if (p.mean) p.mean[row * p.groups + t.group] = mean;
@@ -221,7 +262,7 @@ __global__ void __launch_bounds__(BLOCK ? 512 : kNormThreads, BLOCK ? norm_resid
 }
 
 // With u = d_y w and xh = (x - mean) rstd:  d_x = rstd (u - mean(u) - xh mean(u xh)).
-template <class T, bool PF32, int VEC, int ITEMS, bool BLOCK>
+template <class T, bool PF32, int VEC, int ITEMS, bool BLOCK, bool SHIFT>
 __global__ void __launch_bounds__(BLOCK ? 512 : kNormThreads, BLOCK ? norm_resident(true, VEC * ITEMS) / 512 : norm_resident(true, VEC * ITEMS) / kNormThreads) norm_bwd_kernel(NormParams p) {
   using P = typename NormParam<T, PF32>::type;
   constexpr int EPT = VEC * ITEMS;
@@ -230,14 +271,15 @@ __global__ void __launch_bounds__(BLOCK ? 512 : kNormThreads, BLOCK ? norm_resid
   int turn = 0;
   const NormPlace t = norm_place<BLOCK>(p);
   const int threads = BLOCK ? blockDim.x : p.lanes, lanes = BLOCK ? 32 : p.lanes;
+  const int off = SHIFT ? norm_shift<VEC>(p, t) : 0;
   pdl_trigger();
   float w[EPT], dw[EPT], db[EPT];
 #pragma unroll
   for (int i = 0; i < ITEMS; ++i) {
-    const int c = (i * threads + t.lane) * VEC;
+    const int c = (i * threads + t.lane) * VEC - off;
 #pragma unroll
     for (int j = 0; j < VEC; ++j) { w[i * VEC + j] = 1.f; dw[i * VEC + j] = db[i * VEC + j] = 0.f; }
-    if (p.w && t.active && c < p.n) norm_load<P, VEC>(static_cast<const P*>(p.w) + (int64_t)t.group * p.n + c, w + i * VEC);
+    if (p.w && t.active && c < p.n) norm_param<P, VEC, SHIFT>(static_cast<const P*>(p.w) + (int64_t)t.group * p.n, c, p.n, w + i * VEC);
   }
   const float inv_n = 1.f / (float)p.n;
   const int64_t first = BLOCK ? t.row : (int64_t)(blockIdx.x / p.gblocks) * (p.places / p.per_row);
@@ -250,9 +292,9 @@ __global__ void __launch_bounds__(BLOCK ? 512 : kNormThreads, BLOCK ? norm_resid
     const T* dy = static_cast<const T*>(p.dy) + row * p.dys + (int64_t)t.group * p.n;
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-      const int c = (i * threads + t.lane) * VEC;
-      next_x[i] = on && c < p.n ? norm_raw<T, VEC>(x + c) : norm_nothing<T, VEC>();
-      next_d[i] = on && c < p.n ? norm_raw<T, VEC>(dy + c) : norm_nothing<T, VEC>();
+      const int c = (i * threads + t.lane) * VEC - off;
+      next_x[i] = on ? norm_raw<T, VEC>(x, c, p.n) : norm_nothing<T, VEC>();
+      next_d[i] = on ? norm_raw<T, VEC>(dy, c, p.n) : norm_nothing<T, VEC>();
     }
     next_mean = on ? p.mean[row * p.groups + t.group] : 0.f;
     next_r = on ? p.rstd[row * p.groups + t.group] : 0.f;
@@ -266,16 +308,18 @@ __global__ void __launch_bounds__(BLOCK ? 512 : kNormThreads, BLOCK ? norm_resid
     for (int i = 0; i < ITEMS; ++i) {
       norm_floats<T, VEC>(next_x[i], v + i * VEC);
       norm_floats<T, VEC>(next_d[i], d + i * VEC);
+      norm_inside<VEC, SHIFT>(d + i * VEC, (i * threads + t.lane) * VEC - off, p.n);
     }
     const float mean = next_mean, r = next_r;
     fetch(row + t.step);
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-      const bool in = on && (i * threads + t.lane) * VEC < p.n;
+      const int c = (i * threads + t.lane) * VEC - off;
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
         const int e = i * VEC + j;
+        const bool in = on && (SHIFT ? c + j >= 0 && c + j < p.n : c < p.n);
         v[e] = in ? (v[e] - mean) * r : 0.f;
         dw[e] = fmaf(d[e], v[e], dw[e]);
         db[e] += d[e];
@@ -299,10 +343,10 @@ __global__ void __launch_bounds__(BLOCK ? 512 : kNormThreads, BLOCK ? norm_resid
     T* dx = static_cast<T*>(p.y) + row * p.ys + (int64_t)t.group * p.n;
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-      const int c = (i * threads + t.lane) * VEC;
+      const int c = (i * threads + t.lane) * VEC - off;
 #pragma unroll
       for (int j = 0; j < VEC; ++j) d[i * VEC + j] = r * (d[i * VEC + j] - s1 - v[i * VEC + j] * s2);
-      if (c < p.n) norm_store<T, VEC>(dx + c, d + i * VEC);
+      if (c < p.n) norm_store<T, VEC, SHIFT>(dx + c, d + i * VEC, c, p.n);
     }
   }
   if (!p.part) return;
@@ -310,36 +354,52 @@ __global__ void __launch_bounds__(BLOCK ? 512 : kNormThreads, BLOCK ? norm_resid
   if constexpr (BLOCK) {
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-      const int c = (i * threads + t.lane) * VEC;
+      const int c = (i * threads + t.lane) * VEC - off;
 #pragma unroll
       for (int j = 0; j < VEC; ++j)
-        if (c + j < p.n) {
+        if (c + j < p.n && (!SHIFT || c + j >= 0)) {
           part[c + j] = dw[i * VEC + j];
           part[p.span + c + j] = db[i * VEC + j];
         }
     }
   } else {
-    for (int c = threadIdx.x; c < 2 * p.span; c += kNormThreads) sums[c] = 0.f;
+    // Places of one group add to its columns in turn.  Where a warp has every group of a row the warps have a copy of the sums each, and only its own places wait
+    // for one another (60000 x 64 bf16: 49 us with one copy, a CTA-wide barrier a place).
+    const int copies = norm_copies(p.lanes, p.per_row), in_warp = 32 / p.lanes, warp = threadIdx.x >> 5, size = 2 * p.span;
+    for (int c = threadIdx.x; c < copies * size; c += kNormThreads) sums[c] = 0.f;
     __syncthreads();
-    // one place after the other: each adds to the columns of its group
-    const int rounds = p.places / p.per_row;
-    for (int k = 0; k < rounds; ++k) {
-      if (t.place < p.places && t.place / p.per_row == k) {
-        float* to = sums + (t.place % p.per_row) * p.n;
+    const auto add = [&] {
+      float* to = sums + (copies > 1 ? warp * size : 0) + (t.place % p.per_row) * p.n;
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-          const int c = (i * threads + t.lane) * VEC;
+      for (int i = 0; i < ITEMS; ++i) {
+        const int c = (i * threads + t.lane) * VEC - off;
 #pragma unroll
-          for (int j = 0; j < VEC; ++j)
-            if (c + j < p.n) {
-              to[c + j] += dw[i * VEC + j];
-              to[p.span + c + j] += db[i * VEC + j];
-            }
-        }
+        for (int j = 0; j < VEC; ++j)
+          if (c + j < p.n && (!SHIFT || c + j >= 0)) {
+            to[c + j] += dw[i * VEC + j];
+            to[p.span + c + j] += db[i * VEC + j];
+          }
+      }
+    };
+    const int turn_of = t.place < p.places ? t.place / p.per_row : -1;
+    if (copies > 1) {
+      const int last = (warp * in_warp + in_warp - 1) / p.per_row;
+      for (int k = warp * in_warp / p.per_row; k <= last; ++k) {
+        if (turn_of == k) add();
+        __syncwarp();
       }
       __syncthreads();
+    } else {
+      for (int k = 0; k < p.places / p.per_row; ++k) {
+        if (turn_of == k) add();
+        __syncthreads();
+      }
     }
-    for (int c = threadIdx.x; c < 2 * p.span; c += kNormThreads) part[c] = sums[c];
+    for (int c = threadIdx.x; c < size; c += kNormThreads) {
+      float a = sums[c];
+      for (int i = 1; i < copies; ++i) a += sums[i * size + c];
+      part[c] = a;
+    }
   }
 }
 

@@ -133,6 +133,20 @@ def test_many_rows(cuda_device):
     _check(*_inputs(20000, 1024, torch.float16, torch.float16, 2), G=16)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("cols,G", [(3, 1), (17, 1), (27, 3), (101, 1), (250, 1), (501, 3), (513, 1), (66, 22), (700, 28)])
+def test_many_rows_of_odd_lengths(cuda_device, dtype, cols, G):
+    """Rows that loads of 16 bytes do not divide, far more of them than the device has places: each place's rows begin as far into 16 bytes."""
+    rows = 40000 if cols < 200 else 9001
+    x, w, b, d = _inputs(rows, cols, dtype, torch.float32, cols)
+    _check(x, w, b, d, G=G)
+    apart = torch.zeros(2, rows * (cols + 5) + 9, dtype=dtype, device="cuda")
+    views = [t[3:3 + rows * (cols + 5)].view(rows, cols + 5)[:, 2:2 + cols] for t in apart]
+    views[0].copy_(x)
+    views[1].copy_(d)
+    _check(views[0], w, b, views[1], G=G)
+
+
 def test_gradients_against_differences(cuda_device):
     """Central differences of the float32 call: truncation h^2 / 6 times a third derivative of order one, rounding 2^-22 / h."""
     from flashnystrom_b200 import layer_norm
