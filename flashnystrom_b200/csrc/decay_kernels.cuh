@@ -79,12 +79,14 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
 
 // ---- chunked form ------------------------------------------------------------------------------------------
 // A CTA walks one run of rows, C at a time; tiles in shared memory as FP32.  Thread (ty, tx) of a 16 x 16 grid holds rows
-// ty + 16 i of the score and output tiles and a (D / 16)^2 piece of the state.  Bound by the shared-memory loads of its FP32 products.
+// ty + 16 i of the score and output tiles and a (D / 16)^2 piece of the state.  Bound by the shared-memory loads of its FP32 products
+// (4 x 4 outputs a thread: two values loaded for four products): 2 x 8 x 5001 x 64 fp32, forward and backward, 566 us, 621 before the products were packed in twos;
+// 12 GFLOP, a quarter of what the FP32 units do.  Three-term products on the tensor cores, as the landmark passes have for fp32, are not built.
 constexpr int kDecayC = 64;
 template <int D> struct DecaySmem {
   static constexpr int LD = D + 4, LP = kDecayC + 4;      // (padded rows: 16 rows read at once fall on different banks)
-  static constexpr int kFloats = 3 * kDecayC * LD + kDecayC * LP + D * LD + 80;
-  static constexpr int kBytes = kFloats * 4;
+  static constexpr int kTile = kDecayC * LD, kPowers = 80;
+  static constexpr int bytes(bool out) { return (4 * kTile + kPowers + (out ? kDecayC * LP + D * LD : 0)) * 4; }
 };
 
 template <class T, int D>
@@ -108,6 +110,40 @@ __device__ __forceinline__ void decay_load_tile(float* dst, const DecayRows& t, 
 #pragma unroll
     for (int j = 0; j < V; j += 4) *reinterpret_cast<float4*>(dst + r * LD + c + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
   }
+}
+
+// The same under way while the CTA goes on, where rows can be copied as they are; a group of its own for decay_arrived.
+template <class T, int D>
+__device__ __forceinline__ void decay_fetch_tile(float* dst, const DecayRows& t, int64_t base, int64_t row0, int nv, int vec) {
+  if (sizeof(T) == 4 && vec) {
+    constexpr int CH = D / 4, LD = DecaySmem<D>::LD;
+    const float* src = static_cast<const float*>(t.p) + base + row0 * t.sn;
+    for (int i = threadIdx.x; i < kDecayC * CH; i += kThreads) {
+      const int r = i / CH, c = (i % CH) * 4;
+      float* to = dst + r * LD + c;
+      if (r < nv) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(src + (int64_t)r * t.sn + c) : "memory");
+      else *reinterpret_cast<float4*>(to) = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+  } else if (nv > 0) {
+    decay_load_tile<T, D>(dst, t, base, row0, nv, vec);
+  }
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+// y' in y's place: row t times exp(g (rows behind it, or before it backwards in time)).  (The CTA meets before and behind it.)
+template <int D, bool REV> __device__ __forceinline__ void decay_weigh_tile(float* y, const float* pw, int nv, float scale) {
+  for (int i = threadIdx.x; i < nv * (D / 4); i += kThreads) {
+    const int t = i / (D / 4);
+    const float w = scale * pw[REV ? t + 1 : nv - 1 - t];
+    float4* at = reinterpret_cast<float4*>(y + t * DecaySmem<D>::LD + i % (D / 4) * 4);
+    float4 v = *at;
+    v.x *= w; v.y *= w; v.z *= w; v.w *= w;
+    *at = w == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : v;
+  }
+}
+// all but the last PENDING tiles are there
+template <int PENDING> __device__ __forceinline__ void decay_arrived() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
+  __syncthreads();
 }
 
 // CW consecutive floats from shared memory (CW = 1, 2, 4)
@@ -137,12 +173,14 @@ __global__ void __launch_bounds__(kThreads, D <= 64 ? 2 : 1) decay_chunk_kernel(
   constexpr int LD = L::LD, LP = L::LP, C = kDecayC;
   constexpr int CW = D / 16 < 4 ? D / 16 : 4, CG = D / 16 / CW;      // a thread's columns (and state rows): CG groups of CW
   extern __shared__ float4 smem4[];
-  float* xs = reinterpret_cast<float*>(smem4);
-  float* ys = xs + C * LD;
-  float* zs = ys + C * LD;
-  float* ps = zs + C * LD;
+  // Four tiles take turns.  With outputs: y, x and z of a chunk and the next y; the next x takes x's place and the next z y's as soon as those are done with.
+  float* ys = reinterpret_cast<float*>(smem4);
+  float* xs = ys + L::kTile;
+  float* zs = xs + L::kTile;
+  float* spare = zs + L::kTile;
+  float* pw = spare + L::kTile;      // exp(g n), n = 0 .. C
+  float* ps = pw + L::kPowers;
   float* ss = ps + C * LP;
-  float* pw = ss + D * LD;           // exp(g n), n = 0 .. C
 
   const int bh = blockIdx.x / p.nrun, cut = p.cut0 + blockIdx.x % p.nrun;
   const int b = bh / p.H, h = bh % p.H;
@@ -179,14 +217,27 @@ __global__ void __launch_bounds__(kThreads, D <= 64 ? 2 : 1) decay_chunk_kernel(
         }
   const int64_t bx = b * p.x.sb + h * p.x.sh, by = b * p.y.sb + h * p.y.sh, bz = b * p.z.sb + h * p.z.sh;
   const int chunks = r0 < end ? (int)((end - r0 + C - 1) / C) : 0;
-  for (int ci = 0; ci < chunks; ++ci) {
+  struct Rows { int64_t at; int n; };
+  const auto chunk = [&](int ci) -> Rows {      // (no rows behind the last)
+    if (ci >= chunks) return {r0, 0};
     const int64_t c0 = r0 + (int64_t)(REV ? chunks - 1 - ci : ci) * C;
-    const int nv = end - c0 < C ? (int)(end - c0) : C;
-    __syncthreads();
-    decay_load_tile<T, D>(ys, p.y, by, c0, nv, p.vec);
-    decay_load_tile<T, D>(zs, p.z, bz, c0, nv, p.vec);
+    return {c0, end - c0 < C ? (int)(end - c0) : C};
+  };
+  const auto fetch = [&](float* to, const DecayRows& t, int64_t base, int ci) {
+    const Rows c = chunk(ci);
+    if (c.n > 0) decay_fetch_tile<T, D>(to, t, base, c.at, c.n, p.vec);
+    else asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  fetch(ys, p.y, by, 0);
+  if (OUT) fetch(xs, p.x, bx, 0);
+  fetch(zs, p.z, bz, 0);
+  for (int ci = 0; ci < chunks; ++ci) {
+    const Rows rows = chunk(ci);
+    const int64_t c0 = rows.at;
+    const int nv = rows.n;
+    const bool more = ci + 1 < chunks;
+    __align__(8) float o[4][CG][CW];
     if (OUT) {
-      decay_load_tile<T, D>(xs, p.x, bx, c0, nv, p.vec);
 #pragma unroll
       for (int a = 0; a < CG; ++a)
 #pragma unroll
@@ -195,7 +246,8 @@ __global__ void __launch_bounds__(kThreads, D <= 64 ? 2 : 1) decay_chunk_kernel(
           for (int c = 0; c < CG; ++c)
 #pragma unroll
             for (int j = 0; j < CW; ++j) ss[(a * 64 + ty * CW + i) * LD + c * 64 + tx * CW + j] = S[a][i][c][j];
-      __syncthreads();
+      decay_arrived<1>();      // (y and x)
+      fetch(spare, p.y, by, ci + 1);
       float2 acc[4][4];      // even and odd columns
 #pragma unroll
       for (int i = 0; i < 4; ++i)
@@ -222,16 +274,85 @@ __global__ void __launch_bounds__(kThreads, D <= 64 ? 2 : 1) decay_chunk_kernel(
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int s = ty + 16 * i, t = tx + 16 * j, d = REV ? t - s : s - t;
-          ps[s * LP + t] = d >= 0 ? (acc[i][j].x + acc[i][j].y) * pw[d] : 0.f;
+          ps[s * LP + t] = d >= 0 ? (acc[i][j].x + acc[i][j].y) * pw[d] * p.scale : 0.f;
         }
-      __syncthreads();
-      __align__(8) float o[4][CG][CW], q[4][CG][CW];
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int c = 0; c < CG; ++c)
 #pragma unroll
-          for (int j = 0; j < CW; ++j) o[i][c][j] = q[i][c][j] = 0.f;
+          for (int j = 0; j < CW; ++j) o[i][c][j] = 0.f;
+      for (int k = 0; k < D; k += 4) {
+        float xv[4][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) decay_lds<4>(xs + (ty + 16 * i) * LD + k, xv[i]);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+          for (int c = 0; c < CG; ++c) {
+            __align__(8) float sv[CW];
+            decay_lds<CW>(ss + (k + u) * LD + c * 64 + tx * CW, sv);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) decay_axpy<CW>(xv[i][u], sv, o[i][c]);
+          }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int s = ty + 16 * i;
+        const float w = s < nv ? p.inter * pw[REV ? nv - 1 - s : s + 1] : 0.f;
+#pragma unroll
+        for (int c = 0; c < CG; ++c)
+#pragma unroll
+          for (int j = 0; j < CW; ++j) o[i][c][j] = w == 0.f ? 0.f : w * o[i][c][j];
+      }
+      decay_arrived<1>();      // (z; scores are written, x is done with)
+      fetch(xs, p.x, bx, ci + 1);
+    } else {
+      decay_arrived<0>();
+      fetch(xs, p.y, by, ci + 1);
+      fetch(spare, p.z, bz, ci + 1);
+    }
+    // the state: U = sum over the chunk's rows, then S = exp(g nv) S + U (nothing needs the one behind the last chunk of a run with outputs)
+    if (!OUT || more) {
+      decay_weigh_tile<D, REV>(ys, pw, nv, p.sum_scale);
+      __syncthreads();
+      __align__(8) float U[CG][CW][CG][CW];
+#pragma unroll
+      for (int a = 0; a < CG; ++a)
+#pragma unroll
+        for (int i = 0; i < CW; ++i)
+#pragma unroll
+          for (int c = 0; c < CG; ++c)
+#pragma unroll
+            for (int j = 0; j < CW; ++j) U[a][i][c][j] = 0.f;
+#pragma unroll 4
+      for (int t = 0; t < nv; ++t) {
+        __align__(8) float yv[CG][CW], zv[CG][CW];
+#pragma unroll
+        for (int a = 0; a < CG; ++a) {
+          decay_lds<CW>(ys + t * LD + a * 64 + ty * CW, yv[a]);
+          decay_lds<CW>(zs + t * LD + a * 64 + tx * CW, zv[a]);
+        }
+#pragma unroll
+        for (int a = 0; a < CG; ++a)
+#pragma unroll
+          for (int i = 0; i < CW; ++i)
+#pragma unroll
+            for (int c = 0; c < CG; ++c) decay_axpy<CW>(yv[a][i], zv[c], U[a][i][c]);
+      }
+      const DecayPair by_nv = nv == C ? full : decay_pair(g, nv);
+#pragma unroll
+      for (int a = 0; a < CG; ++a)
+#pragma unroll
+        for (int i = 0; i < CW; ++i)
+#pragma unroll
+          for (int c = 0; c < CG; ++c)
+#pragma unroll
+            for (int j = 0; j < CW; ++j) S[a][i][c][j] = decay_by(by_nv, S[a][i][c][j]) + U[a][i][c][j];
+    }
+    if (OUT) {
+      if (more) __syncthreads();      // (y is done with)
+      fetch(ys, p.z, bz, ci + 1);
 #pragma unroll
       for (int tb = 0; tb < 4; ++tb)
         for (int t = tb * 16; t < tb * 16 + 16; t += 4) {
@@ -250,31 +371,16 @@ __global__ void __launch_bounds__(kThreads, D <= 64 ? 2 : 1) decay_chunk_kernel(
                 if (REV ? i <= tb : i >= tb) decay_axpy<CW>(pv[i][u], zv, o[i][c]);
             }
         }
-      for (int k = 0; k < D; k += 4) {
-        float xv[4][4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) decay_lds<4>(xs + (ty + 16 * i) * LD + k, xv[i]);
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-#pragma unroll
-          for (int c = 0; c < CG; ++c) {
-            __align__(8) float sv[CW];
-            decay_lds<CW>(ss + (k + u) * LD + c * 64 + tx * CW, sv);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) decay_axpy<CW>(xv[i][u], sv, q[i][c]);
-          }
-      }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int s = ty + 16 * i;
         if (s >= nv) continue;
-        const float w = p.inter * pw[REV ? nv - 1 - s : s + 1];
         T* to = out + (c0 + s) * p.out.sn;
 #pragma unroll
         for (int c = 0; c < CG; ++c) {
           T v[CW];
 #pragma unroll
-          for (int j = 0; j < CW; ++j) v[j] = from_f<T>(w == 0.f ? p.scale * o[i][c][j] : fmaf(w, q[i][c][j], p.scale * o[i][c][j]));
+          for (int j = 0; j < CW; ++j) v[j] = from_f<T>(o[i][c][j]);
           if (CW == 4 && p.vec) {
             if (sizeof(T) == 4) *reinterpret_cast<uint4*>(to + c * 64 + tx * CW) = *reinterpret_cast<uint4*>(v);
             else *reinterpret_cast<uint2*>(to + c * 64 + tx * CW) = *reinterpret_cast<uint2*>(v);
@@ -284,47 +390,12 @@ __global__ void __launch_bounds__(kThreads, D <= 64 ? 2 : 1) decay_chunk_kernel(
           }
         }
       }
+      float* const was = zs;
+      zs = ys; ys = spare; spare = was;
     } else {
-      __syncthreads();
+      float* const y = ys; float* const z = zs;
+      ys = xs; zs = spare; xs = y; spare = z;
     }
-    if (OUT && ci + 1 == chunks) break;      // (nothing needs the state behind the last)
-    // the state: U = sum over the chunk's rows, then S = exp(g nv) S + U
-    __align__(8) float U[CG][CW][CG][CW];
-#pragma unroll
-    for (int a = 0; a < CG; ++a)
-#pragma unroll
-      for (int i = 0; i < CW; ++i)
-#pragma unroll
-        for (int c = 0; c < CG; ++c)
-#pragma unroll
-          for (int j = 0; j < CW; ++j) U[a][i][c][j] = 0.f;
-#pragma unroll 4
-    for (int t = 0; t < nv; ++t) {
-      const float w = p.sum_scale * pw[REV ? t + 1 : nv - 1 - t];
-      __align__(8) float yv[CG][CW], zv[CG][CW];
-#pragma unroll
-      for (int a = 0; a < CG; ++a) {
-        decay_lds<CW>(ys + t * LD + a * 64 + ty * CW, yv[a]);
-        decay_lds<CW>(zs + t * LD + a * 64 + tx * CW, zv[a]);
-#pragma unroll
-        for (int i = 0; i < CW; ++i) yv[a][i] = w == 0.f ? 0.f : yv[a][i] * w;
-      }
-#pragma unroll
-      for (int a = 0; a < CG; ++a)
-#pragma unroll
-        for (int i = 0; i < CW; ++i)
-#pragma unroll
-          for (int c = 0; c < CG; ++c) decay_axpy<CW>(yv[a][i], zv[c], U[a][i][c]);
-    }
-    const DecayPair by_nv = nv == C ? full : decay_pair(g, nv);
-#pragma unroll
-    for (int a = 0; a < CG; ++a)
-#pragma unroll
-      for (int i = 0; i < CW; ++i)
-#pragma unroll
-        for (int c = 0; c < CG; ++c)
-#pragma unroll
-          for (int j = 0; j < CW; ++j) S[a][i][c][j] = decay_by(by_nv, S[a][i][c][j]) + U[a][i][c][j];
   }
   if (OUT) return;
   float* to = p.state_out + ((size_t)bh * p.ncut + cut) * D * D;
@@ -340,7 +411,8 @@ __global__ void __launch_bounds__(kThreads, D <= 64 ? 2 : 1) decay_chunk_kernel(
 
 // ---- the runs of a slice joined -----------------------------------------------------------------------------
 // One thread per element of the state of a slice goes through the runs in the order of time: before the first run of a segment
-// the state so far is what enters that segment.  What depends on the run alone is formed once a CTA.
+// the state so far is what enters that segment.  What depends on the run alone is formed once a CTA.  A chain over the runs, its loads fetched ahead:
+// 9 us for 16 slices in 9 segments of two runs (19 MB), 17 us for 64 slices with heads of 128 in two segments.
 struct DecayJoinParams {
   const float* sums;          // [BH][ncut][D][D]: each run alone
   const float* state_in;      // [BH][D][D] or null
@@ -396,7 +468,8 @@ __global__ void __launch_bounds__(kThreads) decay_join_kernel(DecayJoinParams p)
 
 // ---- one token ----------------------------------------------------------------------------------------------
 // A CTA takes W columns of one head's state: LPR = W / 4 threads hold a row's columns as float4, the rows are spread over the CTA.
-// Columns are independent of one another, the sum over the rows ends in shared memory.  Bound by the state, read and written once.
+// Columns are independent of one another, the sum over the rows ends in shared memory.  Bound by the state,
+// read and written once: 4096 heads of 128 (541 MB) 84 us, 6.4 TB/s, which is the rate of a copy.
 struct DecayStepParams {
   const void *q, *k, *v;
   void* out;

@@ -5,7 +5,7 @@
 //     P = x y^T (C x C)             -> times exp(g |s - t|) and the mask, rounded to 16 bits
 //     out = P z + exp(g (s + 1)) x S
 //     S = exp(g C) S + y'^T z,      y' = exp(g (C - 1 - t)) y, as one 16-bit term for the outputs, as two or three
-//                                                                 for the sums that join segments and for the state that is handed out
+//                                                                 for the state that is handed out
 // S takes part in x S as the sum of two 16-bit terms.  So each term of an output is rounded once on its way to 16 bits (its score inside a chunk, its y'
 // outside), and the output once.
 #pragma once
@@ -29,15 +29,6 @@ __device__ __forceinline__ uint64_t along_row(uint32_t base, int k, int rows) {
 __device__ __forceinline__ uint64_t along_rows(uint32_t base, int k, int rows) {
   return smem_desc_sw128(base + k * 2048, rows * 128, 1024);
 }
-template <int NC> __device__ __forceinline__ void ld_cols(uint32_t taddr, float* v) {
-  if (NC == 16) {
-    tmem_ld16(taddr, v);
-  } else {
-#pragma unroll
-    for (int c = 0; c < NC; c += 32) tmem_ld32(taddr + c, v + c);
-  }
-}
-
 struct DecayTcParams {
   const float* log_decay;
   const int32_t* seq_lens;
@@ -56,7 +47,7 @@ struct DecayTcForm {
   int transposed;             // the state is read as its transpose
 };
 // Two forms that read mostly the same rows (dv and dk: q and do in both, k or v) run side by side, the same segment of both in neighbouring CTAs: what one
-// reads the other finds in L2 (B=4, H=16, N=16384, D=128: 425 us one after the other, see kForms below for both together).
+// reads the other finds in L2 (1 x 16 x 65536 x 64 bf16: 246 us one after the other, 231 together; 4 x 16 x 16384 x 128: 425 and 430).
 template <int FORMS> struct DecayTcForms { DecayTcForm f[FORMS]; };
 
 template <class T> __device__ __forceinline__ float2 unpack2(uint32_t u);
@@ -101,6 +92,8 @@ __device__ __forceinline__ void scaled_terms(uint4 raw, float w, uint4* terms) {
 // tensor memory over kSpan rows (weights reach back that far) before the group takes them out and decays what it has.
 // EXACT: two terms of fp16, three of bf16, 22 and 24 bits: the sums are FP32 sums, as a state that is handed out has to be.  Where the sums only join
 // segments, one term, as the chunks inside a segment have it: what an output gets from before its segment is then rounded once, like the rest.
+// Bound by what the eight warps do (a value into terms, two swizzled stores).  1 x 16 x 65536 x 64, 268 MB read: 58 us with one term (4.6 TB/s), 74 with two (fp16),
+// 87 with three (bf16); 4 x 16 x 16384 x 128, 537 MB, one term, half of the rows (what the first of two segments needs): 68 us.
 template <class T, int D, bool EXACT> struct SumsCfg {
   static constexpr int C = D == 64 ? 64 : 32, kStages = 3, kTerms = !EXACT ? 1 : UmmaFmt<T>::v == 0 ? 2 : 3;
   static constexpr int kSpan = 256;
@@ -289,14 +282,19 @@ decay_tc_sums_kernel(const __grid_constant__ CUtensorMap tm_y, const __grid_cons
 }
 
 // ---- outputs -------------------------------------------------------------------------------------------------
-// One CTA a segment, one CTA an SM, 20 or 28 warps, chunks of 128 rows: group A (eight warps, with heads of 64 two groups that
-// take the chunks in turn) turns P into its 16-bit operand and takes the output
-// tile out, group B (eight) forms y' and carries the state, one warp loads, one issues the products of A, one those of B, one
+// One CTA a segment, one CTA an SM, 28 warps with heads of 64 and 20 with heads of 128, chunks of 128 rows: group A (eight warps; with heads of 64 there are
+// two, which take the chunks in turn) turns P into its 16-bit operand and takes the output tile out, group B (eight) forms y' and carries the state, one warp loads, one issues the products of A, one those of B, one
 // stores.  The two groups meet only in what the products need: while A works on the scores of a chunk, B is at the state behind it.
 //
 // Shared memory is what there is least of, its bandwidth (every operand of a product passes it) and, with heads of 128, its room: so P goes to its product
 // through tensor memory, the output tile takes x's place, and with heads of 128 y' takes y's.  The state stays in tensor memory: B takes it out to form
 // its two 16-bit terms, puts it back decayed, and the products add y'^T z to it.
+//
+// Measured: 1 x 16 x 65536 x 64, a pass of 537 MB, 144 CTAs: bf16 122 us (4.4 TB/s), fp16 142 (its state is scaled by powers of two to stay in range); 4 x 16 x
+// 16384 x 128, 1.07 GB, 128 CTAs: 216 us (5.0 TB/s; 193 is what 128 of 148 SMs move).  Bound with heads of 64 by the warps' arithmetic in turn: of 127 us, 8 go
+// without forming y', 10 without the state, 16 without weighing the scores, 6 without the output tile.  What decides it is code that stays in the instruction
+// cache: loops over 16 columns that are not unrolled took 131 us where pieces of 32 columns, unrolled, took 150 (fp16 152 and 187).
+// Sixteen warps in group B: no change with heads of 64, 238 in place of 216 with 128.  Outputs stored from registers: 195 in place of 162 at the time.
 constexpr int kC = 128;      // rows of a chunk
 template <int D> struct MainCfg {
   static constexpr int kTile = kC * D * 2;
@@ -519,8 +517,7 @@ __global__ void __launch_bounds__(MainCfg<D>::kThreads, 1) decay_tc_kernel(const
     }
   } else if (warp < L::kWarpB) {
     // ---- group A: scores and outputs of every NA-th chunk
-    // (Here and in group B one warp asks the mbarriers for all, the others wait at a barrier, which takes no issue slots: twenty warps that ask took 40 % of
-    // them.  A wait that gave up does not leave the loop: the warps meet at barriers, and the status word has it.)
+    // (Here and in group B one warp asks the mbarriers for all, the others wait at a barrier.  A wait that gave up does not leave the loop: the warps meet at barriers, and the status word has it.)
     const int ga = warp >> 3, quarter = warp & 3, half = warp >> 2 & 1, bar = 1 + 2 * ga;
     const bool asks = (warp & 7) == 0;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;

@@ -24,10 +24,10 @@ struct DecayPlan {
   int64_t seg_rows, sub_rows;
   int runs() const { return nseg * sub; }
 };
-constexpr int kDecayUnit = 128;
 
 static DecayPlan decay_plan(const fnb_decay_shape& s) {
-  const int64_t BH = s.batch * s.heads, units = (s.seq_len + kDecayUnit - 1) / kDecayUnit;
+  const int64_t unit = s.dtype == FNB_F32 ? 64 : 128;      // rows of a chunk
+  const int64_t BH = s.batch * s.heads, units = (s.seq_len + unit - 1) / unit;
   const int sms = current_sm_count();
   // Estimated time of a split, in units that one CTA takes in turn: rounds of CTAs x units of the longest, and, where there is more
   // than one segment, half of that for the pass over the states and about four units' time for two more launches.
@@ -42,11 +42,11 @@ static DecayPlan decay_plan(const fnb_decay_shape& s) {
     if (t < least) { least = t; best = n; }
   }
   DecayPlan p;
-  p.seg_rows = (units + best - 1) / best * kDecayUnit;
+  p.seg_rows = (units + best - 1) / best * unit;
   p.nseg = (int)((s.seq_len + p.seg_rows - 1) / p.seg_rows);
   // two CTAs of the pass over the states fit on an SM
-  int64_t sub = std::max<int64_t>(1, std::min<int64_t>(2 * (int64_t)sms / std::max<int64_t>(1, BH * std::max(1, p.nseg - 1)), p.seg_rows / kDecayUnit));
-  p.sub_rows = (p.seg_rows / kDecayUnit + sub - 1) / sub * kDecayUnit;
+  int64_t sub = std::max<int64_t>(1, std::min<int64_t>(2 * (int64_t)sms / std::max<int64_t>(1, BH * std::max(1, p.nseg - 1)), p.seg_rows / unit));
+  p.sub_rows = (p.seg_rows / unit + sub - 1) / sub * unit;
   p.sub = (int)((p.seg_rows + p.sub_rows - 1) / p.sub_rows);
   return p;
 }
@@ -140,9 +140,10 @@ static int launch_chunks(const DecayCall& c, const DecayParams& p, Launcher& L, 
     using T = decltype(tag);
     constexpr int D = decltype(d)::value;
     auto kern = decay_chunk_kernel<T, D, REV, OUT>;
-    if (int rc = set_smem(kern, DecaySmem<D>::kBytes, c.max_smem, name)) return rc;
+    constexpr int smem = DecaySmem<D>::bytes(OUT);
+    if (int rc = set_smem(kern, smem, c.max_smem, name)) return rc;
     L.begin();
-    kern<<<(unsigned)(c.BH * p.nrun), kThreads, DecaySmem<D>::kBytes, c.stream>>>(p);
+    kern<<<(unsigned)(c.BH * p.nrun), kThreads, smem, c.stream>>>(p);
     return L.end(name);
   });
 }
