@@ -79,9 +79,10 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
 
 // ---- chunked form ------------------------------------------------------------------------------------------
 // A CTA walks one run of rows, C at a time; tiles in shared memory as FP32.  Thread (ty, tx) of a 16 x 16 grid holds rows
-// ty + 16 i of the score and output tiles and a (D / 16)^2 piece of the state.  Bound by the shared-memory loads of its FP32 products
-// (4 x 4 outputs a thread: two values loaded for four products): 2 x 8 x 5001 x 64 fp32, forward and backward, 566 us, 621 before the products were packed in twos;
-// 12 GFLOP, a quarter of what the FP32 units do.  Three-term products on the tensor cores, as the landmark passes have for fp32, are not built.
+// ty + 16 i of the score and output tiles and a (D / 16)^2 piece of the state.  Bound by the shared-memory loads of its FP32 products (4 x 4 outputs a
+// thread: two values loaded for four products; with 128 registers a thread there is no room for more).  fp32, 2 x 8 x 5001 x 64, a pass with outputs / the sums:
+// 79 / 29 us; 4 x 8 x 4096 x 128: 329 / 97.  Before tiles were fetched ahead and y' formed once a chunk: 115 / 46 and 532 / 166.  FP32 units at about half their
+// rate.  Three-term products on the tensor cores, as the landmark passes have for fp32, are not built.
 constexpr int kDecayC = 64;
 template <int D> struct DecaySmem {
   static constexpr int LD = D + 4, LP = kDecayC + 4;      // (padded rows: 16 rows read at once fall on different banks)
@@ -190,7 +191,8 @@ __global__ void __launch_bounds__(kThreads, D <= 64 ? 2 : 1) decay_chunk_kernel(
   const int64_t end = r1 < len ? r1 : len;            // rows that count
   if (!OUT && r0 >= end) return;                       // (what joins the runs knows that there is nothing)
   const double g = decay_log(p.log_decay[h]);
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  // (a warp's threads 8 x 4: the 16 bytes that they load for their columns are 128 together)
+  const int tx = (threadIdx.x & 7) + (threadIdx.x >> 2 & 8), ty = (threadIdx.x >> 3 & 3) + (threadIdx.x >> 6) * 4;
   for (int i = threadIdx.x; i <= C; i += kThreads) pw[i] = (float)exp(g * i);
   const DecayPair full = decay_pair(g, C);
 
