@@ -63,8 +63,9 @@ static int check_decay_shape(const fnb_decay_shape* s) {
     return fail(FNB_ERR_INVALID_ARGUMENT, "Supported dtypes: float32, float16, bfloat16 (got code %d)", s->dtype);
   if (!(s->head_dim == 16 || s->head_dim == 32 || s->head_dim == 64 || s->head_dim == 128))
     return fail(FNB_ERR_INVALID_ARGUMENT, "head_dim must be 16, 32, 64 or 128, got %d", s->head_dim);
-  if (!std::isfinite(s->scale) || s->scale == 0.f)
-    return fail(FNB_ERR_INVALID_ARGUMENT, "scale must be finite and not 0 (got %g)", (double)s->scale);
+  // (gradients of states have the scale in them, and their share of a product is divided by it)
+  if (!(std::fabs(s->scale) >= 0x1p-64f && std::fabs(s->scale) <= 0x1p64f))
+    return fail(FNB_ERR_INVALID_ARGUMENT, "scale must be finite and not 0, between 2^-64 and 2^64 in magnitude (got %g)", (double)s->scale);
   if (s->flags & ~FNB_FLAG_FORCE_GENERIC) return fail(FNB_ERR_INVALID_ARGUMENT, "unknown flags 0x%x", s->flags);
   return 0;
 }

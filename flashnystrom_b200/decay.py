@@ -4,8 +4,6 @@
 
 One float32 D x D state for each (batch, head) takes the place of a cache of keys and values, so that a token costs the same after any
 number of others, and a sequence of N tokens costs N."""
-import math
-
 import torch
 import torch.nn as nn
 
@@ -15,8 +13,8 @@ from .norm import layer_norm
 
 def _scale(scale, D):
     scale = float(D) ** -0.5 if scale is None and D > 0 else 1.0 if scale is None else float(scale)
-    if not math.isfinite(scale) or scale == 0.0:
-        raise RuntimeError(f"scale must be finite and not 0 (got {scale})")
+    if not 2.0 ** -64 <= abs(scale) <= 2.0 ** 64:
+        raise RuntimeError(f"scale must be finite and not 0, between 2^-64 and 2^64 in magnitude (got {scale})")
     return scale
 
 
@@ -35,7 +33,7 @@ def decay_attention(q, k, v, log_decay, scale=None, initial_state=None, seq_lens
     q, k, v: (B, H, N, D) CUDA tensors of one dtype (fp16 / bf16 / fp32), D 16, 32, 64 or 128, any strides (the head-split view of a
     (B, N, H * D) projection is read in place, and the output and the gradients come back in that order of memory).
     log_decay: (H,) float32, <= 0: 0 keeps everything, -inf only the token itself; a constant, without a gradient.
-    scale: D ** -0.5 unless given.
+    scale: D ** -0.5 unless given; 2^-64 to 2^64 in magnitude.
     initial_state: (B, H, D, D) float32, S[i, j] = sum k_i v_j, or None for zeros.  Differentiable.
     seq_lens: (B,) int32 on the GPU: rows past a sequence's length take no part, whatever they hold (infinities and NaN too), and
         come out as zeros; values outside 0..N count as the nearest of these.  None: all sequences have N rows.

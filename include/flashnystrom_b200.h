@@ -332,7 +332,7 @@ typedef struct fnb_decay_shape {
   int64_t batch, heads, seq_len;
   int32_t head_dim;       /* 16, 32, 64 or 128 */
   int32_t dtype;          /* fnb_dtype of q, k, v, out and the gradients; states are FP32 */
-  float scale;            /* finite, not 0 */
+  float scale;            /* 2^-64 to 2^64 in magnitude */
   uint32_t flags;         /* 0 or FNB_FLAG_FORCE_GENERIC */
 } fnb_decay_shape;
 typedef struct fnb_rows {

@@ -345,6 +345,16 @@ def test_empty(cuda_device):
     assert torch.equal(s0.grad, torch.ones_like(s0))
     out, state = decay_attention(q[:0], q[:0], q[:0], torch.zeros(3, device="cuda"), return_state=True)
     assert out.shape == (0, 3, 0, 64) and state.shape == (0, 3, 64, 64)
+    leaves = [torch.zeros(2, 3, 0, 64, device="cuda", requires_grad=True) for _ in range(3)]
+    grads = torch.autograd.grad(decay_attention(*leaves, torch.zeros(3, device="cuda")).sum(), leaves)
+    assert all(g.shape == (2, 3, 0, 64) for g in grads)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("scale", [2.0 ** -64, 2.0 ** 64])
+def test_scale_at_its_ends(cuda_device, dtype, scale):
+    """(fp16 outputs would leave their range; those of the others and their sums, 2^64 times a few hundred, do not.)"""
+    _check(*_inputs(1, 2, 700, 64, dtype, 23), scale=scale)
 
 
 def test_c_abi_writes_nothing_but_its_rows(cuda_device):

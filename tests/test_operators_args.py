@@ -20,7 +20,7 @@ def _shape(B=1, H=2, N=100, D=64, dtype=_lib.FNB_F16, scale=0.125, flags=0):
 
 @pytest.mark.parametrize("kw,message", [
     (dict(B=0), "must be positive"), (dict(H=0), "must be positive"), (dict(N=0), "must be positive"), (dict(D=48), "head_dim must be"), (dict(D=256), "head_dim must be"),
-    (dict(dtype=7), "Supported dtypes"), (dict(scale=0.0), "scale must be"), (dict(scale=float("inf")), "scale must be"), (dict(flags=4), "unknown flags"),
+    (dict(dtype=7), "Supported dtypes"), (dict(scale=0.0), "scale must be"), (dict(scale=float("inf")), "scale must be"), (dict(scale=1e-20), "scale must be"), (dict(scale=-1e20), "scale must be"), (dict(flags=4), "unknown flags"),
     (dict(B=300, H=300), "exceeds 65535"), (dict(N=2 ** 31), "exceeds 2"), (dict(B=2 ** 40, H=2 ** 40), "exceeds 65535")])
 def test_decay_shapes(lib, kw, message):
     s = _shape(**kw)
