@@ -314,7 +314,8 @@ static NormPlan norm_plan(const fnb_norm_shape& s, NormLoads how, bool backward,
   p.vec = how == kNormSingle ? 1 : V;
   // Up to 512 columns a warp (or a part of one) holds a run, 16 elements a thread and two loads where there are as many; above that a CTA, 16 elements a
   // thread while it has threads (65536 x 1024 fp16, backward: 95 us, with a warp a run 168).  The forward keeps to warps up to 1024 columns of 16 bits
-  // (56 us, a CTA a run 76).
+  // (56 us, a CTA a run 76), and to 32 elements a thread above: fewer warps meet once a row, and an SM has several CTAs, which wait for their own row alone
+  // (bf16, 16384 x 4096: 54 us, with 16 elements 77; 8192 x 8192: 56 and 79; not where ends are picked out, which takes registers: fp32, 3000 x 7001, 55 and 41).
   p.block = n > (!backward && how == kNormWhole && V == 8 ? 1024 : 512);
   const int loads = how == kNormShifted ? (n + 2 * V - 2) / V : (n + p.vec - 1) / p.vec;
   if (!p.block) {
@@ -331,7 +332,9 @@ static NormPlan norm_plan(const fnb_norm_shape& s, NormLoads how, bool backward,
   } else {
     p.lanes = 32;
     p.threads = 64;
-    while (p.threads < 512 && loads * p.vec > p.threads * 16) p.threads *= 2;
+    const bool few = !backward && how == kNormWhole;
+    const int each = few ? 32 : 16, most = few && n <= 8192 ? 256 : 512;
+    while (p.threads < most && loads * p.vec > p.threads * each) p.threads *= 2;
     p.items = (loads + p.threads - 1) / p.threads;
     p.per_row = p.places = 1;
     p.gblocks = s.groups;
