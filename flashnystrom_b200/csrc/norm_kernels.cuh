@@ -5,8 +5,9 @@
 // group of its own that it keeps over all its rows: weight and bias stay in registers, and the backward adds up its share
 // of d_weight and d_bias there; places are joined in shared memory in their order, CTAs by a second kernel in theirs.
 // Bound by HBM: x (and d_y) read once, y (d_x) written once.  Forward / backward, us, with the share of a copy's 6.4 TB/s: 65536 x 1024 fp16 in 16 groups
-// 50 / 78 (83 / 80 %), in one 48 / 80; bf16, 16384 x 4096 54 / 86, 8192 x 8192 56 / 90, 4096 x 16384 64 / -; rows of odd lengths, which take the same loads with
-// their ends picked out, 20000 x 2002 bf16 60 / 65 (42 / 57 %: the picking).  The kernel that joins the CTAs' sums takes 5 to 10.
+// 52 / 78 (80 %), in one 50 / 80; bf16, 16384 x 4096 54 / 86, 8192 x 8192 56 / 90, 4096 x 16384 64 / -; rows of odd lengths, which take the same loads with
+// their ends picked out, 20000 x 2002 bf16 59 / 65 (42 / 57 %: the picking).  The kernel that joins the CTAs' sums takes 5 to 10.  A second row under way
+// ahead, forward: no faster (65536 x 1024 52, 16384 x 4096 56), short rows slower (200000 x 128 bf16 25.5 against 23.9: registers).
 #pragma once
 #include "common.cuh"
 
@@ -161,9 +162,6 @@ __host__ __device__ constexpr int norm_copies(int lanes, int per_row) { return p
 __host__ __device__ constexpr int norm_resident(bool backward, int elements) {
   return elements <= 8 ? 1024 : elements <= 16 && !backward ? 768 : 512;
 }
-// Rows that a thread of the forward has under way beside its own: two where there are registers for them (65536 x 1024 fp16 in 16 groups: 50 us, with one 54; where a
-// CTA holds a run they cost it a third of the CTAs: fp32, 65536 x 1024, 104 and 99).
-__host__ __device__ constexpr int norm_ahead(bool block, int elements) { return !block && elements <= 16 ? 2 : 1; }
 template <class T, bool PF32, int VEC, int ITEMS, bool BLOCK, bool SHIFT>
 __global__ void __launch_bounds__(BLOCK ? 512 : kNormThreads, BLOCK ? norm_resident(false, VEC * ITEMS) / 512 : norm_resident(false, VEC * ITEMS) / kNormThreads) norm_fwd_kernel(NormParams p) {
   using P = typename NormParam<T, PF32>::type;
@@ -197,26 +195,27 @@ __global__ void __launch_bounds__(BLOCK ? 512 : kNormThreads, BLOCK ? norm_resid
   // (every thread of a warp goes round as often as the others: the sums are shuffles of whole warps)
   const int64_t first = BLOCK ? t.row : (int64_t)(blockIdx.x / p.gblocks) * (p.places / p.per_row);
   const int apart = BLOCK ? 0 : t.place / p.per_row;
-  // the next rows' loads are under way while one is worked on
-  constexpr int AHEAD = norm_ahead(BLOCK, EPT);
-  NormRaw<T, VEC> next[AHEAD][ITEMS];
-  const auto fetch = [&](NormRaw<T, VEC>* to, int64_t row) {
+  // the next row's loads are under way while one is worked on
+  NormRaw<T, VEC> next[ITEMS];
+  const auto fetch = [&](int64_t row) {
     const T* x = static_cast<const T*>(p.x) + row * p.xs + (int64_t)t.group * p.n;
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
       const int c = (i * threads + t.lane) * VEC - off;
-      to[i] = t.active && row < p.rows ? norm_raw<T, VEC>(x, c, p.n) : norm_nothing<T, VEC>();
+      next[i] = t.active && row < p.rows ? norm_raw<T, VEC>(x, c, p.n) : norm_nothing<T, VEC>();
     }
   };
-  const auto work = [&](NormRaw<T, VEC>* raw, int64_t row) {
+  fetch(first + apart);
+  for (int64_t base = first; base < p.rows; base += t.step) {
+    const int64_t row = base + apart;
     const bool on = t.active && row < p.rows;
     float v[EPT];
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-      norm_floats<T, VEC>(raw[i], v + i * VEC);
+      norm_floats<T, VEC>(next[i], v + i * VEC);
       norm_inside<VEC, SHIFT>(v + i * VEC, (i * threads + t.lane) * VEC - off, p.n);
     }
-    fetch(raw, row + AHEAD * t.step);
+    fetch(row + t.step);
     float s = 0.f;
 #pragma unroll
     for (int j = 0; j < EPT; ++j) s += v[j];
@@ -249,7 +248,7 @@ __global__ void __launch_bounds__(BLOCK ? 512 : kNormThreads, BLOCK ? norm_resid
       for (int j = 0; j < EPT; ++j) v[j] += own - mean;
     }
     const float r = 1.f / sqrtf(q * inv_n + p.eps);
-    if (!on) return;
+    if (!on) continue;
     T* y = static_cast<T*>(p.y) + row * p.ys + (int64_t)t.group * p.n;
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
@@ -262,13 +261,7 @@ __global__ void __launch_bounds__(BLOCK ? 512 : kNormThreads, BLOCK ? norm_resid
       if (p.mean) p.mean[row * p.groups + t.group] = mean;
       if (p.rstd) p.rstd[row * p.groups + t.group] = r;
     }
-  };
-#pragma unroll
-  for (int a = 0; a < AHEAD; ++a) fetch(next[a], first + a * t.step + apart);
-  for (int64_t base = first; base < p.rows; base += AHEAD * t.step)
-#pragma unroll
-    for (int a = 0; a < AHEAD; ++a)
-      if (base + a * t.step < p.rows) work(next[a], base + a * t.step + apart);
+  }
 }
 
 // With u = d_y w and xh = (x - mean) rstd:  d_x = rstd (u - mean(u) - xh mean(u xh)).
