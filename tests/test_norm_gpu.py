@@ -78,6 +78,12 @@ def test_forward_and_backward(cuda_device, dtype, params, rows, cols, G):
     _check(*_inputs(rows, cols, dtype, params, rows + cols), G=G)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("cols", [512, 520, 1024, 1032, 2048, 2056, 4096, 4100, 8192, 8200, 16376])
+def test_lengths_around_what_threads_hold(cuda_device, dtype, cols):
+    _check(*_inputs(1200, cols, dtype, torch.float32, cols))
+
+
 @pytest.mark.parametrize("cols,G", [(512, 1), (512, 8), (3000, 1)])
 def test_without_weight_or_bias(cuda_device, cols, G):
     x, w, b, d = _inputs(37, cols, torch.float16, torch.float32, 3)
