@@ -296,8 +296,7 @@ static int check_norm_shape(const fnb_norm_shape* s) {
   return 0;
 }
 
-// How a norm is spread over threads and CTAs.  The grid follows the shape and the SM count alone, whatever the alignment: it sizes the
-// workspace.
+// How a norm is spread over threads and CTAs: by the shape, the SM count and how rows can be read.  The workspace has room for any of the three ways.
 struct NormPlan {
   int how;                   // NormLoads
   int vec, items;            // elements of a load; loads of a thread
@@ -323,7 +322,6 @@ static NormPlan norm_plan(const fnb_norm_shape& s, NormLoads how, bool backward,
     while (p.lanes < 32 && p.lanes * (p.vec > 1 ? 2 : 1) < loads) p.lanes *= 2;
     p.items = (loads + p.lanes - 1) / p.lanes;
     p.threads = kNormThreads;
-    // (places are those of the widest load: the grid and the sums' layout do not follow the alignment)
     const int spc = kNormThreads / p.lanes;
     p.per_row = std::min(s.groups, spc);
     p.places = spc / p.per_row * p.per_row;
