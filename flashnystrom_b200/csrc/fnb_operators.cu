@@ -437,8 +437,13 @@ int fnb_decay_forward(const fnb_decay_fwd_args* a) {
               (cudaStream_t)a->stream, a->device_status};
   if (int rc = check_decay_common(c, a->segment_states, a->workspace, a->workspace_bytes)) return rc;
   Launcher L(c.stream, a->device);
+  const bool cut = c.plan.nseg > 1;
+  const DecayForm out{a->q, a->k, a->v, a->out, false, false};
+  // (one segment: its outputs read initial_state itself, which final_state may be, so they come before the sums)
+  if (!cut)
+    if (int rc = decay_form(c, out, a->initial_state, L, "decay_fwd")) return rc;
   if (int rc = decay_states(c, a->k, a->v, false, a->initial_state, a->segment_states, a->final_state, L)) return rc;
-  return decay_form(c, {a->q, a->k, a->v, a->out, false, false}, c.plan.nseg > 1 ? a->segment_states : a->initial_state, L, "decay_fwd");
+  return cut ? decay_form(c, out, a->segment_states, L, "decay_fwd") : 0;
 }
 
 int fnb_decay_backward(const fnb_decay_bwd_args* a) {
@@ -459,13 +464,19 @@ int fnb_decay_backward(const fnb_decay_bwd_args* a) {
   const bool cut = c.plan.nseg > 1;
   // E = dL/dS runs backwards in time; its states at the cuts lie behind the sums in the workspace
   float* e_states = (float*)((char*)a->workspace + align256(slice_floats(c.s) * c.plan.runs() * sizeof(float)));
-  if (int rc = decay_states(c, a->q, a->d_out, true, a->d_final_state, e_states, a->d_initial_state, L)) return rc;
+  const auto states = [&] { return decay_states(c, a->q, a->d_out, true, a->d_final_state, e_states, a->d_initial_state, L); };
+  if (cut)
+    if (int rc = states()) return rc;
   const float* e_in = cut ? e_states : a->d_final_state;
   if (int rc = decay_form(c, {a->d_out, a->v, a->k, a->dq, false, true}, cut ? a->segment_states : a->initial_state, L, "decay_dq")) return rc;
   const DecayForm dv{a->k, a->q, a->d_out, a->dv, true, false}, dk{a->v, a->d_out, a->q, a->dk, true, true};
-  if (tma_form(c, dv) && tma_form(c, dk)) return launch_tc_forms<true, 2>(c, {&dv, &dk}, e_in, L, "decay_dv_dk");
-  if (int rc = decay_form(c, dv, e_in, L, "decay_dv")) return rc;
-  return decay_form(c, dk, e_in, L, "decay_dk");
+  if (tma_form(c, dv) && tma_form(c, dk)) {
+    if (int rc = launch_tc_forms<true, 2>(c, {&dv, &dk}, e_in, L, "decay_dv_dk")) return rc;
+  } else {
+    if (int rc = decay_form(c, dv, e_in, L, "decay_dv")) return rc;
+    if (int rc = decay_form(c, dk, e_in, L, "decay_dk")) return rc;
+  }
+  return cut ? 0 : states();      // (one segment: d_initial_state may be the memory of a state that the gradients read)
 }
 
 int fnb_decay_step(const fnb_decay_step_args* a) {

@@ -362,7 +362,7 @@ typedef struct fnb_decay_bwd_args {
   const int32_t* seq_lens;
   const float* initial_state;
   const float* d_final_state;   /* (B,H,D,D) or NULL: zeros */
-  float* d_initial_state;       /* (B,H,D,D) or NULL: not wanted */
+  float* d_initial_state;       /* (B,H,D,D) or NULL: not wanted; may be d_final_state's own memory */
   const float* segment_states;  /* what the forward wrote */
   void* workspace;
   size_t workspace_bytes;

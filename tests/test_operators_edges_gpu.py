@@ -1,0 +1,60 @@
+"""Calls of the attention with a decay and of the layer norm at the edges of what their documentation allows."""
+import ctypes as C
+
+import pytest
+import torch
+
+from oracle import operators_oracle as O
+
+pytestmark = pytest.mark.gpu
+
+INF = float("inf")
+
+
+def _normal(*shape, seed=0, dtype=torch.float32, mul=1.0):
+    return (torch.randn(*shape, generator=torch.Generator().manual_seed(seed)) * mul).to(dtype).cuda()
+
+
+def _c_rows(t):
+    from flashnystrom_b200 import _lib
+    return _lib.Rows(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2))
+
+
+def _c_call(q, k, v, d, log_decay, initial, final, d_final, d_initial, flags):
+    """Forward and backward through the C ABI: (out, dq, dk, dv); the states are read and written where the caller says."""
+    from flashnystrom_b200 import _C, _lib
+    lib = _lib.load()
+    B, H, N, D = q.shape
+    shape = _lib.DecayShape(B, H, N, D, _C._DTYPES[q.dtype], D ** -0.5, flags)
+    out, dq, dk, dv = (torch.full_like(q, float("nan")) for _ in range(4))
+    ws = torch.empty(lib.fnb_decay_workspace_bytes(C.byref(shape)), dtype=torch.uint8, device="cuda")
+    seg = torch.empty(lib.fnb_decay_segment_floats(C.byref(shape)) + 1, device="cuda")
+    stream, status = torch.cuda.current_stream().cuda_stream, _C._status(q.device).data_ptr()
+    entered = initial.clone()      # (the backward is handed what entered, wherever the forward's final state went)
+    a = _lib.DecayFwdArgs(shape, *(_c_rows(t) for t in (q, k, v, out)), log_decay.data_ptr(), None, initial.data_ptr(), final.data_ptr(), seg.data_ptr(),
+                          ws.data_ptr(), ws.numel(), 0, stream, status)
+    _lib.check(lib.fnb_decay_forward(C.byref(a)))
+    b = _lib.DecayBwdArgs(shape, *(_c_rows(t) for t in (q, k, v, d, dq, dk, dv)), log_decay.data_ptr(), None, entered.data_ptr(), d_final.data_ptr(),
+                          d_initial.data_ptr(), seg.data_ptr(), ws.data_ptr(), ws.numel(), 0, stream, status)
+    _lib.check(lib.fnb_decay_backward(C.byref(b)))
+    torch.cuda.synchronize()
+    return out, dq, dk, dv
+
+
+@pytest.mark.parametrize("dtype,D,generic", [(torch.float16, 64, False), (torch.bfloat16, 128, False), (torch.float16, 64, True), (torch.float32, 32, False)])
+@pytest.mark.parametrize("N", [1, 100, 5000])
+def test_states_updated_where_they_lie(cuda_device, dtype, D, generic, N):
+    """The final state in the initial state's memory, and its gradient likewise: one segment or many, the same bits as with buffers of their own."""
+    from flashnystrom_b200 import _lib
+    flags = _lib.FNB_FLAG_FORCE_GENERIC if generic else 0
+    q, k, v, d = (_normal(1, 3, N, D, seed=i, dtype=dtype) for i in range(4))
+    s0, ds = (_normal(1, 3, D, D, seed=i) for i in (5, 6))
+    log_decay = torch.tensor([-0.1, -0.01, -1e-3], device="cuda")
+    final, d_initial = torch.empty_like(s0), torch.empty_like(s0)
+    apart = _c_call(q, k, v, d, log_decay, s0, final, ds, d_initial, flags)
+    ref, _ = O.decay_attention(q.double(), k.double(), v.double(), log_decay, None, s0.double())
+    O.within(apart[0], ref, O.decay_bounds(q.double(), k.double(), v.double(), None, log_decay, O.isqrt(D), s0.double(), None, None, dtype)[0], dtype)
+    state, grad = s0.clone(), ds.clone()
+    there = _c_call(q, k, v, d, log_decay, state, state, grad, grad, flags)
+    assert all(torch.equal(a, b) for a, b in zip(apart, there))
+    assert torch.equal(state, final) and torch.equal(grad, d_initial)
