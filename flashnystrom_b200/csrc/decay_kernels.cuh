@@ -502,7 +502,8 @@ __global__ void __launch_bounds__(D * W / 4 < 256 ? D * W / 4 : 256) decay_step_
   float4 s[ITERS];
 #pragma unroll
   for (int i = 0; i < ITERS; ++i) s[i] = S[(size_t)(row + i * RPI) * (D / 4)];
-  const float decay = (float)exp(decay_log(p.log_decay[h]));
+  // (two floats: one alone is off by up to 2^-25 each token in the same direction, 1e-4 of the state with a memory of 4096 tokens)
+  const DecayPair decay = decay_pair(decay_log(p.log_decay[h]), 1);
   int b = b0;
   if (p.slots) {
     // rows of the batch that name one state are tokens in a row: the first of them takes all, the others leave
@@ -528,8 +529,10 @@ __global__ void __launch_bounds__(D * W / 4 < 256 ? D * W / 4 : 256) decay_step_
     for (int i = 0; i < ITERS; ++i) {
       const float kr = s_k[row + i * RPI], qr = s_q[row + i * RPI];
       float4& x = s[i];
-      x.x = fmaf(kr, v0, decay == 0.f ? 0.f : decay * x.x); x.y = fmaf(kr, v1, decay == 0.f ? 0.f : decay * x.y);
-      x.z = fmaf(kr, v2, decay == 0.f ? 0.f : decay * x.z); x.w = fmaf(kr, v3, decay == 0.f ? 0.f : decay * x.w);
+      if (decay.hi == 0.f) x = make_float4(0.f, 0.f, 0.f, 0.f);      // (nothing of the past, whatever it holds)
+      // (the token joins the low part: what is added to the state is rounded once, and not the decay before it)
+      x.x = fmaf(x.x, decay.hi, fmaf(kr, v0, x.x * decay.lo)); x.y = fmaf(x.y, decay.hi, fmaf(kr, v1, x.y * decay.lo));
+      x.z = fmaf(x.z, decay.hi, fmaf(kr, v2, x.z * decay.lo)); x.w = fmaf(x.w, decay.hi, fmaf(kr, v3, x.w * decay.lo));
       o.x = fmaf(qr, x.x, o.x); o.y = fmaf(qr, x.y, o.y); o.z = fmaf(qr, x.z, o.z); o.w = fmaf(qr, x.w, o.w);
     }
     *reinterpret_cast<float4*>(&s_sum[row][(threadIdx.x % LPR) * 4]) = o;

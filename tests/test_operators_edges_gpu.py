@@ -58,3 +58,27 @@ def test_states_updated_where_they_lie(cuda_device, dtype, D, generic, N):
     there = _c_call(q, k, v, d, log_decay, state, state, grad, grad, flags)
     assert all(torch.equal(a, b) for a, b in zip(apart, there))
     assert torch.equal(state, final) and torch.equal(grad, d_initial)
+
+
+@pytest.mark.parametrize("decay", [-2.0 ** -12.1, -1.23e-5])
+@pytest.mark.parametrize("rows", [1, 2048])
+def test_many_tokens_with_a_slow_decay(cuda_device, decay, rows):
+    """16384 tokens, one a call or 2048 that name the same state.  Each token rounds the state once, by at most half a step (2^-24, rms 2^-24 / sqrt 3 of it), in no
+    direction: over the tokens that are remembered, 1 / (2 |g|) or all, that adds up as a random walk over the 4096 elements; four times its length is allowed.  A
+    factor that is off by 2^-25 a token adds up in one direction instead: 5e-5 for the first of these decays."""
+    from flashnystrom_b200 import decay_attention, decay_attention_step
+    N, D = 16384, 64
+    q, k, v = (_normal(1, 1, N, D, seed=i) for i in range(3))
+    log_decay = torch.tensor([decay], device="cuda")
+    state = torch.zeros(1, 1, D, D, device="cuda")
+    t = lambda x: x[0, 0].view(N // rows, rows, 1, D)  # noqa: E731
+    slots = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    for a, b, c in zip(t(q), t(k), t(v)):
+        decay_attention_step(a, b, c, state, log_decay, slots=slots)
+    w = torch.exp(log_decay.double() * torch.arange(N - 1, -1, -1, device="cuda").double()).unsqueeze(-1)
+    ref = (k[0, 0].double() * w).T @ v[0, 0].double()
+    off = lambda s: float((s[0, 0].double() - ref).norm() / ref.norm())  # noqa: E731
+    room = 4 * 2.0 ** -24 / 3 ** 0.5 * min(N, 0.5 / abs(decay)) ** 0.5
+    assert off(state) <= room
+    _, whole = decay_attention(q, k, v, log_decay, return_state=True)
+    assert off(whole) <= room
