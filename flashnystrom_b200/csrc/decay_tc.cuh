@@ -626,6 +626,9 @@ __global__ void __launch_bounds__(MainCfg<D>::kThreads, 1) decay_tc_kernel(const
           if (wi != 0.f) a[j] = fma2(e[j], make_float2(wi, wi), a[j]);
           u[j] = pack2<T>(a[j].x, a[j].y);
         }
+        if (s >= nv)      // (cleared rows times an infinity or NaN of one that counts are not zero)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) u[j] = 0u;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const int cc = (col >> 3) + j;

@@ -82,3 +82,27 @@ def test_many_tokens_with_a_slow_decay(cuda_device, decay, rows):
     assert off(state) <= room
     _, whole = decay_attention(q, k, v, log_decay, return_state=True)
     assert off(whole) <= room
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("bad", [INF, float("nan")])
+def test_rows_behind_a_length_are_zeros_beside_rows_that_are_not_finite(cuda_device, dtype, D, bad):
+    """An infinity or NaN in a row that counts, in the chunk in which its sequence ends, or in the state that enters it."""
+    from flashnystrom_b200 import decay_attention
+    N, lens = 300, [200, 130, 299, 70]
+    log_decay = torch.tensor([-0.1, -0.01], device="cuda")
+    for where in range(5):
+        t = [_normal(4, 2, N, D, seed=i, dtype=dtype) for i in range(4)] + [_normal(4, 2, D, D, seed=5)]
+        for b, n in enumerate(lens):
+            if where < 4:
+                t[where][b, :, n - 3, 1] = bad
+            else:
+                t[4][b, :, 1, 1] = bad
+        leaves = [x.requires_grad_(True) for x in t[:3] + t[4:]]
+        out = decay_attention(*leaves[:3], log_decay, initial_state=leaves[3], seq_lens=torch.tensor(lens, dtype=torch.int32, device="cuda"))
+        grads = torch.autograd.grad(out, leaves, t[3])
+        for b, n in enumerate(lens):
+            for x in (out, *grads[:3]):
+                assert not x[b, :, n:].any()
+            assert where == 3 or not torch.isfinite(out[b]).all()
