@@ -63,7 +63,8 @@ __device__ __forceinline__ DecayPair decay_pair(double g, int64_t n) {
   p.lo = p.hi < INFINITY ? (float)(w - (double)p.hi) : 0.f;
   return p;
 }
-__device__ __forceinline__ float decay_by(const DecayPair& p, float s) { return s == 0.f ? 0.f : fmaf(s, p.hi, s * p.lo); }
+// (a weight of zero takes what it is given with it, infinities and NaN too)
+__device__ __forceinline__ float decay_by(const DecayPair& p, float s) { return s == 0.f || p.hi == 0.f ? 0.f : fmaf(s, p.hi, s * p.lo); }
 
 // two FP32 values in one instruction
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {

@@ -701,7 +701,7 @@ __global__ void __launch_bounds__(MainCfg<D>::kThreads, 1) decay_tc_kernel(const
         if (i + 1 < count) {
           float2 d[8];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) d[j] = fma2(f[j], make_float2(w.hi, w.hi), mul2(f[j], make_float2(w.lo, w.lo)));
+          for (int j = 0; j < 8; ++j) d[j] = w.hi == 0.f ? make_float2(0.f, 0.f) : fma2(f[j], make_float2(w.hi, w.hi), mul2(f[j], make_float2(w.lo, w.lo)));
           tmem_st16(t_state + q * 16, reinterpret_cast<const float*>(d));
         }
         if (F16)

@@ -106,3 +106,24 @@ def test_rows_behind_a_length_are_zeros_beside_rows_that_are_not_finite(cuda_dev
             for x in (out, *grads[:3]):
                 assert not x[b, :, n:].any()
             assert where == 3 or not torch.isfinite(out[b]).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("N,D", [(3, 64), (300, 64), (300, 128), (700, 16), (5000, 64)])
+def test_a_decay_to_nothing_takes_what_is_not_finite_with_it(cuda_device, dtype, N, D):
+    """log_decay -inf: nothing of the state that enters is left, whatever it holds, as in the step; backwards the gradient of the final state reaches the
+    last row alone."""
+    from flashnystrom_b200 import decay_attention
+    q, k, v, d = (_normal(1, 2, N, D, seed=i, dtype=dtype) for i in range(4))
+    log_decay = torch.tensor([-INF, -300.0], device="cuda")
+    s0, ds = _normal(1, 2, D, D, seed=4), _normal(1, 2, D, D, seed=5)
+    s0[:, :, 0, 0], s0[:, :, 1, 1], ds[:, :, 2, 2] = float("nan"), INF, float("nan")
+    leaves = [t.requires_grad_(True) for t in (q, k, v, s0)]
+    out, state = decay_attention(*leaves[:3], log_decay, initial_state=leaves[3], return_state=True)
+    grads = torch.autograd.grad((out, state), leaves, (d, ds))
+    for t in (out, state, grads[0], grads[1][:, :, :max(0, N - 128)], grads[2][:, :, :max(0, N - 128)], grads[3]):
+        assert torch.isfinite(t).all()
+    ref, ref_state = O.decay_attention(q.detach().double(), k.detach().double(), v.detach().double(), log_decay)
+    b = O.decay_bounds(q.detach().double(), k.detach().double(), v.detach().double(), None, log_decay, O.isqrt(D), None, None, None, dtype)
+    O.within(out, ref, b[0], dtype)
+    O.within(state, ref_state, b[1], torch.float32)
