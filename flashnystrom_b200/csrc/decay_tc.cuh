@@ -87,6 +87,15 @@ __device__ __forceinline__ void scaled_terms(uint4 raw, float w, uint4* terms) {
   for (int k = 0; k < TERMS; ++k) terms[k] = make_uint4(t[k][0], t[k][1], t[k][2], t[k][3]);
 }
 
+// Powers of two that take values of up to m into fp16's range and back: m * down lies in 2^14 .. 2^15, so that what is rounded below the normal numbers is 2^-39 of m
+// at most.  1 where m is infinite (or zero exponents say that there is nothing).
+__device__ __forceinline__ void into_range(float m, float& up, float& down) {
+  int e = (int)(__float_as_uint(m) >> 23) - 127;
+  e = e == 128 ? 14 : min(max(e, -100), 100);
+  down = __uint_as_float((uint32_t)(14 - e + 127) << 23);
+  up = __uint_as_float((uint32_t)(e - 14 + 127) << 23);
+}
+
 // ---- sums over runs ------------------------------------------------------------------------------------------
 // One CTA a run, two CTAs an SM: a group of eight warps forms the terms of y', double-buffered, one thread issues the products, which add up in
 // tensor memory over kSpan rows (weights reach back that far) before the group takes them out and decays what it has.
@@ -537,33 +546,26 @@ __global__ void __launch_bounds__(MainCfg<D>::kThreads, 1) decay_tc_kernel(const
       if (asks) mbar_wait(p_full + (i & 3), (i >> 2) & 1, ab, 0x8900 + i);
       named_barrier(bar, kGroup);
       tc_fence_after();
-      // Scores, weighted and packed, 16 columns at a time.  In fp16 the largest is looked at first: where some might leave that type's range
-      // (rare), all go in divided by a power of two.  (Loops are not unrolled: the warps' ways through this kernel have to share the instruction cache.)
-      const uint32_t t_scores = tmem + L::kScores + ga * 128 + lane_base + half * 64, t_packed = t_scores;
-      float up = 1.f, down = 1.f;      // (unweighted scores, masked ones among them: what is too large of them costs a factor that does no harm)
+      // Scores, weighted and packed, 16 columns at a time.  In fp16 a row's are taken into that type's range by a power of two, its largest (of the blocks that are not
+      // masked, unweighted) to 2^14 and more: neither large nor small ones lose more than their rounding.  Each half of a row is looked at by both of its warps, so
+      // these meet before either packs.  (Loops are not unrolled: the warps' ways through this kernel have to share the instruction cache.)
+      const uint32_t t_row = tmem + L::kScores + ga * 128 + lane_base, t_scores = t_row + half * 64, t_packed = t_scores;
+      float up = 1.f, down = 1.f;
       if (F16) {
         float most = 0.f;
 #pragma unroll 1
-        for (int n = 0; n < 2; ++n) {
+        for (int n = 0; n < 4; ++n) {
+          if (REV ? 32 * n < w0 : 32 * n > w0) continue;
           float v[32];
-          tmem_ld32(t_scores + n * 32, v);
+          tmem_ld32(t_row + n * 32, v);
           tmem_ld_wait();
 #pragma unroll
           for (int j = 0; j < 32; ++j) most = fmaxf(most, fabsf(v[j]));
         }
-        most *= largest;
-        if (named_barrier_or(bar, kGroup, most > 32768.f)) {
-          float m = most < INFINITY ? most : 0.f;
-          for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-          if (lane == 0) s_max[warp] = m;
-          named_barrier(bar, kGroup);
-          for (int k = 0; k < 8; ++k) m = fmaxf(m, s_max[8 * ga + k]);
-          int e = 0;
-          frexpf(m, &e);
-          up = ldexpf(1.f, max(0, e - 15));
-          down = 1.f / up;
-          named_barrier(bar, kGroup);
-        }
+        into_range(most * largest, up, down);
+        tc_fence_before();
+        named_barrier(bar, kGroup);
+        tc_fence_after();
       }
 #pragma unroll 1
       for (int n = 0; n < 4; ++n) {

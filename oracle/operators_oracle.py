@@ -94,14 +94,23 @@ def _small_state_steps(y, z, log_decay, scale, seq_lens, backwards):
     return torch.stack(out)
 
 
-def decay_bounds(q, k, v, d, log_decay, scale, initial_state, d_state, seq_lens, dtype):
+def _range_steps(x, y, z, state, scale):
+    """The same where a row's scores, and a tile of y' or of the state, are taken into fp16's range by a power of two of their largest: what is lost lies 2^-39 below
+    that.  A score is at most scale |x|_1 max|y|, the state at most max|y| sum|z| more than what enters; three such roundings."""
+    most = y.abs().amax((2, 3), keepdim=True) * z.abs().sum(2, keepdim=True).amax(3, keepdim=True)
+    if state is not None:
+        most = most + state.abs().amax((2, 3), keepdim=True)
+    return 3 * 2.0 ** -39 * scale * x.abs().sum(-1, keepdim=True) * most
+
+
+def decay_bounds(q, k, v, d, log_decay, scale, initial_state, d_state, seq_lens, dtype, in_range=False):
     """How far the kernels' (out, state, dq, dk, dv, d_initial) may be off, element by element, given the float64 inputs.
 
     Every output is a sum of products of three factors (a pair of rows) or four (with a weight); `mass` is the same sum of absolute values.
     A float32 sum of n terms in any order is off by at most n 2^-24 mass; the tensor cores cut off where others round, two half
     steps.  n is at most the head size, the rows of a chunk and the number of chunks, as a sum of sums.  16-bit calls round each
     pair's score, or the key's part of the state, once to their type (half a step of mass), and the result once; fp16 has a smallest step
-    on top (_small_steps)."""
+    on top (_small_steps; in_range: _range_steps, and no such step for states)."""
     a = lambda t: None if t is None else t.abs()  # noqa: E731
     D, N = q.shape[-1], q.shape[2]
     n = 2 * (D + 128 + N / 64 + 8) * 2.0 ** -24
@@ -118,7 +127,16 @@ def decay_bounds(q, k, v, d, log_decay, scale, initial_state, d_state, seq_lens,
     big = lambda t: None if t is None else (n + 1.01 * u) * t.detach()  # noqa: E731
     small = lambda t: None if t is None else n * t.detach()  # noqa: E731
     bounds = [big(out), small(state), big(grads[0]), big(grads[1]), big(grads[2]), small(grads[3])]
-    if dtype == torch.float16:
+    if dtype == torch.float16 and in_range:
+        s0, ds = initial_state, None if d_state is None else d_state / scale      # (the gradient of the state has the scale in it)
+        bounds[0] = bounds[0] + _range_steps(q, k, v, s0, scale)
+        bounds[1] = bounds[1] + 2.0 ** -38 * k.abs().amax((2, 3), keepdim=True) * v.abs().sum(2).unsqueeze(2)
+        if d is not None:
+            for i, f, s in ((2, (d, v, k), s0), (3, (v, d, q), ds), (4, (k, q, d), ds)):
+                bounds[i] = bounds[i] + _range_steps(*f, s, scale)
+            if bounds[5] is not None:
+                bounds[5] = bounds[5] + 2.0 ** -38 * scale * q.abs().amax((2, 3), keepdim=True) * d.abs().sum(2).unsqueeze(2)
+    elif dtype == torch.float16:
         forms = [(0, (q, k, v), False)] + ([(2, (d, v, k), False), (3, (v, d, q), True), (4, (k, q, d), True)] if d is not None else [])
         for i, f, backwards in forms:
             bounds[i] = bounds[i] + _small_steps(*f, log_decay, scale, seq_lens, backwards)

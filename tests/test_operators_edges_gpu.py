@@ -127,3 +127,37 @@ def test_a_decay_to_nothing_takes_what_is_not_finite_with_it(cuda_device, dtype,
     b = O.decay_bounds(q.detach().double(), k.detach().double(), v.detach().double(), None, log_decay, O.isqrt(D), None, None, None, dtype)
     O.within(out, ref, b[0], dtype)
     O.within(state, ref_state, b[1], torch.float32)
+
+
+def _check_range(t, log_decay, s0=None, ds=None, scale=None, lens=None, final=True):
+    """Outputs, states and gradients of fp16 calls within the roundings of values that are in range (no smallest step of fp16 but that of the result)."""
+    from flashnystrom_b200 import _C, decay_attention
+    leaves = [x.detach().requires_grad_(True) for x in t[:3]] + ([] if s0 is None else [s0.detach().requires_grad_(True)])
+    out, state = decay_attention(*leaves[:3], log_decay, scale=scale, initial_state=None if s0 is None else leaves[3], seq_lens=lens, return_state=True)
+    grads = torch.autograd.grad(out if ds is None else (out, state), leaves, t[3] if ds is None else (t[3], ds))
+    torch.cuda.synchronize()
+    _C.check_device_status()
+    wide = [x.detach().double() for x in t]
+    w0, ws = (None if x is None else x.double() for x in (s0, ds))
+    asked = [x.clone().requires_grad_(True) for x in wide[:3]] + ([] if s0 is None else [w0.clone().requires_grad_(True)])
+    ref, ref_state = O.decay_attention(*asked[:3], log_decay, scale, None if s0 is None else asked[3], lens)
+    refs = torch.autograd.grad((ref * wide[3]).sum() + (0 if ds is None else (ref_state * ws).sum()), asked)
+    bounds = O.decay_bounds(*wide, log_decay, O.isqrt(t[0].shape[-1]) if scale is None else scale, w0, ws, lens, t[0].dtype, in_range=True)
+    O.within(out, ref, bounds[0], t[0].dtype)
+    if final:
+        O.within(state, ref_state, bounds[1], torch.float32)
+    for g, r, b in zip(grads, refs, bounds[2:]):
+        O.within(g, r, b, g.dtype)
+
+
+# magnitudes of q, k, v and the gradient, and the scale (None: D^-1/2)
+SMALL = [(1.0, 1.0, 1.0, 1e-5, None), (1.0, 1.0, 2.0 ** 12, 1.0, 2.0 ** -24), (1e-3, 1e-3, 2.0 ** 12, 1e-3, None), (1.0, 1e-4, 1.0, 1.0, 100.0), (30.0, 30.0, 1e-4, 0.3, None)]
+
+
+@pytest.mark.parametrize("D", [64, 128, 16])
+@pytest.mark.parametrize("size", SMALL)
+def test_small_scores_in_fp16(cuda_device, D, size):
+    """Scores far below fp16's normal numbers, one chunk: their products are as exact as those of any others."""
+    t = [_normal(2, 3, 120, D, seed=i, mul=m).half() for i, m in enumerate(size[:4])]
+    t[0][:, :, 5:50:3] *= 1e-2      # (rows of their own magnitude)
+    _check_range(t, torch.tensor([-0.2, -0.01, 0.0], device="cuda"), scale=size[4], final=False)
