@@ -88,10 +88,10 @@ __device__ __forceinline__ void scaled_terms(uint4 raw, float w, uint4* terms) {
 }
 
 // Powers of two that take values of up to m into fp16's range and back: m * down lies in 2^14 .. 2^15, so that what is rounded below the normal numbers is 2^-39 of m
-// at most.  1 where m is infinite (or zero exponents say that there is nothing).
+// at most.  1 where m is infinite or nothing.
 __device__ __forceinline__ void into_range(float m, float& up, float& down) {
   int e = (int)(__float_as_uint(m) >> 23) - 127;
-  e = e == 128 ? 14 : min(max(e, -100), 100);
+  e = e == 128 || e == -127 ? 14 : min(max(e, -100), 100);
   down = __uint_as_float((uint32_t)(14 - e + 127) << 23);
   up = __uint_as_float((uint32_t)(e - 14 + 127) << 23);
 }
@@ -350,7 +350,7 @@ __global__ void __launch_bounds__(MainCfg<D>::kThreads, 1) decay_tc_kernel(const
   float* s_diag = reinterpret_cast<float*>(s_s + 2 * L::kS);      // [32][16]: weights beside the diagonal, see below
   float* s_pow = s_diag + 32 * 16;                    // powers of exp(g): forwards that of C - k at k, backwards that of k
   float* s_mul = s_pow + C + 4;                       // [4]: what x S of chunk i is to be multiplied by, in s_mul[i & 3] (B may be ahead)
-  float* s_max = s_mul + 4;                           // [24]
+  float* s_max = s_mul + 4;                           // [24], of the state's largest [8]: one a warp of group B
   DecayPair* s_pair = reinterpret_cast<DecayPair*>(s_max + 24);      // [2]: what a chunk decays the state by, a whole one and the first
   uint64_t* bars = reinterpret_cast<uint64_t*>(s_pair + 2);
   uint64_t* full = bars;             // [NS]
@@ -666,12 +666,12 @@ __global__ void __launch_bounds__(MainCfg<D>::kThreads, 1) decay_tc_kernel(const
       }
       tmem_st_wait();
     }
-    // The state as two 16-bit terms for x S (in fp16 divided by a power of two where it would leave the range), and, decayed by the chunk's
+    // The state as two 16-bit terms for x S (in fp16 taken into range by a power of two), and, decayed by the chunk's
     // rows, back to tensor memory, where y'^T z is added to it.
     const auto put_state = [&](int i) {
       float down = 1.f;
       if (F16) {
-        float most = 0.f, up = 1.f;
+        float most = 0.f, up;
 #pragma unroll 1
         for (int q = 0; q < HC / 32; ++q) {
           float f[32];
@@ -680,18 +680,13 @@ __global__ void __launch_bounds__(MainCfg<D>::kThreads, 1) decay_tc_kernel(const
 #pragma unroll
           for (int j = 0; j < 32; ++j) most = fmaxf(most, fabsf(f[j]));
         }
-        if (named_barrier_or(2, kGroup, owner && most > 32768.f)) {
-          float m = owner && most < INFINITY ? most : 0.f;
-          for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-          if (lane == 0) s_max[warp] = m;
-          named_barrier(2, kGroup);
-          for (int k = 0; k < 8; ++k) m = fmaxf(m, s_max[L::kWarpB + k]);
-          int e = 0;
-          frexpf(m, &e);
-          up = ldexpf(1.f, max(0, e - 15));
-          down = 1.f / up;
-          named_barrier(2, kGroup);
-        }
+        const unsigned w = __reduce_max_sync(0xffffffffu, owner && most < INFINITY ? __float_as_uint(most) : 0u);
+        if (lane == 0) s_max[warp - L::kWarpB] = __uint_as_float(w);
+        named_barrier(2, kGroup);
+        float m = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) m = fmaxf(m, s_max[k]);
+        into_range(m, up, down);
         if (tid == 0) s_mul[i & 3] = up;
       }
       const DecayPair w = i == 0 ? first_chunk : full_chunk;

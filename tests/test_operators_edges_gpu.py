@@ -161,3 +161,16 @@ def test_small_scores_in_fp16(cuda_device, D, size):
     t = [_normal(2, 3, 120, D, seed=i, mul=m).half() for i, m in enumerate(size[:4])]
     t[0][:, :, 5:50:3] *= 1e-2      # (rows of their own magnitude)
     _check_range(t, torch.tensor([-0.2, -0.01, 0.0], device="cuda"), scale=size[4], final=False)
+
+
+@pytest.mark.parametrize("D", [64, 128, 16])
+@pytest.mark.parametrize("size", [2.0 ** -22, 2.0 ** -40, 2.0 ** 40])
+def test_states_of_any_size_in_fp16(cuda_device, D, size):
+    """States that enter a chunk, and their gradients, far below fp16's numbers and far above, brought back by the scale."""
+    scale = 2.0 ** -10 / size
+    t = [_normal(2, 3, 120, D, seed=i, mul=m).half() for i, m in enumerate((1.0, 2.0 ** -10, 2.0 ** -10, 1.0))]
+    t[0], t[3] = (x if size < 1 else x * 2.0 ** -6 for x in (t[0], t[3]))
+    s0, ds = (_normal(2, 3, D, D, seed=i, mul=m) for i, m in ((4, size), (5, size * scale)))
+    if size < 2.0 ** -30:      # (pairs would leave the range with so large a scale)
+        t[1], t[2] = t[1] * 0, t[2] * 0
+    _check_range(t, torch.tensor([-0.2, -0.01, 0.0], device="cuda"), s0, ds, scale=scale, final=False)
