@@ -63,8 +63,9 @@ __device__ __forceinline__ DecayPair decay_pair(double g, int64_t n) {
   p.lo = p.hi < INFINITY ? (float)(w - (double)p.hi) : 0.f;
   return p;
 }
-// (a weight of zero takes what it is given with it, infinities and NaN too)
-__device__ __forceinline__ float decay_by(const DecayPair& p, float s) { return s == 0.f || p.hi == 0.f ? 0.f : fmaf(s, p.hi, s * p.lo); }
+__device__ __forceinline__ float decay_by(const DecayPair& p, float s) { return s == 0.f ? 0.f : fmaf(s, p.hi, s * p.lo); }
+// A weight of zero takes what it is given with it, infinities and NaN too.  (Asked once where the weight is the same for all of a state, so not in decay_by.)
+__device__ __forceinline__ bool leaves_something(const DecayPair& p) { return p.hi != 0.f; }
 
 // two FP32 values in one instruction
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
@@ -344,6 +345,7 @@ __global__ void __launch_bounds__(kThreads, D <= 64 ? 2 : 1) decay_chunk_kernel(
             for (int c = 0; c < CG; ++c) decay_axpy<CW>(yv[a][i], zv[c], U[a][i][c]);
       }
       const DecayPair by_nv = nv == C ? full : decay_pair(g, nv);
+      const bool past = leaves_something(by_nv);
 #pragma unroll
       for (int a = 0; a < CG; ++a)
 #pragma unroll
@@ -351,7 +353,7 @@ __global__ void __launch_bounds__(kThreads, D <= 64 ? 2 : 1) decay_chunk_kernel(
 #pragma unroll
           for (int c = 0; c < CG; ++c)
 #pragma unroll
-            for (int j = 0; j < CW; ++j) S[a][i][c][j] = decay_by(by_nv, S[a][i][c][j]) + U[a][i][c][j];
+            for (int j = 0; j < CW; ++j) S[a][i][c][j] = (past ? decay_by(by_nv, S[a][i][c][j]) : 0.f) + U[a][i][c][j];
     }
     if (OUT) {
       if (more) __syncthreads();      // (y is done with)
@@ -463,7 +465,8 @@ __global__ void __launch_bounds__(kThreads) decay_join_kernel(DecayJoinParams p)
       if (k0 + k < walk) {
         const DecayJoinRun run = runs[k0 + k];
         if (to && run.seg >= 0) to[(size_t)run.seg * DD] = s;
-        if (run.rows > 0) s = decay_by({run.hi, run.lo}, s) + u[k];
+        const DecayPair w{run.hi, run.lo};
+        if (run.rows > 0) s = (leaves_something(w) ? decay_by(w, s) : 0.f) + u[k];
       }
   }
   if (p.state_out) p.state_out[(size_t)bh * DD + e] = s;
@@ -530,7 +533,7 @@ __global__ void __launch_bounds__(D * W / 4 < 256 ? D * W / 4 : 256) decay_step_
     for (int i = 0; i < ITERS; ++i) {
       const float kr = s_k[row + i * RPI], qr = s_q[row + i * RPI];
       float4& x = s[i];
-      if (decay.hi == 0.f) x = make_float4(0.f, 0.f, 0.f, 0.f);      // (nothing of the past, whatever it holds)
+      if (!leaves_something(decay)) x = make_float4(0.f, 0.f, 0.f, 0.f);
       // (the token joins the low part: what is added to the state is rounded once, and not the decay before it)
       x.x = fmaf(x.x, decay.hi, fmaf(kr, v0, x.x * decay.lo)); x.y = fmaf(x.y, decay.hi, fmaf(kr, v1, x.y * decay.lo));
       x.z = fmaf(x.z, decay.hi, fmaf(kr, v2, x.z * decay.lo)); x.w = fmaf(x.w, decay.hi, fmaf(kr, v3, x.w * decay.lo));

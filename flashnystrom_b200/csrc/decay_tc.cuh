@@ -255,14 +255,15 @@ decay_tc_sums_kernel(const __grid_constant__ CUtensorMap tm_y, const __grid_cons
         named_barrier(1, kGroup);
         tc_fence_after();
         const DecayPair w = in_span == L::kSpan ? whole : last;      // (the first one has nothing to decay)
+        const bool past = spans > 0 && leaves_something(w);
 #pragma unroll 1
         for (int q = 0; q < D / 32; ++q) {
           float U[16], S[16];
           tmem_ld16(t_sum + q * 16, U);
-          if (spans > 0) tmem_ld16(t_state + q * 16, S);
+          if (past) tmem_ld16(t_state + q * 16, S);
           tmem_ld_wait();
 #pragma unroll
-          for (int j = 0; j < 16; ++j) S[j] = (spans > 0 ? decay_by(w, S[j]) : 0.f) + p.sum_scale * U[j];
+          for (int j = 0; j < 16; ++j) S[j] = (past ? decay_by(w, S[j]) : 0.f) + p.sum_scale * U[j];
           tmem_st16(t_state + q * 16, S);
         }
         tmem_st_wait();
@@ -690,6 +691,7 @@ __global__ void __launch_bounds__(MainCfg<D>::kThreads, 1) decay_tc_kernel(const
         if (tid == 0) s_mul[i & 3] = up;
       }
       const DecayPair w = i == 0 ? first_chunk : full_chunk;
+      const bool past = leaves_something(w);
 #pragma unroll 1
       for (int q = 0; q < HC / 16; ++q) {
         float2 f[8];
@@ -697,9 +699,15 @@ __global__ void __launch_bounds__(MainCfg<D>::kThreads, 1) decay_tc_kernel(const
         tmem_ld_wait();
         if (i + 1 < count) {
           float2 d[8];
+          if (past) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) d[j] = w.hi == 0.f ? make_float2(0.f, 0.f) : fma2(f[j], make_float2(w.hi, w.hi), mul2(f[j], make_float2(w.lo, w.lo)));
-          tmem_st16(t_state + q * 16, reinterpret_cast<const float*>(d));
+            for (int j = 0; j < 8; ++j) d[j] = fma2(f[j], make_float2(w.hi, w.hi), mul2(f[j], make_float2(w.lo, w.lo)));
+            tmem_st16(t_state + q * 16, reinterpret_cast<const float*>(d));
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) d[j] = make_float2(0.f, 0.f);
+            tmem_st16(t_state + q * 16, reinterpret_cast<const float*>(d));
+          }
         }
         if (F16)
 #pragma unroll
