@@ -96,6 +96,19 @@ __device__ __forceinline__ void into_range(float m, float& up, float& down) {
   up = __uint_as_float((uint32_t)(e - 14 + 127) << 23);
 }
 
+// y' of a tile gets a power of two in fp16 where all of y is below 2^-7 (rare): down to there what y' = y e^(..) loses below the normal numbers is 2^-18 of y's largest at
+// most.  Whether it is so shows in two bits of the exponents, so that the bits of all values together tell; the exponent that they have together is at most three
+// above the largest.  That goes to 14 by the factor, or the factor is 2^24, which leaves a state that is multiplied by it in FP32's range.
+__device__ __forceinline__ uint32_t bits_of(uint4 v) { return v.x | v.y | v.z | v.w; }
+__device__ __forceinline__ bool not_small(uint32_t bits) { return bits & 0x60006000u; }
+__device__ __forceinline__ float factor_of(uint32_t bits) {
+  const float m = __half2float(__ushort_as_half((unsigned short)((bits | bits >> 16) & 0x7fffu)));
+  const int e = (int)(__float_as_uint(m) >> 23) - 127;
+  return e == -127 ? 1.f : __uint_as_float((uint32_t)(min(14 - e, 24) + 127) << 23);
+}
+// (of a power of two, exactly)
+__device__ __forceinline__ float inverse_of(float power) { return __uint_as_float(0x7f000000u - __float_as_uint(power)); }
+
 // ---- sums over runs ------------------------------------------------------------------------------------------
 // One CTA a run, two CTAs an SM: a group of eight warps forms the terms of y', double-buffered, one thread issues the products, which add up in
 // tensor memory over kSpan rows (weights reach back that far) before the group takes them out and decays what it has.
@@ -351,7 +364,7 @@ __global__ void __launch_bounds__(MainCfg<D>::kThreads, 1) decay_tc_kernel(const
   float* s_diag = reinterpret_cast<float*>(s_s + 2 * L::kS);      // [32][16]: weights beside the diagonal, see below
   float* s_pow = s_diag + 32 * 16;                    // powers of exp(g): forwards that of C - k at k, backwards that of k
   float* s_mul = s_pow + C + 4;                       // [4]: what x S of chunk i is to be multiplied by, in s_mul[i & 3] (B may be ahead)
-  float* s_max = s_mul + 4;                           // [24], of the state's largest [8]: one a warp of group B
+  float* s_max = s_mul + 4;                           // [8], one a warp of group B: the largest of the state; then [8]: bits of a tile of y; [8] not used
   DecayPair* s_pair = reinterpret_cast<DecayPair*>(s_max + 24);      // [2]: what a chunk decays the state by, a whole one and the first
   uint64_t* bars = reinterpret_cast<uint64_t*>(s_pair + 2);
   uint64_t* full = bars;             // [NS]
@@ -667,6 +680,22 @@ __global__ void __launch_bounds__(MainCfg<D>::kThreads, 1) decay_tc_kernel(const
       }
       tmem_st_wait();
     }
+    // In fp16 y' of a chunk may have a power of two in it (factor_of); the state that it is added to is put back times that.  (With what finds it 1.5 to 4 % of a call:
+    // 1 x 16 x 65536 x 64 forward 237 us, 228 without; 4 x 16 x 16384 x 128 479 and 472.)
+    float y_factor = 1.f, held = 1.f;      // of the chunk that put_state is at; the one that the state in tensor memory has
+    uint32_t seen = 0;                     // the bits of y that this thread has seen
+    constexpr int PIECES = L::kTile / 16 / kGroup;
+    const auto rows_in = [&](int i) { const int64_t n = end - row_of(i); return n < C ? (int)n : C; };
+    // the factor by what all threads have seen of a small y
+    const auto find_factor = [&] {
+      uint32_t* s_seen = reinterpret_cast<uint32_t*>(s_max + 8);
+      uint32_t bits = __reduce_or_sync(0xffffffffu, seen);
+      if (lane == 0) s_seen[warp - L::kWarpB] = bits;
+      named_barrier(2, kGroup);
+      for (int k = 0; k < 8; ++k) bits |= s_seen[k];
+      named_barrier(2, kGroup);
+      return factor_of(bits);
+    };
     // The state as two 16-bit terms for x S (in fp16 taken into range by a power of two), and, decayed by the chunk's
     // rows, back to tensor memory, where y'^T z is added to it.
     const auto put_state = [&](int i) {
@@ -687,11 +716,18 @@ __global__ void __launch_bounds__(MainCfg<D>::kThreads, 1) decay_tc_kernel(const
         float m = 0.f;
 #pragma unroll
         for (int k = 0; k < 8; ++k) m = fmaxf(m, s_max[k]);
-        into_range(m, up, down);
+        const float unheld = inverse_of(held);
+        into_range(m * unheld, up, down);
+        down *= unheld;
         if (tid == 0) s_mul[i & 3] = up;
       }
-      const DecayPair w = i == 0 ? first_chunk : full_chunk;
+      DecayPair w = i == 0 ? first_chunk : full_chunk;
       const bool past = leaves_something(w);
+      if (F16) {
+        const float change = y_factor * inverse_of(held);
+        w = {w.hi * change, w.lo * change};
+        held = y_factor;
+      }
 #pragma unroll 1
       for (int q = 0; q < HC / 16; ++q) {
         float2 f[8];
@@ -729,53 +765,135 @@ __global__ void __launch_bounds__(MainCfg<D>::kThreads, 1) decay_tc_kernel(const
       fence_proxy_async();
       mbar_arrive_warp(s_ready);
     };
-    // y' of chunk i (in y's place: once the scores have been formed from it); rows that do not count are cleared before these
-    const auto put_y = [&](int i) {
-      const int64_t c0 = row_of(i);
-      const int nv = end - c0 < C ? (int)(end - c0) : C;
-      if (i == dirty) {
-        for (int j = 0; j < 3; ++j) {
-          landed(3 * i + j, 0x8b00);
-          for (int idx = tid; idx < L::kTile / 16; idx += kGroup)
-            if (((idx >> 3) & (C - 1)) >= nv) *reinterpret_cast<uint4*>(tile(3 * i + j) + idx * 16) = make_uint4(0, 0, 0, 0);
-        }
-        fence_proxy_async();
-        mbar_arrive_warp(clean);
-        named_barrier(2, kGroup);
+    // the state again, times a power of two that it has not got yet (the first chunk's, found while its state is on the way)
+    const auto scale_state = [&](float factor) {
+#pragma unroll 1
+      for (int q = 0; q < HC / 16; ++q) {
+        float f[16];
+        tmem_ld16(t_state + q * 16, f);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) f[j] *= factor;
+        tmem_st16(t_state + q * 16, f);
       }
-      if (i + 1 >= count) return;
+      tmem_st_wait();
+      tc_fence_before();
+      held = factor;
+    };
+    // rows of chunk i that do not count, before anything reads them
+    const auto clear_rows = [&](int i) {
+      const int nv = rows_in(i);
+      for (int j = 0; j < 3; ++j) {
+        landed(3 * i + j, 0x8b00);
+        for (int idx = tid; idx < L::kTile / 16; idx += kGroup)
+          if (((idx >> 3) & (C - 1)) >= nv) *reinterpret_cast<uint4*>(tile(3 * i + j) + idx * 16) = make_uint4(0, 0, 0, 0);
+      }
+      fence_proxy_async();
+      mbar_arrive_warp(clean);
+      named_barrier(2, kGroup);
+    };
+    // y' of chunk i (in y's place: once the scores have been formed from it)
+    const auto form_y = [&](int i, float factor) {
+      const int nv = rows_in(i);
+      const uint8_t* src = tile(3 * i);
+      uint8_t* dst = D == 64 ? s_y + (i & 1) * L::kTile : tile(3 * i);
+      uint32_t bits = 0;
+#pragma unroll 1
+      for (int q = 0; q < PIECES; ++q) {
+        const int idx = tid + q * kGroup, r = (idx >> 3) & (C - 1);
+        const uint4 raw = *reinterpret_cast<const uint4*>(src + idx * 16);
+        float w = r < nv ? power(REV ? r + 1 : nv - 1 - r) : 0.f;
+        if (F16) w *= factor;
+        uint4 term;
+        scaled_terms<T, 1>(raw, w, &term);
+        *reinterpret_cast<uint4*>(dst + idx * 16) = term;
+        if (F16 && D == 64) bits |= bits_of(raw);
+      }
+      if (F16 && D == 64) seen = bits;
+      fence_proxy_async();
+    };
+    const auto await_y = [&](int i) {
       if (warp == L::kWarpB) {
         landed(3 * i, 0x8c80);
         if (D == 128) mbar_wait(p_full + (i & 3), (i >> 2) & 1, ab, 0x8c00 + i);
       }
       named_barrier(2, kGroup);
-      const uint8_t* src = tile(3 * i);
-      uint8_t* dst = D == 64 ? s_y + (i & 1) * L::kTile : tile(3 * i);
-#pragma unroll 1
-      for (int q = 0; q < L::kTile / 16 / kGroup; ++q) {
-        const int idx = tid + q * kGroup, r = (idx >> 3) & (C - 1);
-        uint4 term;
-        scaled_terms<T, 1>(*reinterpret_cast<const uint4*>(src + idx * 16), r < nv ? power(REV ? r + 1 : nv - 1 - r) : 0.f, &term);
-        *reinterpret_cast<uint4*>(dst + idx * 16) = term;
-      }
-      fence_proxy_async();
-      mbar_arrive_warp(y_ready + (i & 1));
     };
-    if (count > 0) {
-      put_state(0);
-      put_y(0);
-    }
-    // (heads of 64: y' a chunk ahead, while the products that end this one run; its tile is free since u_full of the chunk before)
-    for (int i = 0; i + 1 < count; ++i) {
-      if (D == 64) put_y(i + 1);
+    const auto await_products = [&](int i) {      // those of chunk i that the state takes part in
       if (warp == L::kWarpB) {
         mbar_wait(s_done, i & 1, ab, 0x8e00 + i);
         mbar_wait(u_full, i & 1, ab, 0x8d00 + i);
       }
-      named_barrier(2, kGroup);
-      tc_fence_after();
-      put_state(i + 1);
-      if (D == 128) put_y(i + 1);
+    };
+    if constexpr (!F16) {
+      const auto put_y = [&](int i) {
+        if (i == dirty) clear_rows(i);
+        if (i + 1 >= count) return;
+        await_y(i);
+        form_y(i, 1.f);
+        mbar_arrive_warp(y_ready + (i & 1));
+      };
+      if (count > 0) {
+        put_state(0);
+        put_y(0);
+      }
+      // (heads of 64: y' a chunk ahead, while the products that end this one run; its tile is free since u_full of the chunk before)
+      for (int i = 0; i + 1 < count; ++i) {
+        if (D == 64) put_y(i + 1);
+        await_products(i);
+        named_barrier(2, kGroup);
+        tc_fence_after();
+        put_state(i + 1);
+        if (D == 128) put_y(i + 1);
+      }
+    } else if constexpr (D == 64) {
+      // the same order; y' is formed without a factor, and again where the barrier behind the products tells that y is small (y is still there)
+      for (int c = 0; c < count; ++c) {
+        put_state(c);
+        for (int i = c ? c + 1 : 0; i <= c + 1 && i < count; ++i) {
+          const bool forms = i + 1 < count;
+          if (i == dirty) clear_rows(i);
+          if (forms) {
+            await_y(i);
+            form_y(i, 1.f);
+          }
+          if (i > 0) await_products(i - 1);
+          const bool small = !named_barrier_or(2, kGroup, not_small(seen));
+          tc_fence_after();
+          if (forms) {
+            y_factor = 1.f;
+            if (small) {
+              y_factor = find_factor();
+              if (i == 0) scale_state(y_factor);
+              if (y_factor != 1.f) form_y(i, y_factor);
+            }
+            mbar_arrive_warp(y_ready + (i & 1));
+          }
+        }
+      }
+    } else {
+      // y' takes y's place: y is looked at before the state is put, while products run
+      for (int c = 0; c < count; ++c) {
+        if (c == dirty) clear_rows(c);
+        const bool forms = c + 1 < count;
+        if (forms) {
+          landed(3 * c, 0x8c90);
+          uint32_t bits = 0;
+#pragma unroll 4
+          for (int q = 0; q < PIECES; ++q) bits |= bits_of(*reinterpret_cast<const uint4*>(tile(3 * c) + (tid + q * kGroup) * 16));
+          seen = bits;
+        }
+        if (c > 0) await_products(c - 1);
+        const bool small = !named_barrier_or(2, kGroup, not_small(seen));
+        tc_fence_after();
+        y_factor = small && forms ? find_factor() : 1.f;
+        put_state(c);
+        if (forms) {
+          await_y(c);
+          form_y(c, y_factor);
+          mbar_arrive_warp(y_ready + (c & 1));
+        }
+      }
     }
   }
   tc_fence_before();

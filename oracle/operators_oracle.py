@@ -95,12 +95,12 @@ def _small_state_steps(y, z, log_decay, scale, seq_lens, backwards):
 
 
 def _range_steps(x, y, z, state, scale):
-    """The same where a row's scores, and a tile of y' or of the state, are taken into fp16's range by a power of two of their largest: what is lost lies 2^-39 below
-    that.  A score is at most scale |x|_1 max|y|, the state at most max|y| sum|z| more than what enters; three such roundings."""
-    most = y.abs().amax((2, 3), keepdim=True) * z.abs().sum(2, keepdim=True).amax(3, keepdim=True)
-    if state is not None:
-        most = most + state.abs().amax((2, 3), keepdim=True)
-    return 3 * 2.0 ** -39 * scale * x.abs().sum(-1, keepdim=True) * most
+    """The same where a row's scores and the terms of the state are taken into fp16's range by a power of two of their largest, so that what is lost lies 2^-39 below
+    that, and a tile of y' where its largest is below 2^-7: 2^-25 / 2^-7 of it is lost otherwise.  A score is at most scale |x|_1 max|y|, the state at most
+    max|y| sum|z| more than what enters."""
+    pairs = y.abs().amax((2, 3), keepdim=True) * z.abs().sum(2, keepdim=True).amax(3, keepdim=True)
+    entered = 0 if state is None else state.abs().amax((2, 3), keepdim=True)
+    return scale * x.abs().sum(-1, keepdim=True) * (2.0 ** -18 * pairs + 2 * 2.0 ** -39 * (pairs + entered))
 
 
 def decay_bounds(q, k, v, d, log_decay, scale, initial_state, d_state, seq_lens, dtype, in_range=False):

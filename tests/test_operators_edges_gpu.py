@@ -174,3 +174,19 @@ def test_states_of_any_size_in_fp16(cuda_device, D, size):
     if size < 2.0 ** -30:      # (pairs would leave the range with so large a scale)
         t[1], t[2] = t[1] * 0, t[2] * 0
     _check_range(t, torch.tensor([-0.2, -0.01, 0.0], device="cuda"), s0, ds, scale=scale, final=False)
+
+
+@pytest.mark.parametrize("D", [64, 128, 16])
+@pytest.mark.parametrize("size", SMALL)
+@pytest.mark.parametrize("padded", [False, True])
+def test_small_keys_over_chunks_in_fp16(cuda_device, D, size, padded):
+    """The same over three chunks of sequences of one segment (there are more slices than SMs): what reaches a row from the chunks before it goes through the state.
+    Chunks of their own magnitudes."""
+    t = [_normal(50, 3, 300, D, seed=i, mul=m).half() for i, m in enumerate(size[:4])]
+    for x in t:
+        x[:, :, 128:256] *= 0.125
+    lens = None
+    if padded:
+        lens = torch.tensor([300, 299, 257, 130, 1] * 10, dtype=torch.int32, device="cuda")
+    scale = size[4] if size[4] is None else min(size[4], 10.0)      # (times 100 the gradient of k, scale sqrt(D rows), would leave the range)
+    _check_range(t, torch.tensor([-0.2, -0.01, 0.0], device="cuda"), scale=scale, lens=lens, final=False)
