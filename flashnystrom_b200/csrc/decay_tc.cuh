@@ -106,6 +106,12 @@ __device__ __forceinline__ float factor_of(uint32_t bits) {
   const int e = (int)(__float_as_uint(m) >> 23) - 127;
   return e == -127 ? 1.f : __uint_as_float((uint32_t)(min(14 - e, 24) + 127) << 23);
 }
+// The same for the sums over runs.  Where they are to have FP32's bits y below 2 gets 2^13 already, so that what is lost is 2^-25 of y's largest at most.  Nothing but zeros
+// may have any.
+template <bool EXACT> __device__ __forceinline__ float sums_factor_of(uint32_t bits) {
+  if (bits & (EXACT ? 0x40004000u : 0x60006000u)) return 1.f;
+  return bits & 0x20002000u ? 8192.f : bits & 0x7fff7fffu ? factor_of(bits) : 16777216.f;
+}
 // (of a power of two, exactly)
 __device__ __forceinline__ float inverse_of(float power) { return __uint_as_float(0x7f000000u - __float_as_uint(power)); }
 
@@ -139,18 +145,19 @@ decay_tc_sums_kernel(const __grid_constant__ CUtensorMap tm_y, const __grid_cons
   uint64_t* empty = bars + 3;        // [3]
   uint64_t* y_ready = bars + 6;      // [2]
   uint64_t* y_free = bars + 8;       // [2]
-  uint64_t* u_full = bars + 10;
-  uint64_t* u_free = bars + 11;
-  uint64_t* fin = bars + 12;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 13);
+  uint64_t* fin = bars + 10;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 11);
   int* abort_word = reinterpret_cast<int*>(tmem_slot + 1);
+  uint32_t* s_seen = reinterpret_cast<uint32_t*>((reinterpret_cast<uintptr_t>(abort_word + 1) + 15) & ~(uintptr_t)15);      // fp16: [2][8], by chunk parity, bits of y by warp
+  volatile int* s_fresh = reinterpret_cast<volatile int*>(s_seen + 16);      // fp16: [2], likewise: the sums in tensor memory have been taken out before this chunk
+  constexpr bool F16 = UmmaFmt<T>::v == 0;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int bh = blockIdx.x / p.nrun, cut = p.cut0 + blockIdx.x % p.nrun, b = bh / p.H, h = bh % p.H;
   if (threadIdx.x == 0) {
     for (int i = 0; i < NST; ++i) { mbar_init(full + i, 1); mbar_init(empty + i, 1); }
     for (int i = 0; i < 2; ++i) { mbar_init(y_ready + i, kGroup / 32); mbar_init(y_free + i, 1); }
-    mbar_init(u_full, 1); mbar_init(u_free, kGroup / 32); mbar_init(fin, 1);
+    mbar_init(fin, 1);
     *abort_word = 0;
     fence_mbar_init();
   }
@@ -202,14 +209,13 @@ decay_tc_sums_kernel(const __grid_constant__ CUtensorMap tm_y, const __grid_cons
     // (the whole warp walks this code and one lane issues: descriptors stay in uniform registers)
     if (count > 0) {
       constexpr uint32_t idesc = make_idesc<T>(D, D, true, true);
-      int spans = 0;
       for (int i = 0; i < count; ++i) {
         const int st = i % NST, u = i & 1;
-        bool ok = mbar_wait(full + st, (i / NST) & 1, ab, 0x7280 + i) && mbar_wait(y_ready + u, (i >> 1) & 1, ab, 0x7200 + i);
-        const bool fresh = first_of_span(i);
-        if (fresh && spans > 0) ok = ok && mbar_wait(u_free, (spans - 1) & 1, ab, 0x7300 + i);
+        const bool ok = mbar_wait(full + st, (i / NST) & 1, ab, 0x7280 + i) && mbar_wait(y_ready + u, (i >> 1) & 1, ab, 0x7200 + i);
         if (!__all_sync(0xffffffffu, ok)) break;
         tc_fence_after();
+        // (what was added up before a new sum has been taken out by the time y' is ready)
+        const bool fresh = first_of_span(i) || (F16 && __any_sync(0xffffffffu, s_fresh[u]));
         const uint32_t a_z = smem_u32(s_in + st * 2 * L::kTile + L::kTile), a_y = smem_u32(s_y + u * L::kTerms * L::kTile);
 #pragma unroll 1
         for (int t = L::kTerms - 1; t >= 0; --t)
@@ -218,7 +224,6 @@ decay_tc_sums_kernel(const __grid_constant__ CUtensorMap tm_y, const __grid_cons
             umma_elect(tmem, along_rows(a_y + t * L::kTile, k, C), along_rows(a_z, k, C), idesc, !(fresh && t == L::kTerms - 1 && k == 0));
         umma_commit_elect(empty + st);
         umma_commit_elect(y_free + u);
-        if (last_of_span(i)) { umma_commit_elect(u_full); ++spans; }
       }
       umma_commit_elect(fin);          // nothing of the CTA is given back while a product runs
       mbar_drain(fin, 0);
@@ -229,46 +234,56 @@ decay_tc_sums_kernel(const __grid_constant__ CUtensorMap tm_y, const __grid_cons
     const int row = D == 64 ? quarter * 16 + lane : quarter * 32 + lane;
     const uint32_t t_sum = tmem + lane_base + half * (D / 2), t_state = t_sum + D;
     // (a wait that gave up does not leave the loop: the warps meet at barriers, and the status word has it)
-    int spans = 0, in_span = 0;
     const DecayPair whole = s_pair[0], last = s_pair[1];
+    constexpr int PIECES = L::kTile / 16 / kGroup;
+    int in_span = 0;
     int64_t span_end = 0;        // forwards: the row behind the span; backwards: its first row
-    for (int i = 0; i < count; ++i) {
+    float factor = 1.f;          // fp16: of y' in the sums that are in tensor memory now
+    bool some = false;           // there is something in what was taken out so far
+    bool decayed = false;        // fp16: and that has been decayed by the span's rows (something of this span has been taken out)
+    // Iteration i takes out the sums that chunk i - 1 ended, a span's or (fp16) those that chunk i is too large for, and forms y' of chunk i.
+    for (int i = 0; i <= count; ++i) {
       const int st = i % NST, u = i & 1;
-      if (first_of_span(i)) {
-        const int n = i == 0 ? first_span : PER;
-        span_end = REV ? row_of(i + n - 1) : row_of(i + n - 1) + C;
-        if (!REV && span_end > end) span_end = end;
-        in_span = REV ? (int)((i == 0 ? end : row_of(i) + C) - span_end) : (int)(span_end - row_of(i));
-      }
-      if (warp == 0) {      // (one warp asks for all)
-        mbar_wait(full + st, (i / NST) & 1, ab, 0x7400 + i);
-        if (i >= 2) mbar_wait(y_free + u, ((i >> 1) & 1) ^ 1, ab, 0x7500 + i);
-      }
-      named_barrier(1, kGroup);
+      const bool any = i < count, ends = i > 0 && last_of_span(i - 1), first = i == 0 || ends;
       uint8_t* src = s_in + st * 2 * L::kTile;
       uint8_t* dst = s_y + u * L::kTerms * L::kTile;
       const int64_t c0 = row_of(i);
       const int nv = end - c0 < C ? (int)(end - c0) : C;
-#pragma unroll
-      for (int q = 0; q < L::kTile / 16 / kGroup; ++q) {
-        const int idx = threadIdx.x + q * kGroup, r = (idx >> 3) & (C - 1);
-        uint4 terms[L::kTerms];
-#pragma unroll
-        for (int t = 0; t < L::kTerms; ++t) terms[t] = make_uint4(0, 0, 0, 0);
-        // weights: forwards exp(g (rows of the span behind this one)), backwards exp(g (rows of the span up to and with this one))
-        if (r < nv) scaled_terms<T, L::kTerms>(*reinterpret_cast<const uint4*>(src + idx * 16), pw[REV ? (int)(c0 + r - span_end) + 1 : (int)(span_end - 1 - c0 - r)], terms);
-        else *reinterpret_cast<uint4*>(src + L::kTile + idx * 16) = make_uint4(0, 0, 0, 0);      // (z's row too: it may hold anything)
-#pragma unroll
-        for (int t = 0; t < L::kTerms; ++t) *reinterpret_cast<uint4*>(dst + t * L::kTile + idx * 16) = terms[t];
+      // fp16: sums share a factor of y'.  A span begins with that of its first chunk, and does not look at others where that is 1 (the usual).
+      const bool looks = F16 && any && (first || factor != 1.f);
+      if (warp == 0) {      // (one warp asks for all)
+        if (any) mbar_wait(full + st, (i / NST) & 1, ab, 0x7400 + i);
+        if (ends) mbar_wait(y_free + (u ^ 1), ((i - 1) >> 1) & 1, ab, 0x7600 + i);      // (the products of the chunk before)
+        else if (i >= 2) mbar_wait(y_free + u, ((i >> 1) & 1) ^ 1, ab, 0x7500 + i);
       }
-      fence_proxy_async();
-      mbar_arrive_warp(y_ready + u);
-      if (last_of_span(i)) {
-        if (warp == 0) mbar_wait(u_full, spans & 1, ab, 0x7600 + i);
-        named_barrier(1, kGroup);
+      if (looks) {
+        mbar_wait(full + st, (i / NST) & 1, ab, 0x7480 + i);
+        uint32_t bits = 0;
+#pragma unroll
+        for (int q = 0; q < PIECES; ++q) {
+          const int idx = threadIdx.x + q * kGroup;
+          if (((idx >> 3) & (C - 1)) < nv) bits |= bits_of(*reinterpret_cast<const uint4*>(src + idx * 16));
+        }
+        bits = __reduce_or_sync(0xffffffffu, bits);
+        if (lane == 0) s_seen[u * 8 + warp] = bits;
+      }
+      named_barrier(1, kGroup);
+      float own = 1.f;
+      bool less = false;
+      if (looks) {
+        const uint4 a = *reinterpret_cast<const uint4*>(s_seen + u * 8), b = *reinterpret_cast<const uint4*>(s_seen + u * 8 + 4);
+        own = sums_factor_of<EXACT>(bits_of(a) | bits_of(b));
+        less = !first && own < factor;
+        if (less) {
+          if (warp == 0) mbar_wait(y_free + (u ^ 1), ((i - 1) >> 1) & 1, ab, 0x7580 + i);
+          named_barrier(1, kGroup);
+        }
+      }
+      if (ends || less) {
         tc_fence_after();
-        const DecayPair w = in_span == L::kSpan ? whole : last;      // (the first one has nothing to decay)
-        const bool past = spans > 0 && leaves_something(w);
+        const DecayPair w = in_span == L::kSpan ? whole : last;
+        const bool past = some && (decayed || leaves_something(w));
+        const float mul = F16 ? p.sum_scale * inverse_of(factor) : p.sum_scale;
 #pragma unroll 1
         for (int q = 0; q < D / 32; ++q) {
           float U[16], S[16];
@@ -276,14 +291,43 @@ decay_tc_sums_kernel(const __grid_constant__ CUtensorMap tm_y, const __grid_cons
           if (past) tmem_ld16(t_state + q * 16, S);
           tmem_ld_wait();
 #pragma unroll
-          for (int j = 0; j < 16; ++j) S[j] = (past ? decay_by(w, S[j]) : 0.f) + p.sum_scale * U[j];
+          for (int j = 0; j < 16; ++j) S[j] = (past ? decayed ? S[j] : decay_by(w, S[j]) : 0.f) + mul * U[j];
           tmem_st16(t_state + q * 16, S);
         }
         tmem_st_wait();
         tc_fence_before();
-        mbar_arrive_warp(u_free);
-        ++spans;
+        some = true;
+        decayed = less;
       }
+      if (!any) break;
+      if (first) {
+        const int n = i == 0 ? first_span : PER;
+        span_end = REV ? row_of(i + n - 1) : row_of(i + n - 1) + C;
+        if (!REV && span_end > end) span_end = end;
+        in_span = REV ? (int)((i == 0 ? end : row_of(i) + C) - span_end) : (int)(span_end - row_of(i));
+      }
+      if (F16) {
+        if (first || less) factor = own;
+        if (threadIdx.x == 0) s_fresh[u] = less;
+      }
+#pragma unroll
+      for (int q = 0; q < PIECES; ++q) {
+        const int idx = threadIdx.x + q * kGroup, r = (idx >> 3) & (C - 1);
+        uint4 terms[L::kTerms];
+#pragma unroll
+        for (int t = 0; t < L::kTerms; ++t) terms[t] = make_uint4(0, 0, 0, 0);
+        // weights: forwards exp(g (rows of the span behind this one)), backwards exp(g (rows of the span up to and with this one))
+        if (r < nv) {
+          const float w = pw[REV ? (int)(c0 + r - span_end) + 1 : (int)(span_end - 1 - c0 - r)];
+          scaled_terms<T, L::kTerms>(*reinterpret_cast<const uint4*>(src + idx * 16), F16 ? factor * w : w, terms);
+        } else {
+          *reinterpret_cast<uint4*>(src + L::kTile + idx * 16) = make_uint4(0, 0, 0, 0);      // (z's row too: it may hold anything)
+        }
+#pragma unroll
+        for (int t = 0; t < L::kTerms; ++t) *reinterpret_cast<uint4*>(dst + t * L::kTile + idx * 16) = terms[t];
+      }
+      fence_proxy_async();
+      mbar_arrive_warp(y_ready + u);
     }
     if (count > 0) {
       float* to = p.sums + ((size_t)bh * p.ncut + cut) * p.Dr * p.Dr + row * p.Dr;

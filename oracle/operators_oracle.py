@@ -110,7 +110,7 @@ def decay_bounds(q, k, v, d, log_decay, scale, initial_state, d_state, seq_lens,
     A float32 sum of n terms in any order is off by at most n 2^-24 mass; the tensor cores cut off where others round, two half
     steps.  n is at most the head size, the rows of a chunk and the number of chunks, as a sum of sums.  16-bit calls round each
     pair's score, or the key's part of the state, once to their type (half a step of mass), and the result once; fp16 has a smallest step
-    on top (_small_steps; in_range: _range_steps, and no such step for states)."""
+    on top (_small_steps; in_range: _range_steps, and of a state that is handed out 2^-25 of the largest key, as its sums' tiles are brought to 1 and more)."""
     a = lambda t: None if t is None else t.abs()  # noqa: E731
     D, N = q.shape[-1], q.shape[2]
     n = 2 * (D + 128 + N / 64 + 8) * 2.0 ** -24
@@ -130,12 +130,12 @@ def decay_bounds(q, k, v, d, log_decay, scale, initial_state, d_state, seq_lens,
     if dtype == torch.float16 and in_range:
         s0, ds = initial_state, None if d_state is None else d_state / scale      # (the gradient of the state has the scale in it)
         bounds[0] = bounds[0] + _range_steps(q, k, v, s0, scale)
-        bounds[1] = bounds[1] + 2.0 ** -38 * k.abs().amax((2, 3), keepdim=True) * v.abs().sum(2).unsqueeze(2)
+        bounds[1] = bounds[1] + 2.0 ** -25 * k.abs().amax((2, 3), keepdim=True) * v.abs().sum(2).unsqueeze(2)
         if d is not None:
             for i, f, s in ((2, (d, v, k), s0), (3, (v, d, q), ds), (4, (k, q, d), ds)):
                 bounds[i] = bounds[i] + _range_steps(*f, s, scale)
             if bounds[5] is not None:
-                bounds[5] = bounds[5] + 2.0 ** -38 * scale * q.abs().amax((2, 3), keepdim=True) * d.abs().sum(2).unsqueeze(2)
+                bounds[5] = bounds[5] + 2.0 ** -25 * scale * q.abs().amax((2, 3), keepdim=True) * d.abs().sum(2).unsqueeze(2)
     elif dtype == torch.float16:
         forms = [(0, (q, k, v), False)] + ([(2, (d, v, k), False), (3, (v, d, q), True), (4, (k, q, d), True)] if d is not None else [])
         for i, f, backwards in forms:

@@ -190,3 +190,34 @@ def test_small_keys_over_chunks_in_fp16(cuda_device, D, size, padded):
         lens = torch.tensor([300, 299, 257, 130, 1] * 10, dtype=torch.int32, device="cuda")
     scale = size[4] if size[4] is None else min(size[4], 10.0)      # (times 100 the gradient of k, scale sqrt(D rows), would leave the range)
     _check_range(t, torch.tensor([-0.2, -0.01, 0.0], device="cuda"), scale=scale, lens=lens, final=False)
+
+
+@pytest.mark.parametrize("D", [64, 128, 16])
+@pytest.mark.parametrize("N", [100, 700, 5000])
+@pytest.mark.parametrize("size", [1e-5, 3e-4, 0.02, 0.5])
+def test_small_keys_in_sums_in_fp16(cuda_device, D, N, size):
+    """States that are handed out, of a sequence and of its segments, and their gradients: the sums of small keys (and queries, backwards) have FP32's bits."""
+    t = [_normal(1, 2, N, D, seed=i, mul=m).half() for i, m in enumerate((size, size, 1.0, 1.0))]
+    _check_range(t, torch.tensor([-0.02, -1e-3], device="cuda"), _normal(1, 2, D, D, seed=7, mul=size), _normal(1, 2, D, D, seed=8, mul=size), scale=1 / size)
+
+
+@pytest.mark.parametrize("D", [64, 128, 32])
+@pytest.mark.parametrize("N,lens", [(300, None), (1500, None), (6000, None), (1100, [1100, 1000, 513, 77])])
+def test_keys_whose_size_changes_in_fp16(cuda_device, D, N, lens):
+    """Rows that grow and shrink by many powers of two from block to block, zeros among them: sums begin small and meet what their factor is too large for, in
+    either direction of time."""
+    B = 1 if lens is None else len(lens)
+    t = [_normal(B, 2, N, D, seed=i).half() for i in range(4)]
+    sizes = torch.tensor([1e-5, 0.0, 1e-3, 1e-2, 0.1, 1.0, 20.0, 3.0, 1e-4, 0.05, 5.0, 1e-6, 1e-2], dtype=torch.float16, device="cuda")
+    at = torch.arange(N, device="cuda")
+    for x, rows in ((t[0], 45), (t[1], 32)):
+        x *= sizes[at // rows % len(sizes)].view(1, 1, N, 1)
+    lens = None if lens is None else torch.tensor(lens, dtype=torch.int32, device="cuda")
+    _check_range(t, torch.tensor([-0.02, -1e-3], device="cuda"), _normal(B, 2, D, D, seed=7), _normal(B, 2, D, D, seed=8), lens=lens)
+    again = [_call_state(t, lens) for _ in range(2)]
+    assert all(torch.equal(a, b) for a, b in zip(*again))
+
+
+def _call_state(t, lens):
+    from flashnystrom_b200 import decay_attention
+    return decay_attention(*t[:3], torch.tensor([-0.02, -1e-3], device="cuda"), seq_lens=lens, return_state=True)
