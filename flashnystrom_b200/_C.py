@@ -291,6 +291,12 @@ def being_transformed():
     return torch._C._get_tracing_state() is not None or torch._C._are_functorch_transforms_active()
 
 
+def wants_operators(*tensors):
+    """Whether a call goes through the registered operators: something traces, transforms or records it, or a tensor (those that are given) is a subclass, so that the C++
+    module would do work that is not seen."""
+    return being_transformed() or torch._C._len_torch_dispatch_stack() > 0 or any(t is not None and type(t) not in _PLAIN for t in tensors)
+
+
 def attention(q, k, v, num_landmarks, newton_iter, kappa_star, weight=None):
     """Attention (and the convolution residual) through the C++ module, differentiable; None for a call that is not plainly one of
     plain tensors and numbers, which then takes the autograd functions of flash_nystrom.py."""

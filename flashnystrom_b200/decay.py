@@ -46,7 +46,7 @@ def decay_attention(q, k, v, log_decay, scale=None, initial_state=None, seq_lens
     the rows after it by definition, and may reach up to 127 rows before it.  There is no second derivative, and no CPU path."""
     _check_tensors("decay_attention", q=q, k=k, v=v, log_decay=log_decay)
     scale = _scale(scale, q.shape[-1] if q.dim() else 0)
-    if torch.compiler.is_compiling() or _C.being_transformed():
+    if torch.compiler.is_compiling() or _C.wants_operators(q, k, v, log_decay, initial_state, seq_lens):
         from . import _ops
         out, state = _ops.decay_attention_via_ops(q, k, v, log_decay, scale, initial_state, seq_lens)
     else:
@@ -64,7 +64,7 @@ def decay_attention_step(q, k, v, state, log_decay, scale=None, slots=None):
     Returns (B, H, D).  No gradient: with one wanted the call is refused (decay_attention has one)."""
     _check_tensors("decay_attention_step", q=q, k=k, v=v, state=state, log_decay=log_decay)
     scale = _scale(scale, q.shape[-1] if q.dim() else 0)
-    if torch.compiler.is_compiling():
+    if torch.compiler.is_compiling() or _C.wants_operators(q, k, v, state, log_decay, slots):
         from . import _ops
         return _ops.decay_step(q, k, v, state, log_decay, scale, slots)
     return _C.native().decay_step(q, k, v, state, log_decay, scale, slots)

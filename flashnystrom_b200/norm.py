@@ -18,7 +18,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, num_groups=1):
     fixed order, so that two calls give the same bits.  There is no second derivative, and no CPU path."""
     if not isinstance(x, torch.Tensor):
         raise RuntimeError("layer_norm: x must be a tensor")
-    if torch.compiler.is_compiling() or _C.being_transformed():
+    if torch.compiler.is_compiling() or _C.wants_operators(x, weight, bias):
         from . import _ops
         return _ops.layer_norm_via_ops(x, weight, bias, float(eps), int(num_groups))
     return _C.native().layer_norm(x, weight, bias, float(eps), int(num_groups))

@@ -221,3 +221,49 @@ def test_keys_whose_size_changes_in_fp16(cuda_device, D, N, lens):
 def _call_state(t, lens):
     from flashnystrom_b200 import decay_attention
     return decay_attention(*t[:3], torch.tensor([-0.02, -1e-3], device="cuda"), seq_lens=lens, return_state=True)
+
+
+def _three():
+    """The three calls, each of one tensor, with what they are called on."""
+    from flashnystrom_b200 import decay_attention, decay_attention_step, layer_norm
+    q, k, v = (_normal(1, 2, 100, 64, seed=i, dtype=torch.float16) for i in range(3))
+    log_decay, state, x = torch.tensor([-0.1, -0.01], device="cuda"), _normal(1, 2, 64, 64, seed=4), _normal(5, 64, seed=5)
+    t = lambda a: a[:, :, 0].contiguous()  # noqa: E731
+    kt, vt = t(k), t(v)
+    return {"attention": (lambda a: decay_attention(a, k, v, log_decay), q), "step": (lambda a: decay_attention_step(a, kt, vt, state, log_decay), t(q)),
+            "norm": (layer_norm, x)}, state
+
+
+@pytest.mark.parametrize("name", ["attention", "step", "norm"])
+def test_traced_and_recorded(cuda_device, name):
+    """A trace, a mode that records operators and a subclass see the whole call: an operator that writes its result, and the state that a step writes."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+    calls, state = _three()
+    f, x = calls[name]
+    before = state.clone()
+    want = f(x)
+    after = state.clone()
+    state.copy_(before)
+    traced = torch.jit.trace(f, (x,), check_trace=False)
+    state.copy_(before)
+    assert torch.equal(traced(x), want) and torch.equal(state, after)
+    assert torch.equal(traced(-x) if name != "step" else want, f(-x) if name != "step" else want)
+
+    class Recorder(TorchDispatchMode):
+        def __init__(self):
+            super().__init__()
+            self.seen = []
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+    state.copy_(before)
+    with Recorder() as recorder:
+        got = f(x)
+    assert torch.equal(got, want) and torch.equal(state, after)
+    assert any(s.startswith("flashnystrom_b200.") for s in recorder.seen), recorder.seen
+
+    class Sub(torch.Tensor):
+        pass
+    state.copy_(before)
+    assert torch.equal(f(x.as_subclass(Sub)).as_subclass(torch.Tensor), want) and torch.equal(state, after)
