@@ -297,6 +297,15 @@ def wants_operators(*tensors):
     return being_transformed() or torch._C._len_torch_dispatch_stack() > 0 or any(t is not None and type(t) not in _PLAIN for t in tensors)
 
 
+def refuse_tangents(name, *tensors):
+    """Forward-mode derivatives have no formula here: refused, so that a tangent is not taken for zero."""
+    if torch.autograd.forward_ad._current_level < 0:
+        return
+    for t in tensors:
+        if t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{name} has no forward-mode derivative")
+
+
 def attention(q, k, v, num_landmarks, newton_iter, kappa_star, weight=None):
     """Attention (and the convolution residual) through the C++ module, differentiable; None for a call that is not plainly one of
     plain tensors and numbers, which then takes the autograd functions of flash_nystrom.py."""

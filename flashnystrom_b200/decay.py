@@ -43,9 +43,11 @@ def decay_attention(q, k, v, log_decay, scale=None, initial_state=None, seq_lens
     Sums and states are float32.  fp16 and bf16 calls round each pair's score, or the key's share of the state, once to their type on the way;
     a state that is handed out does not have that rounding, and asking for it may change the last bit of the output of long sequences.  Scores
     and states may leave fp16's range as long as the output does not.  A row of q, k or v that counts and holds an infinity or NaN reaches
-    the rows after it by definition, and may reach up to 127 rows before it.  There is no second derivative, and no CPU path."""
+    the rows after it by definition, and may reach up to 127 rows before it.  There is no second derivative, no forward-mode one, and no CPU path."""
     _check_tensors("decay_attention", q=q, k=k, v=v, log_decay=log_decay)
     scale = _scale(scale, q.shape[-1] if q.dim() else 0)
+    if not torch.compiler.is_compiling():
+        _C.refuse_tangents("decay_attention", q, k, v, log_decay, initial_state)
     if torch.compiler.is_compiling() or _C.wants_operators(q, k, v, log_decay, initial_state, seq_lens):
         from . import _ops
         out, state = _ops.decay_attention_via_ops(q, k, v, log_decay, scale, initial_state, seq_lens)
@@ -64,6 +66,8 @@ def decay_attention_step(q, k, v, state, log_decay, scale=None, slots=None):
     Returns (B, H, D).  No gradient: with one wanted the call is refused (decay_attention has one)."""
     _check_tensors("decay_attention_step", q=q, k=k, v=v, state=state, log_decay=log_decay)
     scale = _scale(scale, q.shape[-1] if q.dim() else 0)
+    if not torch.compiler.is_compiling():
+        _C.refuse_tangents("decay_attention_step", q, k, v, state, log_decay)
     if torch.compiler.is_compiling() or _C.wants_operators(q, k, v, state, log_decay, slots):
         from . import _ops
         return _ops.decay_step(q, k, v, state, log_decay, scale, slots)

@@ -15,9 +15,11 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, num_groups=1):
     every head's output by itself.  x: CUDA tensor, fp16 / bf16 / fp32, any strides (read in place where rows of the last
     dimension are contiguous and one stride apart, copied otherwise); weight, bias: float32 or of x's dtype, or None.  At most 16384
     elements are normalised together.  Statistics and sums are float32; the gradients of weight and bias are summed in a
-    fixed order, so that two calls give the same bits.  There is no second derivative, and no CPU path."""
+    fixed order, so that two calls give the same bits.  There is no second derivative, no forward-mode one, and no CPU path."""
     if not isinstance(x, torch.Tensor):
         raise RuntimeError("layer_norm: x must be a tensor")
+    if not torch.compiler.is_compiling():
+        _C.refuse_tangents("layer_norm", x, weight, bias)
     if torch.compiler.is_compiling() or _C.wants_operators(x, weight, bias):
         from . import _ops
         return _ops.layer_norm_via_ops(x, weight, bias, float(eps), int(num_groups))

@@ -267,3 +267,19 @@ def test_traced_and_recorded(cuda_device, name):
         pass
     state.copy_(before)
     assert torch.equal(f(x.as_subclass(Sub)).as_subclass(torch.Tensor), want) and torch.equal(state, after)
+
+
+@pytest.mark.parametrize("name", ["attention", "step", "norm"])
+def test_tangents_are_refused(cuda_device, name):
+    """A forward-mode derivative is an error, not zero; outside of one the call is as before."""
+    from torch.autograd import forward_ad
+    calls, state = _three()
+    f, x = calls[name]
+    with forward_ad.dual_level():
+        f(x)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="no forward-mode derivative"):
+            f(forward_ad.make_dual(x, torch.ones_like(x)))
+        with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+            f(forward_ad.make_dual(x, torch.ones_like(x)))
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(f, (x,), (torch.ones_like(x),))
