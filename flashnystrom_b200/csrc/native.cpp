@@ -392,7 +392,8 @@ variable_list once_differentiable(variable_list grads, const char* what, const v
 }
 
 // (B, H, N, D) rows that the kernels can read where they lie: last dimension contiguous, no dimension spread out of one element
-at::Tensor rows_in_place(const at::Tensor& t) {
+at::Tensor rows_in_place(const at::Tensor& given) {
+  const at::Tensor t = given.resolve_neg();
   bool fine = t.stride(3) == 1 || t.size(3) == 1;
   for (int i = 0; i < 3; ++i) fine = fine && (t.size(i) == 1 || t.stride(i) > 0);
   return fine ? t : t.contiguous();
@@ -445,13 +446,15 @@ DecayArgs decay_args(const at::Tensor& q, const at::Tensor& k, const at::Tensor&
   }
   return {q, k, v, log_decay, initial ? *initial : at::Tensor(), seq_lens ? *seq_lens : at::Tensor(), scale, status};
 }
-at::Tensor contiguous_or_none(const at::Tensor& t) { return t.defined() ? t.contiguous() : t; }
+// (memory that holds what the tensor says: no negative bit)
+at::Tensor in_memory(const at::Tensor& t) { return t.resolve_neg().contiguous(); }
+at::Tensor contiguous_or_none(const at::Tensor& t) { return t.defined() ? in_memory(t) : t; }
 
 // out, the state behind the last row (undefined unless wanted), the states at the cuts
 struct DecayResult { at::Tensor out, final, segments; };
 DecayResult run_decay_forward(const DecayArgs& c, bool want_state) {
   const at::Tensor q = rows_in_place(c.q), k = rows_in_place(c.k), v = rows_in_place(c.v);
-  const at::Tensor g = c.log_decay.contiguous(), initial = contiguous_or_none(c.initial), lens = contiguous_or_none(c.seq_lens);
+  const at::Tensor g = in_memory(c.log_decay), initial = contiguous_or_none(c.initial), lens = contiguous_or_none(c.seq_lens);
   fnb_decay_fwd_args a{};
   a.shape = decay_shape(q, c.scale);
   check(fnb_check_decay_shape(&a.shape));
@@ -476,7 +479,7 @@ DecayResult run_decay_forward(const DecayArgs& c, bool want_state) {
 // dq, dk, dv, d_initial (undefined unless wanted)
 variable_list run_decay_backward(const DecayArgs& c, const at::Tensor& segments, const at::Tensor& d_out, const at::Tensor& d_final, bool want_initial) {
   const at::Tensor q = rows_in_place(c.q), k = rows_in_place(c.k), v = rows_in_place(c.v), d = rows_in_place(d_out);
-  const at::Tensor g = c.log_decay.contiguous(), initial = contiguous_or_none(c.initial), lens = contiguous_or_none(c.seq_lens),
+  const at::Tensor g = in_memory(c.log_decay), initial = contiguous_or_none(c.initial), lens = contiguous_or_none(c.seq_lens),
                    df = contiguous_or_none(d_final);
   fnb_decay_bwd_args a{};
   a.shape = decay_shape(q, c.scale);
@@ -600,16 +603,17 @@ at::Tensor decay_step(const at::Tensor& q_, const at::Tensor& k_, const at::Tens
   }
   TORCH_CHECK(!(at::GradMode::is_enabled() && (q_.requires_grad() || k_.requires_grad() || v_.requires_grad() || state.requires_grad())),
               "decay_attention_step updates the state in place and has no gradient: use decay_attention, or torch.no_grad()");
+  TORCH_CHECK(!state.is_neg(), "state must not be a negative view: it is written where it lies");
   TORCH_CHECK(!state.is_inference() || c10::InferenceMode::is_enabled(), "an inference tensor cannot be updated in place outside InferenceMode");
   py::gil_scoped_release nogil;
   c10::cuda::CUDAGuard guard(q_.device());
   at::AutoGradMode off(false);
-  const auto in_place = [](const at::Tensor& t) { return t.stride(2) == 1 ? t : t.contiguous(); };
-  const at::Tensor q = in_place(q_), k = in_place(k_), v = in_place(v_), g = log_decay.contiguous();
+  const auto in_place = [](const at::Tensor& t) { return t.stride(2) == 1 ? t.resolve_neg() : in_memory(t); };
+  const at::Tensor q = in_place(q_), k = in_place(k_), v = in_place(v_), g = in_memory(log_decay);
   at::Tensor out = at::empty({B, H, D}, q.options());
   if (B == 0 || H == 0) return out;
   if (state.size(0) == 0) return out.zero_();      // (slots of no state: every row is idle)
-  const at::Tensor s = slots ? slots->contiguous() : at::Tensor();
+  const at::Tensor s = slots ? in_memory(*slots) : at::Tensor();
   fnb_decay_step_args a{};
   const auto arg = [](const at::Tensor& t) { return fnb_rows{t.data_ptr(), t.stride(0), t.stride(1), 0}; };
   a.batch = B; a.heads = H; a.num_states = state.size(0); a.head_dim = (int32_t)std::min<int64_t>(D, INT32_MAX); a.dtype = dtype_of(q);
@@ -624,7 +628,8 @@ at::Tensor decay_step(const at::Tensor& q_, const at::Tensor& k_, const at::Tens
 }
 
 // x as rows of its last dimension that lie one stride apart; contiguous where it is not so
-at::Tensor norm_rows(const at::Tensor& x) {
+at::Tensor norm_rows(const at::Tensor& given) {
+  const at::Tensor x = given.resolve_neg();
   const int64_t C = x.size(-1);
   if (C == 1 || x.stride(-1) == 1) {
     int64_t stride = -1, size = 1;      // of the innermost leading dimension that counts; rows so far

@@ -283,3 +283,32 @@ def test_tangents_are_refused(cuda_device, name):
             f(forward_ad.make_dual(x, torch.ones_like(x)))
     with pytest.raises(RuntimeError):
         torch.func.jvp(f, (x,), (torch.ones_like(x),))
+
+
+def test_negative_views(cuda_device):
+    """Tensors whose negative bit is set hold the opposite of what they are: read as what they are, in every place that takes one."""
+    from flashnystrom_b200 import decay_attention, decay_attention_step, layer_norm
+    neg = torch._neg_view
+    q, k, v, d = (_normal(1, 2, 200, 64, seed=i) for i in range(4))
+    s0, ds = _normal(1, 2, 64, 64, seed=5), _normal(1, 2, 64, 64, seed=6)
+    log_decay = torch.tensor([-0.1, -0.01], device="cuda")
+
+    def run(q, k, v, g, s0, d, ds):
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v, s0)]
+        out, state = decay_attention(*leaves[:3], g, initial_state=leaves[3], return_state=True)
+        return [out, state, *torch.autograd.grad((out, state), leaves, (d, ds))]
+    plain = run(-q, -k, -v, log_decay, -s0, -d, -ds)
+    views = run(neg(q), neg(k), neg(v), neg(-log_decay), neg(s0), neg(d), neg(ds))
+    assert all(torch.equal(a, b) for a, b in zip(plain, views))
+    t = lambda a: a[:, :, 0]  # noqa: E731
+    a, b = s0.clone(), s0.clone()
+    assert torch.equal(decay_attention_step(t(-q), t(-k), t(-v), a, log_decay), decay_attention_step(neg(t(q)), neg(t(k)), neg(t(v)), b, neg(-log_decay))) and torch.equal(a, b)
+    with pytest.raises(RuntimeError, match="negative view"):
+        decay_attention_step(t(q), t(k), t(v), neg(a), log_decay)
+    x, w, bias, dy = _normal(7, 64, seed=1), _normal(64, seed=2), _normal(64, seed=3), _normal(7, 64, seed=4)
+
+    def norm(*p):
+        leaves = [t.detach().requires_grad_(True) for t in p[:3]]
+        y = layer_norm(*leaves)
+        return [y, *torch.autograd.grad(y, leaves, p[3])]
+    assert all(torch.equal(a, b) for a, b in zip(norm(-x, -w, -bias, -dy), norm(neg(x), neg(w), neg(bias), neg(dy))))
