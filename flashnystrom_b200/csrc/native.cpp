@@ -537,6 +537,12 @@ struct DecayNode : torch::autograd::Function<DecayNode> {
   }
 };
 
+// the state behind a sequence without rows
+at::Tensor state_of_nothing(const DecayArgs& c) {
+  TORCH_CHECK(c.q.size(3) > 0, "head_dim must be 16, 32, 64 or 128, got 0");
+  return c.initial.defined() ? c.initial.clone() : at::zeros({c.q.size(0), c.q.size(1), c.q.size(3), c.q.size(3)}, c.q.options().dtype(at::kFloat));
+}
+
 // (out, final state or nothing)
 std::pair<at::Tensor, OptTensor> decay_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& log_decay,
                                                  double scale, const OptTensor& initial, const OptTensor& seq_lens, bool want_state,
@@ -545,9 +551,8 @@ std::pair<at::Tensor, OptTensor> decay_attention(const at::Tensor& q, const at::
   py::gil_scoped_release nogil;
   c10::cuda::CUDAGuard guard(q.device());
   if (q.numel() == 0) {      // nothing to attend to: the state goes through
-    TORCH_CHECK(q.size(3) > 0, "head_dim must be 16, 32, 64 or 128, got 0");
-    OptTensor state;
-    if (want_state) state = initial ? initial->clone() : at::zeros({q.size(0), q.size(1), q.size(3), q.size(3)}, q.options().dtype(at::kFloat));
+    OptTensor state = state_of_nothing(c);
+    if (!want_state) state = std::nullopt;
     return {q + k + v, state};      // (no elements, and a graph to all three)
   }
   if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() || (initial && initial->requires_grad()))) {
@@ -564,6 +569,10 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> decay_forward(const at::Tensor& q
   at::AutoGradMode off(false);
   const DecayArgs c = decay_args(q, k, v, log_decay, scale, initial, seq_lens, status);
   c10::cuda::CUDAGuard guard(q.device());
+  if (q.numel() == 0) {
+    const auto f32 = q.options().dtype(at::kFloat);
+    return {empty_rows_like(rows_in_place(q)), state_of_nothing(c), at::empty({0}, f32)};
+  }
   const DecayResult r = run_decay_forward(c, true);
   return {r.out, r.final, r.segments};
 }
@@ -576,6 +585,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> decay_backward(const 
   TORCH_CHECK(d.sizes() == q.sizes() && d.scalar_type() == q.scalar_type() && d.device() == q.device(), "d_out does not match q");
   check_state(df, "d_final_state", q);
   c10::cuda::CUDAGuard guard(q.device());
+  if (q.numel() == 0) return {empty_rows_like(rows_in_place(q)), empty_rows_like(rows_in_place(k)), empty_rows_like(rows_in_place(v)), df.clone()};
   const variable_list g = run_decay_backward(c, segments, d, df, true);
   return {g[0], g[1], g[2], g[3]};
 }
@@ -773,7 +783,12 @@ at::Tensor layer_norm(const at::Tensor& x, const OptTensor& weight, const OptTen
 std::tuple<at::Tensor, at::Tensor, at::Tensor> norm_forward(const at::Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps, int64_t groups) {
   at::AutoGradMode off(false);
   c10::cuda::CUDAGuard guard(x.device());
-  const NormResult r = run_norm_forward(norm_args(x, weight, bias, eps, groups), true);
+  const NormArgs c = norm_args(x, weight, bias, eps, groups);
+  if (x.numel() == 0) {
+    const auto f32 = x.options().dtype(at::kFloat);
+    return {at::empty(x.sizes(), x.options()), at::empty({0}, f32), at::empty({0}, f32)};
+  }
+  const NormResult r = run_norm_forward(c, true);
   return {r.y, r.mean.clone(), r.rstd.clone()};
 }
 std::tuple<at::Tensor, at::Tensor, at::Tensor> norm_backward(const at::Tensor& d, const at::Tensor& x, const OptTensor& weight, const at::Tensor& mean,
@@ -782,6 +797,10 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> norm_backward(const at::Tensor& d
   c10::cuda::CUDAGuard guard(x.device());
   norm_args(x, weight, std::nullopt, eps, groups);
   TORCH_CHECK(d.sizes() == x.sizes() && d.scalar_type() == x.scalar_type() && d.device() == x.device(), "d_y does not match x");
+  if (x.numel() == 0) {
+    const auto p = x.options().dtype(param_f32 ? at::kFloat : x.scalar_type());
+    return {at::empty(x.sizes(), x.options()), at::zeros({x.size(-1)}, p), at::zeros({x.size(-1)}, p)};
+  }
   const variable_list g = run_norm_backward(x, weight ? *weight : at::Tensor(), mean, rstd, d, groups, eps, param_f32 ? at::kFloat : x.scalar_type(), true, true,
                                             true);
   return {g[0], g[1], g[2]};

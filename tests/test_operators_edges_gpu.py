@@ -312,3 +312,26 @@ def test_negative_views(cuda_device):
         y = layer_norm(*leaves)
         return [y, *torch.autograd.grad(y, leaves, p[3])]
     assert all(torch.equal(a, b) for a, b in zip(norm(-x, -w, -bias, -dy), norm(neg(x), neg(w), neg(bias), neg(dy))))
+
+
+@pytest.mark.parametrize("shape", [(2, 3, 0, 64), (0, 3, 10, 64)])
+def test_empty_calls_compiled(cuda_device, shape):
+    """Nothing to attend to or to normalise: a compiled call gives what the eager one does, its gradients too."""
+    from flashnystrom_b200 import decay_attention, layer_norm
+    log_decay = torch.zeros(3, device="cuda")
+
+    def f(q, s0):
+        return decay_attention(q, q, q, log_decay, initial_state=s0, return_state=True)
+
+    def g(x, w, b):
+        return layer_norm(x, w, b)
+    for fn, sizes in ((f, (shape, (shape[0], 3, 64, 64))), (g, ((0, 5, 48), (48,), (48,)))):
+        torch._dynamo.reset()
+        results = []
+        for call in (fn, torch.compile(fn, fullgraph=True, backend="aot_eager")):
+            leaves = [_normal(*s, seed=1).requires_grad_(True) for s in sizes]
+            out = call(*leaves)
+            out = out if isinstance(out, tuple) else (out,)
+            results.append([*out, *torch.autograd.grad(sum(o.sum() for o in out), leaves)])
+        for a, b in zip(*results):
+            assert a.shape == b.shape and a.dtype == b.dtype and torch.equal(a, b)
