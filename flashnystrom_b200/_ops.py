@@ -8,11 +8,12 @@ graph).
     torch.ops.flashnystrom_b200.nystrom_bwd(d_out, q, k, v, <the ten saved tensors>, ...)
         -> (dq, dk, dv)
 
-    torch.ops.flashnystrom_b200.decay_fwd(q, k, v, log_decay, scale, initial_state, seq_lens) -> (out, final_state, states at the cuts)
-    torch.ops.flashnystrom_b200.decay_bwd(...) -> (dq, dk, dv, d_initial_state)
+    torch.ops.flashnystrom_b200.decay_fwd(q, k, v, log_decay, scale, initial_state, seq_lens, want_state=True, bounded=False)
+        -> (out, final_state, states at the cuts)
+    torch.ops.flashnystrom_b200.decay_bwd(..., want_initial=True) -> (dq, dk, dv, d_initial_state)
     torch.ops.flashnystrom_b200.decay_step(q, k, v, state, log_decay, scale, slots) -> out, with state written
-    torch.ops.flashnystrom_b200.norm_fwd(x, weight, bias, eps, num_groups) -> (y, mean, rstd)
-    torch.ops.flashnystrom_b200.norm_bwd(...) -> (dx, d_weight, d_bias)
+    torch.ops.flashnystrom_b200.norm_fwd(x, weight, bias, eps, num_groups, keep=True) -> (y, mean, rstd)
+    torch.ops.flashnystrom_b200.norm_bwd(..., want_x=True, want_weight=True, want_bias=True) -> (dx, d_weight, d_bias)
 
 All have fake (meta) implementations, and the forward ones have their autograd formulas registered, so the
 operators work under FakeTensorMode, AOT autograd and opcheck.  Eager calls go through the C++ module
@@ -92,11 +93,28 @@ def attention_via_ops(q, k, v, num_landmarks, newton_iter, kappa_star):
 
 
 # ---- causal attention with a decay ------------------------------------------------------------------------
-# (an operator's outputs have one layout, whatever its inputs': contiguous)
-@torch.library.custom_op(f"{_LIB}::decay_fwd", mutates_args=(), device_types="cuda")
-def decay_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, scale: float,
-              initial_state: Optional[torch.Tensor], seq_lens: Optional[torch.Tensor]) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    return _C.native().decay_forward(q.contiguous(), k.contiguous(), v.contiguous(), log_decay, scale, initial_state, seq_lens, _C._status(q.device))
+# Tensors are taken and given back in the order of memory that they have, as by eager calls; what is not wanted has no elements.
+def _rows_like(t):
+    """Uninitialised, in the order that t's heads and rows have in memory (t itself where it can be read in place, its contiguous copy otherwise)."""
+    B, H, N, D = t.shape
+    in_place = t.size(3) == 1 or t.stride(3) == 1
+    for i in range(3):
+        in_place = in_place and (t.size(i) == 1 or t.stride(i) > 0)
+    if in_place and t.stride(1) < t.stride(2):
+        return t.new_empty_strided((B, H, N, D), (N * H * D, D, H * D, 1))
+    return t.new_empty((B, H, N, D))
+
+
+def _segment_bound(B, H, N, D, dtype, sms):
+    """Floats that the states at the cuts take at most, for sizes that need not be numbers yet: a slice has no more segments than units of 64 (float32) or 128
+    rows, all slices together no more than two rounds of CTAs, or one each."""
+    unit, slots = (64, 2 * sms if D <= 64 else sms) if dtype == torch.float32 else (128, sms)
+    units = (N + unit - 1) // unit
+    return D * D * torch.sym_min(B * H * units, torch.sym_max(B * H, 2 * slots))
+
+
+def _bound_of(q):
+    return _segment_bound(*q.shape, q.dtype, torch.cuda.get_device_properties(q.device).multi_processor_count)
 
 
 def _segment_floats(q):
@@ -107,47 +125,60 @@ def _segment_floats(q):
         return _lib.load().fnb_decay_segment_floats(C.byref(shape))
 
 
+@torch.library.custom_op(f"{_LIB}::decay_fwd", mutates_args=(), device_types="cuda")
+def decay_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, scale: float,
+              initial_state: Optional[torch.Tensor], seq_lens: Optional[torch.Tensor], want_state: bool = True,
+              bounded: bool = False) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """bounded: the states at the cuts in room by _segment_bound, whose size holds for symbols, in place of what this very length takes."""
+    return _C.native().decay_forward(q, k, v, log_decay, scale, initial_state, seq_lens, want_state, int(_bound_of(q)) if bounded else -1, _C._status(q.device))
+
+
 @decay_fwd.register_fake
-def _(q, k, v, log_decay, scale, initial_state, seq_lens):
+def _(q, k, v, log_decay, scale, initial_state, seq_lens, want_state=True, bounded=False):
     B, H, N, D = q.shape
-    return (torch.empty_like(q, memory_format=torch.contiguous_format), torch.empty(B, H, D, D, dtype=torch.float32, device=q.device),
-            torch.empty(_segment_floats(q), dtype=torch.float32, device=q.device))
+    f32 = dict(dtype=torch.float32, device=q.device)
+    return (_rows_like(q), torch.empty((B, H, D, D) if want_state else (0,), **f32), torch.empty(_bound_of(q) if bounded else _segment_floats(q), **f32))
 
 
 @torch.library.custom_op(f"{_LIB}::decay_bwd", mutates_args=(), device_types="cuda")
-def decay_bwd(d_out: torch.Tensor, d_state: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, scale: float,
-              initial_state: Optional[torch.Tensor], seq_lens: Optional[torch.Tensor],
-              segments: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
-    return _C.native().decay_backward(d_out.contiguous(), d_state.contiguous(), q.contiguous(), k.contiguous(), v.contiguous(), log_decay, scale, initial_state, seq_lens,
-                                      segments, _C._status(q.device))
+def decay_bwd(d_out: torch.Tensor, d_state: Optional[torch.Tensor], q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, scale: float,
+              initial_state: Optional[torch.Tensor], seq_lens: Optional[torch.Tensor], segments: torch.Tensor,
+              want_initial: bool = True) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    return _C.native().decay_backward(d_out, d_state, q, k, v, log_decay, scale, initial_state, seq_lens, segments, want_initial, _C._status(q.device))
 
 
 @decay_bwd.register_fake
-def _(d_out, d_state, q, k, v, log_decay, scale, initial_state, seq_lens, segments):
-    c = torch.contiguous_format
-    return (torch.empty_like(q, memory_format=c), torch.empty_like(k, memory_format=c), torch.empty_like(v, memory_format=c),
-            torch.empty_like(d_state, memory_format=c))
+def _(d_out, d_state, q, k, v, log_decay, scale, initial_state, seq_lens, segments, want_initial=True):
+    B, H, N, D = q.shape
+    return _rows_like(q), _rows_like(k), _rows_like(v), torch.empty((B, H, D, D) if want_initial else (0,), dtype=torch.float32, device=q.device)
 
 
 def _decay_context(ctx, inputs, output):
-    q, k, v, log_decay, scale, initial_state, seq_lens = inputs
+    q, k, v, log_decay, scale, initial_state, seq_lens, want_state, _ = inputs
     ctx.save_for_backward(q, k, v, log_decay, initial_state, seq_lens, output[2])
-    ctx.scale = scale
+    ctx.scale, ctx.want_state = scale, want_state
+    ctx.set_materialize_grads(False)
 
 
 def _decay_backward(ctx, d_out, d_state, _unused):
     q, k, v, log_decay, initial_state, seq_lens, segments = ctx.saved_tensors
-    dq, dk, dv, ds = decay_bwd(d_out, d_state, q, k, v, log_decay, ctx.scale, initial_state, seq_lens, segments)
-    return dq, dk, dv, None, None, ds if initial_state is not None else None, None
+    if not ctx.want_state:
+        d_state = None
+    if d_out is None and d_state is None:
+        return (None,) * 9
+    want_initial = initial_state is not None and ctx.needs_input_grad[5]
+    dq, dk, dv, ds = decay_bwd(torch.zeros_like(q) if d_out is None else d_out, d_state, q, k, v, log_decay, ctx.scale, initial_state, seq_lens, segments,
+                               want_initial)
+    return dq, dk, dv, None, None, ds if want_initial else None, None, None, None
 
 
 decay_fwd.register_autograd(_decay_backward, setup_context=_decay_context)
 
 
-def decay_attention_via_ops(q, k, v, log_decay, scale, initial_state, seq_lens):
+def decay_attention_via_ops(q, k, v, log_decay, scale, initial_state, seq_lens, want_state):
     if log_decay.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("log_decay is a constant here: it has no gradient")
-    out, state, _ = decay_fwd(q, k, v, log_decay, scale, initial_state, seq_lens)
+    out, state, _ = decay_fwd(q, k, v, log_decay, scale, initial_state, seq_lens, want_state, torch.compiler.is_compiling())
     return out, state
 
 
@@ -164,32 +195,34 @@ def _(q, k, v, state, log_decay, scale, slots):
 
 # ---- layer norm -------------------------------------------------------------------------------------------
 @torch.library.custom_op(f"{_LIB}::norm_fwd", mutates_args=(), device_types="cuda")
-def norm_fwd(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor], eps: float,
-             num_groups: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    return _C.native().norm_forward(x, weight, bias, eps, num_groups)
+def norm_fwd(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor], eps: float, num_groups: int,
+             keep: bool = True) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """keep: the statistics too, which the backward reads."""
+    return _C.native().norm_forward(x, weight, bias, eps, num_groups, keep)
 
 
 @norm_fwd.register_fake
-def _(x, weight, bias, eps, num_groups):
-    runs = x.numel() // x.shape[-1] * num_groups
+def _(x, weight, bias, eps, num_groups, keep=True):
+    runs = x.numel() // x.shape[-1] * num_groups if keep else 0
     f32 = dict(dtype=torch.float32, device=x.device)
     return torch.empty_like(x, memory_format=torch.contiguous_format), torch.empty(runs, **f32), torch.empty(runs, **f32)
 
 
 @torch.library.custom_op(f"{_LIB}::norm_bwd", mutates_args=(), device_types="cuda")
 def norm_bwd(d_y: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor], mean: torch.Tensor, rstd: torch.Tensor, eps: float, num_groups: int,
-             param_f32: bool) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    return _C.native().norm_backward(d_y, x, weight, mean, rstd, eps, num_groups, param_f32)
+             param_f32: bool, want_x: bool = True, want_weight: bool = True, want_bias: bool = True) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    return _C.native().norm_backward(d_y, x, weight, mean, rstd, eps, num_groups, param_f32, want_x, want_weight, want_bias)
 
 
 @norm_bwd.register_fake
-def _(d_y, x, weight, mean, rstd, eps, num_groups, param_f32):
+def _(d_y, x, weight, mean, rstd, eps, num_groups, param_f32, want_x=True, want_weight=True, want_bias=True):
     p = dict(dtype=torch.float32 if param_f32 else x.dtype, device=x.device)
-    return torch.empty_like(x, memory_format=torch.contiguous_format), torch.empty(x.shape[-1], **p), torch.empty(x.shape[-1], **p)
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format) if want_x else x.new_empty(0)
+    return dx, torch.empty(x.shape[-1] if want_weight else 0, **p), torch.empty(x.shape[-1] if want_bias else 0, **p)
 
 
 def _norm_context(ctx, inputs, output):
-    x, weight, bias, eps, num_groups = inputs
+    x, weight, bias, eps, num_groups, _ = inputs
     ctx.save_for_backward(x, weight, output[1], output[2])
     ctx.eps, ctx.num_groups, ctx.has_bias = eps, num_groups, bias is not None
     param = weight if weight is not None else bias
@@ -198,12 +231,13 @@ def _norm_context(ctx, inputs, output):
 
 def _norm_backward(ctx, d_y, _mean, _rstd):
     x, weight, mean, rstd = ctx.saved_tensors
-    dx, dw, db = norm_bwd(d_y, x, weight, mean, rstd, ctx.eps, ctx.num_groups, ctx.param_f32)
-    return dx, dw if weight is not None else None, db if ctx.has_bias else None, None, None
+    want = ctx.needs_input_grad[0], weight is not None and ctx.needs_input_grad[1], ctx.has_bias and ctx.needs_input_grad[2]
+    grads = norm_bwd(d_y, x, weight, mean, rstd, ctx.eps, ctx.num_groups, ctx.param_f32, *want)
+    return (*(g if w else None for g, w in zip(grads, want)), None, None, None)
 
 
 norm_fwd.register_autograd(_norm_backward, setup_context=_norm_context)
 
 
 def layer_norm_via_ops(x, weight, bias, eps, num_groups):
-    return norm_fwd(x, weight, bias, eps, num_groups)[0]
+    return norm_fwd(x, weight, bias, eps, num_groups, torch.is_grad_enabled())[0]

@@ -452,7 +452,8 @@ at::Tensor contiguous_or_none(const at::Tensor& t) { return t.defined() ? in_mem
 
 // out, the state behind the last row (undefined unless wanted), the states at the cuts
 struct DecayResult { at::Tensor out, final, segments; };
-DecayResult run_decay_forward(const DecayArgs& c, bool want_state) {
+// segment_floats: room for the states at the cuts, what they take where it is below zero
+DecayResult run_decay_forward(const DecayArgs& c, bool want_state, int64_t segment_floats = -1) {
   const at::Tensor q = rows_in_place(c.q), k = rows_in_place(c.k), v = rows_in_place(c.v);
   const at::Tensor g = in_memory(c.log_decay), initial = contiguous_or_none(c.initial), lens = contiguous_or_none(c.seq_lens);
   fnb_decay_fwd_args a{};
@@ -463,7 +464,8 @@ DecayResult run_decay_forward(const DecayArgs& c, bool want_state) {
   r.out = empty_rows_like(q);
   if (want_state) r.final = at::empty({q.size(0), q.size(1), q.size(3), q.size(3)}, f32);
   const int64_t cuts = (int64_t)fnb_decay_segment_floats(&a.shape);
-  r.segments = at::empty({cuts}, f32);
+  TORCH_CHECK(segment_floats < 0 || segment_floats >= cuts, "room for ", segment_floats, " floats of states at the cuts, ", cuts, " are needed");
+  r.segments = at::empty({segment_floats < 0 ? cuts : segment_floats}, f32);
   const at::Tensor ws = bytes(fnb_decay_workspace_bytes(&a.shape), q);
   a.q = rows_arg(q); a.k = rows_arg(k); a.v = rows_arg(v); a.out = rows_arg(r.out);
   a.log_decay = g.data_ptr<float>(); a.seq_lens = lens_or_null(lens);
@@ -485,7 +487,7 @@ variable_list run_decay_backward(const DecayArgs& c, const at::Tensor& segments,
   a.shape = decay_shape(q, c.scale);
   check(fnb_check_decay_shape(&a.shape));
   TORCH_CHECK(segments.scalar_type() == at::kFloat && segments.device() == q.device() && segments.is_contiguous() &&
-                  segments.numel() == (int64_t)fnb_decay_segment_floats(&a.shape),
+                  segments.numel() >= (int64_t)fnb_decay_segment_floats(&a.shape),
               "the saved states do not match q");
   at::Tensor dq = empty_rows_like(q), dk = empty_rows_like(k), dv = empty_rows_like(v), d_initial;
   if (want_initial) d_initial = at::empty({q.size(0), q.size(1), q.size(3), q.size(3)}, q.options().dtype(at::kFloat));
@@ -563,31 +565,34 @@ std::pair<at::Tensor, OptTensor> decay_attention(const at::Tensor& q, const at::
   const DecayResult r = run_decay_forward(c, want_state);
   return {r.out, want_state ? OptTensor(r.final) : std::nullopt};
 }
+// For the registered operators: every result a tensor, without elements where it is not wanted.
+at::Tensor or_nothing(const at::Tensor& t, const at::Tensor& like) { return t.defined() ? t : at::empty({0}, like.options()); }
 std::tuple<at::Tensor, at::Tensor, at::Tensor> decay_forward(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& log_decay,
-                                                             double scale, const OptTensor& initial, const OptTensor& seq_lens,
-                                                             const at::Tensor& status) {
+                                                             double scale, const OptTensor& initial, const OptTensor& seq_lens, bool want_state,
+                                                             int64_t segment_floats, const at::Tensor& status) {
   at::AutoGradMode off(false);
   const DecayArgs c = decay_args(q, k, v, log_decay, scale, initial, seq_lens, status);
   c10::cuda::CUDAGuard guard(q.device());
-  if (q.numel() == 0) {
-    const auto f32 = q.options().dtype(at::kFloat);
-    return {empty_rows_like(rows_in_place(q)), state_of_nothing(c), at::empty({0}, f32)};
-  }
-  const DecayResult r = run_decay_forward(c, true);
-  return {r.out, r.final, r.segments};
+  if (q.numel() == 0)
+    return {empty_rows_like(rows_in_place(q)), or_nothing(want_state ? state_of_nothing(c) : at::Tensor(), log_decay), at::empty({std::max<int64_t>(segment_floats, 0)}, log_decay.options())};
+  const DecayResult r = run_decay_forward(c, want_state, segment_floats);
+  return {r.out, or_nothing(r.final, log_decay), r.segments};
 }
-std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> decay_backward(const at::Tensor& d, const at::Tensor& df, const at::Tensor& q,
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> decay_backward(const at::Tensor& d, const OptTensor& df, const at::Tensor& q,
                                                                           const at::Tensor& k, const at::Tensor& v, const at::Tensor& log_decay,
                                                                           double scale, const OptTensor& initial, const OptTensor& seq_lens,
-                                                                          const at::Tensor& segments, const at::Tensor& status) {
+                                                                          const at::Tensor& segments, bool want_initial, const at::Tensor& status) {
   at::AutoGradMode off(false);
   const DecayArgs c = decay_args(q, k, v, log_decay, scale, initial, seq_lens, status);
   TORCH_CHECK(d.sizes() == q.sizes() && d.scalar_type() == q.scalar_type() && d.device() == q.device(), "d_out does not match q");
-  check_state(df, "d_final_state", q);
+  if (df) check_state(*df, "d_final_state", q);
   c10::cuda::CUDAGuard guard(q.device());
-  if (q.numel() == 0) return {empty_rows_like(rows_in_place(q)), empty_rows_like(rows_in_place(k)), empty_rows_like(rows_in_place(v)), df.clone()};
-  const variable_list g = run_decay_backward(c, segments, d, df, true);
-  return {g[0], g[1], g[2], g[3]};
+  if (q.numel() == 0) {
+    const at::Tensor ds = !want_initial ? at::Tensor() : df ? df->clone() : at::zeros({q.size(0), q.size(1), q.size(3), q.size(3)}, log_decay.options());
+    return {empty_rows_like(rows_in_place(q)), empty_rows_like(rows_in_place(k)), empty_rows_like(rows_in_place(v)), or_nothing(ds, log_decay)};
+  }
+  const variable_list g = run_decay_backward(c, segments, d, df ? *df : at::Tensor(), want_initial);
+  return {g[0], g[1], g[2], or_nothing(g[3], log_decay)};
 }
 
 at::Tensor decay_step(const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_, const at::Tensor& state, const at::Tensor& log_decay,
@@ -689,13 +694,16 @@ NormArgs norm_args(const at::Tensor& x, const OptTensor& weight, const OptTensor
 const void* data_or_null(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 struct NormResult { at::Tensor y, mean, rstd; };
-NormResult run_norm_forward(const NormArgs& c, bool keep) {
+NormResult run_norm_forward(const NormArgs& c, bool keep, bool apart = false) {      // apart: statistics in memory of their own each
   NormResult r;
   fnb_norm_fwd_args a{};
   a.shape = norm_shape(c.x, norm_param_type(c), c.groups, c.eps);
   const at::Tensor x = norm_rows(c.x), w = contiguous_or_none(c.weight), b = contiguous_or_none(c.bias);
   r.y = at::empty(c.x.sizes(), c.x.options());
-  if (keep) {
+  if (keep && apart) {
+    r.mean = at::empty({a.shape.rows * c.groups}, c.x.options().dtype(at::kFloat));
+    r.rstd = at::empty_like(r.mean);
+  } else if (keep) {
     const at::Tensor stats = at::empty({2, a.shape.rows * c.groups}, c.x.options().dtype(at::kFloat));
     r.mean = stats.select(0, 0);
     r.rstd = stats.select(0, 1);
@@ -780,30 +788,31 @@ at::Tensor layer_norm(const at::Tensor& x, const OptTensor& weight, const OptTen
   at::AutoGradMode off(false);
   return run_norm_forward(c, false).y;
 }
-std::tuple<at::Tensor, at::Tensor, at::Tensor> norm_forward(const at::Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps, int64_t groups) {
+std::tuple<at::Tensor, at::Tensor, at::Tensor> norm_forward(const at::Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps, int64_t groups,
+                                                            bool keep) {
   at::AutoGradMode off(false);
   c10::cuda::CUDAGuard guard(x.device());
   const NormArgs c = norm_args(x, weight, bias, eps, groups);
-  if (x.numel() == 0) {
-    const auto f32 = x.options().dtype(at::kFloat);
-    return {at::empty(x.sizes(), x.options()), at::empty({0}, f32), at::empty({0}, f32)};
-  }
-  const NormResult r = run_norm_forward(c, true);
-  return {r.y, r.mean.clone(), r.rstd.clone()};
+  const at::Tensor none = at::empty({0}, x.options().dtype(at::kFloat));
+  if (x.numel() == 0) return {at::empty(x.sizes(), x.options()), none, at::empty_like(none)};
+  const NormResult r = run_norm_forward(c, keep, true);
+  return {r.y, or_nothing(r.mean, none), or_nothing(r.rstd, none)};
 }
 std::tuple<at::Tensor, at::Tensor, at::Tensor> norm_backward(const at::Tensor& d, const at::Tensor& x, const OptTensor& weight, const at::Tensor& mean,
-                                                             const at::Tensor& rstd, double eps, int64_t groups, bool param_f32) {
+                                                             const at::Tensor& rstd, double eps, int64_t groups, bool param_f32, bool want_x, bool want_w,
+                                                             bool want_b) {
   at::AutoGradMode off(false);
   c10::cuda::CUDAGuard guard(x.device());
   norm_args(x, weight, std::nullopt, eps, groups);
   TORCH_CHECK(d.sizes() == x.sizes() && d.scalar_type() == x.scalar_type() && d.device() == x.device(), "d_y does not match x");
+  const at::ScalarType param = param_f32 ? at::kFloat : x.scalar_type();
+  const at::Tensor none = at::empty({0}, x.options().dtype(param));
   if (x.numel() == 0) {
-    const auto p = x.options().dtype(param_f32 ? at::kFloat : x.scalar_type());
-    return {at::empty(x.sizes(), x.options()), at::zeros({x.size(-1)}, p), at::zeros({x.size(-1)}, p)};
+    const auto zeros = [&](bool want) { return want ? at::zeros({x.size(-1)}, none.options()) : at::empty_like(none); };
+    return {want_x ? at::empty(x.sizes(), x.options()) : at::empty({0}, x.options()), zeros(want_w), zeros(want_b)};
   }
-  const variable_list g = run_norm_backward(x, weight ? *weight : at::Tensor(), mean, rstd, d, groups, eps, param_f32 ? at::kFloat : x.scalar_type(), true, true,
-                                            true);
-  return {g[0], g[1], g[2]};
+  const variable_list g = run_norm_backward(x, weight ? *weight : at::Tensor(), mean, rstd, d, groups, eps, param, want_x, want_w, want_b);
+  return {or_nothing(g[0], x), or_nothing(g[1], none), or_nothing(g[2], none)};
 }
 
 }  // namespace

@@ -50,7 +50,7 @@ def decay_attention(q, k, v, log_decay, scale=None, initial_state=None, seq_lens
         _C.refuse_tangents("decay_attention", q, k, v, log_decay, initial_state)
     if torch.compiler.is_compiling() or _C.wants_operators(q, k, v, log_decay, initial_state, seq_lens):
         from . import _ops
-        out, state = _ops.decay_attention_via_ops(q, k, v, log_decay, scale, initial_state, seq_lens)
+        out, state = _ops.decay_attention_via_ops(q, k, v, log_decay, scale, initial_state, seq_lens, bool(return_state))
     else:
         out, state = _C.native().decay_attention(q, k, v, log_decay, scale, initial_state, seq_lens, bool(return_state), _C._status(q.device))
     return (out, state) if return_state else out

@@ -1,0 +1,24 @@
+"""Sizes and refusals of the attention with a decay and of the layer norm that no device is needed for."""
+import ctypes as C
+import random
+
+import pytest
+import torch
+
+from flashnystrom_b200 import _lib, _ops
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return _lib.load()
+
+
+def test_bound_of_the_states_at_the_cuts(lib):
+    """What a traced call sets aside for the states at the cuts is enough for every length: the split never has more segments than the bound allows."""
+    r = random.Random(1)
+    for _ in range(3000):
+        B, H, N, D = r.randint(1, 40), r.randint(1, 40), int(2 ** r.uniform(0, 20)), r.choice([16, 32, 64, 128])
+        for code, dtype in ((_lib.FNB_F32, torch.float32), (_lib.FNB_F16, torch.float16), (_lib.FNB_BF16, torch.bfloat16)):
+            s = _lib.DecayShape(B, H, N, D, code, 0.125, 0)
+            # (the SM count without a device is that of a B200)
+            assert lib.fnb_decay_segment_floats(C.byref(s)) <= _ops._segment_bound(B, H, N, D, dtype, 148)

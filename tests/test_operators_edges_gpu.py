@@ -3,6 +3,7 @@ import ctypes as C
 
 import pytest
 import torch
+import torch._dynamo.testing
 
 from oracle import operators_oracle as O
 
@@ -335,3 +336,64 @@ def test_empty_calls_compiled(cuda_device, shape):
             results.append([*out, *torch.autograd.grad(sum(o.sum() for o in out), leaves)])
         for a, b in zip(*results):
             assert a.shape == b.shape and a.dtype == b.dtype and torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("split,state", [(True, False), (False, True)])
+def test_compiled_calls_are_the_eager_ones(cuda_device, dtype, split, state):
+    """Bits, order of memory and gradients of a compiled call, over lengths that it was not compiled for: one compilation serves them all."""
+    from flashnystrom_b200 import decay_attention, layer_norm
+    log_decay = torch.tensor([-0.1, -0.01], device="cuda")
+    torch._dynamo.reset()
+    counter = torch._dynamo.testing.CompileCounterWithBackend("aot_eager")
+
+    def f(q, k, v, s0):
+        return decay_attention(q, k, v, log_decay, initial_state=s0, return_state=state)
+    compiled = torch.compile(f, fullgraph=True, backend=counter, dynamic=True)
+    for N in (300, 130, 4097, 700):
+        def make(seed):
+            t = _normal(2, N, 2, 64, seed=seed, dtype=dtype).transpose(1, 2)
+            return t if split else t.contiguous()
+        d, ds, results = make(5), _normal(2, 2, 64, 64, seed=6), []
+        for call in (f, compiled):
+            leaves = [make(i).requires_grad_(True) for i in range(3)]
+            s0 = _normal(2, 2, 64, 64, seed=7).requires_grad_(True) if state else None
+            r = call(*leaves, s0)
+            leaves += [s0] if state else []
+            results.append([*(r if state else (r,)), *torch.autograd.grad(r, leaves, (d, ds) if state else d)])
+        for a, b in zip(*results):
+            assert torch.equal(a, b) and a.stride() == b.stride()
+    assert counter.frame_count == 1
+    x, w, b = _normal(30, 96, seed=1, dtype=dtype), _normal(96, seed=2), _normal(96, seed=3)
+    for wanted in ((True, True, True), (False, True, False), (True, False, True), (False, False, False)):
+        results = []
+        for call in (layer_norm, torch.compile(lambda *a: layer_norm(*a), fullgraph=True, backend="aot_eager")):
+            leaves = [t.clone().requires_grad_(q) for t, q in zip((x, w, b), wanted)]
+            y = call(*leaves)
+            results.append([y, *torch.autograd.grad(y, [t for t in leaves if t.requires_grad], x)] if any(wanted) else [y])
+        assert all(torch.equal(p, q) for p, q in zip(*results))
+    with torch.no_grad():
+        assert torch.equal(torch.compile(lambda *a: layer_norm(*a), fullgraph=True, backend="aot_eager")(x, w, b), layer_norm(x, w, b))
+
+
+def test_registered_operators(cuda_device):
+    """Their schemas, fake results (sizes, strides, types) and autograd formulas against real calls."""
+    ops = torch.ops.flashnystrom_b200
+    log_decay, s0 = torch.tensor([-0.1, -0.01], device="cuda"), _normal(1, 2, 64, 64, seed=4)
+    for split in (False, True):
+        q, k, v = (_normal(1, 200, 2, 64, seed=i, dtype=torch.float32).transpose(1, 2) for i in range(3))
+        if not split:
+            q, k, v = (t.contiguous() for t in (q, k, v))
+        for want_state, bounded in ((True, False), (False, True)):
+            torch.library.opcheck(ops.decay_fwd.default, (q, k, v, log_decay, 0.125, s0, None, want_state, bounded), test_utils=("test_schema", "test_faketensor"))
+        segments = ops.decay_fwd(q, k, v, log_decay, 0.125, s0, None)[2]
+        for d_state, want_initial in ((None, False), (s0, True)):
+            torch.library.opcheck(ops.decay_bwd.default, (v, d_state, q, k, v, log_decay, 0.125, s0, None, segments, want_initial), test_utils=("test_schema", "test_faketensor"))
+    t = lambda a: a[:, :, 0].contiguous()  # noqa: E731
+    torch.library.opcheck(ops.decay_step.default, (t(q), t(k), t(v), s0.clone(), log_decay, 0.125, None), test_utils=("test_schema", "test_faketensor"))
+    x, w = _normal(7, 96, seed=1), _normal(96, seed=2)
+    for keep in (True, False):
+        torch.library.opcheck(ops.norm_fwd.default, (x, w, None, 1e-5, 3, keep), test_utils=("test_schema", "test_faketensor"))
+    _, mean, rstd = ops.norm_fwd(x, w, None, 1e-5, 3)
+    for want in ((True, True, True), (False, True, False)):
+        torch.library.opcheck(ops.norm_bwd.default, (x, x, w, mean, rstd, 1e-5, 3, True, *want), test_utils=("test_schema", "test_faketensor"))
