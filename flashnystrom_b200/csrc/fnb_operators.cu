@@ -77,6 +77,12 @@ static int check_rows(const fnb_rows& t, const char* name, int dtype) {
   if (t.stride_b < 0 || t.stride_h < 0 || t.stride_n < 0) return fail(FNB_ERR_INVALID_ARGUMENT, "%s has a negative stride", name);
   return 0;
 }
+// FP32 and int32 arrays of the caller are read and written element by element: at their type's alignment, or not at all
+template <class... P>
+static int check_words(const P*... p) {
+  if (((reinterpret_cast<uintptr_t>(p) & 3u) | ...)) return fail(FNB_ERR_INVALID_ARGUMENT, "a float or int32 array is not aligned to its type");
+  return 0;
+}
 static bool vec_rows(const fnb_rows& t, int dtype) {
   const int64_t v = 16 / (int64_t)elem_bytes(dtype);
   return aligned16(t.data) && t.stride_b % v == 0 && t.stride_h % v == 0 && t.stride_n % v == 0;
@@ -429,6 +435,7 @@ int fnb_decay_forward(const fnb_decay_fwd_args* a) {
   const struct { const fnb_rows* t; const char* name; } big[] = {{&a->q, "q"}, {&a->k, "k"}, {&a->v, "v"}, {&a->out, "out"}};
   for (const auto& e : big)
     if (int rc = check_rows(*e.t, e.name, a->shape.dtype)) return rc;
+  if (int rc = check_words(a->log_decay, a->seq_lens, a->initial_state, a->final_state, a->segment_states)) return rc;
   DeviceGuard g(a->device);
   if (!g.ok) return fail(FNB_ERR_CUDA, "cannot select CUDA device %d", a->device);
   int max_smem = 0, cc = 0, sms = 0;
@@ -453,6 +460,7 @@ int fnb_decay_backward(const fnb_decay_bwd_args* a) {
                                                                  {&a->dq, "dq"}, {&a->dk, "dk"}, {&a->dv, "dv"}};
   for (const auto& e : big)
     if (int rc = check_rows(*e.t, e.name, a->shape.dtype)) return rc;
+  if (int rc = check_words(a->log_decay, a->seq_lens, a->initial_state, a->d_final_state, a->d_initial_state, a->segment_states)) return rc;
   DeviceGuard g(a->device);
   if (!g.ok) return fail(FNB_ERR_CUDA, "cannot select CUDA device %d", a->device);
   int max_smem = 0, cc = 0, sms = 0;
@@ -491,6 +499,7 @@ int fnb_decay_step(const fnb_decay_step_args* a) {
   for (const auto& e : big)
     if (int rc = check_rows(*e.t, e.name, a->dtype)) return rc;
   if (!a->log_decay || !a->states) return fail(FNB_ERR_INVALID_ARGUMENT, "log_decay and states must not be NULL");
+  if (int rc = check_words(a->log_decay, a->slots)) return rc;
   if (!aligned16(a->states)) return fail(FNB_ERR_INVALID_ARGUMENT, "states must be 16-byte aligned");
   if (a->num_states <= 0 || (!a->slots && a->num_states < a->batch))
     return fail(FNB_ERR_INVALID_ARGUMENT, "%lld states for %lld rows", (long long)a->num_states, (long long)a->batch);
