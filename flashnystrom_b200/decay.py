@@ -94,7 +94,7 @@ class DecayAttention(nn.Module):
         if self.head_dim not in (16, 32, 64, 128):
             raise ValueError(f"head_dim must be 16, 32, 64 or 128, got {self.head_dim}")
         g = default_log_decay(heads) if log_decay is None else torch.as_tensor(log_decay, dtype=torch.float32).detach().clone()
-        if g.shape != (heads,) or not bool((g <= 0).all()):
+        if g.shape != (heads,) or not (g.is_meta or bool((g <= 0).all())):
             raise ValueError("log_decay must hold one value <= 0 for each head")
         self.register_buffer("log_decay", g)
         self.q_proj = nn.Linear(dim, dim, bias=False)

@@ -5,7 +5,7 @@ import random
 import pytest
 import torch
 
-from flashnystrom_b200 import _lib, _ops
+from flashnystrom_b200 import DecayAttention, _lib, _ops
 
 
 @pytest.fixture(scope="module")
@@ -42,3 +42,13 @@ def test_words_off_their_alignment(lib, where):
         args.log_decay = 64
         setattr(args, where, 66)
         assert call(C.byref(args)) == -1 and "not aligned to its type" in _lib.last_error()
+
+
+def test_module_without_memory():
+    """Built on the meta device, given memory, then a checkpoint's values."""
+    whole = DecayAttention(128, heads=2)
+    with torch.device("meta"):
+        m = DecayAttention(128, heads=2)
+    assert m.log_decay.is_meta and m.q_proj.weight.is_meta
+    m.to_empty(device="cpu").load_state_dict(whole.state_dict())
+    assert torch.equal(m.log_decay, whole.log_decay) and m.log_decay.dtype == torch.float32
