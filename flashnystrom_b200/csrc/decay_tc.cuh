@@ -149,7 +149,6 @@ decay_tc_sums_kernel(const __grid_constant__ CUtensorMap tm_y, const __grid_cons
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 11);
   int* abort_word = reinterpret_cast<int*>(tmem_slot + 1);
   uint32_t* s_seen = reinterpret_cast<uint32_t*>((reinterpret_cast<uintptr_t>(abort_word + 1) + 15) & ~(uintptr_t)15);      // fp16: [2][8], by chunk parity, bits of y by warp
-  volatile int* s_fresh = reinterpret_cast<volatile int*>(s_seen + 16);      // fp16: [2], likewise: the sums in tensor memory have been taken out before this chunk
   constexpr bool F16 = UmmaFmt<T>::v == 0;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -215,7 +214,7 @@ decay_tc_sums_kernel(const __grid_constant__ CUtensorMap tm_y, const __grid_cons
         if (!__all_sync(0xffffffffu, ok)) break;
         tc_fence_after();
         // (what was added up before a new sum has been taken out by the time y' is ready)
-        const bool fresh = first_of_span(i) || (F16 && __any_sync(0xffffffffu, s_fresh[u]));
+        const bool fresh = first_of_span(i);
         const uint32_t a_z = smem_u32(s_in + st * 2 * L::kTile + L::kTile), a_y = smem_u32(s_y + u * L::kTerms * L::kTile);
 #pragma unroll 1
         for (int t = L::kTerms - 1; t >= 0; --t)
@@ -293,6 +292,11 @@ decay_tc_sums_kernel(const __grid_constant__ CUtensorMap tm_y, const __grid_cons
 #pragma unroll
           for (int j = 0; j < 16; ++j) S[j] = (past ? decayed ? S[j] : decay_by(w, S[j]) : 0.f) + mul * U[j];
           tmem_st16(t_state + q * 16, S);
+          if (less) {      // (the span's sum goes on from nothing)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) U[j] = 0.f;
+            tmem_st16(t_sum + q * 16, U);
+          }
         }
         tmem_st_wait();
         tc_fence_before();
@@ -306,10 +310,7 @@ decay_tc_sums_kernel(const __grid_constant__ CUtensorMap tm_y, const __grid_cons
         if (!REV && span_end > end) span_end = end;
         in_span = REV ? (int)((i == 0 ? end : row_of(i) + C) - span_end) : (int)(span_end - row_of(i));
       }
-      if (F16) {
-        if (first || less) factor = own;
-        if (threadIdx.x == 0) s_fresh[u] = less;
-      }
+      if (F16 && (first || less)) factor = own;
 #pragma unroll
       for (int q = 0; q < PIECES; ++q) {
         const int idx = threadIdx.x + q * kGroup, r = (idx >> 3) & (C - 1);
