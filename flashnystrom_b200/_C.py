@@ -23,6 +23,7 @@ import math
 import os as _os
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 from . import _lib
 
@@ -291,18 +292,16 @@ def being_transformed():
     return torch._C._get_tracing_state() is not None or torch._C._are_functorch_transforms_active()
 
 
-def wants_operators(*tensors):
-    """Whether a call goes through the registered operators: something traces, transforms or records it, or a tensor (those that are given) is a subclass, so that the C++
-    module would do work that is not seen."""
-    return being_transformed() or torch._C._len_torch_dispatch_stack() > 0 or any(t is not None and type(t) not in _PLAIN for t in tensors)
+def wants_operators():
+    """Whether a call goes through the registered operators: something traces, transforms or records it, so that the C++ module would do work that is not seen.  (Tensors
+    whose class does that the C++ module hands back.)"""
+    return torch._C._len_torch_dispatch_stack() > 0 or being_transformed()
 
 
 def refuse_tangents(name, *tensors):
-    """Forward-mode derivatives have no formula here: refused, so that a tangent is not taken for zero."""
-    if torch.autograd.forward_ad._current_level < 0:
-        return
+    """Forward-mode derivatives have no formula here: refused, so that a tangent is not taken for zero.  (Asked where a level of them is open.)"""
     for t in tensors:
-        if t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+        if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
             raise RuntimeError(f"{name} has no forward-mode derivative")
 
 

@@ -545,25 +545,31 @@ at::Tensor state_of_nothing(const DecayArgs& c) {
   return c.initial.defined() ? c.initial.clone() : at::zeros({c.q.size(0), c.q.size(1), c.q.size(3), c.q.size(3)}, c.q.options().dtype(at::kFloat));
 }
 
+// A subclass that does its own work on operators: the calls below return nothing for one, and the caller goes through the registered operators.
+bool own_dispatch(const at::Tensor& t) { return at::isTensorSubclassLike(t); }
+bool own_dispatch(const OptTensor& t) { return t && at::isTensorSubclassLike(*t); }
+template <class... Ts> bool any_own_dispatch(const Ts&... t) { return (own_dispatch(t) || ...); }
+
 // (out, final state or nothing)
-std::pair<at::Tensor, OptTensor> decay_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& log_decay,
+std::optional<std::pair<at::Tensor, OptTensor>> decay_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& log_decay,
                                                  double scale, const OptTensor& initial, const OptTensor& seq_lens, bool want_state,
                                                  const at::Tensor& status) {
+  if (any_own_dispatch(q, k, v, log_decay, initial, seq_lens)) return std::nullopt;
   const DecayArgs c = decay_args(q, k, v, log_decay, scale, initial, seq_lens, status);
   py::gil_scoped_release nogil;
   c10::cuda::CUDAGuard guard(q.device());
   if (q.numel() == 0) {      // nothing to attend to: the state goes through
     OptTensor state = state_of_nothing(c);
     if (!want_state) state = std::nullopt;
-    return {q + k + v, state};      // (no elements, and a graph to all three)
+    return std::make_pair(q + k + v, state);      // (no elements, and a graph to all three)
   }
   if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() || (initial && initial->requires_grad()))) {
     const variable_list r = DecayNode::apply(q, k, v, initial, c, want_state);
-    return {r[0], want_state ? OptTensor(r[1]) : std::nullopt};
+    return std::make_pair(r[0], want_state ? OptTensor(r[1]) : std::nullopt);
   }
   at::AutoGradMode off(false);
   const DecayResult r = run_decay_forward(c, want_state);
-  return {r.out, want_state ? OptTensor(r.final) : std::nullopt};
+  return std::make_pair(r.out, want_state ? OptTensor(r.final) : std::nullopt);
 }
 // For the registered operators: every result a tensor, without elements where it is not wanted.
 at::Tensor or_nothing(const at::Tensor& t, const at::Tensor& like) { return t.defined() ? t : at::empty({0}, like.options()); }
@@ -595,8 +601,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> decay_backward(const 
   return {g[0], g[1], g[2], or_nothing(g[3], log_decay)};
 }
 
-at::Tensor decay_step(const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_, const at::Tensor& state, const at::Tensor& log_decay,
+std::optional<at::Tensor> decay_step(const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_, const at::Tensor& state, const at::Tensor& log_decay,
                       double scale, const OptTensor& slots) {
+  if (any_own_dispatch(q_, k_, v_, state, log_decay, slots)) return std::nullopt;
   TORCH_CHECK(q_.is_cuda(), "q must be a CUDA tensor (flashnystrom_b200 has no CPU path)");
   TORCH_CHECK(q_.dim() == 3 && k_.dim() == 3 && v_.dim() == 3, "q, k, v must be 3D (B, H, D)");
   check_cuda(q_, "q", q_);
@@ -774,7 +781,8 @@ struct NormNode : torch::autograd::Function<NormNode> {
     return once_differentiable(std::move(g), "layer_norm", {x, kept[1], d});
   }
 };
-at::Tensor layer_norm(const at::Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps, int64_t groups) {
+std::optional<at::Tensor> layer_norm(const at::Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps, int64_t groups) {
+  if (any_own_dispatch(x, weight, bias)) return std::nullopt;
   const NormArgs c = norm_args(x, weight, bias, eps, groups);
   py::gil_scoped_release nogil;
   c10::cuda::CUDAGuard guard(x.device());

@@ -6,6 +6,7 @@ One float32 D x D state for each (batch, head) takes the place of a cache of key
 number of others, and a sequence of N tokens costs N."""
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad as _forward_ad
 
 from . import _C
 from .norm import layer_norm
@@ -46,13 +47,16 @@ def decay_attention(q, k, v, log_decay, scale=None, initial_state=None, seq_lens
     the rows after it by definition, and may reach up to 127 rows before it.  There is no second derivative, no forward-mode one, and no CPU path."""
     _check_tensors("decay_attention", q=q, k=k, v=v, log_decay=log_decay)
     scale = _scale(scale, q.shape[-1] if q.dim() else 0)
+    r = None
     if not torch.compiler.is_compiling():
-        _C.refuse_tangents("decay_attention", q, k, v, log_decay, initial_state)
-    if torch.compiler.is_compiling() or _C.wants_operators(q, k, v, log_decay, initial_state, seq_lens):
+        if _forward_ad._current_level >= 0:
+            _C.refuse_tangents("decay_attention", q, k, v, log_decay, initial_state)
+        if not _C.wants_operators():
+            r = _C.native().decay_attention(q, k, v, log_decay, scale, initial_state, seq_lens, bool(return_state), _C._status(q.device))
+    if r is None:
         from . import _ops
-        out, state = _ops.decay_attention_via_ops(q, k, v, log_decay, scale, initial_state, seq_lens, bool(return_state))
-    else:
-        out, state = _C.native().decay_attention(q, k, v, log_decay, scale, initial_state, seq_lens, bool(return_state), _C._status(q.device))
+        r = _ops.decay_attention_via_ops(q, k, v, log_decay, scale, initial_state, seq_lens, bool(return_state))
+    out, state = r
     return (out, state) if return_state else out
 
 
@@ -67,11 +71,14 @@ def decay_attention_step(q, k, v, state, log_decay, scale=None, slots=None):
     _check_tensors("decay_attention_step", q=q, k=k, v=v, state=state, log_decay=log_decay)
     scale = _scale(scale, q.shape[-1] if q.dim() else 0)
     if not torch.compiler.is_compiling():
-        _C.refuse_tangents("decay_attention_step", q, k, v, state, log_decay)
-    if torch.compiler.is_compiling() or _C.wants_operators(q, k, v, state, log_decay, slots):
-        from . import _ops
-        return _ops.decay_step(q, k, v, state, log_decay, scale, slots)
-    return _C.native().decay_step(q, k, v, state, log_decay, scale, slots)
+        if _forward_ad._current_level >= 0:
+            _C.refuse_tangents("decay_attention_step", q, k, v, state, log_decay)
+        if not _C.wants_operators():
+            out = _C.native().decay_step(q, k, v, state, log_decay, scale, slots)
+            if out is not None:
+                return out
+    from . import _ops
+    return _ops.decay_step(q, k, v, state, log_decay, scale, slots)
 
 
 def default_log_decay(heads):

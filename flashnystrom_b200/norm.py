@@ -1,6 +1,7 @@
 """Layer norm over the last dimension, whole or in groups, forward and backward as the library's own kernels."""
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad as _forward_ad
 
 from . import _C
 
@@ -19,11 +20,14 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, num_groups=1):
     if not isinstance(x, torch.Tensor):
         raise RuntimeError("layer_norm: x must be a tensor")
     if not torch.compiler.is_compiling():
-        _C.refuse_tangents("layer_norm", x, weight, bias)
-    if torch.compiler.is_compiling() or _C.wants_operators(x, weight, bias):
-        from . import _ops
-        return _ops.layer_norm_via_ops(x, weight, bias, float(eps), int(num_groups))
-    return _C.native().layer_norm(x, weight, bias, float(eps), int(num_groups))
+        if _forward_ad._current_level >= 0:
+            _C.refuse_tangents("layer_norm", x, weight, bias)
+        if not _C.wants_operators():
+            y = _C.native().layer_norm(x, weight, bias, float(eps), int(num_groups))
+            if y is not None:
+                return y
+    from . import _ops
+    return _ops.layer_norm_via_ops(x, weight, bias, float(eps), int(num_groups))
 
 
 class LayerNorm(nn.Module):

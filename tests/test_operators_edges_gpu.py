@@ -271,6 +271,25 @@ def test_traced_and_recorded(cuda_device, name):
 
 
 @pytest.mark.parametrize("name", ["attention", "step", "norm"])
+def test_fake_tensors(cuda_device, name):
+    """Tensors without memory, under their mode and outside of it: the call gives one like its result, and touches nothing."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    calls, state = _three()
+    f, x = calls[name]
+    want = f(x)
+    mode = FakeTensorMode(allow_non_fake_inputs=True)
+    fake, before = mode.from_tensor(x), state.clone()
+    with mode:
+        got = f(fake)
+    assert got.shape == want.shape and got.dtype == want.dtype and got.device == want.device and got.stride() == want.stride()
+    if name != "step":      # (the state of the step is not one of these: it has to be under the mode)
+        got = f(fake)
+        assert got.shape == want.shape
+    torch.cuda.synchronize()
+    assert torch.equal(state, before)
+
+
+@pytest.mark.parametrize("name", ["attention", "step", "norm"])
 def test_tangents_are_refused(cuda_device, name):
     """A forward-mode derivative is an error, not zero; outside of one the call is as before."""
     from torch.autograd import forward_ad
