@@ -119,9 +119,10 @@ __device__ __forceinline__ float inverse_of(float power) { return __uint_as_floa
 // One CTA a run, two CTAs an SM: a group of eight warps forms the terms of y', double-buffered, one thread issues the products, which add up in
 // tensor memory over kSpan rows (weights reach back that far) before the group takes them out and decays what it has.
 // EXACT: two terms of fp16, three of bf16, 22 and 24 bits: the sums are FP32 sums, as a state that is handed out has to be.  Where the sums only join
-// segments, one term, as the chunks inside a segment have it: what an output gets from before its segment is then rounded once, like the rest.
-// Bound by what the eight warps do (a value into terms, two swizzled stores).  1 x 16 x 65536 x 64, 268 MB read: 58 us with one term (4.6 TB/s), 74 with two (fp16),
-// 87 with three (bf16); 4 x 16 x 16384 x 128, 537 MB, one term, half of the rows (what the first of two segments needs): 68 us.
+// segments, one term, as the chunks inside a segment have it: what an output gets from before its segment is then rounded once, like the rest.  In fp16 y' may have a power
+// of two in it (sums_factor_of), so that small keys keep these bits.
+// Bound by what the eight warps do (a value into terms, two swizzled stores).  1 x 16 x 65536 x 64, 268 MB read: 58 us with one term (4.6 TB/s) in bf16 and 74 in fp16 (58 before
+// it looked at y's size), 86 with two (fp16, 74), 80 with three (bf16); 4 x 16 x 16384 x 128, 537 MB, one term, half of the rows (what the first of two segments needs): 68 us.
 template <class T, int D, bool EXACT> struct SumsCfg {
   static constexpr int C = D == 64 ? 64 : 32, kStages = 3, kTerms = !EXACT ? 1 : UmmaFmt<T>::v == 0 ? 2 : 3;
   static constexpr int kSpan = 256;
@@ -358,8 +359,8 @@ decay_tc_sums_kernel(const __grid_constant__ CUtensorMap tm_y, const __grid_cons
 // through tensor memory, the output tile takes x's place, and with heads of 128 y' takes y's.  The state stays in tensor memory: B takes it out to form
 // its two 16-bit terms, puts it back decayed, and the products add y'^T z to it.
 //
-// Measured: 1 x 16 x 65536 x 64, a pass of 537 MB, 144 CTAs: bf16 122 us (4.4 TB/s), fp16 142 (its state is scaled by powers of two to stay in range); 4 x 16 x
-// 16384 x 128, 1.07 GB, 128 CTAs: 216 us (5.0 TB/s; 193 is what 128 of 148 SMs move).  Bound with heads of 64 by the warps' arithmetic in turn: of 127 us, 8 go
+// Measured: 1 x 16 x 65536 x 64, a pass of 537 MB, 144 CTAs: bf16 123 us (4.4 TB/s), fp16 151 (scores, y' and the state are taken into its range by powers of two); 4 x 16 x
+// 16384 x 128, 1.07 GB, 128 CTAs: 220 us (4.9 TB/s; 193 is what 128 of 148 SMs move), fp16 250.  Bound with heads of 64 by the warps' arithmetic in turn: of 127 us, 8 go
 // without forming y', 10 without the state, 16 without weighing the scores, 6 without the output tile.  What decides it is code that stays in the instruction
 // cache: loops over 16 columns that are not unrolled took 131 us where pieces of 32 columns, unrolled, took 150 (fp16 152 and 187).
 // Sixteen warps in group B: no change with heads of 64, 238 in place of 216 with 128.  Outputs stored from registers: 195 in place of 162 at the time.

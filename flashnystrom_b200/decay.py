@@ -41,10 +41,12 @@ def decay_attention(q, k, v, log_decay, scale=None, initial_state=None, seq_lens
     return_state: also return the state behind each sequence's last row (B, H, D, D), float32, differentiable: what the next
         call takes as initial_state, or decay_attention_step as its state.
 
-    Sums and states are float32.  fp16 and bf16 calls round each pair's score, or the key's share of the state, once to their type on the way;
-    a state that is handed out does not have that rounding, and asking for it may change the last bit of the output of long sequences.  Scores
-    and states may leave fp16's range as long as the output does not.  A row of q, k or v that counts and holds an infinity or NaN reaches
-    the rows after it by definition, and may reach up to 127 rows before it.  There is no second derivative, no forward-mode one, and no CPU path."""
+    Sums and states are float32.  fp16 and bf16 calls round each pair's score, or the key's share of the state, once to their type on the way: outputs and gradients are off by
+    1.25 to 1.45 times what rounding the result alone leaves.  A state that is handed out does not have that rounding, and asking for it may change the last
+    bit of the output of long sequences.  Scores, states and tensors may lie far above or below fp16's range as long as the result does not.  fp16 and bf16 tensors whose start or
+    strides are not multiples of 16 bytes take float32 arithmetic on the CUDA cores, several times slower.  A row of q, k or v that counts and holds an
+    infinity or NaN reaches the rows after it by definition, and may reach up to 127 rows before it; rows behind a length stay zeros.  There is no second
+    derivative, no forward-mode one, and no CPU path."""
     _check_tensors("decay_attention", q=q, k=k, v=v, log_decay=log_decay)
     scale = _scale(scale, q.shape[-1] if q.dim() else 0)
     r = None
@@ -67,7 +69,7 @@ def decay_attention_step(q, k, v, state, log_decay, scale=None, slots=None):
     slots: (B,) int32 on the GPU, the state of each row; a row whose slot is not in 0..S-1 (-1, say) is idle: its output is zero and no state
         is touched.  Rows that name the same slot are taken in the order of the batch, as tokens that follow one another.
         None: row b has state b, and S is B.
-    Returns (B, H, D).  No gradient: with one wanted the call is refused (decay_attention has one)."""
+    Returns (B, H, D).  No gradient: with one wanted, or a tangent given, the call is refused (decay_attention has a gradient)."""
     _check_tensors("decay_attention_step", q=q, k=k, v=v, state=state, log_decay=log_decay)
     scale = _scale(scale, q.shape[-1] if q.dim() else 0)
     if not torch.compiler.is_compiling():

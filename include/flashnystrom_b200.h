@@ -325,6 +325,8 @@ FNB_API int fnb_conv_residual_dweight(const fnb_conv_dw_args* args);
  * are clamped to 0 .. seq_len) do not take part, whatever they hold: outputs and gradients are zero there and
  * the final state is the one behind the last row that counts.
  *
+ * States, decays, lengths and slots are read word by word: pointers that are not aligned to their type are refused.
+ *
  * segment_states: FP32, fnb_decay_segment_floats() of them (0: may be NULL), written by the forward and read by the backward:
  * the states at the cuts where the sequence is split over SMs.  workspace: fnb_decay_workspace_bytes(), 256-byte aligned,
  * for either direction.  Both sizes follow the SM count of the device that is current when they are asked for. */
