@@ -236,6 +236,7 @@ decay_tc_sums_kernel(const __grid_constant__ CUtensorMap tm_y, const __grid_cons
     // (a wait that gave up does not leave the loop: the warps meet at barriers, and the status word has it)
     const DecayPair whole = s_pair[0], last = s_pair[1];
     constexpr int PIECES = L::kTile / 16 / kGroup;
+    const bool grows = pw[L::kSpan] > 1.f;      // (a decay above 0: y' may be larger than y, so no factor)
     int in_span = 0;
     int64_t span_end = 0;        // forwards: the row behind the span; backwards: its first row
     float factor = 1.f;          // fp16: of y' in the sums that are in tensor memory now
@@ -250,7 +251,7 @@ decay_tc_sums_kernel(const __grid_constant__ CUtensorMap tm_y, const __grid_cons
       const int64_t c0 = row_of(i);
       const int nv = end - c0 < C ? (int)(end - c0) : C;
       // fp16: sums share a factor of y'.  A span begins with that of its first chunk, and does not look at others where that is 1 (the usual).
-      const bool looks = F16 && any && (first || factor != 1.f);
+      const bool looks = F16 && any && !grows && (first || factor != 1.f);
       if (warp == 0) {      // (one warp asks for all)
         if (any) mbar_wait(full + st, (i / NST) & 1, ab, 0x7400 + i);
         if (ends) mbar_wait(y_free + (u ^ 1), ((i - 1) >> 1) & 1, ab, 0x7600 + i);      // (the products of the chunk before)
@@ -730,6 +731,7 @@ __global__ void __launch_bounds__(MainCfg<D>::kThreads, 1) decay_tc_kernel(const
     // 1 x 16 x 65536 x 64 forward 237 us, 228 without; 4 x 16 x 16384 x 128 479 and 472.)
     float y_factor = 1.f, held = 1.f;      // of the chunk that put_state is at; the one that the state in tensor memory has
     uint32_t seen = 0;                     // the bits of y that this thread has seen
+    const bool grows = power(C - 1) > 1.f;      // (a decay above 0: y' may be larger than y, so no factor)
     constexpr int PIECES = L::kTile / 16 / kGroup;
     const auto rows_in = [&](int i) { const int64_t n = end - row_of(i); return n < C ? (int)n : C; };
     // the factor by what all threads have seen of a small y
@@ -904,7 +906,7 @@ __global__ void __launch_bounds__(MainCfg<D>::kThreads, 1) decay_tc_kernel(const
             form_y(i, 1.f);
           }
           if (i > 0) await_products(i - 1);
-          const bool small = !named_barrier_or(2, kGroup, not_small(seen));
+          const bool small = !named_barrier_or(2, kGroup, grows || not_small(seen));
           tc_fence_after();
           if (forms) {
             y_factor = 1.f;
@@ -930,7 +932,7 @@ __global__ void __launch_bounds__(MainCfg<D>::kThreads, 1) decay_tc_kernel(const
           seen = bits;
         }
         if (c > 0) await_products(c - 1);
-        const bool small = !named_barrier_or(2, kGroup, not_small(seen));
+        const bool small = !named_barrier_or(2, kGroup, grows || not_small(seen));
         tc_fence_after();
         y_factor = small && forms ? find_factor() : 1.f;
         put_state(c);

@@ -130,7 +130,7 @@ def test_a_decay_to_nothing_takes_what_is_not_finite_with_it(cuda_device, dtype,
     O.within(state, ref_state, b[1], torch.float32)
 
 
-def _check_range(t, log_decay, s0=None, ds=None, scale=None, lens=None, final=True):
+def _check_range(t, log_decay, s0=None, ds=None, scale=None, lens=None, final=True, in_range=True):
     """Outputs, states and gradients of fp16 calls within the roundings of values that are in range (no smallest step of fp16 but that of the result)."""
     from flashnystrom_b200 import _C, decay_attention
     leaves = [x.detach().requires_grad_(True) for x in t[:3]] + ([] if s0 is None else [s0.detach().requires_grad_(True)])
@@ -143,7 +143,7 @@ def _check_range(t, log_decay, s0=None, ds=None, scale=None, lens=None, final=Tr
     asked = [x.clone().requires_grad_(True) for x in wide[:3]] + ([] if s0 is None else [w0.clone().requires_grad_(True)])
     ref, ref_state = O.decay_attention(*asked[:3], log_decay, scale, None if s0 is None else asked[3], lens)
     refs = torch.autograd.grad((ref * wide[3]).sum() + (0 if ds is None else (ref_state * ws).sum()), asked)
-    bounds = O.decay_bounds(*wide, log_decay, O.isqrt(t[0].shape[-1]) if scale is None else scale, w0, ws, lens, t[0].dtype, in_range=True)
+    bounds = O.decay_bounds(*wide, log_decay, O.isqrt(t[0].shape[-1]) if scale is None else scale, w0, ws, lens, t[0].dtype, in_range=in_range)
     O.within(out, ref, bounds[0], t[0].dtype)
     if final:
         O.within(state, ref_state, bounds[1], torch.float32)
@@ -416,3 +416,13 @@ def test_registered_operators(cuda_device):
     _, mean, rstd = ops.norm_fwd(x, w, None, 1e-5, 3)
     for want in ((True, True, True), (False, True, False)):
         torch.library.opcheck(ops.norm_bwd.default, (x, x, w, mean, rstd, 1e-5, 3, True, *want), test_utils=("test_schema", "test_faketensor"))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("size", [1e-4, 0.3, 1.0])
+@pytest.mark.parametrize("B,N", [(1, 700), (1, 4000), (160, 300)])
+def test_growing_decays_in_fp16(cuda_device, D, size, B, N):
+    """log_decay above 0 is the caller's affair, and not refused: weights above 1 leave no type's range that the result and its terms keep to.  (Growth of e^0.8 over
+    4000 rows, e^3 over 300.)"""
+    t = [_normal(B, 2, N, D, seed=i, mul=m).half() for i, m in enumerate((1.0, size, 1.0, 0.1))]
+    _check_range(t, torch.tensor([0.01 if N == 300 else 2e-4, 1e-4], device="cuda"), scale=0.01, in_range=False)
